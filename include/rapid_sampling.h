@@ -37,6 +37,7 @@ extern "C" {
 #define RS_ERR_DEVICE      -9   /* a kernel gave up waiting for its peer workgroups           */
 #define RS_ERR_SCRATCH     -10  /* rs_sample_static: the call needs more than RS_STATIC_SCRATCH_BYTES */
 #define RS_ERR_UNSUPPORTED -11  /* the current device is not a whole MI355X (256 compute units)     */
+#define RS_ERR_SHAPE       -12  /* rs_quantize_blocks, rs_linear_blocks: a size or a row stride out of range */
 
 /* Bytes of RNG state per row.  Same size as the reference's
  * curandStatePhilox4_32_10_t record (sampling.cu:9,141) so that the opaque
@@ -445,6 +446,96 @@ int rs_floor_read(const float *logits_device, int64_t row_stride, int32_t *out_d
  * are not cleared.  For tests; no counterpart in the reference.
  */
 int rs_exp_error(int32_t below, int64_t *out_device, void *stream);
+
+/*
+ * Log probabilities of given tokens, with the entropy of their rows, their ranks
+ * and the likeliest alternatives.  No counterpart in the reference.  One launch.
+ *
+ * With z = x / temperature, m = max z and S = sum e^(z - m) over the V logits x
+ * of a row, for the row's token t:
+ *   logprobs      (z_t - m) - ln S
+ *   entropy       ln S - sum e^(z - m) (z - m) / S, with 0 * -inf = 0
+ *   rank          1 + (tokens with a larger logit) + (tokens of a lower index with
+ *                 an equal one): 1 is the likeliest token, and a token of rank
+ *                 r <= top is the r-th alternative
+ *   top_*         the `top` largest logits' log probabilities and tokens, likeliest
+ *                 first, equal ones by the lower index
+ * float32 throughout, whatever the logits' type; the sums do not depend on chance
+ * (no floating-point atomics).
+ *
+ *   logits        V logits for each of B x T rows; row (b, t) begins stride_b * b +
+ *                 stride_t * t elements on (either stride may be 0).  Rows need no
+ *                 alignment but the element's own.  1 <= V <= 1048576.
+ *   tokens        row (b, t)'s token, token_stride_b * b + token_stride_t * t on,
+ *                 int32 or (tokens_64 = 1) int64.  A negative one is none: its
+ *                 logprobs is 0, its rank 0.  One of V or more has NaN and rank 0.
+ *   temperature   0.001 to 1000
+ *   top           0 to RS_LOGPROBS_TOP_MAX, at most V
+ *   logprobs, entropy, rank   B*T each, contiguous; any may be NULL
+ *   top_logprobs, top_tokens  (B*T, top); may be NULL if top is 0
+ *   stats         NULL, or (B*T, 4) floats, 16-byte aligned, for the gradient
+ *   workspace     rs_logprobs_workspace_bytes() bytes of device memory, 256-byte
+ *                 aligned, cleared once with rs_workspace_init and not shared with
+ *                 other entry points; calls that share it are ordered on one stream.
+ *
+ * A row of nothing but -inf has log probabilities of -inf and entropy 0.  A row
+ * with a NaN or +inf has NaN for its log probabilities and its entropy; in the
+ * orders NaN comes after -inf.
+ */
+#define RS_LOGPROBS_TOP_MAX 64
+size_t rs_logprobs_workspace_bytes(void);
+int rs_token_logprobs(const void *logits_device, int32_t logits_dtype, int64_t stride_b, int64_t stride_t,
+                      const void *tokens_device, int32_t tokens_64, int64_t token_stride_b, int64_t token_stride_t,
+                      int32_t B, int32_t T, int32_t V, double temperature, int32_t top,
+                      float *logprobs_device, float *entropy_device, int32_t *rank_device,
+                      float *top_logprobs_device, int32_t *top_tokens_device, float *stats_device,
+                      void *workspace_device, size_t workspace_bytes, void *stream);
+
+/*
+ * Gradient of the logits from the gradients g of logprobs, h of entropy and a of
+ * top_logprobs (any may be NULL: none):
+ *   dx_i = (g [i = t] + sum_j a_j [i = id_j] - p_i (g + sum_j a_j + h (ln p_i + entropy))) / temperature
+ * rounded once to the logits' type.  logits, tokens, temperature and top as in the
+ * call whose `stats` and `top_tokens` are passed.  A gradient's stride is 1
+ * (contiguous) or 0 (one number for all).  grad_logits: contiguous rows.  A row
+ * with a negative token has no g; one of nothing but -inf has gradient 0.
+ * One launch, no workspace.
+ */
+int rs_token_logprobs_backward(const void *logits_device, int32_t logits_dtype, int64_t stride_b, int64_t stride_t,
+                               const void *tokens_device, int32_t tokens_64, int64_t token_stride_b, int64_t token_stride_t,
+                               int32_t B, int32_t T, int32_t V, double temperature, int32_t top,
+                               const float *stats_device, const int32_t *top_tokens_device,
+                               const float *grad_logprobs_device, int32_t grad_logprobs_stride,
+                               const float *grad_entropy_device, int32_t grad_entropy_stride,
+                               const float *grad_top_device, int32_t grad_top_stride,
+                               void *grad_logits_device, void *stream);
+
+/*
+ * Values in 8 bits (e4m3fn: 4 bits of exponent, 3 of significand, no infinity)
+ * with a float32 scale for each block of block_rows x 128 values, block_rows 1
+ * (activations) or 128 (weights):
+ *   scale = max(max |x| / 448, 2^-126)      q = x / scale, to nearest, ties to even
+ * Blocks at the ends are what is left.  x: R rows of K values, x_row_stride
+ * elements apart.  q: rows q_row_stride bytes apart, a multiple of 16 and at least K
+ * rounded up to one, 16-byte aligned; bytes behind column K are cleared up to the
+ * stride, or to a multiple of 128 if that is less.  scale: ceil(R / block_rows) x
+ * ceil(K / 128), contiguous.  A NaN or an infinity gives NaN in its place.
+ * One launch.  No counterpart in the reference.
+ */
+#define RS_LINEAR_MAX (1 << 24)
+int rs_quantize_blocks(const void *x_device, int32_t x_dtype, int64_t x_row_stride, int32_t block_rows,
+                       int32_t R, int32_t K, void *q_device, int64_t q_row_stride, float *scale_device, void *stream);
+
+/*
+ * y = x w^T for such values: x (M, K) with scales of 1 x 128 (M, ceil(K / 128)), w
+ * (N, K) with scales of 128 x 128 (ceil(N / 128), ceil(K / 128)), both scales
+ * contiguous, y (M, N) float32, bfloat16 or float16 (RS_DTYPE_*).  Rows of x and w
+ * 16-byte aligned; bytes behind column K are not looked at.  Sums in float32, one
+ * rounding.  No counterpart in the reference.
+ */
+int rs_linear_blocks(const void *x_device, int64_t x_row_stride, const float *x_scale_device,
+                     const void *w_device, int64_t w_row_stride, const float *w_scale_device,
+                     int32_t M, int32_t N, int32_t K, void *y_device, int32_t y_dtype, int64_t y_row_stride, void *stream);
 
 #ifdef __cplusplus
 }

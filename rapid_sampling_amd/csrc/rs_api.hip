@@ -729,7 +729,7 @@ using namespace rs;
 
 extern "C" {
 
-int rs_version(void) { return 420; }
+int rs_version(void) { return 500; }
 
 const char *rs_error_string(int code)
 {
@@ -746,6 +746,7 @@ const char *rs_error_string(int code)
     case RS_ERR_DEVICE:      return "a workgroup gave up waiting for its peers";
     case RS_ERR_SCRATCH:     return "the call needs a larger workspace than the static scratch of rs_sample_static (RS_STATIC_SCRATCH_BYTES)";
     case RS_ERR_UNSUPPORTED: return "the device is not a whole MI355X (256 compute units in 8 XCDs): the kernels' waits are only known to end on one";
+    case RS_ERR_SHAPE:       return "a size or a row stride is out of range";
     default:                 return "unknown error";
     }
 }

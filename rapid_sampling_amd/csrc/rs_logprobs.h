@@ -1,0 +1,548 @@
+// Log probabilities of given tokens, with the row's entropy, the token's rank and the likeliest alternatives, and the
+// gradient of the logits.  z = x / T, m = max z, S = sum e^(z - m):
+//
+//   logprob = (z_t - m) - ln S            entropy H = ln S - sum e^(z - m) (z - m) / S
+//   rank    = 1 + #{x > x_t} + #{x = x_t, i < t}
+//   top     = the largest logits, equal ones by the lower index
+//   dx_i    = ([i = t] g + sum_j [i = id_j] a_j - p_i (g + sum_j a_j + h (ln p_i + H))) / T,   p_i = e^(z_i - m) / S
+//
+// NaN counts as less than -inf in the orders; a row that holds NaN or +inf has NaN for its sums.  A row of nothing but
+// -inf has no distribution: its log probabilities are -inf, its entropy 0, its gradient 0.
+#pragma once
+
+#include "rs_common.h"
+
+namespace rs {
+
+constexpr int kLpThreads = 256;
+constexpr int kLpWaves   = kLpThreads / kWave;
+constexpr int kLpTopMax  = RS_LOGPROBS_TOP_MAX;
+constexpr int kLpCap     = 512;          // candidates that are put in order
+constexpr float kLn2 = 0.693147180559945309f;
+
+// What a workgroup of a split row leaves for the last of the row's workgroups.
+struct alignas(16) LpSlice {
+    float    m, s, t;                    // see LpSums
+    uint32_t above;                      // tokens of the slice that come before the given one
+    float    top[kLpThreads];            // largest logit of each thread
+};
+static_assert(sizeof(LpSlice) == 1040, "rs_logprobs_workspace_bytes");
+
+struct LpParams {
+    const void *logits;
+    int64_t     stride_b, stride_t;      // elements from a batch, from a position to the next
+    const void *tokens;
+    int64_t     token_b, token_t;
+    int32_t     tokens_64;               // int64 token ids, else int32
+    int32_t     T, V;
+    int32_t     top;
+    float       c, inv_t;                // log2(e) / T, 1 / T
+    float      *logprobs, *entropy;
+    int32_t    *rank;
+    float      *top_logprobs;
+    int32_t    *top_tokens;
+    float4     *stats;                   // for the gradient: max, log2 of the sum, entropy; or null
+    uint32_t    S, J;                    // workgroups per row; windows per thread and slice
+    LpSlice    *slices;                  // split rows: what the workgroups of a row leave for the last of them
+    uint32_t   *arrived;                 // ... and how many have, per row; zero between calls
+};
+
+struct LpGradParams {
+    const void   *logits;
+    int64_t       stride_b, stride_t;
+    const void   *tokens;
+    int64_t       token_b, token_t;
+    int32_t       tokens_64;
+    int32_t       T, V;
+    int32_t       top;
+    float         c, inv_t;
+    const float4 *stats;
+    const int32_t *top_tokens;
+    const float  *g, *h, *a;             // gradients of logprob, entropy, alternatives; any may be null
+    int32_t       g_stride, h_stride, a_stride;
+    void         *grad;                  // contiguous rows of the logits' type
+    uint32_t      chunks;                // workgroups per row
+};
+
+// ------------------------------------------------------------- element types --
+// A window is 16 bytes of a row: 4 or 8 logits.  Rows begin at any multiple of the element's size, so windows are read
+// and written without a claim on alignment: the hardware takes 16 bytes at any address.
+template <int DT> struct Elem;
+template <> struct Elem<RS_DTYPE_F32> {
+    using T = float;
+    static constexpr int kVec = 4, kBits = 32;     // bits of an order key that tell values apart
+    static __device__ __forceinline__ void wide(const uint4 r, float (&x)[4])
+    {
+        x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
+    }
+    static __device__ __forceinline__ uint4 narrow(const float (&x)[4])
+    {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+    static __device__ __forceinline__ float one(T v) { return v; }
+    static __device__ __forceinline__ T round(float x) { return x; }
+};
+template <> struct Elem<RS_DTYPE_BF16> {
+    using T = uint16_t;
+    static constexpr int kVec = 8, kBits = 16;
+    static __device__ __forceinline__ void wide(const uint4 r, float (&x)[8])
+    {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    }
+    static __device__ __forceinline__ T round(float x)       // to nearest, ties to even; NaN stays one
+    {
+        const __bf16 b = (__bf16)x;
+        return __builtin_bit_cast(uint16_t, b);
+    }
+    static __device__ __forceinline__ uint4 narrow(const float (&x)[8])
+    {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)round(x[2 * i]) | (uint32_t)round(x[2 * i + 1]) << 16;
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ float one(T v) { return __uint_as_float((uint32_t)v << 16); }
+};
+template <> struct Elem<RS_DTYPE_F16> {
+    using T = uint16_t;
+    static constexpr int kVec = 8, kBits = 19;     // sign, 5 + 3 bits of exponent once widened, 10 of significand
+    static __device__ __forceinline__ float one(T v) { return (float)__builtin_bit_cast(_Float16, v); }
+    static __device__ __forceinline__ T round(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+    static __device__ __forceinline__ void wide(const uint4 r, float (&x)[8])
+    {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { x[2 * i] = one((T)w[i]); x[2 * i + 1] = one((T)(w[i] >> 16)); }
+    }
+    static __device__ __forceinline__ uint4 narrow(const float (&x)[8])
+    {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)round(x[2 * i]) | (uint32_t)round(x[2 * i + 1]) << 16;
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+template <int DT>
+__device__ __forceinline__ uint4 load_window(const typename Elem<DT>::T *row, uint32_t n)
+{
+    uint4 r;
+    __builtin_memcpy(&r, row + (size_t)n * Elem<DT>::kVec, 16);
+    return r;
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Order of the logits as whole numbers: 0 nothing, 1 NaN, then the numbers; -0 is 0.
+__device__ __forceinline__ uint32_t lp_key(float x) { return x != x ? 1u : fkey(x + 0.0f); }
+// ... and of the tokens: by the logit, equal ones by the lower index.  All are distinct.
+__device__ __forceinline__ uint64_t lp_token(float x, uint32_t i) { return (uint64_t)lp_key(x) << 32 | (0xFFFFFFFFu - i); }
+
+// ------------------------------------------------------------- running sums --
+struct LpSums {
+    float m, s, t;      // largest logit x; sum of e = 2^((x - m) c); sum of e (x - m) c
+};
+
+// The sums as they are for a maximum of `m` (at least a.m).  Where nothing but -inf was seen a.s and a.t are 0, and stay so.
+__device__ __forceinline__ void lp_rebase(LpSums &a, float m, float c)
+{
+    const float d = fmaxf((a.m - m) * c, -1e30f);       // -inf - (-inf) and the like: NaN -> -1e30
+    const float f = exp2_hw(d);
+    a.t = f * __builtin_fmaf(a.s, d, a.t);
+    a.s = f * a.s;
+    a.m = m;
+}
+
+// N more logits.  Two exponents of a lane's window share the sums' chains; the terms of (x - m) c below -200 have e = 0
+// and must not make 0 * inf.
+template <int N>
+__device__ __forceinline__ void lp_take(LpSums &a, const float (&x)[N], float c)
+{
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+    lp_rebase(a, fmaxf(a.m, top), c);
+    const float base = a.m == -__builtin_inff() ? 0.0f : a.m;
+    float s[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float z = (x[i] - base) * c;
+        const float e = exp2_hw(z);
+        s[i & 1] += e;
+        t[i & 1] = __builtin_fmaf(e, fmaxf(z, -200.0f), t[i & 1]);
+    }
+    a.s += s[0] + s[1];
+    a.t += t[0] + t[1];
+}
+
+__device__ __forceinline__ float wave_max_f(float v)
+{
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    return v;
+}
+__device__ __forceinline__ float wave_sum_f(float v)
+{
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+struct LpShared {
+    float    m[kLpWaves], s[kLpWaves], t[kLpWaves];
+    uint32_t above[kLpWaves];
+    uint32_t key[kLpThreads];            // order key of each thread's largest logit
+    uint64_t lane_top[kLpThreads];
+    uint64_t cand[kLpCap];
+    uint32_t n;
+    uint32_t last;
+    uint16_t hot[kLpThreads];
+};
+
+// The sums of the workgroup, in every thread.
+__device__ __forceinline__ void lp_block(LpSums &a, uint32_t &above, float c, LpShared &sh)
+{
+    const uint32_t w = threadIdx.x / kWave;
+    lp_rebase(a, wave_max_f(a.m), c);
+    a.s = wave_sum_f(a.s);
+    a.t = wave_sum_f(a.t);
+    if (threadIdx.x % kWave == 0) { sh.m[w] = a.m; sh.s[w] = a.s; sh.t[w] = a.t; sh.above[w] = above; }
+    __syncthreads();
+    float m = sh.m[0];
+#pragma unroll
+    for (int i = 1; i < kLpWaves; ++i) m = fmaxf(m, sh.m[i]);
+    LpSums all{m, 0.0f, 0.0f};
+    above = 0;
+#pragma unroll
+    for (int i = 0; i < kLpWaves; ++i) {
+        LpSums one{sh.m[i], sh.s[i], sh.t[i]};
+        lp_rebase(one, m, c);
+        all.s += one.s; all.t += one.t;
+        above += sh.above[i];
+    }
+    a = all;
+}
+
+// --------------------------------------------------------- the alternatives --
+// The `top` largest tokens of the row.  A thread's largest logit is known from the pass.  The top-th largest of those, tau,
+// is no larger than the top-th largest logit (that many threads hold one as large), so every token wanted is at least tau,
+// and only threads whose own largest is at least tau hold such tokens.  Only their windows are read again, by
+// all lanes: about `top` threads' worth of the row.  What is at least tau goes to a list, a few tokens more than are
+// wanted, and a token's place is the number of tokens in the list before it.
+//
+// A list that does not fit (rows of thousands of equal logits, or of large ones that all fall to a few threads) is cut by the
+// same bound over the lanes of the second reading, with the index as part of the order, and, if that is not enough,
+// by halving the range of the bound until it is.  That ends: the orders are distinct.
+template <int DT>
+struct LpRow {
+    using E = Elem<DT>;
+    const typename E::T *row;
+    uint32_t V, full, J;                 // logits; whole windows; windows of a thread, over the whole row
+
+    // f(logit, index) for the windows of the n_hot threads in sh.hot, spread over the workgroup, and for the row's last few
+    template <typename F>
+    __device__ __forceinline__ void each(const LpShared &sh, uint32_t n_hot, F f) const
+    {
+        const uint32_t items = n_hot * J;
+        for (uint32_t i = threadIdx.x; i < items; i += kLpThreads) {
+            const uint32_t h = i / J, j = i - h * J;
+            const uint32_t n = j * kLpThreads + sh.hot[h];
+            if (n < full) {
+                float x[E::kVec];
+                E::wide(load_window<DT>(row, n), x);
+#pragma unroll
+                for (int k = 0; k < E::kVec; ++k) f(x[k], n * E::kVec + k);
+            }
+        }
+        const uint32_t i = full * E::kVec + threadIdx.x;
+        if (i < V) f(E::one(row[i]), i);
+    }
+};
+
+// The largest t with at least `k` of the workgroup's keys >= t (0 if k > kLpThreads); only the upper BITS bits matter.
+template <int BITS, typename K>
+__device__ __forceinline__ K lp_kth(const K *key, uint32_t k)
+{
+    constexpr int kAll = (int)sizeof(K) * 8;
+    K mine[kLpWaves];
+#pragma unroll
+    for (int i = 0; i < kLpWaves; ++i) mine[i] = key[i * kWave + threadIdx.x % kWave];
+    K t = 0;
+    for (int bit = kAll - 1; bit >= kAll - BITS; --bit) {
+        const K c = t | (K)1 << bit;
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < kLpWaves; ++i) n += (uint32_t)__popcll(__ballot(mine[i] >= c));
+        if (n >= k) t = c;
+        if (n == k) break;
+    }
+    return t;
+}
+
+template <int DT>
+__device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float largest, const LpSums &a, float log_s, float inv_t, uint32_t top,
+                                                float *out_logprobs, int32_t *out_tokens, LpShared &sh)
+{
+    const uint32_t tid = threadIdx.x, lane = tid % kWave, w = tid / kWave;
+    sh.key[tid] = lp_key(largest);
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    uint32_t tau = lp_kth<Elem<DT>::kBits>(sh.key, top);
+    if (tau <= fkey(-__builtin_inff())) tau = 1u;        // fewer numbers than are wanted, perhaps: NaN too
+    uint32_t n_hot = 0;
+#pragma unroll
+    for (int i = 0; i < kLpWaves; ++i) {
+        const uint64_t is = __ballot(sh.key[i * kWave + lane] >= tau);
+        if (i == (int)w && ((is >> lane) & 1)) sh.hot[n_hot + __popcll(is & ((1ull << lane) - 1))] = (uint16_t)tid;
+        n_hot += (uint32_t)__popcll(is);
+    }
+    __syncthreads();
+    row.each(sh, n_hot, [&](float x, uint32_t i) {
+        if (lp_key(x) >= tau) {
+            const uint32_t at = atomicAdd(&sh.n, 1u);
+            if (at < kLpCap) sh.cand[at] = lp_token(x, i);
+        }
+    });
+    __syncthreads();
+    if (sh.n > kLpCap) {
+        uint64_t best = 0;
+        row.each(sh, n_hot, [&](float x, uint32_t i) { best = max(best, lp_token(x, i)); });
+        sh.lane_top[tid] = best;
+        __syncthreads();
+        uint64_t lo = max(lp_kth<64>(sh.lane_top, top), (uint64_t)tau << 32), hi = ~0ull;
+        for (uint64_t t = lo;; t = lo + (hi - lo) / 2) {
+            __syncthreads();
+            if (tid == 0) sh.n = 0;
+            __syncthreads();
+            row.each(sh, n_hot, [&](float x, uint32_t i) {
+                const uint64_t k = lp_token(x, i);
+                if (k >= t) {
+                    const uint32_t at = atomicAdd(&sh.n, 1u);
+                    if (at < kLpCap) sh.cand[at] = k;
+                }
+            });
+            __syncthreads();
+            if (sh.n > kLpCap) lo = t;
+            else if (sh.n < top) hi = t;
+            else break;
+        }
+    }
+    const uint32_t n = sh.n;
+    for (uint32_t i = tid; i < n; i += kLpThreads) {
+        const uint64_t k = sh.cand[i];
+        uint32_t place = 0;
+        for (uint32_t j = 0; j < n; ++j) place += sh.cand[j] > k;
+        if (place < top) {
+            const uint32_t id = 0xFFFFFFFFu - (uint32_t)k;
+            const float x = Elem<DT>::one(row.row[id]);
+            out_tokens[place] = (int32_t)id;
+            out_logprobs[place] = x == -__builtin_inff() && a.s == a.s ? x : (x - a.m) * inv_t - log_s;
+        }
+    }
+}
+
+// ------------------------------------------------------------------- forward --
+// U windows of each thread are in flight at a time.
+template <int DT, int U, bool GUARD>
+__device__ __forceinline__ void lp_batch(const typename Elem<DT>::T *row, uint32_t n0, uint32_t full, uint32_t token_window, float before, float after,
+                                         float c, LpSums &a, uint32_t &above)
+{
+    using E = Elem<DT>;
+    constexpr float kNone = -__builtin_inff();
+    float x[U * E::kVec], edge[U];
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t n = n0 + u * kLpThreads;
+        if (!GUARD || n < full) raw[u] = load_window<DT>(row, n);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t n = n0 + u * kLpThreads;
+        float v[E::kVec];
+        E::wide(raw[u], v);
+        edge[u] = n < token_window ? before : after;
+        if (GUARD && n >= full) edge[u] = __builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < E::kVec; ++i) x[u * E::kVec + i] = GUARD && n >= full ? kNone : v[i];
+    }
+    lp_take(a, x, c);
+#pragma unroll
+    for (int i = 0; i < U * E::kVec; ++i) above += (uint32_t)__popcll(__ballot(x[i] >= edge[i / E::kVec]));
+}
+
+// One workgroup per row, or S of them (SPLIT), each on a stretch of the row, of which the last to arrive finishes the row.
+// Nothing waits.
+template <int DT, bool SPLIT>
+__global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
+{
+    using E = Elem<DT>;
+    constexpr int U = 4;
+    __shared__ LpShared sh;
+    const uint32_t r = SPLIT ? blockIdx.x / p.S : blockIdx.x, slice = SPLIT ? blockIdx.x - r * p.S : 0;
+    const uint32_t b = r / (uint32_t)p.T, pos = r - b * (uint32_t)p.T;
+    const uint32_t V = (uint32_t)p.V, full = V / E::kVec, tid = threadIdx.x;
+    const typename E::T *row = (const typename E::T *)p.logits + (int64_t)b * p.stride_b + (int64_t)pos * p.stride_t;
+    const int64_t at = (int64_t)b * p.token_b + (int64_t)pos * p.token_t;
+    const int64_t token = p.tokens_64 ? ((const int64_t *)p.tokens)[at] : (int64_t)((const int32_t *)p.tokens)[at];
+    const bool given = token >= 0 && token < (int64_t)V;
+    const uint32_t tok = given ? (uint32_t)token : 0u;
+    const float x_t = E::one(row[tok]);
+    // a window before the token's counts x >= x_t, one behind it x > x_t, that is x >= the next number up; in the token's own
+    // window the equal ones before it are counted at the end.  Below -inf there is nothing but NaN.
+    float before = x_t, after;
+    {
+        const uint32_t bits = __float_as_uint(x_t + 0.0f);
+        after = __uint_as_float(bits & 0x80000000u ? bits - 1u : bits + 1u);
+        if (x_t != x_t) before = after = -__builtin_inff();
+    }
+    const uint32_t token_window = tok / E::kVec;
+
+    LpSums a{-__builtin_inff(), 0.0f, 0.0f};
+    uint32_t above = 0;
+    const uint32_t first = slice * p.J * kLpThreads, end = min(full, first + p.J * kLpThreads);
+    uint32_t n = first;
+    for (; n + U * kLpThreads <= end; n += U * kLpThreads) lp_batch<DT, U, false>(row, n + tid, end, token_window, before, after, p.c, a, above);
+    for (; n < end; n += kLpThreads) lp_batch<DT, 1, true>(row, n + tid, end, token_window, before, after, p.c, a, above);
+    const float largest = a.m;
+    if (!SPLIT || slice == p.S - 1u) {
+        const uint32_t i = full * E::kVec + tid;
+        const float x[1] = {i < V ? E::one(row[i]) : -__builtin_inff()};
+        lp_take(a, x, p.c);
+        above += (uint32_t)__popcll(__ballot(x[0] >= (i < V ? (i < tok ? before : after) : __builtin_nanf(""))));
+    }
+    lp_block(a, above, p.c, sh);
+
+    float mine = largest;
+    if constexpr (SPLIT) {
+        LpSlice *slices = p.slices + (size_t)r * p.S;
+        a_store(&slices[slice].top[tid], largest);
+        if (tid == 0) {
+            a_store(&slices[slice].m, a.m); a_store(&slices[slice].s, a.s); a_store(&slices[slice].t, a.t);
+            a_store(&slices[slice].above, above);
+        }
+        wait_vmem();
+        __syncthreads();
+        if (tid == 0) {
+            sh.last = __hip_atomic_fetch_add(&p.arrived[r], 1u, __ATOMIC_RELAXED, RS_AGENT) == p.S - 1u;
+            if (sh.last) a_store(&p.arrived[r], 0u);
+        }
+        __syncthreads();
+        if (!sh.last) return;
+        // the row's sums, from the slices' in turn; the largest logit of each thread over them
+        a = LpSums{-__builtin_inff(), 0.0f, 0.0f};
+        above = 0;
+        for (uint32_t s = tid; s < p.S; s += kLpThreads) {
+            LpSums o{a_load(&slices[s].m), a_load(&slices[s].s), a_load(&slices[s].t)};
+            const float m = fmaxf(a.m, o.m);
+            lp_rebase(a, m, p.c);
+            lp_rebase(o, m, p.c);
+            a.s += o.s; a.t += o.t;
+            above += a_load(&slices[s].above);
+        }
+        above = wave_sum(above);
+        if (p.top) for (uint32_t s = 0; s < p.S; ++s) mine = fmaxf(mine, a_load(&slices[s].top[tid]));
+        __syncthreads();
+        lp_block(a, above, p.c, sh);
+    }
+
+    const float log_s = logf(a.s);
+    const bool empty = a.s == 0.0f;                     // nothing but -inf
+    if (tid < kWave) {
+        // equal logits before the token in its own window
+        const uint32_t i = token_window * E::kVec + tid;
+        const bool eq = tid < (uint32_t)E::kVec && i < tok && i < full * E::kVec && E::one(row[i]) == x_t;
+        above += (uint32_t)__popcll(__ballot(eq));
+        if (x_t != x_t)                                 // NaN: behind every number, among its like by the index
+            for (uint32_t j = tid; j < ((tok + kWave - 1u) & ~(kWave - 1u)); j += kWave) {
+                const float x = j < tok ? E::one(row[j]) : 0.0f;
+                above += (uint32_t)__popcll(__ballot(x != x));
+            }
+        if (tid == 0) {
+            const float h = log_s - a.t * kLn2 / a.s;
+            const float lp = x_t == -__builtin_inff() && a.s == a.s ? x_t : (x_t - a.m) * p.inv_t - log_s;
+            const float entropy = empty ? 0.0f : h;
+            if (p.logprobs) p.logprobs[r] = given ? lp : token < 0 ? 0.0f : __builtin_nanf("");
+            if (p.entropy) p.entropy[r] = entropy;
+            if (p.rank) p.rank[r] = given ? (int32_t)above + 1 : 0;
+            if (p.stats) p.stats[r] = empty ? make_float4(0.0f, __builtin_inff(), 0.0f, 0.0f) : make_float4(a.m, log2f(a.s), entropy, 0.0f);
+        }
+    }
+    if (p.top) {
+        const LpRow<DT> all{row, V, full, (full + kLpThreads - 1u) / kLpThreads};
+        lp_alternatives<DT>(all, mine, a, log_s, p.inv_t, (uint32_t)p.top, p.top_logprobs + (size_t)r * p.top, p.top_tokens + (size_t)r * p.top, sh);
+    }
+}
+
+// ------------------------------------------------------------------ gradient --
+// dx_i = p_i (alpha + beta ln2 (z_i - ..)): one exponential and a product per logit; the few tokens that were named are then
+// written once more, whole, by the workgroup that wrote them first.
+template <int DT>
+__global__ __launch_bounds__(kLpThreads) void logprobs_grad_kernel(LpGradParams p)
+{
+    using E = Elem<DT>;
+    constexpr int U = 4;
+    const uint32_t r = blockIdx.x / p.chunks, chunk = blockIdx.x - r * p.chunks;
+    const uint32_t b = r / (uint32_t)p.T, pos = r - b * (uint32_t)p.T;
+    const uint32_t V = (uint32_t)p.V, full = V / E::kVec, tid = threadIdx.x, lane = tid % kWave;
+    const typename E::T *row = (const typename E::T *)p.logits + (int64_t)b * p.stride_b + (int64_t)pos * p.stride_t;
+    typename E::T *out = (typename E::T *)p.grad + (size_t)r * V;
+    const uint32_t n0 = chunk * (U * kLpThreads) + tid;
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) if (n0 + u * kLpThreads < full) raw[u] = load_window<DT>(row, n0 + u * kLpThreads);
+
+    const float4 st = p.stats[r];
+    const int64_t at = (int64_t)b * p.token_b + (int64_t)pos * p.token_t;
+    const int64_t token = p.tokens_64 ? ((const int64_t *)p.tokens)[at] : (int64_t)((const int32_t *)p.tokens)[at];
+    float g = p.g && token >= 0 ? p.g[(int64_t)r * p.g_stride] : 0.0f;
+    if (token >= (int64_t)V) g = __builtin_nanf("");
+    const float h = p.h ? p.h[(int64_t)r * p.h_stride] : 0.0f;
+    float a = 0.0f;
+    int64_t id = -1;
+    if (p.a && lane < (uint32_t)p.top) {
+        id = p.top_tokens[(size_t)r * p.top + lane];
+        a = p.a[((int64_t)r * p.top + lane) * p.a_stride];
+    }
+    float a_sum = p.a ? wave_sum_f(a) : 0.0f;
+    const float alpha = -(g + a_sum + h * st.z) * p.inv_t, beta = -h * kLn2 * p.inv_t;
+    const float m = st.x, log2_s = st.y;
+    auto grad = [&](float x) {
+        const float z = (x - m) * p.c - log2_s;
+        return exp2_hw(z) * __builtin_fmaf(beta, fmaxf(z, -200.0f), alpha);
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t n = n0 + u * kLpThreads;
+        if (n < full) {
+            float x[E::kVec];
+            E::wide(raw[u], x);
+#pragma unroll
+            for (int i = 0; i < E::kVec; ++i) x[i] = grad(x[i]);
+            const uint4 v = E::narrow(x);
+            __builtin_memcpy(out + (size_t)n * E::kVec, &v, 16);
+        }
+    }
+    const bool last = chunk == p.chunks - 1u;
+    if (last) {
+        const uint32_t i = full * E::kVec + tid;
+        if (i < V) out[i] = E::round(grad(E::one(row[i])));
+    }
+    // the named tokens of this chunk
+    const int64_t begin = (int64_t)chunk * (U * kLpThreads * E::kVec);
+    const int64_t end = last ? (int64_t)V : begin + U * kLpThreads * E::kVec;
+    const bool token_here = token >= begin && token < end;
+    const bool id_here = id >= begin && id < end;
+    const uint64_t any = __ballot(id_here || token_here);
+    if (any == 0 || log2_s == __builtin_inff()) return;
+    wait_vmem();
+    __syncthreads();
+    if (tid >= (uint32_t)kWave) return;
+    const uint64_t both = __ballot(id_here && id == token);
+    if (id_here) out[id] = E::round(grad(E::one(row[id])) + (a + (id == token ? g : 0.0f)) * p.inv_t);
+    if (token_here && !both && lane == 0) out[token] = E::round(grad(E::one(row[token])) + g * p.inv_t);
+}
+
+}  // namespace rs

@@ -1,0 +1,112 @@
+// Instantiations, launchers and C entry points of the log probabilities and their gradient.
+#include "rs_logprobs.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace rs {
+
+constexpr uint32_t kLpSplitMost = 1024;   // workgroups of a call whose rows are split: four to a compute unit
+
+// Workgroups per row: one, or enough for about four to a compute unit, each with at least four windows per thread.
+static uint32_t lp_split(uint32_t rows, uint32_t windows)
+{
+    const uint32_t most = kLpSplitMost / rows, per = (windows + 4u * kLpThreads - 1u) / (4u * kLpThreads);
+    return std::max(1u, std::min(most, per));
+}
+
+static int lp_check(const void *logits, int32_t dtype, const void *tokens, int32_t tokens_64, int64_t B, int64_t T, int64_t V, double temperature, int32_t top)
+{
+    if (!(V > 0 && V <= 1048576)) return RS_ERR_VOCAB;
+    if (B <= 0 || T <= 0 || B > 0x7FFFFFFF || T > 0x7FFFFFFF || B * T > 0x7FFFFFFF) return RS_ERR_BATCH;
+    if (!(temperature >= 0.001 && temperature <= 1000.0)) return RS_ERR_TEMPERATURE;
+    if (!logits || !tokens) return RS_ERR_NULL;
+    if (dtype != RS_DTYPE_F32 && dtype != RS_DTYPE_BF16 && dtype != RS_DTYPE_F16) return RS_ERR_ARG;
+    if (tokens_64 != 0 && tokens_64 != 1) return RS_ERR_ARG;
+    if (top < 0 || top > kLpTopMax || top > V) return RS_ERR_ARG;
+    if (((uintptr_t)logits & (dtype == RS_DTYPE_F32 ? 3 : 1)) || ((uintptr_t)tokens & (tokens_64 ? 7 : 3))) return RS_ERR_ALIGN;
+    return RS_OK;
+}
+
+template <int DT>
+static void lp_launch(const LpParams &p, uint32_t rows, hipStream_t st)
+{
+    if (p.S > 1) hipLaunchKernelGGL((logprobs_kernel<DT, true>), dim3(rows * p.S), dim3(kLpThreads), 0, st, p);
+    else hipLaunchKernelGGL((logprobs_kernel<DT, false>), dim3(rows), dim3(kLpThreads), 0, st, p);
+}
+
+}  // namespace rs
+
+using namespace rs;
+
+extern "C" {
+
+size_t rs_logprobs_workspace_bytes(void) { return (size_t)kLpSplitMost * (sizeof(LpSlice) + 16); }
+
+int rs_token_logprobs(const void *logits, int32_t dtype, int64_t stride_b, int64_t stride_t,
+                      const void *tokens, int32_t tokens_64, int64_t token_stride_b, int64_t token_stride_t,
+                      int32_t B, int32_t T, int32_t V, double temperature, int32_t top,
+                      float *logprobs, float *entropy, int32_t *rank, float *top_logprobs, int32_t *top_tokens,
+                      float *stats, void *workspace, size_t workspace_bytes, void *stream)
+{
+    const int bad = lp_check(logits, dtype, tokens, tokens_64, B, T, V, temperature, top);
+    if (bad != RS_OK) return bad;
+    if (!workspace || (top && (!top_logprobs || !top_tokens))) return RS_ERR_NULL;
+    if (workspace_bytes < rs_logprobs_workspace_bytes() || ((uintptr_t)workspace & 255)) return RS_ERR_WORKSPACE;
+    if ((uintptr_t)stats & 15) return RS_ERR_ALIGN;
+    const uint32_t rows = (uint32_t)B * (uint32_t)T;
+    const uint32_t vec = dtype == RS_DTYPE_F32 ? 4 : 8, windows = (uint32_t)V / vec;
+    LpParams p;
+    p.logits = logits; p.stride_b = stride_b; p.stride_t = stride_t;
+    p.tokens = tokens; p.tokens_64 = tokens_64; p.token_b = token_stride_b; p.token_t = token_stride_t;
+    p.T = T; p.V = V; p.top = top;
+    p.c = (float)(1.4426950408889634 / temperature); p.inv_t = (float)(1.0 / temperature);
+    p.logprobs = logprobs; p.entropy = entropy; p.rank = rank; p.top_logprobs = top_logprobs; p.top_tokens = top_tokens;
+    p.stats = (float4 *)stats;
+    p.S = lp_split(rows, windows);
+    p.J = (windows + p.S * kLpThreads - 1) / (p.S * kLpThreads);
+    p.arrived = (uint32_t *)workspace;
+    p.slices = (LpSlice *)((char *)workspace + 16 * (size_t)kLpSplitMost);
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == RS_DTYPE_F32) lp_launch<RS_DTYPE_F32>(p, rows, st);
+    else if (dtype == RS_DTYPE_BF16) lp_launch<RS_DTYPE_BF16>(p, rows, st);
+    else lp_launch<RS_DTYPE_F16>(p, rows, st);
+    return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
+}
+
+int rs_token_logprobs_backward(const void *logits, int32_t dtype, int64_t stride_b, int64_t stride_t,
+                               const void *tokens, int32_t tokens_64, int64_t token_stride_b, int64_t token_stride_t,
+                               int32_t B, int32_t T, int32_t V, double temperature, int32_t top,
+                               const float *stats, const int32_t *top_tokens,
+                               const float *grad_logprobs, int32_t grad_logprobs_stride,
+                               const float *grad_entropy, int32_t grad_entropy_stride,
+                               const float *grad_top, int32_t grad_top_stride,
+                               void *grad_logits, void *stream)
+{
+    const int bad = lp_check(logits, dtype, tokens, tokens_64, B, T, V, temperature, top);
+    if (bad != RS_OK) return bad;
+    if (!stats || !grad_logits || (grad_top && top && !top_tokens)) return RS_ERR_NULL;
+    if (((uintptr_t)stats & 15) || ((uintptr_t)grad_logits & (dtype == RS_DTYPE_F32 ? 3 : 1))) return RS_ERR_ALIGN;
+    for (const int32_t s : {grad_logprobs_stride, grad_entropy_stride, grad_top_stride}) if (s != 0 && s != 1) return RS_ERR_ARG;
+    const uint32_t rows = (uint32_t)B * (uint32_t)T;
+    const uint32_t vec = dtype == RS_DTYPE_F32 ? 4 : 8, windows = (uint32_t)V / vec;
+    LpGradParams p;
+    p.logits = logits; p.stride_b = stride_b; p.stride_t = stride_t;
+    p.tokens = tokens; p.tokens_64 = tokens_64; p.token_b = token_stride_b; p.token_t = token_stride_t;
+    p.T = T; p.V = V; p.top = top;
+    p.c = (float)(1.4426950408889634 / temperature); p.inv_t = (float)(1.0 / temperature);
+    p.stats = (const float4 *)stats; p.top_tokens = top_tokens;
+    p.g = grad_logprobs; p.h = grad_entropy; p.a = top ? grad_top : nullptr;
+    p.g_stride = grad_logprobs_stride; p.h_stride = grad_entropy_stride; p.a_stride = grad_top_stride;
+    p.grad = grad_logits;
+    p.chunks = std::max(1u, (windows + 4 * kLpThreads - 1) / (4 * kLpThreads));
+    if ((uint64_t)rows * p.chunks > 0x7FFFFFFFull) return RS_ERR_BATCH;
+    const dim3 grid(rows * p.chunks), block(kLpThreads);
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == RS_DTYPE_F32) hipLaunchKernelGGL(logprobs_grad_kernel<RS_DTYPE_F32>, grid, block, 0, st, p);
+    else if (dtype == RS_DTYPE_BF16) hipLaunchKernelGGL(logprobs_grad_kernel<RS_DTYPE_BF16>, grid, block, 0, st, p);
+    else hipLaunchKernelGGL(logprobs_grad_kernel<RS_DTYPE_F16>, grid, block, 0, st, p);
+    return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
+}
+
+}  // extern "C"

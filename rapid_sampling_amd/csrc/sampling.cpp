@@ -45,6 +45,7 @@ struct Entry {
     at::Tensor ws;
     int64_t B = 0, V = 0;
     rs_policy *policy = nullptr;
+    at::Tensor logprobs_ws;                 // workspace of token_logprobs: of one size, so never replaced
     bool captured = false;                  // a stream capture has recorded calls that point into ws
     std::vector<at::Tensor> retired;        // outgrown workspaces a captured graph may still point into
     std::vector<rs_policy *> retired_policies;   // replaced policies whose pinned words a captured graph's kernels may still write
@@ -246,7 +247,287 @@ at::Tensor run(const at::Tensor &logits, const Shape &s, at::Tensor *penalties, 
     return out;
 }
 
+// ------------------------------------------------ log probabilities of given tokens --
+
+// The workspace of token_logprobs on this stream: of one size for every call.
+at::Tensor &logprobs_workspace(const at::Tensor &like, void *stream)
+{
+    Entry &e = entry_for((int)like.device().index(), stream);
+    if (!e.logprobs_ws.defined()) {
+        if (is_capturing(stream))
+            throw std::runtime_error("rapid_sampling: token_logprobs has no workspace on this stream yet, which is being captured; "
+                                     "call reserve_workspace(B, V) on this stream before the capture begins");
+        auto ws = at::empty({(int64_t)rs_logprobs_workspace_bytes()}, at::TensorOptions().dtype(at::kChar).device(like.device()));
+        const int rc = rs_workspace_init(ws.data_ptr(), (size_t)ws.numel(), stream);
+        if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+        e.logprobs_ws = ws;
+    }
+    return e.logprobs_ws;
+}
+
+int32_t float_dtype(const at::Tensor &t, const char *what)
+{
+    if (t.dtype() == at::kFloat) return RS_DTYPE_F32;
+    if (t.dtype() == at::kBFloat16) return RS_DTYPE_BF16;
+    if (t.dtype() == at::kHalf) return RS_DTYPE_F16;
+    throw std::invalid_argument(std::string(what) + " must be of type float32, bfloat16 or float16, got " +
+                                std::string(t.dtype().name()) + " !\n");
+}
+
+// Rows of logits and their tokens, as the kernels walk them.
+struct TokenRows {
+    int64_t B, T, V, stride_b, stride_t, token_b, token_t;
+    int32_t dtype, tokens_64;
+};
+
+TokenRows read_rows(const at::Tensor &logits, const at::Tensor &tokens, double temperature, int64_t top)
+{
+    TokenRows s;
+    s.dtype = float_dtype(logits, "Logits tensor");
+    const int64_t dim = logits.dim();
+    if (dim < 1 || dim > 3) throw std::invalid_argument("Logits tensor must have shape (V,), (B, V) or (B, T, V) !\n");
+    s.V = logits.size(-1);
+    s.B = dim >= 2 ? logits.size(0) : 1;
+    s.T = dim == 3 ? logits.size(1) : 1;
+    if (s.V < 1 || s.V > 1048576)
+        throw std::invalid_argument("Vocabulary size must be positive, and no larger than 1048576, got " + std::to_string(s.V) + " !\n");
+    if (tokens.dtype() != at::kInt && tokens.dtype() != at::kLong)
+        throw std::invalid_argument("tokens must be of type int32 or int64, got " + std::string(tokens.dtype().name()) + " !\n");
+    if (tokens.sizes() != logits.sizes().slice(0, dim - 1))
+        throw std::invalid_argument("tokens must have the logits' shape without the vocabulary: (), (B,) or (B, T) !\n");
+    if (!(temperature >= 0.001 && temperature <= 1000.0)) throw_for(RS_ERR_TEMPERATURE, s.B, s.T, s.V, temperature);
+    if (top < 0 || top > RS_LOGPROBS_TOP_MAX || top > s.V)
+        throw std::invalid_argument("top outside range, got " + std::to_string(top) + ", expect 0 to " +
+                                    std::to_string(std::min<int64_t>(RS_LOGPROBS_TOP_MAX, s.V)) + " !\n");
+    if (!logits.is_cuda() || tokens.device() != logits.device())
+        throw std::invalid_argument("Logits and tokens must live on the same GPU !\n");
+    if (logits.stride(-1) != 1 && s.V > 1) throw std::invalid_argument("Logits tensor must be contiguous along the vocabulary axis !\n");
+    if (s.B > 0 && s.T > 0 && s.B > 0x7FFFFFFF / s.T) throw std::invalid_argument("B*T is too large !\n");
+    s.stride_b = dim >= 2 ? logits.stride(0) : 0;
+    s.stride_t = dim == 3 ? logits.stride(1) : 0;
+    s.tokens_64 = tokens.dtype() == at::kLong;
+    s.token_b = dim >= 2 ? tokens.stride(0) : 0;
+    s.token_t = dim == 3 ? tokens.stride(1) : 0;
+    return s;
+}
+
+struct LogprobsResult {
+    at::Tensor logprobs, entropy, rank, top_logprobs, top_tokens, stats;
+};
+
+LogprobsResult logprobs_forward(const at::Tensor &logits, const at::Tensor &tokens, double temperature, int64_t top, bool want_stats)
+{
+    const TokenRows s = read_rows(logits, tokens, temperature, top);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+    const auto f32 = at::TensorOptions().dtype(at::kFloat).device(logits.device()), i32 = f32.dtype(at::kInt);
+    std::vector<int64_t> rows = tokens.sizes().vec(), alternatives = rows, four = rows;
+    alternatives.push_back(top);
+    four.push_back(4);
+    LogprobsResult o;
+    o.logprobs = at::empty(rows, f32);
+    o.entropy = at::empty(rows, f32);
+    o.rank = at::empty(rows, i32);
+    o.top_logprobs = at::empty(alternatives, f32);
+    o.top_tokens = at::empty(alternatives, i32);
+    if (want_stats) o.stats = at::empty(four, f32);
+    if (s.B == 0 || s.T == 0) return o;
+    void *stream = current_stream(logits);
+    at::Tensor &ws = logprobs_workspace(logits, stream);
+    const int rc = rs_token_logprobs(logits.data_ptr(), s.dtype, s.stride_b, s.stride_t, tokens.data_ptr(), s.tokens_64, s.token_b, s.token_t,
+                                     (int32_t)s.B, (int32_t)s.T, (int32_t)s.V, temperature, (int32_t)top,
+                                     o.logprobs.data_ptr<float>(), o.entropy.data_ptr<float>(), o.rank.data_ptr<int32_t>(),
+                                     o.top_logprobs.data_ptr<float>(), o.top_tokens.data_ptr<int32_t>(),
+                                     want_stats ? o.stats.data_ptr<float>() : nullptr, ws.data_ptr(), (size_t)ws.numel(), stream);
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    return o;
+}
+
+// A gradient as the kernel reads it: one float for each output, or one for all of them (what sum() hands back).
+at::Tensor gradient_in(const at::Tensor &g, int32_t *stride)
+{
+    *stride = 1;
+    if (!g.defined()) return g;
+    at::Tensor f = g.to(at::kFloat);
+    bool one = f.numel() > 0;
+    for (int64_t d = 0; d < f.dim(); ++d) one = one && (f.stride(d) == 0 || f.size(d) == 1);
+    if (one) { *stride = 0; return f; }
+    return f.contiguous();
+}
+
+at::Tensor logprobs_backward(const at::Tensor &logits, const at::Tensor &tokens, const at::Tensor &top_tokens, const at::Tensor &stats,
+                             double temperature, int64_t top, const at::Tensor &g, const at::Tensor &h, const at::Tensor &a)
+{
+    const TokenRows s = read_rows(logits, tokens, temperature, top);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+    at::Tensor grad = at::empty(logits.sizes(), logits.options());
+    if (s.B == 0 || s.T == 0) return grad;
+    int32_t gs, hs, as;
+    const at::Tensor g1 = gradient_in(g, &gs), h1 = gradient_in(h, &hs), a1 = gradient_in(a, &as);
+    auto ptr = [](const at::Tensor &t) { return t.defined() && t.numel() ? (const float *)t.data_ptr() : nullptr; };
+    const int rc = rs_token_logprobs_backward(logits.data_ptr(), s.dtype, s.stride_b, s.stride_t, tokens.data_ptr(), s.tokens_64, s.token_b,
+                                              s.token_t, (int32_t)s.B, (int32_t)s.T, (int32_t)s.V, temperature, (int32_t)top,
+                                              stats.data_ptr<float>(), top_tokens.data_ptr<int32_t>(), ptr(g1), gs, ptr(h1), hs, ptr(a1), as,
+                                              grad.data_ptr(), current_stream(logits));
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    return grad;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// The gradient's own gradient is not provided: it raises where it is asked for, in the place of a silent zero.
+struct LogprobsBackward : torch::autograd::Function<LogprobsBackward> {
+    static at::Tensor forward(AutogradContext *, at::Tensor logits, at::Tensor tokens, at::Tensor top_tokens, at::Tensor stats, double temperature,
+                              int64_t top, std::optional<at::Tensor> g, std::optional<at::Tensor> h, std::optional<at::Tensor> a)
+    {
+        return logprobs_backward(logits, tokens, top_tokens, stats, temperature, top, g.value_or(at::Tensor()), h.value_or(at::Tensor()),
+                                 a.value_or(at::Tensor()));
+    }
+    static variable_list backward(AutogradContext *, variable_list)
+    {
+        throw std::runtime_error("rapid_sampling: token_logprobs can be differentiated once only");
+    }
+};
+
+struct Logprobs : torch::autograd::Function<Logprobs> {
+    static variable_list forward(AutogradContext *ctx, at::Tensor logits, at::Tensor tokens, double temperature, int64_t top)
+    {
+        LogprobsResult o = logprobs_forward(logits, tokens, temperature, top, true);
+        ctx->save_for_backward({logits, tokens, o.top_tokens, o.stats});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["top"] = top;
+        ctx->mark_non_differentiable({o.rank, o.top_tokens});
+        ctx->set_materialize_grads(false);
+        return {o.logprobs, o.entropy, o.rank, o.top_logprobs, o.top_tokens};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const auto saved = ctx->get_saved_variables();
+        const double temperature = ctx->saved_data["temperature"].toDouble();
+        const int64_t top = ctx->saved_data["top"].toInt();
+        if (!grads[0].defined() && !grads[1].defined() && !grads[3].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        auto given = [&](int i) { return grads[i].defined() ? std::optional<at::Tensor>(grads[i]) : std::nullopt; };
+        const at::Tensor grad = at::GradMode::is_enabled()
+            ? LogprobsBackward::apply(saved[0], saved[1], saved[2], saved[3], temperature, top, given(0), given(1), given(3))
+            : logprobs_backward(saved[0], saved[1], saved[2], saved[3], temperature, top, grads[0], grads[1], grads[3]);
+        return {grad, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+// ------------------------------------------------------- values and products in 8 bits --
+
+at::Tensor rows_of_16_bytes(std::vector<int64_t> sizes, const at::Device &device)
+{
+    const int64_t K = sizes.back();
+    sizes.back() = (K + 15) / 16 * 16;
+    return at::empty(sizes, at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(device)).narrow(-1, 0, K);
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize(const at::Tensor &x, int64_t block_rows)
+{
+    const int32_t dtype = float_dtype(x, "x");
+    if (block_rows != 1 && block_rows != 128)
+        throw std::invalid_argument("block_rows must be 1 or 128, got " + std::to_string(block_rows) + " !\n");
+    if (x.dim() < 1 || (block_rows == 128 && x.dim() != 2))
+        throw std::invalid_argument("x must have shape (..., K), or (N, K) for blocks of 128 x 128 !\n");
+    if (!x.is_cuda()) throw std::invalid_argument("x must live on the GPU !\n");
+    const int64_t K = x.size(-1), rows = K ? x.numel() / K : 0;
+    if (K < 1 || K > RS_LINEAR_MAX || rows > 0x7FFFFFFF / ((K + 127) / 128))
+        throw std::invalid_argument("x has no columns, or too many elements !\n");
+    if (x.stride(-1) != 1 && K > 1) throw std::invalid_argument("x must be contiguous along its last axis !\n");
+    if (x.requires_grad() && at::GradMode::is_enabled())
+        throw std::invalid_argument("quantize_fp8 has no gradient: call it under torch.no_grad(), or on x.detach() !\n");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    std::vector<int64_t> blocks = x.sizes().vec();
+    blocks.back() = (K + 127) / 128;
+    if (block_rows == 128) blocks[0] = (blocks[0] + 127) / 128;
+    at::Tensor q = rows_of_16_bytes(x.sizes().vec(), x.device());
+    at::Tensor scale = at::empty(blocks, at::TensorOptions().dtype(at::kFloat).device(x.device()));
+    if (!rows) return {q, scale};
+    const at::Tensor flat = x.reshape({rows, K});
+    const int rc = rs_quantize_blocks(flat.data_ptr(), dtype, flat.stride(0), (int32_t)block_rows, (int32_t)rows, (int32_t)K, q.data_ptr(),
+                                      (K + 15) / 16 * 16, scale.data_ptr<float>(), current_stream(x));
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    return {q, scale};
+}
+
+// (..., K) as rows a fixed number of bytes apart; what does not lie so, or is not aligned, is refused.
+at::Tensor fp8_rows(const at::Tensor &t, const char *what)
+{
+    const int64_t K = t.size(-1);
+    at::Tensor flat;
+    try {
+        flat = t.dim() == 2 ? t : t.view({K ? t.numel() / K : 0, K});
+    } catch (const c10::Error &) {
+        throw std::invalid_argument(std::string(what) + " must have its rows at a fixed distance from each other !\n");
+    }
+    if ((flat.stride(1) != 1 && K > 1) || (flat.size(0) > 1 && (flat.stride(0) % 16 || flat.stride(0) < K)) || ((uintptr_t)flat.data_ptr() & 15))
+        throw std::invalid_argument(std::string(what) + " must be contiguous along its last axis, with rows that begin at multiples of 16 bytes "
+                                    "(as quantize_fp8 returns them) !\n");
+    return flat;
+}
+
+void check_scale(const at::Tensor &scale, const at::Tensor &like, int64_t rows, int64_t blocks, const char *what)
+{
+    if (scale.dtype() != at::kFloat || scale.device() != like.device() || !scale.is_contiguous() || scale.size(-1) != blocks ||
+        scale.numel() != rows * blocks)
+        throw std::invalid_argument(std::string(what) + " must be a contiguous float32 GPU tensor of " + std::to_string(rows) + " x " +
+                                    std::to_string(blocks) + " scales !\n");
+}
+
+at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &weight_scale, const std::optional<at::Tensor> &x_scale,
+                  const std::optional<at::ScalarType> &out_dtype)
+{
+    const at::ScalarType to = out_dtype ? *out_dtype : at::kFloat;
+    if (to != at::kFloat && to != at::kBFloat16 && to != at::kHalf) throw std::invalid_argument("out_dtype must be float32, bfloat16 or float16 !\n");
+    if (weight.dtype() != at::kFloat8_e4m3fn || weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1)
+        throw std::invalid_argument("weight must be of type float8_e4m3fn and shape (N, K) !\n");
+    if (x.dim() < 1 || x.size(-1) != weight.size(1)) throw std::invalid_argument("x must have shape (..., K), with the weight's K !\n");
+    if (!x.is_cuda() || weight.device() != x.device()) throw std::invalid_argument("x and weight must live on the same GPU !\n");
+    const bool given = x.dtype() == at::kFloat8_e4m3fn;
+    if (given != x_scale.has_value()) throw std::invalid_argument("x_scale goes with an x of type float8_e4m3fn, and only with one !\n");
+    if (at::GradMode::is_enabled() && (x.requires_grad() || weight_scale.requires_grad() || (x_scale && x_scale->requires_grad())))
+        throw std::invalid_argument("linear_fp8 has no gradient: call it under torch.no_grad(), or on x.detach() !\n");
+    const int64_t K = weight.size(1), N = weight.size(0), blocks = (K + 127) / 128, M = x.numel() / K;
+    if (M > RS_LINEAR_MAX || N > RS_LINEAR_MAX || K > RS_LINEAR_MAX) throw std::invalid_argument("x or weight is too large !\n");
+    const at::Tensor w = fp8_rows(weight, "weight");
+    check_scale(weight_scale, weight, (N + 127) / 128, blocks, "weight_scale");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    std::vector<int64_t> sizes = x.sizes().vec();
+    sizes.back() = N;
+    at::Tensor y = at::empty(sizes, at::TensorOptions().dtype(to).device(x.device()));
+    if (!M) return y;
+    at::Tensor q, scale;
+    if (given) { q = x; scale = *x_scale; check_scale(scale, x, M, blocks, "x_scale"); }
+    else std::tie(q, scale) = quantize(x, 1);
+    q = fp8_rows(q, "x");
+    const int rc = rs_linear_blocks(q.data_ptr(), q.stride(0), scale.data_ptr<float>(), w.data_ptr(), w.stride(0), weight_scale.data_ptr<float>(),
+                                    (int32_t)M, (int32_t)N, (int32_t)K, y.data_ptr(), float_dtype(y, "y"), N, current_stream(x));
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    return y;
+}
+
 }  // namespace
+
+// (logprobs, entropy, rank, top_logprobs, top_tokens); under autograd where the logits ask for a gradient.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(const at::Tensor &logits, const at::Tensor &tokens,
+                                                                                     double temperature, int64_t top)
+{
+    if (logits.requires_grad() && at::GradMode::is_enabled()) {
+        variable_list o = Logprobs::apply(logits, tokens, temperature, top);
+        return {o[0], o[1], o[2], o[3], o[4]};
+    }
+    LogprobsResult o = logprobs_forward(logits, tokens, temperature, top, false);
+    return {o.logprobs, o.entropy, o.rank, o.top_logprobs, o.top_tokens};
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_fp8(const at::Tensor &x, int64_t block_rows) { return quantize(x, block_rows); }
+
+at::Tensor linear_fp8(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &weight_scale, std::optional<at::Tensor> x_scale,
+                      std::optional<at::ScalarType> out_dtype)
+{
+    return linear(x, weight, weight_scale, x_scale, out_dtype);
+}
 
 // sampling.cu:140-144.  State is 64 bytes per row, opaque to the caller.
 at::Tensor setup_rand(int64_t seed, int64_t B)
@@ -309,6 +590,7 @@ void reserve_workspace(int64_t B, int64_t V, std::optional<int64_t> device)
     c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
     auto like = at::empty({1}, at::TensorOptions().dtype(at::kChar).device(dev));
     workspace_for(like, current_stream(like), B, V);
+    logprobs_workspace(like, current_stream(like));
 }
 
 // Synchronises the current stream of `device` and returns the sticky error word of its workspace:
@@ -441,6 +723,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           py::arg("uniforms") = py::none(), py::arg("accept_half") = false);
     m.def("floor_read", &floor_read, py::arg("logits"), py::arg("variant") = 1);
     m.def("reserve_workspace", &reserve_workspace, py::arg("B"), py::arg("V"), py::arg("device") = py::none());
+    m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("tokens"), py::arg("temperature") = 1.0, py::kw_only(),
+          py::arg("top") = 0);
+    m.def("quantize_fp8", &quantize_fp8, py::arg("x"), py::kw_only(), py::arg("block_rows") = 1);
+    m.def("linear_fp8", &linear_fp8, py::arg("x"), py::arg("weight"), py::arg("weight_scale"), py::kw_only(), py::arg("x_scale") = py::none(),
+          py::arg("out_dtype") = py::none());
+    m.attr("LOGPROBS_TOP_MAX") = RS_LOGPROBS_TOP_MAX;
     m.def("workspace_status", &workspace_status, py::arg("device") = py::none());
     m.def("policy_state", &policy_state, py::arg("device") = py::none());
     m.def("force_path", &force_path, py::arg("name"));

@@ -1,0 +1,235 @@
+"""quantize_fp8 and linear_fp8 against the formulas: the values in 8 bits bit for bit, the product in 64 bits.
+
+With eps = 2^-24 a block's sum of 128 products is within 128 eps of the sum of their magnitudes, the scales and the sums over the
+blocks add two roundings a block: eps (128 + 2 blocks + 8) sum |x| |w| bounds the error before the one rounding of the output."""
+import math
+
+import pytest
+import torch
+
+EPS = 2.0 ** -24
+F8 = torch.float8_e4m3fn
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+UNIT = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+gpu = pytest.mark.gpu
+
+
+def blocks_of(x, rows):
+    R, K = x.shape
+    x = torch.nn.functional.pad(x, (0, -K % 128, 0, -R % rows))
+    return x.view(-1, rows, x.shape[1] // 128, 128)
+
+
+def quantized(x, rows):
+    R, K = x.shape
+    b = blocks_of(x.cpu().float(), rows)
+    scale = (b.abs().amax(dim=(1, 3)) / 448.0).clamp(min=2.0 ** -126)
+    q = (b / scale[:, None, :, None]).to(F8)
+    return q.view(torch.uint8).view(b.shape[0] * rows, -1)[:R, :K], scale
+
+
+def values(q, scale, rows):
+    R, K = q.shape
+    return (blocks_of(q.cpu().float(), rows).double() * scale.cpu().double()[:, None, :, None]).view(-1, -(-K // 128) * 128)[:R, :K]
+
+
+def make(R, K, dtype, seed):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn((R, K), generator=gen) * torch.exp(torch.randn((K,), generator=gen))
+    return x.to(DTYPES[dtype]).cuda()
+
+
+CUT = 7 * 2.0 ** -13
+
+
+def check(y, x, sx, w, sw, out_dtype, cut=0.0):
+    a, b = values(x, sx, 1), values(w, sw, 128)
+    want, size = a @ b.T, a.abs() @ b.abs().T
+    bound = (EPS * (128 + 2 * sx.shape[-1] + 8) + cut) * size + UNIT[out_dtype] * want.abs() * 1.01 + 2.0 ** -25
+    off = (y.cpu().double() - want).abs()
+    assert y.dtype == out_dtype and (off <= bound).all(), (off / bound).max().item()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("R,K", [(1, 1), (3, 7), (1, 128), (2, 129), (130, 255), (257, 1000), (300, 4096)])
+@pytest.mark.parametrize("rows", [1, 128])
+def test_quantize(R, K, dtype, rows):
+    import rapid_sampling_amd as sample
+    print("quantize", R, K, dtype, rows, flush=True)
+    x = make(R, K, dtype, R + K)
+    x[0, :] = 0.0                                                   # a block of nothing
+    if R > 1:
+        x[1, 0] = 1e-30 if dtype != "f16" else 6e-8
+    q, scale = sample.quantize_fp8(x, block_rows=rows)
+    want, want_scale = quantized(x, rows)
+    assert q.dtype == F8 and q.shape == x.shape and q.stride(0) % 16 == 0 and q.data_ptr() % 16 == 0
+    assert torch.equal(scale.cpu(), want_scale)
+    assert torch.equal(q.view(torch.uint8).cpu(), want)
+
+
+@gpu
+def test_quantize_extremes_and_strides():
+    import rapid_sampling_amd as sample
+    x = torch.zeros((4, 256), device="cuda")
+    x[0, 0], x[0, 1] = 3.4e38, -3.4e38
+    x[1, 0], x[1, 1] = 1e-45, -3e-39                                # below the least scale
+    x[2, 5] = math.nan
+    x[3, 200] = math.inf
+    q, scale = sample.quantize_fp8(x)
+    want, want_scale = quantized(x, 1)
+    assert torch.equal(q[:2].view(torch.uint8).cpu(), want[:2]) and torch.equal(scale[:2].cpu(), want_scale[:2])
+    f = q.float()
+    assert f[2, 5].isnan() and f[3, 200].isnan() and not f[2, :5].isnan().any() and not f[3, :128].isnan().any()
+    y = make(10, 700, "bf16", 3)
+    for view in (y[::2, 3:500], y[:, 1:2], y.view(2, 5, 700), y[4]):
+        q, scale = sample.quantize_fp8(view)
+        want, want_scale = quantized(view.reshape(-1, view.shape[-1]), 1)
+        assert torch.equal(q.view(torch.uint8).cpu().reshape(want.shape), want) and torch.equal(scale.cpu().reshape(want_scale.shape), want_scale)
+    assert sample.quantize_fp8(y[:0])[0].shape == (0, 700)
+
+
+@gpu
+@pytest.mark.parametrize("M,K,N", [(1, 16, 1), (1, 100, 50), (2, 128, 16), (1, 4096, 1000), (5, 1000, 257), (16, 512, 384), (17, 256, 129), (33, 2000, 515),
+                                   (64, 144, 640), (77, 2000, 1037), (128, 1024, 256), (129, 128, 128), (257, 300, 700), (512, 2048, 1024), (300, 1, 5)])
+@pytest.mark.parametrize("out", list(DTYPES))
+def test_product(M, K, N, out):
+    import rapid_sampling_amd as sample
+    print("product", M, K, N, out, flush=True)
+    x, w = make(M, K, "bf16", M), make(N, K, "f32", N)
+    qw, sw = sample.quantize_fp8(w, block_rows=128)
+    qx, sx = sample.quantize_fp8(x)
+    y = sample.linear_fp8(qx, qw, sw, x_scale=sx, out_dtype=DTYPES[out])
+    check(y, qx, sx, qw, sw, DTYPES[out], CUT if M > 64 and out != "f32" else 0.0)
+    assert torch.equal(y, sample.linear_fp8(x, qw, sw, out_dtype=DTYPES[out]))      # quantised within the call: the same
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 3, 40, 200])
+def test_shapes_types_and_what_lies_behind_the_columns(M):
+    import rapid_sampling_amd as sample
+    K, N = 200, 300
+    store = torch.full((N, 256), 0x7F, dtype=torch.uint8, device="cuda")             # NaN behind every row
+    w = make(N, K, "f32", 1)
+    qw, sw = sample.quantize_fp8(w, block_rows=128)
+    store[:, :K] = qw.view(torch.uint8)
+    poisoned = store.view(F8)[:, :K]
+    for dtype in DTYPES:
+        x = make(M, K, dtype, M)
+        y = sample.linear_fp8(x, poisoned, sw)
+        qx, sx = sample.quantize_fp8(x)
+        check(y, qx, sx, qw, sw, torch.float32)
+        held = torch.full((M, 208), 0x7F, dtype=torch.uint8, device="cuda")
+        held[:, :K] = qx.view(torch.uint8)
+        assert torch.equal(y, sample.linear_fp8(held.view(F8)[:, :K], poisoned, sw, x_scale=sx))
+    z = sample.linear_fp8(x.view(1, M, K), qw, sw)
+    assert z.shape == (1, M, N) and torch.equal(z[0], sample.linear_fp8(x, qw, sw))
+    assert torch.equal(sample.linear_fp8(x[0], qw, sw), sample.linear_fp8(x[:1], qw, sw)[0])
+    assert sample.linear_fp8(x[:0], qw, sw).shape == (0, N)
+    wide = torch.zeros((M, 2 * K), dtype=x.dtype, device="cuda")                     # rows apart
+    wide[:, 1:K + 1] = x
+    assert torch.equal(sample.linear_fp8(wide[:, 1:K + 1], qw, sw), sample.linear_fp8(x, qw, sw))
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 20, 150])
+def test_values_that_are_no_numbers_stay_in_their_row(M):
+    import rapid_sampling_amd as sample
+    x, w = make(M, 384, "f32", 9), make(260, 384, "f32", 10)
+    qw, sw = sample.quantize_fp8(w, block_rows=128)
+    want = sample.linear_fp8(x, qw, sw)
+    x[M // 2, 200] = math.inf
+    y = sample.linear_fp8(x, qw, sw)
+    assert y[M // 2].isnan().all()
+    rest = torch.arange(M, device="cuda") != M // 2
+    assert torch.equal(y[rest], want[rest])
+
+
+@gpu
+def test_head_sampler_and_logprobs_together():
+    """hidden states -> logits -> a token each -> its log probability, on another stream and from a graph."""
+    import rapid_sampling_amd as sample
+    V, K, B = 4096, 512, 6
+    qw, sw = sample.quantize_fp8(make(V, K, "f32", 1), block_rows=128)
+    u = torch.linspace(0.1, 0.9, B, device="cuda")
+    states = sample.setup_rand(0, B)
+
+    def step(hidden):
+        logits = sample.linear_fp8(hidden, qw, sw)
+        tokens = sample.batch_sampling_temperature_topk_topp(logits, states, 0.9, 5, 1.0, uniforms=u)
+        return (logits, tokens) + tuple(sample.token_logprobs(logits, tokens, 0.9, top=5))
+    hidden = make(B, K, "bf16", 2)
+    logits, tokens, lp, entropy, rank, top_lp, top_tokens = step(hidden)
+    assert (rank <= 5).all() and (rank >= 1).all()
+    at = (rank.long() - 1)[:, None]
+    assert torch.equal(top_tokens.gather(1, at)[:, 0], tokens) and torch.equal(top_lp.gather(1, at)[:, 0], lp)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        sample.reserve_workspace(B, V)
+        held_in = hidden.clone()
+        step(held_in)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = step(held_in)
+    for seed in range(3):
+        fresh = make(B, K, "bf16", 50 + seed)
+        held_in.copy_(fresh)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, step(fresh))), seed
+
+
+def test_refusals():
+    import rapid_sampling_amd as sample
+    x, w, s = torch.zeros((2, 32)), torch.zeros((16, 32), dtype=F8), torch.ones((1, 1))
+    bad = [((x, x, s), {}, "float8"), ((x, w[:, :16], s), {}, "K"), ((x, w[0], s), {}, "shape"), ((x, w, s), {"out_dtype": torch.float64}, "out_dtype"),
+           ((x, w, s), {}, "GPU")]
+    for args, kw, text in bad:
+        with pytest.raises(ValueError, match=text):
+            sample.linear_fp8(*args, **kw)
+    for args, kw, text in [((x.double(),), {}, "float32"), ((x,), {"block_rows": 2}, "block_rows"), ((x[0],), {"block_rows": 128}, "shape"), ((x,), {}, "GPU")]:
+        with pytest.raises(ValueError, match=text):
+            sample.quantize_fp8(*args, **kw)
+
+
+@gpu
+def test_refusals_on_the_gpu():
+    import rapid_sampling_amd as sample
+    x, wf = make(2, 100, "f32", 1), make(20, 100, "f32", 2)
+    learnt = x.clone().requires_grad_()
+    w, s = sample.quantize_fp8(wf, block_rows=128)
+    qx, sx = sample.quantize_fp8(x)
+    tight = torch.empty(20 * 100, dtype=torch.uint8, device="cuda").view(F8).view(20, 100)      # rows of 100 bytes
+    bad = [((x, tight, s), {}, "16 bytes"), ((x, w, s.double()), {}, "weight_scale"), ((x, w, s[:, :0]), {}, "weight_scale"), ((qx, w, s), {}, "x_scale"),
+           ((x, w, s), {"x_scale": sx}, "x_scale"), ((qx, w, s), {"x_scale": sx[:1]}, "x_scale"), ((x.t()[:, :2], w[:, :2], s), {}, "contiguous|16 bytes"),
+           ((learnt, w, s), {}, "gradient")]
+    for args, kw, text in bad:
+        with pytest.raises(ValueError, match=text):
+            sample.linear_fp8(*args, **kw)
+    with pytest.raises(ValueError, match="gradient"):
+        sample.quantize_fp8(learnt)
+    with torch.no_grad():
+        assert sample.linear_fp8(learnt, w, s).shape == (2, 20)
+
+
+def test_refusals_of_the_c_abi():
+    import ctypes as C
+
+    from tests import capi
+    L = capi.lib()
+    p, i32, i64 = C.c_void_p, C.c_int32, C.c_int64
+    L.rs_quantize_blocks.argtypes = [p, i32, i64, i32, i32, i32, p, i64, p, p]
+    L.rs_linear_blocks.argtypes = [p, i64, p, p, i64, p, i32, i32, i32, p, i32, i64, p]
+
+    def quantize(x=256, dtype=0, rows=1, R=2, K=20, q=256, q_stride=32, scale=256):
+        return L.rs_quantize_blocks(x, dtype, K, rows, R, K, q, q_stride, scale, None)
+    assert quantize(x=None) == quantize(q=None) == quantize(scale=None) == -4 and quantize(dtype=5) == quantize(rows=64) == -7
+    assert quantize(R=0) == quantize(K=0) == quantize(q_stride=16) == -12 and quantize(x=258) == quantize(q=264) == quantize(q_stride=40) == -6
+
+    def linear(x=256, xs=32, w=256, ws=32, sx=256, sw=256, M=2, N=20, K=20, y=256, dtype=0, ys=20):
+        return L.rs_linear_blocks(x, xs, sx, w, ws, sw, M, N, K, y, dtype, ys, None)
+    assert linear(x=None) == linear(w=None) == linear(y=None) == linear(sx=None) == linear(sw=None) == -4 and linear(dtype=7) == -7
+    assert linear(M=0) == linear(N=0) == linear(K=0) == linear(xs=16) == linear(ws=16) == linear(ys=19) == -12
+    assert linear(x=264) == linear(w=260) == linear(xs=40) == linear(ws=40) == linear(y=258) == -6
