@@ -514,7 +514,8 @@ int rs_token_logprobs_backward(const void *logits_device, int32_t logits_dtype, 
  * Values in 8 bits (e4m3fn: 4 bits of exponent, 3 of significand, no infinity)
  * with a float32 scale for each block of block_rows x 128 values, block_rows 1
  * (activations) or 128 (weights):
- *   scale = max(max |x| / 448, 2^-126)      q = x / scale, to nearest, ties to even
+ *   scale = max(max |x| * r, 2^-126), r = 1/448 in float32
+ *   q     = x / scale, to nearest, ties to even
  * Blocks at the ends are what is left.  x: R rows of K values, x_row_stride
  * elements apart.  q: rows q_row_stride bytes apart, a multiple of 16 and at least K
  * rounded up to one, 16-byte aligned; bytes behind column K are cleared up to the

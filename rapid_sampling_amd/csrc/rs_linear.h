@@ -1,6 +1,6 @@
 // Values in 8 bits (e4m3fn) with a float32 scale for each block of 128 along the rows, and their matrix product:
 //
-//   scale = max(max |x| over the block / 448, 2^-126)        q = e4m3(x / scale), to nearest, ties to even
+//   scale = max(max |x| over the block * r, 2^-126), r = 1/448 in float32        q = e4m3(x / scale), to nearest, ties to even
 //   y[m, n] = sum over blocks kb of sx[m, kb] sw[n / 128, kb] sum_{k in kb} qx[m, k] qw[n, k]
 //
 // The inner sums are the matrix cores' (products of two such values are exact in float32, the sum over a block is held in
@@ -16,6 +16,7 @@ constexpr int kFpBlock = 128;
 typedef int   v8i __attribute__((ext_vector_type(8)));
 typedef int   v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
@@ -49,7 +50,7 @@ template <int DT> __device__ __forceinline__ void put(void *p, int64_t i, float 
     else ((_Float16 *)p)[i] = (_Float16)v;
 }
 
-__device__ __forceinline__ float block_scale(float peak) { return fmaxf(peak / 448.0f, 0x1p-126f); }
+__device__ __forceinline__ float block_scale(float peak) { return fmaxf(peak * (1.0f / 448.0f), 0x1p-126f); }
 
 // One block of 1 x 128: sixteen lanes, eight values each.
 template <int DT>
@@ -143,6 +144,30 @@ __device__ __forceinline__ v4f block_product(v8i w, v8i x)
     return acc;
 }
 
+// The same on the matrix cores' 8-bit instructions: for outputs of 16 bits, whose own rounding is fifty times as large.
+__device__ __forceinline__ v4f block_product_8(v8i w, v8i x)
+{
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
+}
+
+// Four consecutive float32 values, or eight of 16 bits, in one store.
+template <int DT> __device__ __forceinline__ void put_wide(void *p, int64_t i, v4f a, v4f b)
+{
+    if constexpr (DT == RS_DTYPE_F32) *(v4f *)((float *)p + i) = a;
+    else if constexpr (DT == RS_DTYPE_BF16) {
+        v8bf v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { v[j] = (__bf16)a[j]; v[j + 4] = (__bf16)b[j]; }
+        *(v8bf *)((__bf16 *)p + i) = v;
+    } else {
+        v8h v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { v[j] = (_Float16)a[j]; v[j + 4] = (_Float16)b[j]; }
+        *(v8h *)((_Float16 *)p + i) = v;
+    }
+}
+
 // A wave per 16 rows of w and 16 MT rows of x.
 template <int DT, int MT>
 __global__ __launch_bounds__(256) void linear_kernel(LinearParams p)
@@ -177,6 +202,160 @@ __global__ __launch_bounds__(256) void linear_kernel(LinearParams p)
         for (int j = 0; j < 4; ++j) {
             const uint32_t n = n0 + part * 4u + j;
             if (n < p.N) put<DT>(p.y, (int64_t)m * p.y_stride + n, acc[t][j]);
+        }
+    }
+}
+
+// -------------------------------------------------------------- many rows --
+// A workgroup of eight waves makes 256 rows of w x 64 MT rows of x, a wave 128 x 16 MT of it: a quarter of w's rows in a lane's
+// reach would not do, since every block has to be scaled in the vector unit before it is added (four sums a lane and
+// 16 x 16 product), so the sums sit in ordinary registers, 32 MT of them.
+//
+// A block of 128 columns is one stage: rows of 128 bytes go from memory to LDS without passing through registers, while
+// the stage before is multiplied.  The eight 16-byte pieces of a row are stored in an order that depends on the row
+// (place = piece ^ f(row)), so that the eight rows read at once lie in different banks.  The first operand's rows are
+// dealt so that a lane's sums are 32 consecutive columns of y.
+typedef __attribute__((address_space(1))) const void *GlobalPtr;
+typedef __attribute__((address_space(3))) void *LdsPtr;
+
+constexpr int kTileN = 256;
+constexpr int64_t kTileStride = (1ll << 32) / 256 - kFpBlock;
+
+__device__ __forceinline__ uint32_t w_turn(uint32_t row) { return (row & 3u) | ((row >> 3) & 4u); }
+__device__ __forceinline__ uint32_t x_turn(uint32_t row) { return row & 7u; }
+
+template <int DT, int MT, bool EXACT>
+struct LinearTile {
+    static constexpr uint32_t kTileM = 64 * MT, kRows = kTileN + kTileM, kStage = kRows * kFpBlock;
+    static constexpr uint32_t kLoads = kRows / 64;           // 16-byte pieces of a stage per thread
+
+    // A wave fills eight rows of a stage with one load: thread's row and piece of load i, w's rows first.
+    static __device__ __forceinline__ uint32_t row_of(uint32_t i) { return (i * 8u + threadIdx.x / 64u) * 8u + threadIdx.x % 64u / 8u; }
+
+    struct Source {
+        const uint8_t *w, *x;            // of the tile's first rows
+        uint32_t       at[kLoads];       // bytes from there to the thread's pieces of the first block
+    };
+    static __device__ __forceinline__ Source source(const LinearParams &p, uint32_t n0, uint32_t m0)
+    {
+        Source s;
+        s.w = p.w + (int64_t)n0 * p.w_stride;
+        s.x = p.x + (int64_t)m0 * p.x_stride;
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            const bool is_w = i < kTileN / 64;
+            const uint32_t r = row_of(i) - (is_w ? 0u : kTileN);
+            const uint32_t piece = (threadIdx.x & 7u) ^ (is_w ? w_turn(r) : x_turn(r));
+            s.at[i] = (is_w ? min(r, p.N - 1u - n0) * (uint32_t)p.w_stride : min(r, p.M - 1u - m0) * (uint32_t)p.x_stride) + piece * 16u;
+        }
+        return s;
+    }
+    static __device__ __forceinline__ void fill(const LinearParams &p, const Source &s, uint32_t n0, uint32_t m0, uint32_t kb, uint8_t *lds)
+    {
+        const uint32_t k = kb * kFpBlock;
+        if (k + kFpBlock <= p.K) {
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i)
+                __builtin_amdgcn_global_load_lds((GlobalPtr)((i < kTileN / 64 ? s.w : s.x) + k + s.at[i]), (LdsPtr)(lds + (i * 8u + threadIdx.x / 64u) * 1024u), 16, 0, 0);
+            return;
+        }
+        // the last block where K is no whole number of them
+#pragma unroll 1
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            const bool is_w = i < kTileN / 64;
+            const uint32_t r = row_of(i) - (is_w ? 0u : kTileN);
+            const uint32_t piece = (threadIdx.x & 7u) ^ (is_w ? w_turn(r) : x_turn(r));
+            const uint8_t *from = is_w ? s.w + min(r, p.N - 1u - n0) * p.w_stride : s.x + min(r, p.M - 1u - m0) * p.x_stride;
+            *(v4i *)(lds + row_of(i) * kFpBlock + (threadIdx.x & 7u) * 16u) = load16(from, k + piece * 16u, p.K);
+        }
+    }
+
+    static __device__ __forceinline__ v8i fragment(const uint8_t *lds, uint32_t row, uint32_t turn, uint32_t part)
+    {
+        const uint8_t *r = lds + row * kFpBlock;
+        return join(*(const v4i *)(r + ((part ^ turn) * 16u)), *(const v4i *)(r + (((part + 4u) ^ turn) * 16u)));
+    }
+
+    static __device__ __forceinline__ void step(const LinearParams &p, const Source &source, uint32_t n0, uint32_t m0, uint32_t next,
+                                                const uint8_t *__restrict now_lds, uint8_t *__restrict next_lds, const float (&f)[MT], v4f (&acc)[8][MT])
+    {
+        if (next < p.blocks) fill(p, source, n0, m0, next, next_lds);
+        const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
+        const uint32_t wn = (wave & 1u) * 128u, wm = (wave >> 1) * (16u * MT);
+        v8i x[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const uint32_t r = wm + t * 16u + i;
+            x[t] = fragment(now_lds + kTileN * kFpBlock, r, x_turn(r), part);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const uint32_t r = wn + i / 4u * 32u + u * 4u + i % 4u;
+            const v8i w = fragment(now_lds, r, w_turn(r), part);
+            v4f s[MT];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) s[t] = EXACT ? block_product(w, x[t]) : block_product_8(w, x[t]);
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[u][t][j] = __builtin_fmaf(s[t][j], f[t], acc[u][t][j]);
+        }
+    }
+};
+
+template <int DT, int MT, bool EXACT>
+__global__ __launch_bounds__(512, 2) void linear_tile_kernel(LinearParams p)
+{
+    using L = LinearTile<DT, MT, EXACT>;
+    extern __shared__ uint8_t lds[];
+    // Workgroup b runs on XCD b % 8: each XCD takes a stretch of the tiles, in panels of eight rows of tiles, so that the 32 tiles
+    // it works on at a time share their rows in its L2.
+    const uint32_t tm = (p.M + L::kTileM - 1u) / L::kTileM, tn = (p.N + kTileN - 1u) / kTileN, tiles = tm * tn;
+    const uint32_t each = tiles / 8u, rest = tiles % 8u, xcd = blockIdx.x % 8u;
+    const uint32_t id = xcd * each + min(xcd, rest) + blockIdx.x / 8u;
+    const uint32_t panel = id / (8u * tn), high = min(8u, tm - panel * 8u), in = id - panel * 8u * tn;
+    const uint32_t m0 = (panel * 8u + in % high) * L::kTileM, n0 = in / high * kTileN;
+
+    const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
+    const uint32_t wn = (wave & 1u) * 128u, wm = (wave >> 1) * (16u * MT);
+    const float *sw = p.w_scale + (size_t)min((n0 + wn) / kFpBlock, (p.N - 1u) / kFpBlock) * p.blocks;
+    const float *sx[MT];
+    v4f acc[8][MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        sx[t] = p.x_scale + (size_t)min(m0 + wm + t * 16u + i, p.M - 1u) * p.blocks;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) acc[u][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const typename L::Source source = L::source(p, n0, m0);
+    L::fill(p, source, n0, m0, 0, lds);
+    for (uint32_t kb = 0; kb < p.blocks; ++kb) {
+        float f[MT];
+        const float s = sw[kb];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) f[t] = sx[t][kb] * s;
+        wait_vmem();
+        __syncthreads();
+        const bool odd = kb & 1u;
+        L::step(p, source, n0, m0, kb + 1u, lds + (odd ? L::kStage : 0u), lds + (odd ? 0u : L::kStage), f, acc);
+    }
+    // a lane has columns wn + 32 part .. + 31 of its rows of y
+    const uint32_t n = n0 + wn + part * 32u;
+    constexpr uint32_t kVec = DT == RS_DTYPE_F32 ? 4 : 8;
+    const bool wide = n + 32u <= p.N && !(p.y_stride % kVec) && !((uintptr_t)p.y & 15);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const uint32_t m = m0 + wm + t * 16u + i;
+        if (m >= p.M) continue;
+        const int64_t at = (int64_t)m * p.y_stride + n;
+        if (wide) {
+#pragma unroll
+            for (int u = 0; u < 8; u += kVec / 4) put_wide<DT>(p.y, at + u * 4, acc[u][t], acc[(u + 1) % 8][t]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) if (n + u * 4u + j < p.N) put<DT>(p.y, at + u * 4 + j, acc[u][t][j]);
         }
     }
 }

@@ -10,12 +10,28 @@ static void launch_quantize(const QuantParams &p, bool tiles, hipStream_t st)
     else hipLaunchKernelGGL(quantize_rows_kernel<DT>, dim3((uint32_t)(((uint64_t)p.R * p.blocks + 15) / 16)), dim3(256), 0, st, p);
 }
 
-template <int DT>
-static void launch_linear(const LinearParams &p, hipStream_t st)
+template <int DT, int MT, bool EXACT>
+static hipError_t launch_tiles(const LinearParams &p, hipStream_t st)
 {
+    using L = LinearTile<DT, MT, EXACT>;
+    const uint64_t tiles = (uint64_t)((p.M + L::kTileM - 1) / L::kTileM) * ((p.N + kTileN - 1) / kTileN);
+    if (tiles > 0x7FFFFFFF) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((linear_tile_kernel<DT, MT, EXACT>), dim3((uint32_t)tiles), dim3(512), 2 * L::kStage, st, p);
+    return hipGetLastError();
+}
+
+template <int DT>
+static hipError_t launch_linear(const LinearParams &p, hipStream_t st)
+{
+    // (the tiles' kernel reaches its 256 rows with 32 bits)
+    if (p.M > 64 && p.x_stride <= kTileStride && p.w_stride <= kTileStride) {
+        if constexpr (DT == RS_DTYPE_F32) return launch_tiles<DT, 2, true>(p, st);
+        else return p.M > 128 ? launch_tiles<DT, 4, false>(p, st) : launch_tiles<DT, 2, false>(p, st);
+    }
     const uint32_t nb = (p.N + 63) / 64;
     if (p.M <= 16) hipLaunchKernelGGL((linear_kernel<DT, 1>), dim3(nb, 1), dim3(256), 0, st, p);
     else hipLaunchKernelGGL((linear_kernel<DT, 4>), dim3(nb, (p.M + 63) / 64), dim3(256), 0, st, p);
+    return hipGetLastError();
 }
 
 static bool known(int32_t dtype) { return dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16 || dtype == RS_DTYPE_F16; }
@@ -63,10 +79,9 @@ int rs_linear_blocks(const void *x, int64_t x_row_stride, const float *x_scale,
     p.y = y; p.y_stride = y_row_stride;
     p.M = (uint32_t)M; p.N = (uint32_t)N; p.K = (uint32_t)K; p.blocks = ((uint32_t)K + kFpBlock - 1) / kFpBlock;
     const hipStream_t st = (hipStream_t)stream;
-    if (y_dtype == RS_DTYPE_F32) launch_linear<RS_DTYPE_F32>(p, st);
-    else if (y_dtype == RS_DTYPE_BF16) launch_linear<RS_DTYPE_BF16>(p, st);
-    else launch_linear<RS_DTYPE_F16>(p, st);
-    return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
+    const hipError_t e = y_dtype == RS_DTYPE_F32 ? launch_linear<RS_DTYPE_F32>(p, st)
+                       : y_dtype == RS_DTYPE_BF16 ? launch_linear<RS_DTYPE_BF16>(p, st) : launch_linear<RS_DTYPE_F16>(p, st);
+    return e == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
 }
 
 }  // extern "C"

@@ -23,7 +23,7 @@ def blocks_of(x, rows):
 def quantized(x, rows):
     R, K = x.shape
     b = blocks_of(x.cpu().float(), rows)
-    scale = (b.abs().amax(dim=(1, 3)) / 448.0).clamp(min=2.0 ** -126)
+    scale = (b.abs().amax(dim=(1, 3)) * torch.tensor(1.0 / 448.0)).clamp(min=2.0 ** -126)
     q = (b / scale[:, None, :, None]).to(F8)
     return q.view(torch.uint8).view(b.shape[0] * rows, -1)[:R, :K], scale
 
