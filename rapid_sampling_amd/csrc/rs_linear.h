@@ -16,6 +16,8 @@ constexpr int kFpBlock = 128;
 typedef int   v8i __attribute__((ext_vector_type(8)));
 typedef int   v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
@@ -129,18 +131,23 @@ __device__ __forceinline__ v8bf widen8(int lo, int hi)
     return v8bf{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+__device__ __forceinline__ void widen_block(v8i q, v8bf (&b)[4])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = widen8(q[2 * i], q[2 * i + 1]);
+}
+
 // 16 x 16 sums over a block of 128.  Lane l gives 32 bytes of row l % 16 of either side (any 32 of the block's columns, as
 // long as both sides agree) and has the sums of w's rows 4 (l / 16) + 0..3 with x's row l % 16.
 //
 // The matrix instructions that take 8 bits do not hold their sums in 32: of the eight products that are added at once, what lies
 // 14 binades and more under the largest is dropped (256 * 256 + 4 is 65536; measured 3.1e-5 of a result's size over
 // 4096 random columns).  Those that take bfloat16 keep 24 bits (1.0e-7), at half the rate.
-__device__ __forceinline__ v4f block_product(v8i w, v8i x)
+__device__ __forceinline__ v4f block_product(const v8bf (&w)[4], const v8bf (&x)[4])
 {
     v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(w[2 * i], w[2 * i + 1]), widen8(x[2 * i], x[2 * i + 1]), acc, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], x[i], acc, 0, 0, 0);
     return acc;
 }
 
@@ -149,6 +156,13 @@ __device__ __forceinline__ v4f block_product_8(v8i w, v8i x)
 {
     const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
+}
+
+template <int DT> __device__ __forceinline__ void put_four(void *p, int64_t i, v4f a)
+{
+    if constexpr (DT == RS_DTYPE_F32) *(v4f *)((float *)p + i) = a;
+    else if constexpr (DT == RS_DTYPE_BF16) *(v4bf *)((__bf16 *)p + i) = v4bf{(__bf16)a[0], (__bf16)a[1], (__bf16)a[2], (__bf16)a[3]};
+    else *(v4h *)((_Float16 *)p + i) = v4h{(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3]};
 }
 
 // Four consecutive float32 values, or eight of 16 bits, in one store.
@@ -168,86 +182,174 @@ template <int DT> __device__ __forceinline__ void put_wide(void *p, int64_t i, v
     }
 }
 
-// A wave per 16 rows of w and 16 MT rows of x.
-template <int DT, int MT>
-__global__ __launch_bounds__(256) void linear_kernel(LinearParams p)
-{
-    const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u;
-    const uint32_t n0 = (blockIdx.x * 4u + wave) * 16u, m0 = blockIdx.y * (16u * MT);
-    if (n0 >= p.N) return;
-    const uint32_t i = lane % 16u, part = lane / 16u;
-    const uint8_t *wr = p.w + (int64_t)min(n0 + i, p.N - 1u) * p.w_stride;
-    v4f acc[MT];
+// --------------------------------------------------------------- few rows --
+// Bound by reading w once.  A workgroup makes 16 NT rows of w x 16 MT rows of x; its waves take the blocks of 128 columns in
+// turn, so that it reads 1 KB of each row at a time and nothing is shared but the sums, which go through LDS once, at
+// the end, and are added in the order of the waves.  A wave asks for its next block before it multiplies the one it has.
+// The products are made on bfloat16, whatever y's type: the matrix cores have time to spare here.
+template <int MT, int NT>
+struct LinearFew {
+    struct Block {
+        v8i   w[NT], x[MT];
+        float f[MT];
+    };
+    const uint8_t *w[NT], *x[MT];        // the lane's rows, at its columns of the first block
+    const float   *sw, *sx[MT];
+
+    __device__ __forceinline__ LinearFew(const LinearParams &p, uint32_t n0, uint32_t m0)
+    {
+        const uint32_t lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t kb = 0; kb < p.blocks; ++kb) {
-        const uint32_t k = kb * kFpBlock + part * 32u;
-        const v8i w = join(load16(wr, k, p.K), load16(wr, k + 16u, p.K));
-        const float sw = p.w_scale[(size_t)(n0 / kFpBlock) * p.blocks + kb];
+        for (int u = 0; u < NT; ++u) w[u] = p.w + (int64_t)min(n0 + u * 16u + i, p.N - 1u) * p.w_stride + part * 16u;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             const uint32_t m = min(m0 + t * 16u + i, p.M - 1u);
-            const uint8_t *xr = p.x + (int64_t)m * p.x_stride;
-            const v4f s = block_product(w, join(load16(xr, k, p.K), load16(xr, k + 16u, p.K)));
-            const float f = sw * p.x_scale[(size_t)m * p.blocks + kb];
+            x[t] = p.x + (int64_t)m * p.x_stride + part * 16u;
+            sx[t] = p.x_scale + (size_t)m * p.blocks;
+        }
+        sw = p.w_scale + (size_t)(n0 / kFpBlock) * p.blocks;
+    }
+    // (w is read once and need not stay in the caches; x is read by every workgroup)
+    __device__ __forceinline__ void load(const LinearParams &p, uint32_t kb, Block &b) const
+    {
+        const uint32_t k = kb * kFpBlock;
+        if (k + kFpBlock <= p.K) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[t][j] = __builtin_fmaf(s[j], f, acc[t][j]);
+            for (int u = 0; u < NT; ++u)
+                b.w[u] = join(__builtin_nontemporal_load((const v4i *)(w[u] + k)), __builtin_nontemporal_load((const v4i *)(w[u] + k + 64)));
+#pragma unroll
+            for (int t = 0; t < MT; ++t) b.x[t] = join(*(const v4i *)(x[t] + k), *(const v4i *)(x[t] + k + 64));
+        } else {
+            const uint32_t at = threadIdx.x % 64u / 16u * 16u;
+#pragma unroll
+            for (int u = 0; u < NT; ++u) b.w[u] = join(load16(w[u] - at, k + at, p.K), load16(w[u] - at, k + at + 64u, p.K));
+#pragma unroll
+            for (int t = 0; t < MT; ++t) b.x[t] = join(load16(x[t] - at, k + at, p.K), load16(x[t] - at, k + at + 64u, p.K));
+        }
+        const float s = sw[kb];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) b.f[t] = s * sx[t][kb];
+    }
+    static __device__ __forceinline__ void multiply(const Block &b, v4f (&acc)[NT][MT])
+    {
+        v8bf x[MT][4];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) widen_block(b.x[t], x[t]);
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            v8bf w[4];
+            widen_block(b.w[u], w);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const v4f s = block_product(w, x[t]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[u][t][j] = __builtin_fmaf(s[j], b.f[t], acc[u][t][j]);
+            }
         }
     }
+};
+
+template <int DT, int MT, int NT>
+__global__ __launch_bounds__(512) void linear_few_kernel(LinearParams p)
+{
+    using L = LinearFew<MT, NT>;
+    constexpr int kTiles = NT * MT, kRound = kTiles < 8 ? kTiles : 8;
+    __shared__ v4f sums[8][kRound][64];
+    const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u, waves = blockDim.x / 64u, i = lane % 16u, part = lane / 16u;
+    const uint32_t n0 = blockIdx.x * (16u * NT), m0 = blockIdx.y * (16u * MT);
+    const L rows(p, n0, m0);
+    v4f acc[NT][MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const uint32_t m = m0 + t * 16u + i;
-        if (m >= p.M) continue;
+    for (int u = 0; u < NT; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t n = n0 + part * 4u + j;
-            if (n < p.N) put<DT>(p.y, (int64_t)m * p.y_stride + n, acc[t][j]);
+        for (int t = 0; t < MT; ++t) acc[u][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (wave < p.blocks) {
+        typename L::Block now, next;
+        rows.load(p, wave, now);
+        uint32_t kb = wave + waves;
+        for (; kb < p.blocks; kb += waves) {
+            rows.load(p, kb, next);
+            L::multiply(now, acc);
+            now = next;
+        }
+        L::multiply(now, acc);
+    }
+    const bool aligned = !(p.y_stride % 4) && !((uintptr_t)p.y & 15);
+#pragma unroll
+    for (int r = 0; r < kTiles; r += kRound) {
+        if (r) __syncthreads();
+#pragma unroll
+        for (int c = 0; c < kRound; ++c) sums[wave][c][lane] = acc[(r + c) / MT][(r + c) % MT];
+        __syncthreads();
+        for (uint32_t c = wave; c < (uint32_t)kRound; c += waves) {
+            v4f s = sums[0][c][lane];
+            for (uint32_t o = 1; o < waves; ++o) s += sums[o][c][lane];
+            const uint32_t u = (r + c) / MT, t = (r + c) % MT;
+            const uint32_t m = m0 + t * 16u + i, n = n0 + u * 16u + part * 4u;
+            if (m >= p.M) continue;
+            const int64_t at = (int64_t)m * p.y_stride + n;
+            if (aligned && n + 4u <= p.N) put_four<DT>(p.y, at, s);
+            else
+#pragma unroll
+                for (int j = 0; j < 4; ++j) if (n + j < p.N) put<DT>(p.y, at + j, s[j]);
         }
     }
 }
 
 // -------------------------------------------------------------- many rows --
-// A workgroup of eight waves makes 256 rows of w x 64 MT rows of x, a wave 128 x 16 MT of it: a quarter of w's rows in a lane's
-// reach would not do, since every block has to be scaled in the vector unit before it is added (four sums a lane and
-// 16 x 16 product), so the sums sit in ordinary registers, 32 MT of them.
+// A workgroup of WN x WM waves makes 128 WN rows of w x 16 MT WM rows of x, a wave 128 x 16 MT of it.  Every block has to be
+// scaled in the vector unit before it is added (four sums a lane and 16 x 16 product), so a wave's sums sit in 32 MT ordinary
+// registers; a product's sums are added while the matrix cores make the next.
 //
-// A block of 128 columns is one stage: rows of 128 bytes go from memory to LDS without passing through registers, while
-// the stage before is multiplied.  The eight 16-byte pieces of a row are stored in an order that depends on the row
-// (place = piece ^ f(row)), so that the eight rows read at once lie in different banks.  The first operand's rows are
+// A block of 128 columns is one stage: rows of 128 bytes go from memory to LDS without passing through registers, up to
+// STAGES - 1 blocks ahead of the one that is multiplied.  The eight 16-byte pieces of a row are stored in an order that depends on
+// the row (place = piece ^ turn(row)), so that the eight rows read at once lie in different banks.  The first operand's rows are
 // dealt so that a lane's sums are 32 consecutive columns of y.
 typedef __attribute__((address_space(1))) const void *GlobalPtr;
 typedef __attribute__((address_space(3))) void *LdsPtr;
 
-constexpr int kTileN = 256;
-constexpr int64_t kTileStride = (1ll << 32) / 256 - kFpBlock;
+constexpr int64_t kTileStride = (1ll << 32) / 256 - kFpBlock;   // a tile's rows are reached with 32 bits
 
 __device__ __forceinline__ uint32_t w_turn(uint32_t row) { return (row & 3u) | ((row >> 3) & 4u); }
 __device__ __forceinline__ uint32_t x_turn(uint32_t row) { return row & 7u; }
 
-template <int DT, int MT, bool EXACT>
+__device__ __forceinline__ uint32_t wave_id() { return uniform(threadIdx.x / 64u); }
+
+// All but the newest N loads of this wave are done, and so are every other wave's, and their reads of LDS.
+template <int N> __device__ __forceinline__ void stage_barrier()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
+}
+
+template <int WN, int WM, int MT, int STAGES, bool EXACT>
 struct LinearTile {
-    static constexpr uint32_t kTileM = 64 * MT, kRows = kTileN + kTileM, kStage = kRows * kFpBlock;
-    static constexpr uint32_t kLoads = kRows / 64;           // 16-byte pieces of a stage per thread
+    static constexpr uint32_t kWaves = WN * WM, kThreads = 64 * kWaves, kTileN = 128 * WN, kTileM = 16 * MT * WM;
+    static constexpr uint32_t kRows = kTileN + kTileM, kStage = kRows * kFpBlock, kLds = STAGES * kStage;
+    static constexpr uint32_t kLoads = kRows * 8 / kThreads, kLoadsW = kTileN * 8 / kThreads;    // 16-byte pieces of a stage per thread
+    static_assert(kRows * 8 % kThreads == 0 && kTileN * 8 % kThreads == 0 && kTileN <= 256 && kTileM <= 256, "whole loads; 32-bit offsets");
+    static_assert(kWaves % 4 == 0, "w_turn is the same for every load of a thread, or for every other one");
 
-    // A wave fills eight rows of a stage with one load: thread's row and piece of load i, w's rows first.
-    static __device__ __forceinline__ uint32_t row_of(uint32_t i) { return (i * 8u + threadIdx.x / 64u) * 8u + threadIdx.x % 64u / 8u; }
+    // A wave fills eight rows of a stage with one load: the thread's row of load i, w's rows first.
+    static __device__ __forceinline__ uint32_t row_of(uint32_t i) { return (i * kWaves + wave_id()) * 8u + threadIdx.x % 64u / 8u; }
 
+    // The tile's rows as two buffers; what lies behind their last row reads as 0.
     struct Source {
-        const uint8_t *w, *x;            // of the tile's first rows
-        uint32_t       at[kLoads];       // bytes from there to the thread's pieces of the first block
+        __amdgpu_buffer_rsrc_t w, x;
+        uint32_t w_stride, x_stride;
+        uint32_t w_at[2], x_at;          // the thread's piece of the first block of its row of an even, of an odd load
     };
     static __device__ __forceinline__ Source source(const LinearParams &p, uint32_t n0, uint32_t m0)
     {
+        constexpr int kFlags = 0x00027000;     // untyped, offsets in bytes
         Source s;
-        s.w = p.w + (int64_t)n0 * p.w_stride;
-        s.x = p.x + (int64_t)m0 * p.x_stride;
-#pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i) {
-            const bool is_w = i < kTileN / 64;
-            const uint32_t r = row_of(i) - (is_w ? 0u : kTileN);
-            const uint32_t piece = (threadIdx.x & 7u) ^ (is_w ? w_turn(r) : x_turn(r));
-            s.at[i] = (is_w ? min(r, p.N - 1u - n0) * (uint32_t)p.w_stride : min(r, p.M - 1u - m0) * (uint32_t)p.x_stride) + piece * 16u;
-        }
+        s.w_stride = (uint32_t)p.w_stride;
+        s.x_stride = (uint32_t)p.x_stride;
+        const uint32_t rows_w = min(p.N - n0, kTileN), rows_x = min(p.M - m0, kTileM);
+        s.w = __builtin_amdgcn_make_buffer_rsrc((void *)(p.w + (int64_t)n0 * p.w_stride), 0, (int)((rows_w - 1u) * s.w_stride + p.K), kFlags);
+        s.x = __builtin_amdgcn_make_buffer_rsrc((void *)(p.x + (int64_t)m0 * p.x_stride), 0, (int)((rows_x - 1u) * s.x_stride + p.K), kFlags);
+        const uint32_t r = row_of(0);
+        for (uint32_t i = 0; i < 2; ++i) s.w_at[i] = r * s.w_stride + ((threadIdx.x & 7u) ^ w_turn(r + i * 8u * kWaves)) * 16u;
+        s.x_at = r * s.x_stride + ((threadIdx.x & 7u) ^ x_turn(r)) * 16u;
         return s;
     }
     static __device__ __forceinline__ void fill(const LinearParams &p, const Source &s, uint32_t n0, uint32_t m0, uint32_t kb, uint8_t *lds)
@@ -255,19 +357,23 @@ struct LinearTile {
         const uint32_t k = kb * kFpBlock;
         if (k + kFpBlock <= p.K) {
 #pragma unroll
-            for (uint32_t i = 0; i < kLoads; ++i)
-                __builtin_amdgcn_global_load_lds((GlobalPtr)((i < kTileN / 64 ? s.w : s.x) + k + s.at[i]), (LdsPtr)(lds + (i * 8u + threadIdx.x / 64u) * 1024u), 16, 0, 0);
+            for (uint32_t i = 0; i < kLoads; ++i) {
+                const LdsPtr to = (LdsPtr)(lds + (i * kWaves + wave_id()) * 1024u);
+                if (i < kLoadsW) __builtin_amdgcn_raw_ptr_buffer_load_lds(s.w, to, 16, s.w_at[kWaves % 8 ? i % 2 : 0], k + i * 8u * kWaves * s.w_stride, 0, 0);
+                else __builtin_amdgcn_raw_ptr_buffer_load_lds(s.x, to, 16, s.x_at, k + (i - kLoadsW) * 8u * kWaves * s.x_stride, 0, 0);
+            }
             return;
         }
         // the last block where K is no whole number of them
 #pragma unroll 1
         for (uint32_t i = 0; i < kLoads; ++i) {
-            const bool is_w = i < kTileN / 64;
+            const bool is_w = i < kLoadsW;
             const uint32_t r = row_of(i) - (is_w ? 0u : kTileN);
             const uint32_t piece = (threadIdx.x & 7u) ^ (is_w ? w_turn(r) : x_turn(r));
-            const uint8_t *from = is_w ? s.w + min(r, p.N - 1u - n0) * p.w_stride : s.x + min(r, p.M - 1u - m0) * p.x_stride;
+            const uint8_t *from = is_w ? p.w + (int64_t)min(n0 + r, p.N - 1u) * p.w_stride : p.x + (int64_t)min(m0 + r, p.M - 1u) * p.x_stride;
             *(v4i *)(lds + row_of(i) * kFpBlock + (threadIdx.x & 7u) * 16u) = load16(from, k + piece * 16u, p.K);
         }
+        wait_vmem();
     }
 
     static __device__ __forceinline__ v8i fragment(const uint8_t *lds, uint32_t row, uint32_t turn, uint32_t part)
@@ -276,48 +382,70 @@ struct LinearTile {
         return join(*(const v4i *)(r + ((part ^ turn) * 16u)), *(const v4i *)(r + (((part + 4u) ^ turn) * 16u)));
     }
 
+    // Asks for block `next` and multiplies the one in now_lds.
     static __device__ __forceinline__ void step(const LinearParams &p, const Source &source, uint32_t n0, uint32_t m0, uint32_t next,
                                                 const uint8_t *__restrict now_lds, uint8_t *__restrict next_lds, const float (&f)[MT], v4f (&acc)[8][MT])
     {
         if (next < p.blocks) fill(p, source, n0, m0, next, next_lds);
-        const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
-        const uint32_t wn = (wave & 1u) * 128u, wm = (wave >> 1) * (16u * MT);
+        const uint32_t wave = wave_id(), lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
+        const uint32_t wn = wave % WN * 128u, wm = wave / WN * (16u * MT);
         v8i x[MT];
+        v8bf xb[EXACT ? MT : 1][4];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             const uint32_t r = wm + t * 16u + i;
             x[t] = fragment(now_lds + kTileN * kFpBlock, r, x_turn(r), part);
+            if constexpr (EXACT) widen_block(x[t], xb[t]);
         }
+        const uint32_t r0 = wn + i / 4u * 32u + i % 4u;
+        v8i w = fragment(now_lds, r0, w_turn(r0), part);
+        v4f s[MT];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const uint32_t r = wn + i / 4u * 32u + u * 4u + i % 4u;
-            const v8i w = fragment(now_lds, r, w_turn(r), part);
-            v4f s[MT];
+            v8i ahead = w;
+            if (u < 7) {
+                const uint32_t r = r0 + (u + 1) * 4u;
+                ahead = fragment(now_lds, r, w_turn(r), part);
+            }
+            v4f made[MT];
+            v8bf wb[4];
+            if constexpr (EXACT) widen_block(w, wb);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) s[t] = EXACT ? block_product(w, x[t]) : block_product_8(w, x[t]);
+            for (int t = 0; t < MT; ++t) {
+                if constexpr (EXACT) made[t] = block_product(wb, xb[t]);
+                else made[t] = block_product_8(w, x[t]);
+            }
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+            for (int t = 0; t < MT; ++t) {
+                if (u)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[u][t][j] = __builtin_fmaf(s[t][j], f[t], acc[u][t][j]);
+                    for (int j = 0; j < 4; ++j) acc[u - 1][t][j] = __builtin_fmaf(s[t][j], f[t], acc[u - 1][t][j]);
+                s[t] = made[t];
+            }
+            w = ahead;
         }
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[7][t][j] = __builtin_fmaf(s[t][j], f[t], acc[7][t][j]);
     }
 };
 
-template <int DT, int MT, bool EXACT>
-__global__ __launch_bounds__(512, 2) void linear_tile_kernel(LinearParams p)
+template <int DT, int WN, int WM, int MT, int STAGES, bool EXACT>
+__global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearParams p)
 {
-    using L = LinearTile<DT, MT, EXACT>;
+    using L = LinearTile<WN, WM, MT, STAGES, EXACT>;
     extern __shared__ uint8_t lds[];
     // Workgroup b runs on XCD b % 8: each XCD takes a stretch of the tiles, in panels of eight rows of tiles, so that the 32 tiles
     // it works on at a time share their rows in its L2.
-    const uint32_t tm = (p.M + L::kTileM - 1u) / L::kTileM, tn = (p.N + kTileN - 1u) / kTileN, tiles = tm * tn;
+    const uint32_t tm = (p.M + L::kTileM - 1u) / L::kTileM, tn = (p.N + L::kTileN - 1u) / L::kTileN, tiles = tm * tn;
     const uint32_t each = tiles / 8u, rest = tiles % 8u, xcd = blockIdx.x % 8u;
     const uint32_t id = xcd * each + min(xcd, rest) + blockIdx.x / 8u;
     const uint32_t panel = id / (8u * tn), high = min(8u, tm - panel * 8u), in = id - panel * 8u * tn;
-    const uint32_t m0 = (panel * 8u + in % high) * L::kTileM, n0 = in / high * kTileN;
+    const uint32_t m0 = (panel * 8u + in % high) * L::kTileM, n0 = in / high * L::kTileN;
 
-    const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
-    const uint32_t wn = (wave & 1u) * 128u, wm = (wave >> 1) * (16u * MT);
+    const uint32_t wave = wave_id(), lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
+    const uint32_t wn = wave % WN * 128u, wm = wave / WN * (16u * MT);
     const float *sw = p.w_scale + (size_t)min((n0 + wn) / kFpBlock, (p.N - 1u) / kFpBlock) * p.blocks;
     const float *sx[MT];
     v4f acc[8][MT];
@@ -328,16 +456,29 @@ __global__ __launch_bounds__(512, 2) void linear_tile_kernel(LinearParams p)
         for (int u = 0; u < 8; ++u) acc[u][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const typename L::Source source = L::source(p, n0, m0);
-    L::fill(p, source, n0, m0, 0, lds);
-    for (uint32_t kb = 0; kb < p.blocks; ++kb) {
-        float f[MT];
-        const float s = sw[kb];
+    // (a block's scales are asked for one block ahead, before that block's rows: waiting for them waits for nothing newer)
+    float f[MT], ahead[MT], ahead_w = sw[0];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) f[t] = sx[t][kb] * s;
-        wait_vmem();
-        __syncthreads();
-        const bool odd = kb & 1u;
-        L::step(p, source, n0, m0, kb + 1u, lds + (odd ? L::kStage : 0u), lds + (odd ? 0u : L::kStage), f, acc);
+    for (int t = 0; t < MT; ++t) {
+        ahead[t] = sx[t][0];
+        asm volatile("" : "+v"(ahead[t]));       // here, and not in the loop, where it would wait for the next block's
+    }
+#pragma unroll
+    for (int b = 0; b < STAGES - 1; ++b) if (b < (int)p.blocks) L::fill(p, source, n0, m0, b, lds + b * L::kStage);
+    uint32_t now = 0, next = (STAGES - 1) * L::kStage;
+    for (uint32_t kb = 0; kb < p.blocks; ++kb) {
+        // (towards the end there are no newer stages to leave under way)
+        if (STAGES == 2 || kb + STAGES - 1 > p.blocks) stage_barrier<0>();
+        else stage_barrier<(STAGES - 2) * L::kLoads>();
+#pragma unroll
+        for (int t = 0; t < MT; ++t) f[t] = ahead[t] * ahead_w;
+        const uint32_t k1 = min(kb + 1u, p.blocks - 1u);
+        ahead_w = sw[k1];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) ahead[t] = sx[t][k1];
+        L::step(p, source, n0, m0, kb + STAGES - 1u, lds + now, lds + next, f, acc);
+        now = now == (STAGES - 1) * L::kStage ? 0u : now + L::kStage;
+        next = next == (STAGES - 1) * L::kStage ? 0u : next + L::kStage;
     }
     // a lane has columns wn + 32 part .. + 31 of its rows of y
     const uint32_t n = n0 + wn + part * 32u;

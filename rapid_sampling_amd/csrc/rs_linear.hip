@@ -10,28 +10,33 @@ static void launch_quantize(const QuantParams &p, bool tiles, hipStream_t st)
     else hipLaunchKernelGGL(quantize_rows_kernel<DT>, dim3((uint32_t)(((uint64_t)p.R * p.blocks + 15) / 16)), dim3(256), 0, st, p);
 }
 
-template <int DT, int MT, bool EXACT>
+template <int DT, int WN, int WM, int MT, int STAGES, bool EXACT>
 static hipError_t launch_tiles(const LinearParams &p, hipStream_t st)
 {
-    using L = LinearTile<DT, MT, EXACT>;
-    const uint64_t tiles = (uint64_t)((p.M + L::kTileM - 1) / L::kTileM) * ((p.N + kTileN - 1) / kTileN);
+    using L = LinearTile<WN, WM, MT, STAGES, EXACT>;
+    const uint64_t tiles = (uint64_t)((p.M + L::kTileM - 1) / L::kTileM) * ((p.N + L::kTileN - 1) / L::kTileN);
     if (tiles > 0x7FFFFFFF) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((linear_tile_kernel<DT, MT, EXACT>), dim3((uint32_t)tiles), dim3(512), 2 * L::kStage, st, p);
+    hipLaunchKernelGGL((linear_tile_kernel<DT, WN, WM, MT, STAGES, EXACT>), dim3((uint32_t)tiles), dim3(L::kThreads), L::kLds, st, p);
+    return hipGetLastError();
+}
+
+template <int DT, int MT, int NT>
+static hipError_t launch_few(const LinearParams &p, hipStream_t st)
+{
+    const uint32_t waves = p.blocks >= 8 ? 8 : p.blocks >= 4 ? 4 : p.blocks >= 2 ? 2 : 1;
+    hipLaunchKernelGGL((linear_few_kernel<DT, MT, NT>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)), dim3(64 * waves), 0, st, p);
     return hipGetLastError();
 }
 
 template <int DT>
 static hipError_t launch_linear(const LinearParams &p, hipStream_t st)
 {
-    // (the tiles' kernel reaches its 256 rows with 32 bits)
-    if (p.M > 64 && p.x_stride <= kTileStride && p.w_stride <= kTileStride) {
-        if constexpr (DT == RS_DTYPE_F32) return launch_tiles<DT, 2, true>(p, st);
-        else return p.M > 128 ? launch_tiles<DT, 4, false>(p, st) : launch_tiles<DT, 2, false>(p, st);
-    }
-    const uint32_t nb = (p.N + 63) / 64;
-    if (p.M <= 16) hipLaunchKernelGGL((linear_kernel<DT, 1>), dim3(nb, 1), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((linear_kernel<DT, 4>), dim3(nb, (p.M + 63) / 64), dim3(256), 0, st, p);
-    return hipGetLastError();
+    // (the tiles' kernel reaches its rows with 32 bits)
+    if (p.M <= 16 || p.x_stride > kTileStride || p.w_stride > kTileStride) return launch_few<DT, 1, 2>(p, st);
+    constexpr bool kExact = DT == RS_DTYPE_F32;
+    if (p.M <= 64) return launch_tiles<DT, 1, 4, 1, 3, true>(p, st);
+    if constexpr (kExact) return launch_tiles<DT, 2, 4, 2, 3, true>(p, st);
+    else return p.M <= 128 ? launch_tiles<DT, 2, 4, 2, 3, false>(p, st) : launch_tiles<DT, 2, 4, 4, 2, false>(p, st);
 }
 
 static bool known(int32_t dtype) { return dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16 || dtype == RS_DTYPE_F16; }
