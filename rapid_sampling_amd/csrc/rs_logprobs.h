@@ -42,7 +42,8 @@ struct LpParams {
     float      *top_logprobs;
     int32_t    *top_tokens;
     float4     *stats;                   // for the gradient: max, log2 of the sum, entropy; or null
-    uint32_t    S, J;                    // workgroups per row; windows per thread and slice
+    uint32_t    S, J;                    // workgroups per row (at most 64); windows per thread and slice
+    uint32_t    J_row, step;             // windows per thread of the whole row, and ceil(2^32 / J_row)
     LpSlice    *slices;                  // split rows: what the workgroups of a row leave for the last of them
     uint32_t   *arrived;                 // ... and how many have, per row; zero between calls
 };
@@ -177,17 +178,32 @@ __device__ __forceinline__ void lp_take(LpSums &a, const float (&x)[N], float c)
     a.t += t[0] + t[1];
 }
 
+// Reductions over the 64 lanes, the result in all of them: within rows of 16 lanes, then across the rows; a lane without a
+// source keeps its own maximum, adds nothing.
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_max(float v)
+{
+    return fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)__float_as_uint(v), (int)__float_as_uint(v), CTRL, ROWS, 0xf, false)));
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_sum(float v) { return v + __uint_as_float(dpp0_u32<CTRL, ROWS>(__float_as_uint(v))); }
 __device__ __forceinline__ float wave_max_f(float v)
 {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
+    v = dpp_max<0x111, 0xf>(v); v = dpp_max<0x112, 0xf>(v); v = dpp_max<0x114, 0xf>(v); v = dpp_max<0x118, 0xf>(v);
+    v = dpp_max<0x142, 0xa>(v); v = dpp_max<0x143, 0xc>(v);
+    return __uint_as_float(lane63_u32(__float_as_uint(v)));
 }
 __device__ __forceinline__ float wave_sum_f(float v)
 {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+    v = dpp_sum<0x111, 0xf>(v); v = dpp_sum<0x112, 0xf>(v); v = dpp_sum<0x114, 0xf>(v); v = dpp_sum<0x118, 0xf>(v);
+    v = dpp_sum<0x142, 0xa>(v); v = dpp_sum<0x143, 0xc>(v);
+    return __uint_as_float(lane63_u32(__float_as_uint(v)));
+}
+
+// The sums of a wave, in every lane.
+__device__ __forceinline__ void lp_wave(LpSums &a, float c)
+{
+    lp_rebase(a, wave_max_f(a.m), c);
+    a.s = wave_sum_f(a.s);
+    a.t = wave_sum_f(a.t);
 }
 
 struct LpShared {
@@ -205,9 +221,7 @@ struct LpShared {
 __device__ __forceinline__ void lp_block(LpSums &a, uint32_t &above, float c, LpShared &sh)
 {
     const uint32_t w = threadIdx.x / kWave;
-    lp_rebase(a, wave_max_f(a.m), c);
-    a.s = wave_sum_f(a.s);
-    a.t = wave_sum_f(a.t);
+    lp_wave(a, c);
     if (threadIdx.x % kWave == 0) { sh.m[w] = a.m; sh.s[w] = a.s; sh.t[w] = a.t; sh.above[w] = above; }
     __syncthreads();
     float m = sh.m[0];
@@ -241,19 +255,31 @@ struct LpRow {
     const typename E::T *row;
     uint32_t V, full, J;                 // logits; whole windows; windows of a thread, over the whole row
 
-    // f(logit, index) for the windows of the n_hot threads in sh.hot, spread over the workgroup, and for the row's last few
+    uint32_t step;                       // ceil(2^32 / J): i / J = (i step) >> 32 for i < 256 J, J < 4096
+
+    // f(logit, index) for the windows of the n_hot threads in sh.hot, spread over the workgroup and four of a thread's under way
+    // at a time, and for the row's last few logits
     template <typename F>
     __device__ __forceinline__ void each(const LpShared &sh, uint32_t n_hot, F f) const
     {
+        constexpr int U = 4;
         const uint32_t items = n_hot * J;
-        for (uint32_t i = threadIdx.x; i < items; i += kLpThreads) {
-            const uint32_t h = i / J, j = i - h * J;
-            const uint32_t n = j * kLpThreads + sh.hot[h];
-            if (n < full) {
-                float x[E::kVec];
-                E::wide(load_window<DT>(row, n), x);
+        for (uint32_t i = threadIdx.x; i < items; i += U * kLpThreads) {
+            uint4 raw[U];
+            uint32_t n[U];
 #pragma unroll
-                for (int k = 0; k < E::kVec; ++k) f(x[k], n * E::kVec + k);
+            for (int u = 0; u < U; ++u) {
+                const uint32_t at = i + u * kLpThreads, h = J == 1u ? at : __umulhi(at, step);
+                n[u] = at < items ? (at - h * J) * kLpThreads + sh.hot[h] : full;
+                if (n[u] < full) raw[u] = load_window<DT>(row, n[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (n[u] >= full) continue;
+                float x[E::kVec];
+                E::wide(raw[u], x);
+#pragma unroll
+                for (int k = 0; k < E::kVec; ++k) f(x[k], n[u] * E::kVec + k);
             }
         }
         const uint32_t i = full * E::kVec + threadIdx.x;
@@ -261,9 +287,9 @@ struct LpRow {
     }
 };
 
-// The largest t with at least `k` of the workgroup's keys >= t (0 if k > kLpThreads); only the upper BITS bits matter.
+// A t with at least `k` and, unless keys are equal, at most k + spare of the workgroup's keys >= t; only the upper BITS bits matter.
 template <int BITS, typename K>
-__device__ __forceinline__ K lp_kth(const K *key, uint32_t k)
+__device__ __forceinline__ K lp_kth(const K *key, uint32_t k, uint32_t spare)
 {
     constexpr int kAll = (int)sizeof(K) * 8;
     K mine[kLpWaves];
@@ -276,7 +302,7 @@ __device__ __forceinline__ K lp_kth(const K *key, uint32_t k)
 #pragma unroll
         for (int i = 0; i < kLpWaves; ++i) n += (uint32_t)__popcll(__ballot(mine[i] >= c));
         if (n >= k) t = c;
-        if (n == k) break;
+        if (n >= k && n <= k + spare) break;
     }
     return t;
 }
@@ -289,7 +315,7 @@ __device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float larg
     sh.key[tid] = lp_key(largest);
     if (tid == 0) sh.n = 0;
     __syncthreads();
-    uint32_t tau = lp_kth<Elem<DT>::kBits>(sh.key, top);
+    uint32_t tau = lp_kth<Elem<DT>::kBits>(sh.key, top, top / 4u);
     if (tau <= fkey(-__builtin_inff())) tau = 1u;        // fewer numbers than are wanted, perhaps: NaN too
     uint32_t n_hot = 0;
 #pragma unroll
@@ -311,7 +337,7 @@ __device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float larg
         row.each(sh, n_hot, [&](float x, uint32_t i) { best = max(best, lp_token(x, i)); });
         sh.lane_top[tid] = best;
         __syncthreads();
-        uint64_t lo = max(lp_kth<64>(sh.lane_top, top), (uint64_t)tau << 32), hi = ~0ull;
+        uint64_t lo = max(lp_kth<64>(sh.lane_top, top, 0u), (uint64_t)tau << 32), hi = ~0ull;
         for (uint64_t t = lo;; t = lo + (hi - lo) / 2) {
             __syncthreads();
             if (tid == 0) sh.n = 0;
@@ -330,16 +356,26 @@ __device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float larg
         }
     }
     const uint32_t n = sh.n;
+    auto put = [&](uint64_t k, uint32_t place) {
+        if (place >= top) return;
+        const float x = (uint32_t)(k >> 32) == 1u ? __builtin_nanf("") : fkey_inv((uint32_t)(k >> 32));
+        out_tokens[place] = (int32_t)(0xFFFFFFFFu - (uint32_t)k);
+        out_logprobs[place] = x == -__builtin_inff() && a.s == a.s ? x : (x - a.m) * inv_t - log_s;
+    };
+    if (n <= (uint32_t)kWave) {
+        if (w) return;
+        const uint64_t mine = lane < n ? sh.cand[lane] : 0;
+        uint32_t place = 0;
+        for (uint32_t j = 0; j < n; ++j) place += lane_of(mine, j) > mine;
+        if (lane < n) put(mine, place);
+        return;
+    }
     for (uint32_t i = tid; i < n; i += kLpThreads) {
         const uint64_t k = sh.cand[i];
         uint32_t place = 0;
+#pragma unroll 8
         for (uint32_t j = 0; j < n; ++j) place += sh.cand[j] > k;
-        if (place < top) {
-            const uint32_t id = 0xFFFFFFFFu - (uint32_t)k;
-            const float x = Elem<DT>::one(row.row[id]);
-            out_tokens[place] = (int32_t)id;
-            out_logprobs[place] = x == -__builtin_inff() && a.s == a.s ? x : (x - a.m) * inv_t - log_s;
-        }
+        put(k, place);
     }
 }
 
@@ -418,7 +454,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
     float mine = largest;
     if constexpr (SPLIT) {
         LpSlice *slices = p.slices + (size_t)r * p.S;
-        a_store(&slices[slice].top[tid], largest);
+        if (p.top) a_store(&slices[slice].top[tid], largest);
         if (tid == 0) {
             a_store(&slices[slice].m, a.m); a_store(&slices[slice].s, a.s); a_store(&slices[slice].t, a.t);
             a_store(&slices[slice].above, above);
@@ -431,21 +467,26 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
         }
         __syncthreads();
         if (!sh.last) return;
-        // the row's sums, from the slices' in turn; the largest logit of each thread over them
+        // the row's sums, from the slices' in every wave; the largest logit of each thread over the slices
         a = LpSums{-__builtin_inff(), 0.0f, 0.0f};
         above = 0;
-        for (uint32_t s = tid; s < p.S; s += kLpThreads) {
-            LpSums o{a_load(&slices[s].m), a_load(&slices[s].s), a_load(&slices[s].t)};
-            const float m = fmaxf(a.m, o.m);
-            lp_rebase(a, m, p.c);
-            lp_rebase(o, m, p.c);
-            a.s += o.s; a.t += o.t;
-            above += a_load(&slices[s].above);
+        const uint32_t lane = tid % kWave;
+        if (lane < p.S) {
+            a = LpSums{a_load(&slices[lane].m), a_load(&slices[lane].s), a_load(&slices[lane].t)};
+            above = a_load(&slices[lane].above);
         }
+        if (p.top) {
+            constexpr uint32_t B = 8;
+            for (uint32_t s = 0; s < p.S; s += B) {
+                float more[B];
+#pragma unroll
+                for (uint32_t u = 0; u < B; ++u) more[u] = a_load(&slices[min(s + u, p.S - 1u)].top[tid]);
+#pragma unroll
+                for (uint32_t u = 0; u < B; ++u) mine = fmaxf(mine, more[u]);
+            }
+        }
+        lp_wave(a, p.c);
         above = wave_sum(above);
-        if (p.top) for (uint32_t s = 0; s < p.S; ++s) mine = fmaxf(mine, a_load(&slices[s].top[tid]));
-        __syncthreads();
-        lp_block(a, above, p.c, sh);
     }
 
     const float log_s = logf(a.s);
@@ -471,7 +512,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
         }
     }
     if (p.top) {
-        const LpRow<DT> all{row, V, full, (full + kLpThreads - 1u) / kLpThreads};
+        const LpRow<DT> all{row, V, full, p.J_row, p.step};
         lp_alternatives<DT>(all, mine, a, log_s, p.inv_t, (uint32_t)p.top, p.top_logprobs + (size_t)r * p.top, p.top_tokens + (size_t)r * p.top, sh);
     }
 }

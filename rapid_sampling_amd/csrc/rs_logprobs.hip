@@ -12,7 +12,7 @@ constexpr uint32_t kLpSplitMost = 1024;   // workgroups of a call whose rows are
 static uint32_t lp_split(uint32_t rows, uint32_t windows)
 {
     const uint32_t most = kLpSplitMost / rows, per = (windows + 4u * kLpThreads - 1u) / (4u * kLpThreads);
-    return std::max(1u, std::min(most, per));
+    return std::max(1u, std::min(std::min(most, per), (uint32_t)kWave));
 }
 
 static int lp_check(const void *logits, int32_t dtype, const void *tokens, int32_t tokens_64, int64_t B, int64_t T, int64_t V, double temperature, int32_t top)
@@ -65,6 +65,8 @@ int rs_token_logprobs(const void *logits, int32_t dtype, int64_t stride_b, int64
     p.stats = (float4 *)stats;
     p.S = lp_split(rows, windows);
     p.J = (windows + p.S * kLpThreads - 1) / (p.S * kLpThreads);
+    p.J_row = (windows + kLpThreads - 1) / kLpThreads;
+    p.step = p.J_row ? 0xFFFFFFFFu / p.J_row + 1u : 0u;
     p.arrived = (uint32_t *)workspace;
     p.slices = (LpSlice *)((char *)workspace + 16 * (size_t)kLpSplitMost);
     const hipStream_t st = (hipStream_t)stream;
