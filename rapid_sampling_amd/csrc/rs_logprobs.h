@@ -18,15 +18,18 @@ constexpr int kLpThreads = 256;
 constexpr int kLpWaves   = kLpThreads / kWave;
 constexpr int kLpTopMax  = RS_LOGPROBS_TOP_MAX;
 constexpr int kLpCap     = 512;          // candidates that are put in order
+constexpr int kLpSegs    = 8;            // stretches that a thread's windows of a slice are divided into, at most
+constexpr int kLpStretches = 32;         // ... and a row's, where it is split
+constexpr int kLpUnits   = 1024;         // stretches that are read again
 constexpr float kLn2 = 0.693147180559945309f;
 
 // What a workgroup of a split row leaves for the last of the row's workgroups.
 struct alignas(16) LpSlice {
     float    m, s, t;                    // see LpSums
     uint32_t above;                      // tokens of the slice that come before the given one
-    float    top[kLpThreads];            // largest logit of each thread
+    float    seg[kLpSegs][kLpThreads];   // largest logit of each stretch of each thread's windows
 };
-static_assert(sizeof(LpSlice) == 1040, "rs_logprobs_workspace_bytes");
+static_assert(sizeof(LpSlice) == 16 + 4 * kLpSegs * kLpThreads, "rs_logprobs_workspace_bytes");
 
 struct LpParams {
     const void *logits;
@@ -42,8 +45,8 @@ struct LpParams {
     float      *top_logprobs;
     int32_t    *top_tokens;
     float4     *stats;                   // for the gradient: max, log2 of the sum, entropy; or null
-    uint32_t    S, J;                    // workgroups per row (at most 64); windows per thread and slice
-    uint32_t    J_row, step;             // windows per thread of the whole row, and ceil(2^32 / J_row)
+    uint32_t    S, J;                    // workgroups per row (at most kLpStretches); windows per thread and slice
+    uint32_t    seg_log;                 // a stretch is 2^seg_log windows, four at least
     LpSlice    *slices;                  // split rows: what the workgroups of a row leave for the last of them
     uint32_t   *arrived;                 // ... and how many have, per row; zero between calls
 };
@@ -156,10 +159,11 @@ __device__ __forceinline__ void lp_rebase(LpSums &a, float m, float c)
     a.m = m;
 }
 
-// N more logits.  Two exponents of a lane's window share the sums' chains; the terms of (x - m) c below -200 have e = 0
-// and must not make 0 * inf.
+// N more logits; returns the largest.  Two exponents of a lane's window share the sums' chains; the terms of (x - m) c below -200
+// have e = 0 and must not make 0 * inf.  (One operation less for z, with m c taken off in one step, and one less for t, with the
+// rare NaN looked for afterwards, did not make a call faster: it is bound by what it reads, 5.2 to 5.5 TB/s.)
 template <int N>
-__device__ __forceinline__ void lp_take(LpSums &a, const float (&x)[N], float c)
+__device__ __forceinline__ float lp_take(LpSums &a, const float (&x)[N], float c)
 {
     float top = x[0];
 #pragma unroll
@@ -176,6 +180,7 @@ __device__ __forceinline__ void lp_take(LpSums &a, const float (&x)[N], float c)
     }
     a.s += s[0] + s[1];
     a.t += t[0] + t[1];
+    return top;
 }
 
 // Reductions over the 64 lanes, the result in all of them: within rows of 16 lanes, then across the rows; a lane without a
@@ -210,11 +215,14 @@ struct LpShared {
     float    m[kLpWaves], s[kLpWaves], t[kLpWaves];
     uint32_t above[kLpWaves];
     uint32_t key[kLpThreads];            // order key of each thread's largest logit
-    uint64_t lane_top[kLpThreads];
+    union {
+        float    seg[kLpSegs][kLpThreads];      // largest logit of each stretch (rows that are not split)
+        uint64_t lane_top[kLpThreads];
+    };
     uint64_t cand[kLpCap];
-    uint32_t n;
+    uint32_t unit[kLpUnits];             // stretches to read again: stretch << 8 | thread
+    uint32_t n, n_units;
     uint32_t last;
-    uint16_t hot[kLpThreads];
 };
 
 // The sums of the workgroup, in every thread.
@@ -240,37 +248,42 @@ __device__ __forceinline__ void lp_block(LpSums &a, uint32_t &above, float c, Lp
 }
 
 // --------------------------------------------------------- the alternatives --
-// The `top` largest tokens of the row.  A thread's largest logit is known from the pass.  The top-th largest of those, tau,
-// is no larger than the top-th largest logit (that many threads hold one as large), so every token wanted is at least tau,
-// and only threads whose own largest is at least tau hold such tokens.  Only their windows are read again, by
-// all lanes: about `top` threads' worth of the row.  What is at least tau goes to a list, a few tokens more than are
-// wanted, and a token's place is the number of tokens in the list before it.
+// The `top` largest tokens of the row.  Each thread's largest logit is known from the pass, and that of each stretch of its
+// windows.  The top-th largest of the threads', tau, is no larger than the top-th largest logit (that many threads hold one as
+// large), so every token wanted is at least tau, and only stretches whose own largest is at least tau hold such tokens: about as
+// many stretches as tokens are wanted.  Their windows alone are read again, spread over the workgroup.  What is at least tau goes
+// to a list, a few tokens more than are wanted, and a token's place is the number of tokens in the list before it.
 //
-// A list that does not fit (rows of thousands of equal logits, or of large ones that all fall to a few threads) is cut by the
-// same bound over the lanes of the second reading, with the index as part of the order, and, if that is not enough,
-// by halving the range of the bound until it is.  That ends: the orders are distinct.
+// A list that does not fit (rows of hundreds of equal logits, or of large ones that all fall to a few threads) is cut by the
+// same bound over the threads of a second reading of the whole row, with the index as part of the order, and, if that is not
+// enough, by halving the range of the bound until it is.  That ends: the orders are distinct.
 template <int DT>
 struct LpRow {
     using E = Elem<DT>;
     const typename E::T *row;
-    uint32_t V, full, J;                 // logits; whole windows; windows of a thread, over the whole row
+    uint32_t V, full, J, seg_log, segs;  // logits; whole windows; windows of a thread in a slice, stretches in a slice
 
-    uint32_t step;                       // ceil(2^32 / J): i / J = (i step) >> 32 for i < 256 J, J < 4096
-
-    // f(logit, index) for the windows of the n_hot threads in sh.hot, spread over the workgroup and four of a thread's under way
-    // at a time, and for the row's last few logits
-    template <typename F>
-    __device__ __forceinline__ void each(const LpShared &sh, uint32_t n_hot, F f) const
+    template <typename F> __device__ __forceinline__ void tail(F f) const
+    {
+        const uint32_t i = full * E::kVec + threadIdx.x;
+        if (i < V) f(E::one(row[i]), i);
+    }
+    // f(logit, index) for the windows of the stretches in sh.unit and the row's last few logits
+    template <typename F> __device__ __forceinline__ void units(const LpShared &sh, uint32_t n_units, float least, F f) const
     {
         constexpr int U = 4;
-        const uint32_t items = n_hot * J;
+        const uint32_t items = n_units << seg_log, mask = (1u << seg_log) - 1u;
         for (uint32_t i = threadIdx.x; i < items; i += U * kLpThreads) {
             uint4 raw[U];
             uint32_t n[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const uint32_t at = i + u * kLpThreads, h = J == 1u ? at : __umulhi(at, step);
-                n[u] = at < items ? (at - h * J) * kLpThreads + sh.hot[h] : full;
+                const uint32_t at = i + u * kLpThreads;
+                n[u] = full;
+                if (at < items) {
+                    const uint32_t unit = sh.unit[at >> seg_log], slice = (unit >> 8) / segs, j = (((unit >> 8) - slice * segs) << seg_log) + (at & mask);
+                    if (j < J) n[u] = (slice * J + j) * kLpThreads + (unit & 255u);
+                }
                 if (n[u] < full) raw[u] = load_window<DT>(row, n[u]);
             }
 #pragma unroll
@@ -278,18 +291,33 @@ struct LpRow {
                 if (n[u] >= full) continue;
                 float x[E::kVec];
                 E::wide(raw[u], x);
+                float most = x[0];
 #pragma unroll
-                for (int k = 0; k < E::kVec; ++k) f(x[k], n[u] * E::kVec + k);
+                for (int k = 1; k < E::kVec; ++k) most = fmaxf(most, x[k]);
+                if (most >= least)
+#pragma unroll
+                    for (int k = 0; k < E::kVec; ++k) f(x[k], n[u] * E::kVec + k);
             }
         }
-        const uint32_t i = full * E::kVec + threadIdx.x;
-        if (i < V) f(E::one(row[i]), i);
+        tail(f);
+    }
+    // ... for the whole row
+    template <typename F> __device__ __forceinline__ void all(F f) const
+    {
+        for (uint32_t n = threadIdx.x; n < full; n += kLpThreads) {
+            float x[E::kVec];
+            E::wide(load_window<DT>(row, n), x);
+#pragma unroll
+            for (int k = 0; k < E::kVec; ++k) f(x[k], n * E::kVec + k);
+        }
+        tail(f);
     }
 };
 
 // A t with at least `k` and, unless keys are equal, at most k + spare of the workgroup's keys >= t; only the upper BITS bits matter.
+// No key is larger than `most`.
 template <int BITS, typename K>
-__device__ __forceinline__ K lp_kth(const K *key, uint32_t k, uint32_t spare)
+__device__ __forceinline__ K lp_kth(const K *key, uint32_t k, uint32_t spare, K most)
 {
     constexpr int kAll = (int)sizeof(K) * 8;
     K mine[kLpWaves];
@@ -298,6 +326,7 @@ __device__ __forceinline__ K lp_kth(const K *key, uint32_t k, uint32_t spare)
     K t = 0;
     for (int bit = kAll - 1; bit >= kAll - BITS; --bit) {
         const K c = t | (K)1 << bit;
+        if (c > most) continue;
         uint32_t n = 0;
 #pragma unroll
         for (int i = 0; i < kLpWaves; ++i) n += (uint32_t)__popcll(__ballot(mine[i] >= c));
@@ -307,48 +336,53 @@ __device__ __forceinline__ K lp_kth(const K *key, uint32_t k, uint32_t spare)
     return t;
 }
 
-template <int DT>
-__device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float largest, const LpSums &a, float log_s, float inv_t, uint32_t top,
-                                                float *out_logprobs, int32_t *out_tokens, LpShared &sh)
+// seg[s] is the thread's largest logit of stretch s of the row, `largest` the largest of those.
+template <int DT, int N>
+__device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float largest, const float (&seg)[N], const LpSums &a, float log_s, float inv_t,
+                                                uint32_t top, float *out_logprobs, int32_t *out_tokens, LpShared &sh)
 {
     const uint32_t tid = threadIdx.x, lane = tid % kWave, w = tid / kWave;
     sh.key[tid] = lp_key(largest);
-    if (tid == 0) sh.n = 0;
+    if (tid == 0) sh.n = sh.n_units = 0;
     __syncthreads();
-    uint32_t tau = lp_kth<Elem<DT>::kBits>(sh.key, top, top / 4u);
+    uint32_t tau = lp_kth<Elem<DT>::kBits>(sh.key, top, top / 4u, uniform(lp_key(a.m)));
     if (tau <= fkey(-__builtin_inff())) tau = 1u;        // fewer numbers than are wanted, perhaps: NaN too
-    uint32_t n_hot = 0;
+    const float least = fkey_inv(tau);
+    if (tau != 1u) {
 #pragma unroll
-    for (int i = 0; i < kLpWaves; ++i) {
-        const uint64_t is = __ballot(sh.key[i * kWave + lane] >= tau);
-        if (i == (int)w && ((is >> lane) & 1)) sh.hot[n_hot + __popcll(is & ((1ull << lane) - 1))] = (uint16_t)tid;
-        n_hot += (uint32_t)__popcll(is);
+        for (int i = 0; i < N; ++i)
+            if (seg[i] >= least) {
+                const uint32_t at = atomicAdd(&sh.n_units, 1u);
+                if (at < kLpUnits) sh.unit[at] = (uint32_t)i << 8 | tid;
+            }
+        __syncthreads();
     }
-    __syncthreads();
-    row.each(sh, n_hot, [&](float x, uint32_t i) {
-        if (lp_key(x) >= tau) {
-            const uint32_t at = atomicAdd(&sh.n, 1u);
-            if (at < kLpCap) sh.cand[at] = lp_token(x, i);
-        }
-    });
+    auto list = [&](uint64_t from) {
+        return [&sh, from](float x, uint32_t i) {
+            const uint64_t k = lp_token(x, i);
+            if (k >= from) {
+                const uint32_t at = atomicAdd(&sh.n, 1u);
+                if (at < kLpCap) sh.cand[at] = k;
+            }
+        };
+    };
+    const uint64_t from = (uint64_t)tau << 32;
+    const uint32_t n_units = sh.n_units;
+    if (tau != 1u && n_units <= kLpUnits) row.units(sh, n_units, least, list(from));
+    else row.all(list(from));
     __syncthreads();
     if (sh.n > kLpCap) {
         uint64_t best = 0;
-        row.each(sh, n_hot, [&](float x, uint32_t i) { best = max(best, lp_token(x, i)); });
+        row.all([&](float x, uint32_t i) { best = max(best, lp_token(x, i)); });
+        __syncthreads();                                 // (the stretches' room is used again)
         sh.lane_top[tid] = best;
         __syncthreads();
-        uint64_t lo = max(lp_kth<64>(sh.lane_top, top, 0u), (uint64_t)tau << 32), hi = ~0ull;
+        uint64_t lo = max(lp_kth<64>(sh.lane_top, top, 0u, (uint64_t)~0ull), from), hi = ~0ull;
         for (uint64_t t = lo;; t = lo + (hi - lo) / 2) {
             __syncthreads();
             if (tid == 0) sh.n = 0;
             __syncthreads();
-            row.each(sh, n_hot, [&](float x, uint32_t i) {
-                const uint64_t k = lp_token(x, i);
-                if (k >= t) {
-                    const uint32_t at = atomicAdd(&sh.n, 1u);
-                    if (at < kLpCap) sh.cand[at] = k;
-                }
-            });
+            row.all(list(t));
             __syncthreads();
             if (sh.n > kLpCap) lo = t;
             else if (sh.n < top) hi = t;
@@ -380,20 +414,24 @@ __device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float larg
 }
 
 // ------------------------------------------------------------------- forward --
-// U windows of each thread are in flight at a time.
-template <int DT, int U, bool GUARD>
-__device__ __forceinline__ void lp_batch(const typename Elem<DT>::T *row, uint32_t n0, uint32_t full, uint32_t token_window, float before, float after,
-                                         float c, LpSums &a, uint32_t &above)
+// U windows of each thread, whole ones below `full` only.  A batch is asked for before the one before it is worked on.
+template <int DT, int U>
+__device__ __forceinline__ void lp_ask(const typename Elem<DT>::T *row, uint32_t n0, uint32_t full, uint4 (&raw)[U])
 {
-    using E = Elem<DT>;
-    constexpr float kNone = -__builtin_inff();
-    float x[U * E::kVec], edge[U];
-    uint4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint32_t n = n0 + u * kLpThreads;
-        if (!GUARD || n < full) raw[u] = load_window<DT>(row, n);
+        if (n < full) raw[u] = load_window<DT>(row, n);
     }
+}
+
+// Returns the largest logit of the batch.  GUARD: lanes whose window is not below `full` have none.
+template <int DT, int U, bool GUARD>
+__device__ __forceinline__ float lp_batch(const uint4 *raw, uint32_t n0, uint32_t full, uint32_t token_window, float before, float after,
+                                          float c, LpSums &a, uint32_t &above)
+{
+    using E = Elem<DT>;
+    float x[U * E::kVec], edge[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint32_t n = n0 + u * kLpThreads;
@@ -402,11 +440,18 @@ __device__ __forceinline__ void lp_batch(const typename Elem<DT>::T *row, uint32
         edge[u] = n < token_window ? before : after;
         if (GUARD && n >= full) edge[u] = __builtin_nanf("");
 #pragma unroll
-        for (int i = 0; i < E::kVec; ++i) x[u * E::kVec + i] = GUARD && n >= full ? kNone : v[i];
+        for (int i = 0; i < E::kVec; ++i) x[u * E::kVec + i] = GUARD && n >= full ? -__builtin_inff() : v[i];
     }
-    lp_take(a, x, c);
+    const float top = lp_take(a, x, c);
 #pragma unroll
     for (int i = 0; i < U * E::kVec; ++i) above += (uint32_t)__popcll(__ballot(x[i] >= edge[i / E::kVec]));
+    return top;
+}
+
+__device__ __forceinline__ float lp_stretch(const LpSlice *slices, uint32_t segs, uint32_t s, uint32_t tid)
+{
+    const uint32_t slice = s / segs;
+    return a_load(&slices[slice].seg[s - slice * segs][tid]);
 }
 
 // One workgroup per row, or S of them (SPLIT), each on a stretch of the row, of which the last to arrive finishes the row.
@@ -421,40 +466,70 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
     const uint32_t b = r / (uint32_t)p.T, pos = r - b * (uint32_t)p.T;
     const uint32_t V = (uint32_t)p.V, full = V / E::kVec, tid = threadIdx.x;
     const typename E::T *row = (const typename E::T *)p.logits + (int64_t)b * p.stride_b + (int64_t)pos * p.stride_t;
+    const uint32_t first = slice * p.J * kLpThreads, end = min(full, first + p.J * kLpThreads);
+    uint4 raw[U];
+    lp_ask<DT, U>(row, first + tid, end, raw);
+    const uint32_t last = full * E::kVec + tid;          // the row's last few logits
+    const bool has_last = (!SPLIT || slice == p.S - 1u) && last < V;
+    const float x_last = has_last ? E::one(row[last]) : -__builtin_inff();
     const int64_t at = (int64_t)b * p.token_b + (int64_t)pos * p.token_t;
     const int64_t token = p.tokens_64 ? ((const int64_t *)p.tokens)[at] : (int64_t)((const int32_t *)p.tokens)[at];
     const bool given = token >= 0 && token < (int64_t)V;
     const uint32_t tok = given ? (uint32_t)token : 0u;
     const float x_t = E::one(row[tok]);
-    // a window before the token's counts x >= x_t, one behind it x > x_t, that is x >= the next number up; in the token's own
-    // window the equal ones before it are counted at the end.  Below -inf there is nothing but NaN.
+    const uint32_t token_window = tok / E::kVec, beside = token_window * E::kVec + tid;
+    const bool is_beside = tid < (uint32_t)E::kVec && beside < tok && token_window >= first && token_window < end;
+    const float x_beside = is_beside ? E::one(row[beside]) : __builtin_nanf("");
+    // a window before the token's counts x >= x_t, one behind it x > x_t, that is x >= the next number up; the token's own
+    // window counts the latter, and the equal ones before the token are added.  Below -inf there is nothing but NaN.
     float before = x_t, after;
     {
         const uint32_t bits = __float_as_uint(x_t + 0.0f);
         after = __uint_as_float(bits & 0x80000000u ? bits - 1u : bits + 1u);
         if (x_t != x_t) before = after = -__builtin_inff();
     }
-    const uint32_t token_window = tok / E::kVec;
 
     LpSums a{-__builtin_inff(), 0.0f, 0.0f};
-    uint32_t above = 0;
-    const uint32_t first = slice * p.J * kLpThreads, end = min(full, first + p.J * kLpThreads);
-    uint32_t n = first;
-    for (; n + U * kLpThreads <= end; n += U * kLpThreads) lp_batch<DT, U, false>(row, n + tid, end, token_window, before, after, p.c, a, above);
-    for (; n < end; n += kLpThreads) lp_batch<DT, 1, true>(row, n + tid, end, token_window, before, after, p.c, a, above);
+    uint32_t above = 0, n = first;
+    float seg = -__builtin_inff();
+    for (; n + U * kLpThreads <= end; ) {
+        uint4 now[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) now[u] = raw[u];
+        lp_ask<DT, U>(row, n + U * kLpThreads + tid, end, raw);
+        seg = fmaxf(seg, lp_batch<DT, U, false>(now, n + tid, end, token_window, before, after, p.c, a, above));
+        n += U * kLpThreads;
+        const uint32_t j = (n - first) / kLpThreads;
+        if (!(j & ((1u << p.seg_log) - 1u))) {
+            if (p.top) sh.seg[(j >> p.seg_log) - 1u][tid] = seg;
+            seg = -__builtin_inff();
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (n + u * kLpThreads < end) seg = fmaxf(seg, lp_batch<DT, 1, true>(raw + u, n + u * kLpThreads + tid, end, token_window, before, after, p.c, a, above));
+    const uint32_t segs = (p.J + (1u << p.seg_log) - 1u) >> p.seg_log;
+    if (p.top) {
+        // the stretch that the slice ends in, and those behind it
+        for (uint32_t g = end > first ? (end - first) / kLpThreads >> p.seg_log : 0u; g < segs; ++g) {
+            sh.seg[g][tid] = seg;
+            seg = -__builtin_inff();
+        }
+    }
     const float largest = a.m;
     if (!SPLIT || slice == p.S - 1u) {
-        const uint32_t i = full * E::kVec + tid;
-        const float x[1] = {i < V ? E::one(row[i]) : -__builtin_inff()};
+        const float x[1] = {x_last};
         lp_take(a, x, p.c);
-        above += (uint32_t)__popcll(__ballot(x[0] >= (i < V ? (i < tok ? before : after) : __builtin_nanf(""))));
+        above += (uint32_t)__popcll(__ballot(x_last >= (has_last ? (last < tok ? before : after) : __builtin_nanf(""))));
     }
+    above += (uint32_t)__popcll(__ballot(x_beside == x_t));
     lp_block(a, above, p.c, sh);
 
     float mine = largest;
+    float seg_of[SPLIT ? kLpStretches : kLpSegs];
     if constexpr (SPLIT) {
         LpSlice *slices = p.slices + (size_t)r * p.S;
-        if (p.top) a_store(&slices[slice].top[tid], largest);
+        if (p.top) for (uint32_t g = 0; g < segs; ++g) a_store(&slices[slice].seg[g][tid], sh.seg[g][tid]);
         if (tid == 0) {
             a_store(&slices[slice].m, a.m); a_store(&slices[slice].s, a.s); a_store(&slices[slice].t, a.t);
             a_store(&slices[slice].above, above);
@@ -475,15 +550,12 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
             a = LpSums{a_load(&slices[lane].m), a_load(&slices[lane].s), a_load(&slices[lane].t)};
             above = a_load(&slices[lane].above);
         }
+        // (all under way at once: what other workgroups have written comes from far)
         if (p.top) {
-            constexpr uint32_t B = 8;
-            for (uint32_t s = 0; s < p.S; s += B) {
-                float more[B];
 #pragma unroll
-                for (uint32_t u = 0; u < B; ++u) more[u] = a_load(&slices[min(s + u, p.S - 1u)].top[tid]);
+            for (int s = 0; s < kLpStretches; ++s) seg_of[s] = s < (int)(p.S * segs) ? lp_stretch(slices, segs, s, tid) : -__builtin_inff();
 #pragma unroll
-                for (uint32_t u = 0; u < B; ++u) mine = fmaxf(mine, more[u]);
-            }
+            for (int s = 0; s < kLpStretches; ++s) mine = fmaxf(mine, seg_of[s]);
         }
         lp_wave(a, p.c);
         above = wave_sum(above);
@@ -492,10 +564,6 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
     const float log_s = logf(a.s);
     const bool empty = a.s == 0.0f;                     // nothing but -inf
     if (tid < kWave) {
-        // equal logits before the token in its own window
-        const uint32_t i = token_window * E::kVec + tid;
-        const bool eq = tid < (uint32_t)E::kVec && i < tok && i < full * E::kVec && E::one(row[i]) == x_t;
-        above += (uint32_t)__popcll(__ballot(eq));
         if (x_t != x_t)                                 // NaN: behind every number, among its like by the index
             for (uint32_t j = tid; j < ((tok + kWave - 1u) & ~(kWave - 1u)); j += kWave) {
                 const float x = j < tok ? E::one(row[j]) : 0.0f;
@@ -512,8 +580,13 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
         }
     }
     if (p.top) {
-        const LpRow<DT> all{row, V, full, p.J_row, p.step};
-        lp_alternatives<DT>(all, mine, a, log_s, p.inv_t, (uint32_t)p.top, p.top_logprobs + (size_t)r * p.top, p.top_tokens + (size_t)r * p.top, sh);
+        const LpRow<DT> whole{row, V, full, p.J, p.seg_log, segs};
+        float *const lps = p.top_logprobs + (size_t)r * p.top;
+        int32_t *const ids = p.top_tokens + (size_t)r * p.top;
+        if constexpr (!SPLIT)
+#pragma unroll
+            for (int s = 0; s < kLpSegs; ++s) seg_of[s] = s < (int)segs ? sh.seg[s][tid] : -__builtin_inff();
+        lp_alternatives<DT>(whole, mine, seg_of, a, log_s, p.inv_t, (uint32_t)p.top, lps, ids, sh);
     }
 }
 

@@ -6,13 +6,15 @@
 
 namespace rs {
 
-constexpr uint32_t kLpSplitMost = 1024;   // workgroups of a call whose rows are split: four to a compute unit
+constexpr uint32_t kLpSplitMost = 512;   // workgroups of a call whose rows are split
 
-// Workgroups per row: one, or enough for about four to a compute unit, each with at least four windows per thread.
+// Workgroups per row: one, or enough for about two to a compute unit, each with at least four windows per thread.  (With four to a
+// compute unit 64 rows of 152064 bfloat16 logits and 20 alternatives take 18.5 us in the place of 17.0, 385 of 50257 23.1 in the
+// place of 19.6, with one 16.8 and 19.6, but 48 of 32768 float32 are as fast either way.)
 static uint32_t lp_split(uint32_t rows, uint32_t windows)
 {
     const uint32_t most = kLpSplitMost / rows, per = (windows + 4u * kLpThreads - 1u) / (4u * kLpThreads);
-    return std::max(1u, std::min(std::min(most, per), (uint32_t)kWave));
+    return std::max(1u, std::min(std::min(most, per), (uint32_t)kLpStretches));
 }
 
 static int lp_check(const void *logits, int32_t dtype, const void *tokens, int32_t tokens_64, int64_t B, int64_t T, int64_t V, double temperature, int32_t top)
@@ -63,10 +65,13 @@ int rs_token_logprobs(const void *logits, int32_t dtype, int64_t stride_b, int64
     p.c = (float)(1.4426950408889634 / temperature); p.inv_t = (float)(1.0 / temperature);
     p.logprobs = logprobs; p.entropy = entropy; p.rank = rank; p.top_logprobs = top_logprobs; p.top_tokens = top_tokens;
     p.stats = (float4 *)stats;
-    p.S = lp_split(rows, windows);
-    p.J = (windows + p.S * kLpThreads - 1) / (p.S * kLpThreads);
-    p.J_row = (windows + kLpThreads - 1) / kLpThreads;
-    p.step = p.J_row ? 0xFFFFFFFFu / p.J_row + 1u : 0u;
+    // (a thread's windows are worked on four at a time)
+    const uint32_t per_row = (windows + kLpThreads - 1) / kLpThreads, split = lp_split(rows, windows);
+    p.J = split > 1 ? ((per_row + split - 1) / split + 3) / 4 * 4 : per_row;
+    p.S = split > 1 ? (per_row + p.J - 1) / p.J : 1;
+    // stretches of four windows and more, at most kLpSegs of them in a slice and kLpStretches in a row
+    const uint32_t most = p.S > 1 ? std::min((uint32_t)kLpSegs, (uint32_t)kLpStretches / p.S) : (uint32_t)kLpSegs;
+    for (p.seg_log = 2; p.J > most << p.seg_log; ) ++p.seg_log;
     p.arrived = (uint32_t *)workspace;
     p.slices = (LpSlice *)((char *)workspace + 16 * (size_t)kLpSplitMost);
     const hipStream_t st = (hipStream_t)stream;
