@@ -531,12 +531,22 @@ int rs_quantize_blocks(const void *x_device, int32_t x_dtype, int64_t x_row_stri
  * y = x w^T for such values: x (M, K) with scales of 1 x 128 (M, ceil(K / 128)), w
  * (N, K) with scales of 128 x 128 (ceil(N / 128), ceil(K / 128)), both scales
  * contiguous, y (M, N) float32, bfloat16 or float16 (RS_DTYPE_*).  Rows of x and w
- * 16-byte aligned; bytes behind column K are not looked at.  Sums in float32, one
- * rounding.  No counterpart in the reference.
+ * 16-byte aligned; bytes behind column K are not looked at.  One rounding of the
+ * sums, which are held in float32; outputs of 16 bits from more than 64 rows are
+ * made with the matrix cores' 8-bit instructions, which drop of eight products
+ * that are added at once what lies 14 binades and more under the largest (3e-5
+ * of a result's size, a tenth of those types' own rounding and less).  The sums
+ * do not depend on chance.
+ * workspace: rs_linear_workspace_bytes() bytes of device memory, 256-byte aligned,
+ * cleared once with rs_workspace_init and not shared with other entry points;
+ * calls that share it are ordered on one stream.  One launch.  No counterpart in
+ * the reference.
  */
+size_t rs_linear_workspace_bytes(void);
 int rs_linear_blocks(const void *x_device, int64_t x_row_stride, const float *x_scale_device,
                      const void *w_device, int64_t w_row_stride, const float *w_scale_device,
-                     int32_t M, int32_t N, int32_t K, void *y_device, int32_t y_dtype, int64_t y_row_stride, void *stream);
+                     int32_t M, int32_t N, int32_t K, void *y_device, int32_t y_dtype, int64_t y_row_stride,
+                     void *workspace_device, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -37,6 +37,9 @@ struct LinearParams {
     const float   *x_scale, *w_scale;
     void          *y;
     uint32_t       M, N, K, blocks;
+    uint32_t       split;                // workgroups that share a tile's blocks of columns
+    float         *parts;                // ... their sums, and how many have left theirs, per tile; zero between calls
+    uint32_t      *arrived;
 };
 
 template <int DT> __device__ __forceinline__ float widen(const void *p, int64_t i)
@@ -158,27 +161,32 @@ __device__ __forceinline__ v4f block_product_8(v8i w, v8i x)
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
 }
 
+// Four consecutive values, or eight of 16 bits, in one store.  y's rows begin at any multiple of a value's size (an odd number of
+// columns): the hardware stores at any address, 77 x 50257 x 2000 into bfloat16 took 45 us in single values.
 template <int DT> __device__ __forceinline__ void put_four(void *p, int64_t i, v4f a)
 {
-    if constexpr (DT == RS_DTYPE_F32) *(v4f *)((float *)p + i) = a;
-    else if constexpr (DT == RS_DTYPE_BF16) *(v4bf *)((__bf16 *)p + i) = v4bf{(__bf16)a[0], (__bf16)a[1], (__bf16)a[2], (__bf16)a[3]};
-    else *(v4h *)((_Float16 *)p + i) = v4h{(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3]};
+    if constexpr (DT == RS_DTYPE_F32) __builtin_memcpy((float *)p + i, &a, 16);
+    else if constexpr (DT == RS_DTYPE_BF16) {
+        const v4bf v = {(__bf16)a[0], (__bf16)a[1], (__bf16)a[2], (__bf16)a[3]};
+        __builtin_memcpy((__bf16 *)p + i, &v, 8);
+    } else {
+        const v4h v = {(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3]};
+        __builtin_memcpy((_Float16 *)p + i, &v, 8);
+    }
 }
-
-// Four consecutive float32 values, or eight of 16 bits, in one store.
 template <int DT> __device__ __forceinline__ void put_wide(void *p, int64_t i, v4f a, v4f b)
 {
-    if constexpr (DT == RS_DTYPE_F32) *(v4f *)((float *)p + i) = a;
+    if constexpr (DT == RS_DTYPE_F32) put_four<DT>(p, i, a);
     else if constexpr (DT == RS_DTYPE_BF16) {
         v8bf v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) { v[j] = (__bf16)a[j]; v[j + 4] = (__bf16)b[j]; }
-        *(v8bf *)((__bf16 *)p + i) = v;
+        __builtin_memcpy((__bf16 *)p + i, &v, 16);
     } else {
         v8h v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) { v[j] = (_Float16)a[j]; v[j + 4] = (_Float16)b[j]; }
-        *(v8h *)((_Float16 *)p + i) = v;
+        __builtin_memcpy((_Float16 *)p + i, &v, 16);
     }
 }
 
@@ -264,17 +272,18 @@ __global__ __launch_bounds__(512) void linear_few_kernel(LinearParams p)
 #pragma unroll
         for (int t = 0; t < MT; ++t) acc[u][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (wave < p.blocks) {
+        // (every workgroup begins at another block: see the kernel for many rows)
+        const uint32_t turn = blockIdx.x % p.blocks;
+        auto turned = [&](uint32_t kb) { kb += turn; return kb < p.blocks ? kb : kb - p.blocks; };
         typename L::Block now, next;
-        rows.load(p, wave, now);
-        uint32_t kb = wave + waves;
-        for (; kb < p.blocks; kb += waves) {
-            rows.load(p, kb, next);
+        rows.load(p, turned(wave), now);
+        for (uint32_t j = wave + waves; j < p.blocks; j += waves) {
+            rows.load(p, turned(j), next);
             L::multiply(now, acc);
             now = next;
         }
         L::multiply(now, acc);
     }
-    const bool aligned = !(p.y_stride % 4) && !((uintptr_t)p.y & 15);
 #pragma unroll
     for (int r = 0; r < kTiles; r += kRound) {
         if (r) __syncthreads();
@@ -288,7 +297,7 @@ __global__ __launch_bounds__(512) void linear_few_kernel(LinearParams p)
             const uint32_t m = m0 + t * 16u + i, n = n0 + u * 16u + part * 4u;
             if (m >= p.M) continue;
             const int64_t at = (int64_t)m * p.y_stride + n;
-            if (aligned && n + 4u <= p.N) put_four<DT>(p.y, at, s);
+            if (n + 4u <= p.N) put_four<DT>(p.y, at, s);
             else
 #pragma unroll
                 for (int j = 0; j < 4; ++j) if (n + j < p.N) put<DT>(p.y, at + j, s[j]);
@@ -297,20 +306,20 @@ __global__ __launch_bounds__(512) void linear_few_kernel(LinearParams p)
 }
 
 // -------------------------------------------------------------- many rows --
-// A workgroup of WN x WM waves makes 128 WN rows of w x 16 MT WM rows of x, a wave 128 x 16 MT of it.  Every block has to be
-// scaled in the vector unit before it is added (four sums a lane and 16 x 16 product), so a wave's sums sit in 32 MT ordinary
+// A workgroup of WN x WM waves makes 16 NU WN rows of w x 16 MT WM rows of x, a wave 16 NU x 16 MT of it.  Every block has to be
+// scaled in the vector unit before it is added (four sums a lane and 16 x 16 product), so a wave's sums sit in 4 NU MT ordinary
 // registers; a product's sums are added while the matrix cores make the next.
 //
 // A block of 128 columns is one stage: rows of 128 bytes go from memory to LDS without passing through registers, up to
 // STAGES - 1 blocks ahead of the one that is multiplied.  The eight 16-byte pieces of a row are stored in an order that depends on
 // the row (place = piece ^ turn(row)), so that the eight rows read at once lie in different banks.  The first operand's rows are
-// dealt so that a lane's sums are 32 consecutive columns of y.
+// dealt so that a lane's sums are 4 NU consecutive columns of y.
 typedef __attribute__((address_space(1))) const void *GlobalPtr;
 typedef __attribute__((address_space(3))) void *LdsPtr;
 
 constexpr int64_t kTileStride = (1ll << 32) / 256 - kFpBlock;   // a tile's rows are reached with 32 bits
 
-__device__ __forceinline__ uint32_t w_turn(uint32_t row) { return (row & 3u) | ((row >> 3) & 4u); }
+template <int NU> __device__ __forceinline__ uint32_t w_turn(uint32_t row) { return (row & 3u) | ((row / NU) & 4u); }
 __device__ __forceinline__ uint32_t x_turn(uint32_t row) { return row & 7u; }
 
 __device__ __forceinline__ uint32_t wave_id() { return uniform(threadIdx.x / 64u); }
@@ -321,13 +330,14 @@ template <int N> __device__ __forceinline__ void stage_barrier()
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
 }
 
-template <int WN, int WM, int MT, int STAGES, bool EXACT>
+template <int WN, int WM, int NU, int MT, int STAGES, bool EXACT>
 struct LinearTile {
-    static constexpr uint32_t kWaves = WN * WM, kThreads = 64 * kWaves, kTileN = 128 * WN, kTileM = 16 * MT * WM;
+    static constexpr uint32_t kWaves = WN * WM, kThreads = 64 * kWaves, kTileN = 16 * NU * WN, kTileM = 16 * MT * WM;
     static constexpr uint32_t kRows = kTileN + kTileM, kStage = kRows * kFpBlock, kLds = STAGES * kStage;
     static constexpr uint32_t kLoads = kRows * 8 / kThreads, kLoadsW = kTileN * 8 / kThreads;    // 16-byte pieces of a stage per thread
     static_assert(kRows * 8 % kThreads == 0 && kTileN * 8 % kThreads == 0 && kTileN <= 256 && kTileM <= 256, "whole loads; 32-bit offsets");
     static_assert(kWaves % 4 == 0, "w_turn is the same for every load of a thread, or for every other one");
+    static_assert(NU == 4 || NU == 8, "");
 
     // A wave fills eight rows of a stage with one load: the thread's row of load i, w's rows first.
     static __device__ __forceinline__ uint32_t row_of(uint32_t i) { return (i * kWaves + wave_id()) * 8u + threadIdx.x % 64u / 8u; }
@@ -345,10 +355,11 @@ struct LinearTile {
         s.w_stride = (uint32_t)p.w_stride;
         s.x_stride = (uint32_t)p.x_stride;
         const uint32_t rows_w = min(p.N - n0, kTileN), rows_x = min(p.M - m0, kTileM);
-        s.w = __builtin_amdgcn_make_buffer_rsrc((void *)(p.w + (int64_t)n0 * p.w_stride), 0, (int)((rows_w - 1u) * s.w_stride + p.K), kFlags);
-        s.x = __builtin_amdgcn_make_buffer_rsrc((void *)(p.x + (int64_t)m0 * p.x_stride), 0, (int)((rows_x - 1u) * s.x_stride + p.K), kFlags);
+        const uint32_t bytes = (p.K + 3u) & ~3u;       // of the last row, in whole words: a word is read or it is not
+        s.w = __builtin_amdgcn_make_buffer_rsrc((void *)(p.w + (int64_t)n0 * p.w_stride), 0, (int)((rows_w - 1u) * s.w_stride + bytes), kFlags);
+        s.x = __builtin_amdgcn_make_buffer_rsrc((void *)(p.x + (int64_t)m0 * p.x_stride), 0, (int)((rows_x - 1u) * s.x_stride + bytes), kFlags);
         const uint32_t r = row_of(0);
-        for (uint32_t i = 0; i < 2; ++i) s.w_at[i] = r * s.w_stride + ((threadIdx.x & 7u) ^ w_turn(r + i * 8u * kWaves)) * 16u;
+        for (uint32_t i = 0; i < 2; ++i) s.w_at[i] = r * s.w_stride + ((threadIdx.x & 7u) ^ w_turn<NU>(r + i * 8u * kWaves)) * 16u;
         s.x_at = r * s.x_stride + ((threadIdx.x & 7u) ^ x_turn(r)) * 16u;
         return s;
     }
@@ -364,14 +375,27 @@ struct LinearTile {
             }
             return;
         }
-        // the last block where K is no whole number of them
+        // the last block where K is no whole number of them: through registers, with the bytes from K on cleared
+        constexpr uint32_t kAtOnce = MT > 2 ? 2 : kLoads;
+        static_assert(kLoads % kAtOnce == 0, "");
 #pragma unroll 1
-        for (uint32_t i = 0; i < kLoads; ++i) {
-            const bool is_w = i < kLoadsW;
-            const uint32_t r = row_of(i) - (is_w ? 0u : kTileN);
-            const uint32_t piece = (threadIdx.x & 7u) ^ (is_w ? w_turn(r) : x_turn(r));
-            const uint8_t *from = is_w ? p.w + (int64_t)min(n0 + r, p.N - 1u) * p.w_stride : p.x + (int64_t)min(m0 + r, p.M - 1u) * p.x_stride;
-            *(v4i *)(lds + row_of(i) * kFpBlock + (threadIdx.x & 7u) * 16u) = load16(from, k + piece * 16u, p.K);
+        for (uint32_t i0 = 0; i0 < kLoads; i0 += kAtOnce) {
+            v4i v[kAtOnce];
+#pragma unroll
+            for (uint32_t o = 0; o < kAtOnce; ++o) {
+                const uint32_t i = i0 + o;
+                if (i < kLoadsW) v[o] = __builtin_amdgcn_raw_buffer_load_b128(s.w, kWaves % 8 && i % 2 ? s.w_at[1] : s.w_at[0], k + i * 8u * kWaves * s.w_stride, 0);
+                else v[o] = __builtin_amdgcn_raw_buffer_load_b128(s.x, s.x_at, k + (i - kLoadsW) * 8u * kWaves * s.x_stride, 0);
+            }
+#pragma unroll
+            for (uint32_t o = 0; o < kAtOnce; ++o) {
+                const uint32_t i = i0 + o;
+                const uint32_t r = row_of(i) - (i < kLoadsW ? 0u : kTileN);
+                const int32_t left = (int32_t)(p.K - k) - (int32_t)(((threadIdx.x & 7u) ^ (i < kLoadsW ? w_turn<NU>(r) : x_turn(r))) * 16u);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) v[o][d] &= left >= 4 * d + 4 ? -1 : left <= 4 * d ? 0 : (1 << 8 * (left - 4 * d)) - 1;
+                *(v4i *)(lds + row_of(i) * kFpBlock + (threadIdx.x & 7u) * 16u) = v[o];
+            }
         }
         wait_vmem();
     }
@@ -383,12 +407,15 @@ struct LinearTile {
     }
 
     // Asks for block `next` and multiplies the one in now_lds.
-    static __device__ __forceinline__ void step(const LinearParams &p, const Source &source, uint32_t n0, uint32_t m0, uint32_t next,
-                                                const uint8_t *__restrict now_lds, uint8_t *__restrict next_lds, const float (&f)[MT], v4f (&acc)[8][MT])
+    static __device__ __forceinline__ void step(const LinearParams &p, const Source &source, uint32_t n0, uint32_t m0, uint32_t next, bool more,
+                                                const uint8_t *__restrict now_lds, uint8_t *__restrict next_lds, const float (&f)[MT], v4f (&acc)[NU][MT])
     {
-        if (next < p.blocks) fill(p, source, n0, m0, next, next_lds);
+        // (where one workgroup has the compute unit to itself, after the first products are under way: all its waves leave the barrier
+        // together, and 8192^3 takes 536 us in the place of 567; of two workgroups one works while the other asks)
+        constexpr int kAskAt = kWaves == 8 ? 1 : -1;
+        if (kAskAt < 0 && more) fill(p, source, n0, m0, next, next_lds);
         const uint32_t wave = wave_id(), lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
-        const uint32_t wn = wave % WN * 128u, wm = wave / WN * (16u * MT);
+        const uint32_t wn = wave % WN * (16u * NU), wm = wave / WN * (16u * MT);
         v8i x[MT];
         v8bf xb[EXACT ? MT : 1][4];
 #pragma unroll
@@ -397,15 +424,16 @@ struct LinearTile {
             x[t] = fragment(now_lds + kTileN * kFpBlock, r, x_turn(r), part);
             if constexpr (EXACT) widen_block(x[t], xb[t]);
         }
-        const uint32_t r0 = wn + i / 4u * 32u + i % 4u;
-        v8i w = fragment(now_lds, r0, w_turn(r0), part);
+        const uint32_t r0 = wn + i / 4u * (4u * NU) + i % 4u;
+        v8i w = fragment(now_lds, r0, w_turn<NU>(r0), part);
         v4f s[MT];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
+        for (int u = 0; u < NU; ++u) {
+            if (u == kAskAt && more) fill(p, source, n0, m0, next, next_lds);
             v8i ahead = w;
-            if (u < 7) {
+            if (u < NU - 1) {
                 const uint32_t r = r0 + (u + 1) * 4u;
-                ahead = fragment(now_lds, r, w_turn(r), part);
+                ahead = fragment(now_lds, r, w_turn<NU>(r), part);
             }
             v4f made[MT];
             v8bf wb[4];
@@ -427,63 +455,112 @@ struct LinearTile {
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[7][t][j] = __builtin_fmaf(s[t][j], f[t], acc[7][t][j]);
+            for (int j = 0; j < 4; ++j) acc[NU - 1][t][j] = __builtin_fmaf(s[t][j], f[t], acc[NU - 1][t][j]);
     }
 };
 
-template <int DT, int WN, int WM, int MT, int STAGES, bool EXACT>
+template <int DT, int WN, int WM, int NU, int MT, int STAGES, bool EXACT>
 __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearParams p)
 {
-    using L = LinearTile<WN, WM, MT, STAGES, EXACT>;
+    using L = LinearTile<WN, WM, NU, MT, STAGES, EXACT>;
     extern __shared__ uint8_t lds[];
+    const uint32_t tm = (p.M + L::kTileM - 1u) / L::kTileM, tn = (p.N + L::kTileN - 1u) / L::kTileN, tiles = tm * tn;
     // Workgroup b runs on XCD b % 8: each XCD takes a stretch of the tiles, in panels of eight rows of tiles, so that the 32 tiles
     // it works on at a time share their rows in its L2.
-    const uint32_t tm = (p.M + L::kTileM - 1u) / L::kTileM, tn = (p.N + L::kTileN - 1u) / L::kTileN, tiles = tm * tn;
-    const uint32_t each = tiles / 8u, rest = tiles % 8u, xcd = blockIdx.x % 8u;
-    const uint32_t id = xcd * each + min(xcd, rest) + blockIdx.x / 8u;
+    uint32_t id = blockIdx.x, part_of = 0;
+    if (p.split > 1u) { part_of = id / tiles; id -= part_of * tiles; }
+    else {
+        const uint32_t each = tiles / 8u, rest = tiles % 8u, xcd = id % 8u;
+        id = xcd * each + min(xcd, rest) + id / 8u;
+    }
     const uint32_t panel = id / (8u * tn), high = min(8u, tm - panel * 8u), in = id - panel * 8u * tn;
-    const uint32_t m0 = (panel * 8u + in % high) * L::kTileM, n0 = in / high * L::kTileN;
+    const uint32_t tile_n = in / high, m0 = (panel * 8u + in % high) * L::kTileM, n0 = tile_n * L::kTileN;
+    const uint32_t kb0 = p.blocks * part_of / p.split, count = p.blocks * (part_of + 1u) / p.split - kb0;
 
     const uint32_t wave = wave_id(), lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
-    const uint32_t wn = wave % WN * 128u, wm = wave / WN * (16u * MT);
+    const uint32_t wn = wave % WN * (16u * NU), wm = wave / WN * (16u * MT);
     const float *sw = p.w_scale + (size_t)min((n0 + wn) / kFpBlock, (p.N - 1u) / kFpBlock) * p.blocks;
     const float *sx[MT];
-    v4f acc[8][MT];
+    v4f acc[NU][MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         sx[t] = p.x_scale + (size_t)min(m0 + wm + t * 16u + i, p.M - 1u) * p.blocks;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) acc[u][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = 0; u < NU; ++u) acc[u][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    // Where w is read once, by one row of tiles, every workgroup begins at another block: rows are usually a power of two of bytes
+    // apart, and workgroups in step would ask the same memory channels at a time.
+    uint32_t first = tm == 1u ? kb0 + tile_n % count : kb0;
+    auto after = [&](uint32_t kb) { return kb + 1u == kb0 + count ? kb0 : kb + 1u; };
     const typename L::Source source = L::source(p, n0, m0);
     // (a block's scales are asked for one block ahead, before that block's rows: waiting for them waits for nothing newer)
-    float f[MT], ahead[MT], ahead_w = sw[0];
+    float f[MT], ahead[MT], ahead_w = sw[first];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        ahead[t] = sx[t][0];
+        ahead[t] = sx[t][first];
         asm volatile("" : "+v"(ahead[t]));       // here, and not in the loop, where it would wait for the next block's
     }
+    uint32_t kb = first, to_fill = first;
 #pragma unroll
-    for (int b = 0; b < STAGES - 1; ++b) if (b < (int)p.blocks) L::fill(p, source, n0, m0, b, lds + b * L::kStage);
+    for (int b = 0; b < STAGES - 1; ++b)
+        if (b < (int)count) { L::fill(p, source, n0, m0, to_fill, lds + b * L::kStage); to_fill = after(to_fill); }
     uint32_t now = 0, next = (STAGES - 1) * L::kStage;
-    for (uint32_t kb = 0; kb < p.blocks; ++kb) {
+    for (uint32_t j = 0; j < count; ++j) {
         // (towards the end there are no newer stages to leave under way)
-        if (STAGES == 2 || kb + STAGES - 1 > p.blocks) stage_barrier<0>();
+        if (STAGES == 2 || j + STAGES - 1 > count) stage_barrier<0>();
         else stage_barrier<(STAGES - 2) * L::kLoads>();
 #pragma unroll
         for (int t = 0; t < MT; ++t) f[t] = ahead[t] * ahead_w;
-        const uint32_t k1 = min(kb + 1u, p.blocks - 1u);
-        ahead_w = sw[k1];
+        kb = after(kb);
+        ahead_w = sw[kb];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) ahead[t] = sx[t][k1];
-        L::step(p, source, n0, m0, kb + STAGES - 1u, lds + now, lds + next, f, acc);
+        for (int t = 0; t < MT; ++t) ahead[t] = sx[t][kb];
+        L::step(p, source, n0, m0, to_fill, j + STAGES - 1u < count, lds + now, lds + next, f, acc);
+        to_fill = after(to_fill);
         now = now == (STAGES - 1) * L::kStage ? 0u : now + L::kStage;
         next = next == (STAGES - 1) * L::kStage ? 0u : next + L::kStage;
     }
-    // a lane has columns wn + 32 part .. + 31 of its rows of y
-    const uint32_t n = n0 + wn + part * 32u;
+    if (p.split > 1u) {
+        // every workgroup leaves its sums; the last of the tile's adds them up, in the order of the blocks
+        constexpr uint32_t kPart = L::kThreads * NU * MT * 2;
+        uint64_t *parts = (uint64_t *)p.parts + (size_t)id * p.split * kPart + threadIdx.x;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    a_store(&parts[part_of * kPart + ((u * MT + t) * 2 + h) * L::kThreads],
+                            (uint64_t)__float_as_uint(acc[u][t][2 * h + 1]) << 32 | __float_as_uint(acc[u][t][2 * h]));
+        uint32_t *last = (uint32_t *)lds;
+        wait_vmem();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            *last = __hip_atomic_fetch_add(&p.arrived[id], 1u, __ATOMIC_RELAXED, RS_AGENT) == p.split - 1u;
+            if (*last) a_store(&p.arrived[id], 0u);
+        }
+        __syncthreads();
+        if (!*last) return;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[u][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+        for (uint32_t s = 0; s < p.split; ++s) {
+            uint64_t v[2 * NU * MT];
+#pragma unroll
+            for (int o = 0; o < 2 * NU * MT; ++o) v[o] = a_load(&parts[s * kPart + o * L::kThreads]);
+#pragma unroll
+            for (int o = 0; o < 2 * NU * MT; ++o) {
+                acc[o / 2 / MT][o / 2 % MT][o % 2 * 2] += __uint_as_float((uint32_t)v[o]);
+                acc[o / 2 / MT][o / 2 % MT][o % 2 * 2 + 1] += __uint_as_float((uint32_t)(v[o] >> 32));
+            }
+        }
+    }
+    // a lane has 4 NU columns of its rows of y
+    const uint32_t n = n0 + wn + part * (4u * NU);
     constexpr uint32_t kVec = DT == RS_DTYPE_F32 ? 4 : 8;
-    const bool wide = n + 32u <= p.N && !(p.y_stride % kVec) && !((uintptr_t)p.y & 15);
+    const bool wide = n + 4u * NU <= p.N;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const uint32_t m = m0 + wm + t * 16u + i;
@@ -491,10 +568,10 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearPara
         const int64_t at = (int64_t)m * p.y_stride + n;
         if (wide) {
 #pragma unroll
-            for (int u = 0; u < 8; u += kVec / 4) put_wide<DT>(p.y, at + u * 4, acc[u][t], acc[(u + 1) % 8][t]);
+            for (int u = 0; u < NU; u += kVec / 4) put_wide<DT>(p.y, at + u * 4, acc[u][t], acc[(u + 1) % NU][t]);
         } else {
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
+            for (int u = 0; u < NU; ++u)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) if (n + u * 4u + j < p.N) put<DT>(p.y, at + u * 4 + j, acc[u][t][j]);
         }

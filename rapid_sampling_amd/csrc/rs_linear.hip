@@ -1,6 +1,8 @@
 // Instantiations, launchers and C entry points of the quantisers and the product in 8 bits.
 #include "rs_linear.h"
 
+#include <algorithm>
+
 namespace rs {
 
 template <int DT>
@@ -10,13 +12,21 @@ static void launch_quantize(const QuantParams &p, bool tiles, hipStream_t st)
     else hipLaunchKernelGGL(quantize_rows_kernel<DT>, dim3((uint32_t)(((uint64_t)p.R * p.blocks + 15) / 16)), dim3(256), 0, st, p);
 }
 
-template <int DT, int WN, int WM, int MT, int STAGES, bool EXACT>
-static hipError_t launch_tiles(const LinearParams &p, hipStream_t st)
+constexpr uint32_t kPartTiles = 256;                 // tiles of partial sums that the workspace holds ...
+constexpr size_t   kPartBytes = 128 * 64 * 4;        // ... of 128 x 64
+
+// SPLIT: where there are few tiles their blocks of columns are shared out, for up to one workgroup to a compute unit.  Leaving and
+// adding up the parts costs about 2 us, a block 0.5 us, 0.9 on bfloat16 cores: eight blocks or four to each at least (64 x 1024 x
+// 4096: 24 us whole, 12 in eight; 64 x 4096 x 512: 4.7 whole, 6.6 in two).
+template <int DT, int WN, int WM, int NU, int MT, int STAGES, bool EXACT, bool SPLIT>
+static hipError_t launch_tiles(LinearParams p, hipStream_t st)
 {
-    using L = LinearTile<WN, WM, MT, STAGES, EXACT>;
+    using L = LinearTile<WN, WM, NU, MT, STAGES, EXACT>;
+    static_assert(!SPLIT || L::kTileN * L::kTileM * 4 <= kPartBytes, "a tile's sums fit the workspace");
     const uint64_t tiles = (uint64_t)((p.M + L::kTileM - 1) / L::kTileM) * ((p.N + L::kTileN - 1) / L::kTileN);
     if (tiles > 0x7FFFFFFF) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((linear_tile_kernel<DT, WN, WM, MT, STAGES, EXACT>), dim3((uint32_t)tiles), dim3(L::kThreads), L::kLds, st, p);
+    p.split = SPLIT ? (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({kPartTiles / tiles, p.blocks / (EXACT ? 4 : 8), 8})) : 1;
+    hipLaunchKernelGGL((linear_tile_kernel<DT, WN, WM, NU, MT, STAGES, EXACT>), dim3((uint32_t)tiles * p.split), dim3(L::kThreads), L::kLds, st, p);
     return hipGetLastError();
 }
 
@@ -28,15 +38,33 @@ static hipError_t launch_few(const LinearParams &p, hipStream_t st)
     return hipGetLastError();
 }
 
+// Times in us on one card, weights beyond its caches unless said otherwise.
 template <int DT>
 static hipError_t launch_linear(const LinearParams &p, hipStream_t st)
 {
-    // (the tiles' kernel reaches its rows with 32 bits)
-    if (p.M <= 16 || p.x_stride > kTileStride || p.w_stride > kTileStride) return launch_few<DT, 1, 2>(p, st);
-    constexpr bool kExact = DT == RS_DTYPE_F32;
-    if (p.M <= 64) return launch_tiles<DT, 1, 4, 1, 3, true>(p, st);
-    if constexpr (kExact) return launch_tiles<DT, 2, 4, 2, 3, true>(p, st);
-    else return p.M <= 128 ? launch_tiles<DT, 2, 4, 2, 3, false>(p, st) : launch_tiles<DT, 2, 4, 4, 2, false>(p, st);
+    // Up to 16 rows one 16 x 16 product holds them all, and nothing but w is worth staging (1 x 131072 x 4096: 93, 5.8 TB/s).  32 rows of
+    // w to a workgroup, 16 where there are few (1 x 1024 x 8192: 7.7 against 10.5; 1 x 65536 x 4096: 55.6 against 48.5).
+    // (The tiles' kernel reaches its rows with 32 bits.)
+    if (p.M <= 16 || p.x_stride > kTileStride || p.w_stride > kTileStride)
+        return p.N <= 8192 ? launch_few<DT, 1, 1>(p, st) : launch_few<DT, 1, 2>(p, st);
+    // Tiles of 128 x 64 (rows of w x rows of x) for up to 64 rows, and wherever those of 128 x 128 would not give every compute unit
+    // its own (1000 x 4096 x 4096 into bfloat16: 28.0 against 29.8; 300 x 8192 x 1440: 12.9 against 14.0).  On bfloat16 cores two
+    // waves share w's rows and two x's, since both have to be widened (64 x 50256 x 2000: 25.7 against 29.0 with four and one).
+    const uint64_t n128 = (p.N + 127) / 128, m128 = (p.M + 127) / 128;
+    const bool few_tiles = n128 * m128 <= 256;
+    if (DT == RS_DTYPE_F32 || p.M <= 64) {
+        if (p.M <= 64 || few_tiles) return launch_tiles<DT, 2, 2, 4, 2, 3, true, true>(p, st);
+        // 128 x 128: 4096 x 32768 x 4096 in 1076 (1.02 PFLOP/s), bound by the widening; 1278 in tiles of 128 x 64
+        if constexpr (DT == RS_DTYPE_F32) return launch_tiles<DT, 1, 4, 8, 2, 2, true, false>(p, st);
+    }
+    if constexpr (DT != RS_DTYPE_F32) {
+        if (few_tiles) return launch_tiles<DT, 1, 4, 8, 1, 3, false, true>(p, st);
+        // 256 x 256 where that fills the card and wastes little: 8192^3 536 against 612 in tiles of 128 x 128, 2048 x 16384 x 2048 85
+        // against 92; but 128 x 131072 x 4096 143 against 129
+        const uint64_t n256 = (p.N + 255) / 256, m256 = (p.M + 255) / 256;
+        if (n256 * m256 >= 256 && 20 * m256 <= 11 * m128) return launch_tiles<DT, 2, 4, 8, 4, 2, false, false>(p, st);
+        return launch_tiles<DT, 1, 4, 8, 2, 2, false, false>(p, st);
+    }
 }
 
 static bool known(int32_t dtype) { return dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16 || dtype == RS_DTYPE_F16; }
@@ -67,11 +95,15 @@ int rs_quantize_blocks(const void *x, int32_t dtype, int64_t x_row_stride, int32
     return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
 }
 
+size_t rs_linear_workspace_bytes(void) { return kPartTiles * (kPartBytes + 16); }
+
 int rs_linear_blocks(const void *x, int64_t x_row_stride, const float *x_scale,
                      const void *w, int64_t w_row_stride, const float *w_scale,
-                     int32_t M, int32_t N, int32_t K, void *y, int32_t y_dtype, int64_t y_row_stride, void *stream)
+                     int32_t M, int32_t N, int32_t K, void *y, int32_t y_dtype, int64_t y_row_stride,
+                     void *workspace, size_t workspace_bytes, void *stream)
 {
-    if (!x || !x_scale || !w || !w_scale || !y) return RS_ERR_NULL;
+    if (!x || !x_scale || !w || !w_scale || !y || !workspace) return RS_ERR_NULL;
+    if (workspace_bytes < rs_linear_workspace_bytes() || ((uintptr_t)workspace & 255)) return RS_ERR_WORKSPACE;
     if (!known(y_dtype)) return RS_ERR_ARG;
     if (M <= 0 || N <= 0 || K <= 0 || M > RS_LINEAR_MAX || N > RS_LINEAR_MAX || K > RS_LINEAR_MAX) return RS_ERR_SHAPE;
     if ((M > 1 && x_row_stride < K) || (N > 1 && w_row_stride < K) || (M > 1 && y_row_stride < N)) return RS_ERR_SHAPE;
@@ -82,6 +114,9 @@ int rs_linear_blocks(const void *x, int64_t x_row_stride, const float *x_scale,
     p.x = (const uint8_t *)x; p.x_stride = x_row_stride; p.x_scale = x_scale;
     p.w = (const uint8_t *)w; p.w_stride = w_row_stride; p.w_scale = w_scale;
     p.y = y; p.y_stride = y_row_stride;
+    p.split = 1;
+    p.arrived = (uint32_t *)workspace;
+    p.parts = (float *)((char *)workspace + 16 * kPartTiles);
     p.M = (uint32_t)M; p.N = (uint32_t)N; p.K = (uint32_t)K; p.blocks = ((uint32_t)K + kFpBlock - 1) / kFpBlock;
     const hipStream_t st = (hipStream_t)stream;
     const hipError_t e = y_dtype == RS_DTYPE_F32 ? launch_linear<RS_DTYPE_F32>(p, st)

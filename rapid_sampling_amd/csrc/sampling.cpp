@@ -45,7 +45,7 @@ struct Entry {
     at::Tensor ws;
     int64_t B = 0, V = 0;
     rs_policy *policy = nullptr;
-    at::Tensor logprobs_ws;                 // workspace of token_logprobs: of one size, so never replaced
+    at::Tensor logprobs_ws, linear_ws;      // workspaces of token_logprobs and linear_fp8: of one size, so never replaced
     bool captured = false;                  // a stream capture has recorded calls that point into ws
     std::vector<at::Tensor> retired;        // outgrown workspaces a captured graph may still point into
     std::vector<rs_policy *> retired_policies;   // replaced policies whose pinned words a captured graph's kernels may still write
@@ -249,20 +249,28 @@ at::Tensor run(const at::Tensor &logits, const Shape &s, at::Tensor *penalties, 
 
 // ------------------------------------------------ log probabilities of given tokens --
 
-// The workspace of token_logprobs on this stream: of one size for every call.
-at::Tensor &logprobs_workspace(const at::Tensor &like, void *stream)
+// The workspace of one of the operators on this stream, of `bytes` bytes whatever the call.
+at::Tensor &operator_workspace(at::Tensor Entry::*which, size_t bytes, const char *what, const at::Tensor &like, void *stream)
 {
-    Entry &e = entry_for((int)like.device().index(), stream);
-    if (!e.logprobs_ws.defined()) {
+    at::Tensor &held = entry_for((int)like.device().index(), stream).*which;
+    if (!held.defined()) {
         if (is_capturing(stream))
-            throw std::runtime_error("rapid_sampling: token_logprobs has no workspace on this stream yet, which is being captured; "
+            throw std::runtime_error(std::string("rapid_sampling: ") + what + " has no workspace on this stream yet, which is being captured; "
                                      "call reserve_workspace(B, V) on this stream before the capture begins");
-        auto ws = at::empty({(int64_t)rs_logprobs_workspace_bytes()}, at::TensorOptions().dtype(at::kChar).device(like.device()));
+        auto ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kChar).device(like.device()));
         const int rc = rs_workspace_init(ws.data_ptr(), (size_t)ws.numel(), stream);
         if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
-        e.logprobs_ws = ws;
+        held = ws;
     }
-    return e.logprobs_ws;
+    return held;
+}
+at::Tensor &logprobs_workspace(const at::Tensor &like, void *stream)
+{
+    return operator_workspace(&Entry::logprobs_ws, rs_logprobs_workspace_bytes(), "token_logprobs", like, stream);
+}
+at::Tensor &linear_workspace(const at::Tensor &like, void *stream)
+{
+    return operator_workspace(&Entry::linear_ws, rs_linear_workspace_bytes(), "linear_fp8", like, stream);
 }
 
 int32_t float_dtype(const at::Tensor &t, const char *what)
@@ -501,8 +509,10 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const at::Tenso
     if (given) { q = x; scale = *x_scale; check_scale(scale, x, M, blocks, "x_scale"); }
     else std::tie(q, scale) = quantize(x, 1);
     q = fp8_rows(q, "x");
+    void *stream = current_stream(x);
+    at::Tensor &ws = linear_workspace(x, stream);
     const int rc = rs_linear_blocks(q.data_ptr(), q.stride(0), scale.data_ptr<float>(), w.data_ptr(), w.stride(0), weight_scale.data_ptr<float>(),
-                                    (int32_t)M, (int32_t)N, (int32_t)K, y.data_ptr(), float_dtype(y, "y"), N, current_stream(x));
+                                    (int32_t)M, (int32_t)N, (int32_t)K, y.data_ptr(), float_dtype(y, "y"), N, ws.data_ptr(), (size_t)ws.numel(), stream);
     if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
     return y;
 }
@@ -591,6 +601,7 @@ void reserve_workspace(int64_t B, int64_t V, std::optional<int64_t> device)
     auto like = at::empty({1}, at::TensorOptions().dtype(at::kChar).device(dev));
     workspace_for(like, current_stream(like), B, V);
     logprobs_workspace(like, current_stream(like));
+    linear_workspace(like, current_stream(like));
 }
 
 // Synchronises the current stream of `device` and returns the sticky error word of its workspace:

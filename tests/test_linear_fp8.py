@@ -221,15 +221,18 @@ def test_refusals_of_the_c_abi():
     L = capi.lib()
     p, i32, i64 = C.c_void_p, C.c_int32, C.c_int64
     L.rs_quantize_blocks.argtypes = [p, i32, i64, i32, i32, i32, p, i64, p, p]
-    L.rs_linear_blocks.argtypes = [p, i64, p, p, i64, p, i32, i32, i32, p, i32, i64, p]
+    L.rs_linear_workspace_bytes.restype = C.c_size_t
+    n = L.rs_linear_workspace_bytes()
+    L.rs_linear_blocks.argtypes = [p, i64, p, p, i64, p, i32, i32, i32, p, i32, i64, p, C.c_size_t, p]
 
     def quantize(x=256, dtype=0, rows=1, R=2, K=20, q=256, q_stride=32, scale=256):
         return L.rs_quantize_blocks(x, dtype, K, rows, R, K, q, q_stride, scale, None)
     assert quantize(x=None) == quantize(q=None) == quantize(scale=None) == -4 and quantize(dtype=5) == quantize(rows=64) == -7
     assert quantize(R=0) == quantize(K=0) == quantize(q_stride=16) == -12 and quantize(x=258) == quantize(q=264) == quantize(q_stride=40) == -6
 
-    def linear(x=256, xs=32, w=256, ws=32, sx=256, sw=256, M=2, N=20, K=20, y=256, dtype=0, ys=20):
-        return L.rs_linear_blocks(x, xs, sx, w, ws, sw, M, N, K, y, dtype, ys, None)
-    assert linear(x=None) == linear(w=None) == linear(y=None) == linear(sx=None) == linear(sw=None) == -4 and linear(dtype=7) == -7
+    def linear(x=256, xs=32, w=256, ws=32, sx=256, sw=256, M=2, N=20, K=20, y=256, dtype=0, ys=20, ws_at=256, ws_bytes=n):
+        return L.rs_linear_blocks(x, xs, sx, w, ws, sw, M, N, K, y, dtype, ys, ws_at, ws_bytes, None)
+    assert linear(x=None) == linear(w=None) == linear(y=None) == linear(sx=None) == linear(sw=None) == linear(ws_at=None) == -4 and linear(dtype=7) == -7
+    assert linear(ws_at=264) == linear(ws_bytes=n - 1) == -5
     assert linear(M=0) == linear(N=0) == linear(K=0) == linear(xs=16) == linear(ws=16) == linear(ys=19) == -12
     assert linear(x=264) == linear(w=260) == linear(xs=40) == linear(ws=40) == linear(y=258) == -6
