@@ -548,6 +548,19 @@ int rs_linear_blocks(const void *x_device, int64_t x_row_stride, const float *x_
                      int32_t M, int32_t N, int32_t K, void *y_device, int32_t y_dtype, int64_t y_row_stride,
                      void *workspace_device, size_t workspace_bytes, void *stream);
 
+/*
+ * rs_quantize_blocks and rs_linear_blocks in one launch, without anything in
+ * between, for up to RS_LINEAR_ROWS_MAX rows of up to RS_LINEAR_ROWS_COLUMNS_MAX
+ * columns of x in float32, bfloat16 or float16 (rows x_row_stride elements
+ * apart, at any address).  The same y.  No workspace.  No counterpart in the
+ * reference.
+ */
+#define RS_LINEAR_ROWS_MAX 4
+#define RS_LINEAR_ROWS_COLUMNS_MAX 8192
+int rs_linear_rows(const void *x_device, int32_t x_dtype, int64_t x_row_stride,
+                   const void *w_device, int64_t w_row_stride, const float *w_scale_device,
+                   int32_t M, int32_t N, int32_t K, void *y_device, int32_t y_dtype, int64_t y_row_stride, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

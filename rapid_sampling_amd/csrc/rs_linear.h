@@ -32,7 +32,7 @@ struct QuantParams {
 };
 
 struct LinearParams {
-    const uint8_t *x, *w;
+    const uint8_t *x, *w;                // x in 8 bits, or of another type: then x_scale is null and x_stride counts elements
     int64_t        x_stride, w_stride, y_stride;
     const float   *x_scale, *w_scale;
     void          *y;
@@ -57,56 +57,109 @@ template <int DT> __device__ __forceinline__ void put(void *p, int64_t i, float 
 
 __device__ __forceinline__ float block_scale(float peak) { return fmaxf(peak * (1.0f / 448.0f), 0x1p-126f); }
 
+// x / scale, rounded once: the quotient by way of the reciprocal, and what it is off by divided once more.  (Compared with the
+// division on 4e8 pairs of a block's largest value and another: the same.)
+struct Divisor {
+    float s, r;
+    __device__ __forceinline__ explicit Divisor(float scale) : s(scale < __builtin_inff() ? scale : 0.0f), r(1.0f / scale) {}
+    __device__ __forceinline__ float operator()(float x) const
+    {
+        const float q = x * r;
+        // (-0 stays one; an infinite scale gives 0 for a finite x, NaN for an infinite one)
+        return __builtin_copysignf(__builtin_fmaf(__builtin_fmaf(-q, s, x), r, q), x);
+    }
+};
+__device__ __forceinline__ uint2 quantize8(const float (&x)[8], float scale)
+{
+    const Divisor d(scale);
+    int lo = 0, hi = 0;
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(d(x[0]), d(x[1]), lo, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(d(x[2]), d(x[3]), lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(d(x[4]), d(x[5]), hi, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(d(x[6]), d(x[7]), hi, true);
+    return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+
+// Eight values of a row from column k on, at any address; 0 from column K on.
+template <int DT>
+__device__ __forceinline__ void load8(const void *base, int64_t at, uint32_t k, uint32_t K, float (&x)[8])
+{
+    if (k + 8u <= K) {
+        if constexpr (DT == RS_DTYPE_F32) {
+            v4f a, b;
+            __builtin_memcpy(&a, (const float *)base + at + k, 16);
+            __builtin_memcpy(&b, (const float *)base + at + k + 4, 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { x[j] = a[j]; x[j + 4] = b[j]; }
+        } else {
+            uint16_t v[8];
+            __builtin_memcpy(v, (const uint16_t *)base + at + k, 16);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = DT == RS_DTYPE_BF16 ? __uint_as_float((uint32_t)v[j] << 16) : (float)__builtin_bit_cast(_Float16, v[j]);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) x[j] = k + j < K ? widen<DT>(base, at + k + j) : 0.0f;
+    }
+}
+__device__ __forceinline__ float largest8(const float (&x)[8])
+{
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[j]));
+    return m;
+}
+// Largest over 16 lanes, in all of them.
+template <int CTRL> __device__ __forceinline__ float turn_max(float v)
+{
+    return fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, false)));
+}
+__device__ __forceinline__ float max16(float v)
+{
+    return turn_max<0x121>(turn_max<0x122>(turn_max<0x124>(turn_max<0x128>(v))));       // row_ror 8, 4, 2, 1
+}
+
 // One block of 1 x 128: sixteen lanes, eight values each.
 template <int DT>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantParams p)
 {
     const uint32_t i = blockIdx.x * 16u + threadIdx.x / 16u, part = threadIdx.x % 16u;
-    const bool live = i < p.R * (uint64_t)p.blocks;
+    const bool live = i < (uint64_t)p.R * p.blocks;
     const uint32_t r = live ? i / p.blocks : 0, kb = live ? i - r * p.blocks : 0;
     const uint32_t k0 = kb * kFpBlock + part * 8u;
-    float x[8], peak = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        x[j] = live && k0 + j < p.K ? widen<DT>(p.x, (int64_t)r * p.x_stride + k0 + j) : 0.0f;
-        peak = fmaxf(peak, fabsf(x[j]));
-    }
-#pragma unroll
-    for (int d = 8; d; d >>= 1) peak = fmaxf(peak, __shfl_xor(peak, d));
-    const float scale = block_scale(peak);
+    float x[8];
+    load8<DT>(p.x, (int64_t)r * p.x_stride, k0, p.K, x);
+    const float scale = block_scale(max16(largest8(x)));
     if (!live) return;
     if (part == 0) p.scale[(size_t)r * p.blocks + kb] = scale;
-    if (k0 >= p.q_cols) return;
-    uint2 q;
-    int lo = 0, hi = 0;
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] / scale, x[1] / scale, lo, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] / scale, x[3] / scale, lo, true);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[4] / scale, x[5] / scale, hi, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[6] / scale, x[7] / scale, hi, true);
-    q.x = (uint32_t)lo; q.y = (uint32_t)hi;
-    *(uint2 *)(p.q + (int64_t)r * p.q_stride + k0) = q;      // q_cols is a multiple of 8
+    if (k0 < p.q_cols) *(uint2 *)(p.q + (int64_t)r * p.q_stride + k0) = quantize8(x, scale);       // q_cols is a multiple of 8
 }
 
-// One block of 128 x 128: a workgroup, two threads to a row.
+// One block of 128 x 128: a workgroup, sixteen lanes to a row, eight rows to a thread.
 template <int DT>
 __global__ __launch_bounds__(256) void quantize_tiles_kernel(QuantParams p)
 {
     __shared__ float peaks[4];
     const uint32_t rb = blockIdx.x / p.blocks, kb = blockIdx.x - rb * p.blocks;
-    const uint32_t r = rb * kFpBlock + threadIdx.x / 2u, k0 = kb * kFpBlock + threadIdx.x % 2u * 64u;
-    const int64_t at = (int64_t)r * p.x_stride + k0;
-    float peak = 0.0f;
-    for (uint32_t j = 0; j < 64; ++j) if (r < p.R && k0 + j < p.K) peak = fmaxf(peak, fabsf(widen<DT>(p.x, at + j)));
+    const uint32_t r0 = rb * kFpBlock + threadIdx.x / 16u, k0 = kb * kFpBlock + threadIdx.x % 16u * 8u;
+    float x[8][8], peak = 0.0f;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+        const uint32_t r = r0 + j * 16u;
+        load8<DT>(p.x, (int64_t)min(r, p.R - 1u) * p.x_stride, k0, r < p.R ? p.K : 0u, x[j]);
+        peak = fmaxf(peak, largest8(x[j]));
+    }
 #pragma unroll
     for (int d = 32; d; d >>= 1) peak = fmaxf(peak, __shfl_xor(peak, d));
     if (threadIdx.x % 64 == 0) peaks[threadIdx.x / 64] = peak;
     __syncthreads();
     const float scale = block_scale(fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3])));
     if (threadIdx.x == 0) p.scale[(size_t)rb * p.blocks + kb] = scale;
-    if (r >= p.R) return;
-    for (uint32_t j = 0; j < 64 && k0 + j < p.q_cols; j += 2) {
-        const float a = k0 + j < p.K ? widen<DT>(p.x, at + j) : 0.0f, b = k0 + j + 1 < p.K ? widen<DT>(p.x, at + j + 1) : 0.0f;
-        *(uint16_t *)(p.q + (int64_t)r * p.q_stride + k0 + j) = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(a / scale, b / scale, 0, false);
+    if (k0 >= p.q_cols) return;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+        const uint32_t r = r0 + j * 16u;
+        if (r < p.R) *(uint2 *)(p.q + (int64_t)r * p.q_stride + k0) = quantize8(x[j], scale);
     }
 }
 
@@ -191,30 +244,30 @@ template <int DT> __device__ __forceinline__ void put_wide(void *p, int64_t i, v
 }
 
 // --------------------------------------------------------------- few rows --
-// Bound by reading w once.  A workgroup makes 16 NT rows of w x 16 MT rows of x; its waves take the blocks of 128 columns in
+// Bound by reading w once.  A workgroup makes 16 NT rows of w x up to 16 rows of x; its waves take the blocks of 128 columns in
 // turn, so that it reads 1 KB of each row at a time and nothing is shared but the sums, which go through LDS once, at
 // the end, and are added in the order of the waves.  A wave asks for its next block before it multiplies the one it has.
 // The products are made on bfloat16, whatever y's type: the matrix cores have time to spare here.
-template <int MT, int NT>
+//
+// XT < 0: x is in 8 bits.  Else it is of that type, and every workgroup rounds all of it (a few rows) into LDS while its first
+// rows of w are on their way: one launch in the place of two.
+template <int XT, int NT>
 struct LinearFew {
     struct Block {
-        v8i   w[NT], x[MT];
-        float f[MT];
+        v8i   w[NT], x;
+        float f, s;                      // x's scale (of a row that is in memory), w's
     };
-    const uint8_t *w[NT], *x[MT];        // the lane's rows, at its columns of the first block
-    const float   *sw, *sx[MT];
+    const uint8_t *w[NT], *x;            // the lane's rows, at its columns of the first block; x in memory or in LDS
+    const float   *sw, *sx;
 
-    __device__ __forceinline__ LinearFew(const LinearParams &p, uint32_t n0, uint32_t m0)
+    __device__ __forceinline__ LinearFew(const LinearParams &p, uint32_t n0, uint32_t m0, const uint8_t *lds)
     {
         const uint32_t lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
 #pragma unroll
         for (int u = 0; u < NT; ++u) w[u] = p.w + (int64_t)min(n0 + u * 16u + i, p.N - 1u) * p.w_stride + part * 16u;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const uint32_t m = min(m0 + t * 16u + i, p.M - 1u);
-            x[t] = p.x + (int64_t)m * p.x_stride + part * 16u;
-            sx[t] = p.x_scale + (size_t)m * p.blocks;
-        }
+        const uint32_t m = min(m0 + i, p.M - 1u);
+        x = (XT < 0 ? p.x + (int64_t)m * p.x_stride : lds + m * (p.blocks * kFpBlock)) + part * 16u;
+        sx = (XT < 0 ? p.x_scale : (const float *)(lds + p.M * p.blocks * kFpBlock)) + (size_t)m * p.blocks;
         sw = p.w_scale + (size_t)(n0 / kFpBlock) * p.blocks;
     }
     // (w is read once and need not stay in the caches; x is read by every workgroup)
@@ -225,83 +278,88 @@ struct LinearFew {
 #pragma unroll
             for (int u = 0; u < NT; ++u)
                 b.w[u] = join(__builtin_nontemporal_load((const v4i *)(w[u] + k)), __builtin_nontemporal_load((const v4i *)(w[u] + k + 64)));
-#pragma unroll
-            for (int t = 0; t < MT; ++t) b.x[t] = join(*(const v4i *)(x[t] + k), *(const v4i *)(x[t] + k + 64));
+            if constexpr (XT < 0) b.x = join(*(const v4i *)(x + k), *(const v4i *)(x + k + 64));
         } else {
             const uint32_t at = threadIdx.x % 64u / 16u * 16u;
 #pragma unroll
             for (int u = 0; u < NT; ++u) b.w[u] = join(load16(w[u] - at, k + at, p.K), load16(w[u] - at, k + at + 64u, p.K));
-#pragma unroll
-            for (int t = 0; t < MT; ++t) b.x[t] = join(load16(x[t] - at, k + at, p.K), load16(x[t] - at, k + at + 64u, p.K));
+            if constexpr (XT < 0) b.x = join(load16(x - at, k + at, p.K), load16(x - at, k + at + 64u, p.K));
         }
-        const float s = sw[kb];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) b.f[t] = s * sx[t][kb];
+        b.s = sw[kb];
+        if constexpr (XT < 0) b.f = sx[kb];
     }
-    static __device__ __forceinline__ void multiply(const Block &b, v4f (&acc)[NT][MT])
+    __device__ __forceinline__ void multiply(Block b, uint32_t kb, v4f (&acc)[NT]) const
     {
-        v8bf x[MT][4];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) widen_block(b.x[t], x[t]);
+        if constexpr (XT >= 0) {
+            b.x = join(*(const v4i *)(x + kb * kFpBlock), *(const v4i *)(x + kb * kFpBlock + 64));
+            b.f = sx[kb];
+        }
+        const float f = b.s * b.f;
+        v8bf xb[4];
+        widen_block(b.x, xb);
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            v8bf w[4];
-            widen_block(b.w[u], w);
+            v8bf wb[4];
+            widen_block(b.w[u], wb);
+            const v4f s = block_product(wb, xb);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const v4f s = block_product(w, x[t]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[u][t][j] = __builtin_fmaf(s[j], b.f[t], acc[u][t][j]);
-            }
+            for (int j = 0; j < 4; ++j) acc[u][j] = __builtin_fmaf(s[j], f, acc[u][j]);
         }
     }
 };
 
-template <int DT, int MT, int NT>
+template <int DT, int XT, int NT>
 __global__ __launch_bounds__(512) void linear_few_kernel(LinearParams p)
 {
-    using L = LinearFew<MT, NT>;
-    constexpr int kTiles = NT * MT, kRound = kTiles < 8 ? kTiles : 8;
-    __shared__ v4f sums[8][kRound][64];
+    using L = LinearFew<XT, NT>;
+    __shared__ v4f sums[8][NT][64];
+    extern __shared__ uint8_t lds[];
     const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u, waves = blockDim.x / 64u, i = lane % 16u, part = lane / 16u;
-    const uint32_t n0 = blockIdx.x * (16u * NT), m0 = blockIdx.y * (16u * MT);
-    const L rows(p, n0, m0);
-    v4f acc[NT][MT];
-#pragma unroll
-    for (int u = 0; u < NT; ++u)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) acc[u][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    if (wave < p.blocks) {
-        // (every workgroup begins at another block: see the kernel for many rows)
-        const uint32_t turn = blockIdx.x % p.blocks;
-        auto turned = [&](uint32_t kb) { kb += turn; return kb < p.blocks ? kb : kb - p.blocks; };
-        typename L::Block now, next;
-        rows.load(p, turned(wave), now);
-        for (uint32_t j = wave + waves; j < p.blocks; j += waves) {
-            rows.load(p, turned(j), next);
-            L::multiply(now, acc);
-            now = next;
+    const uint32_t n0 = blockIdx.x * (16u * NT), m0 = blockIdx.y * 16u;
+    const L rows(p, n0, m0, lds);
+    // (every workgroup begins at another block: see the kernel for many rows)
+    const uint32_t turn = blockIdx.x % p.blocks;
+    auto turned = [&](uint32_t kb) { kb += turn; return kb < p.blocks ? kb : kb - p.blocks; };
+    typename L::Block now, next;
+    if (wave < p.blocks) rows.load(p, turned(wave), now);
+    if constexpr (XT >= 0) {
+        for (uint32_t c = threadIdx.x / 16u; c < p.M * p.blocks; c += waves * 4u) {
+            const uint32_t r = c / p.blocks, k = (c - r * p.blocks) * kFpBlock + threadIdx.x % 16u * 8u;
+            float x[8];
+            load8<XT>(p.x, (int64_t)r * p.x_stride, k, p.K, x);
+            const float scale = block_scale(max16(largest8(x)));
+            *(uint2 *)(lds + r * (p.blocks * kFpBlock) + k) = quantize8(x, scale);
+            if (threadIdx.x % 16u == 0) ((float *)(lds + p.M * p.blocks * kFpBlock))[c] = scale;
         }
-        L::multiply(now, acc);
+        __syncthreads();
+    }
+    v4f acc[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) acc[u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (wave < p.blocks) {
+        uint32_t kb = turned(wave);
+        for (uint32_t j = wave + waves; j < p.blocks; j += waves) {
+            const uint32_t following = turned(j);
+            rows.load(p, following, next);
+            rows.multiply(now, kb, acc);
+            now = next;
+            kb = following;
+        }
+        rows.multiply(now, kb, acc);
     }
 #pragma unroll
-    for (int r = 0; r < kTiles; r += kRound) {
-        if (r) __syncthreads();
+    for (int u = 0; u < NT; ++u) sums[wave][u][lane] = acc[u];
+    __syncthreads();
+    for (uint32_t u = wave; u < (uint32_t)NT; u += waves) {
+        v4f s = sums[0][u][lane];
+        for (uint32_t o = 1; o < waves; ++o) s += sums[o][u][lane];
+        const uint32_t m = m0 + i, n = n0 + u * 16u + part * 4u;
+        if (m >= p.M) continue;
+        const int64_t at = (int64_t)m * p.y_stride + n;
+        if (n + 4u <= p.N) put_four<DT>(p.y, at, s);
+        else
 #pragma unroll
-        for (int c = 0; c < kRound; ++c) sums[wave][c][lane] = acc[(r + c) / MT][(r + c) % MT];
-        __syncthreads();
-        for (uint32_t c = wave; c < (uint32_t)kRound; c += waves) {
-            v4f s = sums[0][c][lane];
-            for (uint32_t o = 1; o < waves; ++o) s += sums[o][c][lane];
-            const uint32_t u = (r + c) / MT, t = (r + c) % MT;
-            const uint32_t m = m0 + t * 16u + i, n = n0 + u * 16u + part * 4u;
-            if (m >= p.M) continue;
-            const int64_t at = (int64_t)m * p.y_stride + n;
-            if (n + 4u <= p.N) put_four<DT>(p.y, at, s);
-            else
-#pragma unroll
-                for (int j = 0; j < 4; ++j) if (n + j < p.N) put<DT>(p.y, at + j, s[j]);
-        }
+            for (int j = 0; j < 4; ++j) if (n + j < p.N) put<DT>(p.y, at + j, s[j]);
     }
 }
 

@@ -30,23 +30,35 @@ static hipError_t launch_tiles(LinearParams p, hipStream_t st)
     return hipGetLastError();
 }
 
-template <int DT, int MT, int NT>
+template <int DT, int XT, int NT>
 static hipError_t launch_few(const LinearParams &p, hipStream_t st)
 {
     const uint32_t waves = p.blocks >= 8 ? 8 : p.blocks >= 4 ? 4 : p.blocks >= 2 ? 2 : 1;
-    hipLaunchKernelGGL((linear_few_kernel<DT, MT, NT>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)), dim3(64 * waves), 0, st, p);
+    const uint32_t lds = XT < 0 ? 0 : p.M * p.blocks * (kFpBlock + 4);
+    hipLaunchKernelGGL((linear_few_kernel<DT, XT, NT>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 15) / 16), dim3(64 * waves), lds, st, p);
     return hipGetLastError();
+}
+
+// 32 rows of w to a workgroup, 16 where there are few (1 x 1024 x 8192: 7.7 us against 10.5; 1 x 65536 x 4096: 55.6 against 48.5).
+template <int DT, int XT>
+static hipError_t launch_few(const LinearParams &p, hipStream_t st)
+{
+    return p.N <= 8192 ? launch_few<DT, XT, 1>(p, st) : launch_few<DT, XT, 2>(p, st);
+}
+
+template <int DT>
+static hipError_t launch_rows(const LinearParams &p, int32_t x_dtype, hipStream_t st)
+{
+    return x_dtype == RS_DTYPE_F32 ? launch_few<DT, RS_DTYPE_F32>(p, st) : x_dtype == RS_DTYPE_BF16 ? launch_few<DT, RS_DTYPE_BF16>(p, st) : launch_few<DT, RS_DTYPE_F16>(p, st);
 }
 
 // Times in us on one card, weights beyond its caches unless said otherwise.
 template <int DT>
 static hipError_t launch_linear(const LinearParams &p, hipStream_t st)
 {
-    // Up to 16 rows one 16 x 16 product holds them all, and nothing but w is worth staging (1 x 131072 x 4096: 93, 5.8 TB/s).  32 rows of
-    // w to a workgroup, 16 where there are few (1 x 1024 x 8192: 7.7 against 10.5; 1 x 65536 x 4096: 55.6 against 48.5).
+    // Up to 16 rows one 16 x 16 product holds them all, and nothing but w is worth staging (1 x 131072 x 4096: 93, 5.8 TB/s).
     // (The tiles' kernel reaches its rows with 32 bits.)
-    if (p.M <= 16 || p.x_stride > kTileStride || p.w_stride > kTileStride)
-        return p.N <= 8192 ? launch_few<DT, 1, 1>(p, st) : launch_few<DT, 1, 2>(p, st);
+    if (p.M <= 16 || p.x_stride > kTileStride || p.w_stride > kTileStride) return launch_few<DT, -1>(p, st);
     // Tiles of 128 x 64 (rows of w x rows of x) for up to 64 rows, and wherever those of 128 x 128 would not give every compute unit
     // its own (1000 x 4096 x 4096 into bfloat16: 28.0 against 29.8; 300 x 8192 x 1440: 12.9 against 14.0).  On bfloat16 cores two
     // waves share w's rows and two x's, since both have to be widened (64 x 50256 x 2000: 25.7 against 29.0 with four and one).
@@ -65,6 +77,20 @@ static hipError_t launch_linear(const LinearParams &p, hipStream_t st)
         if (n256 * m256 >= 256 && 20 * m256 <= 11 * m128) return launch_tiles<DT, 2, 4, 8, 4, 2, false, false>(p, st);
         return launch_tiles<DT, 1, 4, 8, 2, 2, false, false>(p, st);
     }
+}
+
+static LinearParams linear_params(const void *x, int64_t x_stride, const float *x_scale, const void *w, int64_t w_stride, const float *w_scale,
+                                  int32_t M, int32_t N, int32_t K, void *y, int64_t y_stride, void *workspace)
+{
+    LinearParams p;
+    p.x = (const uint8_t *)x; p.x_stride = x_stride; p.x_scale = x_scale;
+    p.w = (const uint8_t *)w; p.w_stride = w_stride; p.w_scale = w_scale;
+    p.y = y; p.y_stride = y_stride;
+    p.M = (uint32_t)M; p.N = (uint32_t)N; p.K = (uint32_t)K; p.blocks = ((uint32_t)K + kFpBlock - 1) / kFpBlock;
+    p.split = 1;
+    p.arrived = (uint32_t *)workspace;
+    p.parts = workspace ? (float *)((char *)workspace + 16 * kPartTiles) : nullptr;
+    return p;
 }
 
 static bool known(int32_t dtype) { return dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16 || dtype == RS_DTYPE_F16; }
@@ -110,17 +136,27 @@ int rs_linear_blocks(const void *x, int64_t x_row_stride, const float *x_scale,
     if (((uintptr_t)x & 15) || (M > 1 && (x_row_stride & 15)) || ((uintptr_t)w & 15) || (N > 1 && (w_row_stride & 15)) ||
         ((uintptr_t)x_scale & 3) || ((uintptr_t)w_scale & 3) || ((uintptr_t)y & (y_dtype == RS_DTYPE_F32 ? 3 : 1)))
         return RS_ERR_ALIGN;
-    LinearParams p;
-    p.x = (const uint8_t *)x; p.x_stride = x_row_stride; p.x_scale = x_scale;
-    p.w = (const uint8_t *)w; p.w_stride = w_row_stride; p.w_scale = w_scale;
-    p.y = y; p.y_stride = y_row_stride;
-    p.split = 1;
-    p.arrived = (uint32_t *)workspace;
-    p.parts = (float *)((char *)workspace + 16 * kPartTiles);
-    p.M = (uint32_t)M; p.N = (uint32_t)N; p.K = (uint32_t)K; p.blocks = ((uint32_t)K + kFpBlock - 1) / kFpBlock;
+    const LinearParams p = linear_params(x, x_row_stride, x_scale, w, w_row_stride, w_scale, M, N, K, y, y_row_stride, workspace);
     const hipStream_t st = (hipStream_t)stream;
     const hipError_t e = y_dtype == RS_DTYPE_F32 ? launch_linear<RS_DTYPE_F32>(p, st)
                        : y_dtype == RS_DTYPE_BF16 ? launch_linear<RS_DTYPE_BF16>(p, st) : launch_linear<RS_DTYPE_F16>(p, st);
+    return e == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
+}
+
+int rs_linear_rows(const void *x, int32_t x_dtype, int64_t x_row_stride, const void *w, int64_t w_row_stride, const float *w_scale,
+                   int32_t M, int32_t N, int32_t K, void *y, int32_t y_dtype, int64_t y_row_stride, void *stream)
+{
+    if (!x || !w || !w_scale || !y) return RS_ERR_NULL;
+    if (!known(x_dtype) || !known(y_dtype)) return RS_ERR_ARG;
+    if (M <= 0 || N <= 0 || K <= 0 || M > RS_LINEAR_ROWS_MAX || N > RS_LINEAR_MAX || K > RS_LINEAR_ROWS_COLUMNS_MAX) return RS_ERR_SHAPE;
+    if ((N > 1 && w_row_stride < K) || (M > 1 && y_row_stride < N)) return RS_ERR_SHAPE;
+    if (((uintptr_t)x & (x_dtype == RS_DTYPE_F32 ? 3 : 1)) || ((uintptr_t)w & 15) || (N > 1 && (w_row_stride & 15)) || ((uintptr_t)w_scale & 3) ||
+        ((uintptr_t)y & (y_dtype == RS_DTYPE_F32 ? 3 : 1)))
+        return RS_ERR_ALIGN;
+    const LinearParams p = linear_params(x, x_row_stride, nullptr, w, w_row_stride, w_scale, M, N, K, y, y_row_stride, nullptr);
+    const hipStream_t st = (hipStream_t)stream;
+    const hipError_t e = y_dtype == RS_DTYPE_F32 ? launch_rows<RS_DTYPE_F32>(p, x_dtype, st)
+                       : y_dtype == RS_DTYPE_BF16 ? launch_rows<RS_DTYPE_BF16>(p, x_dtype, st) : launch_rows<RS_DTYPE_F16>(p, x_dtype, st);
     return e == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
 }
 

@@ -431,31 +431,41 @@ at::Tensor rows_of_16_bytes(std::vector<int64_t> sizes, const at::Device &device
     return at::empty(sizes, at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(device)).narrow(-1, 0, K);
 }
 
-std::tuple<at::Tensor, at::Tensor> quantize(const at::Tensor &x, int64_t block_rows)
+// Values to be rounded to 8 bits, (..., K); the rows of the result lie (K + 15) / 16 * 16 bytes apart.
+void check_floats(const at::Tensor &x, int64_t block_rows)
 {
-    const int32_t dtype = float_dtype(x, "x");
-    if (block_rows != 1 && block_rows != 128)
-        throw std::invalid_argument("block_rows must be 1 or 128, got " + std::to_string(block_rows) + " !\n");
+    float_dtype(x, "x");
     if (x.dim() < 1 || (block_rows == 128 && x.dim() != 2))
         throw std::invalid_argument("x must have shape (..., K), or (N, K) for blocks of 128 x 128 !\n");
     if (!x.is_cuda()) throw std::invalid_argument("x must live on the GPU !\n");
-    const int64_t K = x.size(-1), rows = K ? x.numel() / K : 0;
-    if (K < 1 || K > RS_LINEAR_MAX || rows > 0x7FFFFFFF / ((K + 127) / 128))
+    const int64_t K = x.size(-1);
+    if (K < 1 || K > RS_LINEAR_MAX || x.numel() / K > 0x7FFFFFFF / ((K + 127) / 128))
         throw std::invalid_argument("x has no columns, or too many elements !\n");
     if (x.stride(-1) != 1 && K > 1) throw std::invalid_argument("x must be contiguous along its last axis !\n");
+}
+void quantize_into(const at::Tensor &x, int64_t block_rows, void *q, float *scale, void *stream)
+{
+    const int64_t K = x.size(-1), rows = x.numel() / K;
+    const at::Tensor flat = x.dim() == 2 ? x : x.reshape({rows, K});
+    const int rc = rs_quantize_blocks(flat.data_ptr(), float_dtype(x, "x"), flat.stride(0), (int32_t)block_rows, (int32_t)rows, (int32_t)K, q,
+                                      (K + 15) / 16 * 16, scale, stream);
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize(const at::Tensor &x, int64_t block_rows)
+{
+    if (block_rows != 1 && block_rows != 128)
+        throw std::invalid_argument("block_rows must be 1 or 128, got " + std::to_string(block_rows) + " !\n");
+    check_floats(x, block_rows);
     if (x.requires_grad() && at::GradMode::is_enabled())
         throw std::invalid_argument("quantize_fp8 has no gradient: call it under torch.no_grad(), or on x.detach() !\n");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     std::vector<int64_t> blocks = x.sizes().vec();
-    blocks.back() = (K + 127) / 128;
+    blocks.back() = (x.size(-1) + 127) / 128;
     if (block_rows == 128) blocks[0] = (blocks[0] + 127) / 128;
     at::Tensor q = rows_of_16_bytes(x.sizes().vec(), x.device());
     at::Tensor scale = at::empty(blocks, at::TensorOptions().dtype(at::kFloat).device(x.device()));
-    if (!rows) return {q, scale};
-    const at::Tensor flat = x.reshape({rows, K});
-    const int rc = rs_quantize_blocks(flat.data_ptr(), dtype, flat.stride(0), (int32_t)block_rows, (int32_t)rows, (int32_t)K, q.data_ptr(),
-                                      (K + 15) / 16 * 16, scale.data_ptr<float>(), current_stream(x));
-    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    if (x.numel()) quantize_into(x, block_rows, q.data_ptr(), scale.data_ptr<float>(), current_stream(x));
     return {q, scale};
 }
 
@@ -498,6 +508,7 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const at::Tenso
         throw std::invalid_argument("linear_fp8 has no gradient: call it under torch.no_grad(), or on x.detach() !\n");
     const int64_t K = weight.size(1), N = weight.size(0), blocks = (K + 127) / 128, M = x.numel() / K;
     if (M > RS_LINEAR_MAX || N > RS_LINEAR_MAX || K > RS_LINEAR_MAX) throw std::invalid_argument("x or weight is too large !\n");
+    if (!given) check_floats(x, 1);
     const at::Tensor w = fp8_rows(weight, "weight");
     check_scale(weight_scale, weight, (N + 127) / 128, blocks, "weight_scale");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
@@ -505,14 +516,37 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const at::Tenso
     sizes.back() = N;
     at::Tensor y = at::empty(sizes, at::TensorOptions().dtype(to).device(x.device()));
     if (!M) return y;
-    at::Tensor q, scale;
-    if (given) { q = x; scale = *x_scale; check_scale(scale, x, M, blocks, "x_scale"); }
-    else std::tie(q, scale) = quantize(x, 1);
-    q = fp8_rows(q, "x");
+    // One launch for a few rows, where the launch that it saves (2 to 5 us) is more than what the workgroups spend on rounding the same
+    // rows each for itself: 1 x 8192 x 4096 7.7 us against 12.5, 1 x 65536 x 4096 52.8 either way, 4 x 16384 x 4096 16.3
+    // against 18.0, 4 x 65536 x 4096 59.4 against 55.7.
+    if (!given && M <= RS_LINEAR_ROWS_MAX && M * N <= 65536 && K <= RS_LINEAR_ROWS_COLUMNS_MAX) {
+        const at::Tensor flat = x.dim() == 2 ? x : x.reshape({M, K});
+        const int rc = rs_linear_rows(flat.data_ptr(), float_dtype(x, "x"), flat.stride(0), w.data_ptr(), w.stride(0), weight_scale.data_ptr<float>(),
+                                      (int32_t)M, (int32_t)N, (int32_t)K, y.data_ptr(), float_dtype(y, "y"), N, current_stream(x));
+        if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+        return y;
+    }
+    // x's rows in 8 bits and their scales: as given, or made here, side by side in one buffer
+    at::Tensor held;
+    const void *q;
+    const float *scale;
+    int64_t q_stride = (K + 15) / 16 * 16;
     void *stream = current_stream(x);
+    if (given) {
+        check_scale(*x_scale, x, M, blocks, "x_scale");
+        held = fp8_rows(x, "x");
+        q = held.data_ptr();
+        q_stride = held.stride(0);
+        scale = x_scale->data_ptr<float>();
+    } else {
+        held = at::empty({M * (q_stride + blocks * 4)}, at::TensorOptions().dtype(at::kByte).device(x.device()));
+        q = held.data_ptr();
+        scale = (const float *)((const char *)q + M * q_stride);
+        quantize_into(x, 1, (void *)q, (float *)scale, stream);
+    }
     at::Tensor &ws = linear_workspace(x, stream);
-    const int rc = rs_linear_blocks(q.data_ptr(), q.stride(0), scale.data_ptr<float>(), w.data_ptr(), w.stride(0), weight_scale.data_ptr<float>(),
-                                    (int32_t)M, (int32_t)N, (int32_t)K, y.data_ptr(), float_dtype(y, "y"), N, ws.data_ptr(), (size_t)ws.numel(), stream);
+    const int rc = rs_linear_blocks(q, q_stride, scale, w.data_ptr(), w.stride(0), weight_scale.data_ptr<float>(), (int32_t)M, (int32_t)N, (int32_t)K,
+                                    y.data_ptr(), float_dtype(y, "y"), N, ws.data_ptr(), (size_t)ws.numel(), stream);
     if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
     return y;
 }

@@ -90,7 +90,7 @@ def test_quantize_extremes_and_strides():
 
 
 @gpu
-@pytest.mark.parametrize("M,K,N", [(1, 16, 1), (1, 100, 50), (2, 128, 16), (1, 4096, 1000), (5, 1000, 257), (16, 512, 384), (17, 256, 129), (33, 2000, 515),
+@pytest.mark.parametrize("M,K,N", [(1, 16, 1), (1, 100, 50), (2, 128, 16), (1, 4096, 1000), (4, 8192, 70), (3, 8200, 40), (4, 1999, 9000), (5, 1000, 257), (16, 512, 384), (17, 256, 129), (33, 2000, 515),
                                    (64, 144, 640), (77, 2000, 1037), (128, 1024, 256), (129, 128, 128), (257, 300, 700), (512, 2048, 1024), (300, 1, 5)])
 @pytest.mark.parametrize("out", list(DTYPES))
 def test_product(M, K, N, out):
@@ -236,3 +236,10 @@ def test_refusals_of_the_c_abi():
     assert linear(ws_at=264) == linear(ws_bytes=n - 1) == -5
     assert linear(M=0) == linear(N=0) == linear(K=0) == linear(xs=16) == linear(ws=16) == linear(ys=19) == -12
     assert linear(x=264) == linear(w=260) == linear(xs=40) == linear(ws=40) == linear(y=258) == -6
+
+    L.rs_linear_rows.argtypes = [p, i32, i64, p, i64, p, i32, i32, i32, p, i32, i64, p]
+
+    def rows(x=256, dtype=0, w=256, ws=32, sw=256, M=2, N=20, K=20, y=256, y_dtype=0, ys=20):
+        return L.rs_linear_rows(x, dtype, K, w, ws, sw, M, N, K, y, y_dtype, ys, None)
+    assert rows(x=None) == rows(w=None) == rows(sw=None) == rows(y=None) == -4 and rows(dtype=3) == rows(y_dtype=-1) == -7
+    assert rows(M=0) == rows(M=5) == rows(K=8193, ws=8208) == rows(ws=16) == rows(ys=19) == -12 and rows(x=258) == rows(w=260) == rows(ws=40) == -6
