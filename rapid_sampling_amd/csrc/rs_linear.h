@@ -396,6 +396,8 @@ struct LinearTile {
     static_assert(kRows * 8 % kThreads == 0 && kTileN * 8 % kThreads == 0 && kTileN <= 256 && kTileM <= 256, "whole loads; 32-bit offsets");
     static_assert(kWaves % 4 == 0, "w_turn is the same for every load of a thread, or for every other one");
     static_assert(NU == 4 || NU == 8, "");
+    static constexpr int kBufferFlags = 0x00027000;              // untyped, offsets in bytes
+    static constexpr bool kWhole = kWaves == 8;                  // K has to be a whole number of blocks: no registers to spare for anything else
 
     // A wave fills eight rows of a stage with one load: the thread's row of load i, w's rows first.
     static __device__ __forceinline__ uint32_t row_of(uint32_t i) { return (i * kWaves + wave_id()) * 8u + threadIdx.x % 64u / 8u; }
@@ -408,14 +410,13 @@ struct LinearTile {
     };
     static __device__ __forceinline__ Source source(const LinearParams &p, uint32_t n0, uint32_t m0)
     {
-        constexpr int kFlags = 0x00027000;     // untyped, offsets in bytes
         Source s;
         s.w_stride = (uint32_t)p.w_stride;
         s.x_stride = (uint32_t)p.x_stride;
         const uint32_t rows_w = min(p.N - n0, kTileN), rows_x = min(p.M - m0, kTileM);
         const uint32_t bytes = (p.K + 3u) & ~3u;       // of the last row, in whole words: a word is read or it is not
-        s.w = __builtin_amdgcn_make_buffer_rsrc((void *)(p.w + (int64_t)n0 * p.w_stride), 0, (int)((rows_w - 1u) * s.w_stride + bytes), kFlags);
-        s.x = __builtin_amdgcn_make_buffer_rsrc((void *)(p.x + (int64_t)m0 * p.x_stride), 0, (int)((rows_x - 1u) * s.x_stride + bytes), kFlags);
+        s.w = __builtin_amdgcn_make_buffer_rsrc((void *)(p.w + (int64_t)n0 * p.w_stride), 0, (int)((rows_w - 1u) * s.w_stride + bytes), kBufferFlags);
+        s.x = __builtin_amdgcn_make_buffer_rsrc((void *)(p.x + (int64_t)m0 * p.x_stride), 0, (int)((rows_x - 1u) * s.x_stride + bytes), kBufferFlags);
         const uint32_t r = row_of(0);
         for (uint32_t i = 0; i < 2; ++i) s.w_at[i] = r * s.w_stride + ((threadIdx.x & 7u) ^ w_turn<NU>(r + i * 8u * kWaves)) * 16u;
         s.x_at = r * s.x_stride + ((threadIdx.x & 7u) ^ x_turn(r)) * 16u;
@@ -424,7 +425,7 @@ struct LinearTile {
     static __device__ __forceinline__ void fill(const LinearParams &p, const Source &s, uint32_t n0, uint32_t m0, uint32_t kb, uint8_t *lds)
     {
         const uint32_t k = kb * kFpBlock;
-        if (k + kFpBlock <= p.K) {
+        if (kWhole || k + kFpBlock <= p.K) {
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
                 const LdsPtr to = (LdsPtr)(lds + (i * kWaves + wave_id()) * 1024u);
@@ -434,26 +435,20 @@ struct LinearTile {
             return;
         }
         // the last block where K is no whole number of them: through registers, with the bytes from K on cleared
-        constexpr uint32_t kAtOnce = MT > 2 ? 2 : kLoads;
-        static_assert(kLoads % kAtOnce == 0, "");
-#pragma unroll 1
-        for (uint32_t i0 = 0; i0 < kLoads; i0 += kAtOnce) {
-            v4i v[kAtOnce];
+        if constexpr (kWhole) return;
+        v4i v[kLoads];
 #pragma unroll
-            for (uint32_t o = 0; o < kAtOnce; ++o) {
-                const uint32_t i = i0 + o;
-                if (i < kLoadsW) v[o] = __builtin_amdgcn_raw_buffer_load_b128(s.w, kWaves % 8 && i % 2 ? s.w_at[1] : s.w_at[0], k + i * 8u * kWaves * s.w_stride, 0);
-                else v[o] = __builtin_amdgcn_raw_buffer_load_b128(s.x, s.x_at, k + (i - kLoadsW) * 8u * kWaves * s.x_stride, 0);
-            }
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            if (i < kLoadsW) v[i] = __builtin_amdgcn_raw_buffer_load_b128(s.w, kWaves % 8 && i % 2 ? s.w_at[1] : s.w_at[0], k + i * 8u * kWaves * s.w_stride, 0);
+            else v[i] = __builtin_amdgcn_raw_buffer_load_b128(s.x, s.x_at, k + (i - kLoadsW) * 8u * kWaves * s.x_stride, 0);
+        }
 #pragma unroll
-            for (uint32_t o = 0; o < kAtOnce; ++o) {
-                const uint32_t i = i0 + o;
-                const uint32_t r = row_of(i) - (i < kLoadsW ? 0u : kTileN);
-                const int32_t left = (int32_t)(p.K - k) - (int32_t)(((threadIdx.x & 7u) ^ (i < kLoadsW ? w_turn<NU>(r) : x_turn(r))) * 16u);
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            const uint32_t r = row_of(i) - (i < kLoadsW ? 0u : kTileN);
+            const int32_t left = (int32_t)(p.K - k) - (int32_t)(((threadIdx.x & 7u) ^ (i < kLoadsW ? w_turn<NU>(r) : x_turn(r))) * 16u);
 #pragma unroll
-                for (int d = 0; d < 4; ++d) v[o][d] &= left >= 4 * d + 4 ? -1 : left <= 4 * d ? 0 : (1 << 8 * (left - 4 * d)) - 1;
-                *(v4i *)(lds + row_of(i) * kFpBlock + (threadIdx.x & 7u) * 16u) = v[o];
-            }
+            for (int d = 0; d < 4; ++d) v[i][d] &= left >= 4 * d + 4 ? -1 : left <= 4 * d ? 0 : (1 << 8 * (left - 4 * d)) - 1;
+            *(v4i *)(lds + row_of(i) * kFpBlock + (threadIdx.x & 7u) * 16u) = v[i];
         }
         wait_vmem();
     }
@@ -493,20 +488,18 @@ struct LinearTile {
                 const uint32_t r = r0 + (u + 1) * 4u;
                 ahead = fragment(now_lds, r, w_turn<NU>(r), part);
             }
-            v4f made[MT];
             v8bf wb[4];
             if constexpr (EXACT) widen_block(w, wb);
+            // (the sums of the row of products before, each behind a product of this one)
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                if constexpr (EXACT) made[t] = block_product(wb, xb[t]);
-                else made[t] = block_product_8(w, x[t]);
-            }
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
+                v4f made;
+                if constexpr (EXACT) made = block_product(wb, xb[t]);
+                else made = block_product_8(w, x[t]);
                 if (u)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[u - 1][t][j] = __builtin_fmaf(s[t][j], f[t], acc[u - 1][t][j]);
-                s[t] = made[t];
+                s[t] = made;
             }
             w = ahead;
         }
@@ -517,7 +510,7 @@ struct LinearTile {
     }
 };
 
-template <int DT, int WN, int WM, int NU, int MT, int STAGES, bool EXACT>
+template <int DT, int WN, int WM, int NU, int MT, int STAGES, bool EXACT, bool SPLIT>
 __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearParams p)
 {
     using L = LinearTile<WN, WM, NU, MT, STAGES, EXACT>;
@@ -526,7 +519,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearPara
     // Workgroup b runs on XCD b % 8: each XCD takes a stretch of the tiles, in panels of eight rows of tiles, so that the 32 tiles
     // it works on at a time share their rows in its L2.
     uint32_t id = blockIdx.x, part_of = 0;
-    if (p.split > 1u) { part_of = id / tiles; id -= part_of * tiles; }
+    if (SPLIT && p.split > 1u) { part_of = id / tiles; id -= part_of * tiles; }
     else {
         const uint32_t each = tiles / 8u, rest = tiles % 8u, xcd = id % 8u;
         id = xcd * each + min(xcd, rest) + id / 8u;
@@ -538,14 +531,16 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearPara
     const uint32_t wave = wave_id(), lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
     const uint32_t wn = wave % WN * (16u * NU), wm = wave / WN * (16u * MT);
     const float *sw = p.w_scale + (size_t)min((n0 + wn) / kFpBlock, (p.N - 1u) / kFpBlock) * p.blocks;
-    const float *sx[MT];
+    // x's scales as a buffer as well: one address register for all rows, and 0 behind the last
+    const __amdgpu_buffer_rsrc_t sx = __builtin_amdgcn_make_buffer_rsrc((void *)(p.x_scale + (size_t)m0 * p.blocks), 0,
+                                                                        (int)(min(p.M - m0, L::kTileM) * p.blocks * 4u), L::kBufferFlags);
+    const uint32_t sx_at = (wm + i) * p.blocks * 4u;
+    auto x_scale = [&](int t, uint32_t kb) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sx, sx_at, (t * 16u * p.blocks + kb) * 4u, 0)); };
     v4f acc[NU][MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        sx[t] = p.x_scale + (size_t)min(m0 + wm + t * 16u + i, p.M - 1u) * p.blocks;
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int u = 0; u < NU; ++u) acc[u][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    }
     // Where w is read once, by one row of tiles, every workgroup begins at another block: rows are usually a power of two of bytes
     // apart, and workgroups in step would ask the same memory channels at a time.
     uint32_t first = tm == 1u ? kb0 + tile_n % count : kb0;
@@ -555,7 +550,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearPara
     float f[MT], ahead[MT], ahead_w = sw[first];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        ahead[t] = sx[t][first];
+        ahead[t] = x_scale(t, first);
         asm volatile("" : "+v"(ahead[t]));       // here, and not in the loop, where it would wait for the next block's
     }
     uint32_t kb = first, to_fill = first;
@@ -572,13 +567,13 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearPara
         kb = after(kb);
         ahead_w = sw[kb];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) ahead[t] = sx[t][kb];
+        for (int t = 0; t < MT; ++t) ahead[t] = x_scale(t, kb);
         L::step(p, source, n0, m0, to_fill, j + STAGES - 1u < count, lds + now, lds + next, f, acc);
         to_fill = after(to_fill);
         now = now == (STAGES - 1) * L::kStage ? 0u : now + L::kStage;
         next = next == (STAGES - 1) * L::kStage ? 0u : next + L::kStage;
     }
-    if (p.split > 1u) {
+    if (SPLIT && p.split > 1u) {
         // every workgroup leaves its sums; the last of the tile's adds them up, in the order of the blocks
         constexpr uint32_t kPart = L::kThreads * NU * MT * 2;
         uint64_t *parts = (uint64_t *)p.parts + (size_t)id * p.split * kPart + threadIdx.x;

@@ -26,7 +26,7 @@ static hipError_t launch_tiles(LinearParams p, hipStream_t st)
     const uint64_t tiles = (uint64_t)((p.M + L::kTileM - 1) / L::kTileM) * ((p.N + L::kTileN - 1) / L::kTileN);
     if (tiles > 0x7FFFFFFF) return hipErrorInvalidValue;
     p.split = SPLIT ? (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({kPartTiles / tiles, p.blocks / (EXACT ? 4 : 8), 8})) : 1;
-    hipLaunchKernelGGL((linear_tile_kernel<DT, WN, WM, NU, MT, STAGES, EXACT>), dim3((uint32_t)tiles * p.split), dim3(L::kThreads), L::kLds, st, p);
+    hipLaunchKernelGGL((linear_tile_kernel<DT, WN, WM, NU, MT, STAGES, EXACT, SPLIT>), dim3((uint32_t)tiles * p.split), dim3(L::kThreads), L::kLds, st, p);
     return hipGetLastError();
 }
 
@@ -74,7 +74,7 @@ static hipError_t launch_linear(const LinearParams &p, hipStream_t st)
         // 256 x 256 where that fills the card and wastes little: 8192^3 536 against 612 in tiles of 128 x 128, 2048 x 16384 x 2048 85
         // against 92; but 128 x 131072 x 4096 143 against 129
         const uint64_t n256 = (p.N + 255) / 256, m256 = (p.M + 255) / 256;
-        if (n256 * m256 >= 256 && 20 * m256 <= 11 * m128) return launch_tiles<DT, 2, 4, 8, 4, 2, false, false>(p, st);
+        if (p.K % kFpBlock == 0 && n256 * m256 >= 256 && 20 * m256 <= 11 * m128) return launch_tiles<DT, 2, 4, 8, 4, 2, false, false>(p, st);
         return launch_tiles<DT, 1, 4, 8, 2, 2, false, false>(p, st);
     }
 }
