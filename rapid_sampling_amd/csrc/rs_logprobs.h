@@ -14,13 +14,12 @@
 
 namespace rs {
 
-constexpr int kLpThreads = 256;
-constexpr int kLpWaves   = kLpThreads / kWave;
+constexpr int kLpThreads = 256;          // of a workgroup; NT below is this or, for short rows, a single wave
 constexpr int kLpTopMax  = RS_LOGPROBS_TOP_MAX;
-constexpr int kLpCap     = 512;          // candidates that are put in order
+template <int NT> constexpr int kLpCap = NT == kLpThreads ? 512 : 384;      // candidates that are put in order
 constexpr int kLpSegs    = 8;            // stretches that a thread's windows of a slice are divided into, at most
 constexpr int kLpStretches = 32;         // ... and a row's, where it is split
-constexpr int kLpUnits   = 1024;         // stretches that are read again
+template <int NT> constexpr int kLpUnits = NT == kLpThreads ? 1024 : 512;   // stretches that are read again
 constexpr float kLn2 = 0.693147180559945309f;
 
 // What a workgroup of a split row leaves for the last of the row's workgroups.
@@ -211,22 +210,24 @@ __device__ __forceinline__ void lp_wave(LpSums &a, float c)
     a.t = wave_sum_f(a.t);
 }
 
+template <int NT>
 struct LpShared {
-    float    m[kLpWaves], s[kLpWaves], t[kLpWaves];
-    uint32_t above[kLpWaves];
-    uint32_t key[kLpThreads];            // order key of each thread's largest logit
+    float    m[NT / kWave], s[NT / kWave], t[NT / kWave];
+    uint32_t above[NT / kWave];
+    uint32_t key[NT];            // order key of each thread's largest logit
     union {
-        float    seg[kLpSegs][kLpThreads];      // largest logit of each stretch (rows that are not split)
-        uint64_t lane_top[kLpThreads];
+        float    seg[kLpSegs][NT];      // largest logit of each stretch (rows that are not split)
+        uint64_t lane_top[NT];
     };
-    uint64_t cand[kLpCap];
-    uint32_t unit[kLpUnits];             // stretches to read again: stretch << 8 | thread
+    uint64_t cand[kLpCap<NT>];
+    uint32_t unit[kLpUnits<NT>];             // stretches to read again: stretch << 8 | thread
     uint32_t n, n_units;
     uint32_t last;
 };
 
 // The sums of the workgroup, in every thread.
-__device__ __forceinline__ void lp_block(LpSums &a, uint32_t &above, float c, LpShared &sh)
+template <int NT>
+__device__ __forceinline__ void lp_block(LpSums &a, uint32_t &above, float c, LpShared<NT> &sh)
 {
     const uint32_t w = threadIdx.x / kWave;
     lp_wave(a, c);
@@ -234,11 +235,11 @@ __device__ __forceinline__ void lp_block(LpSums &a, uint32_t &above, float c, Lp
     __syncthreads();
     float m = sh.m[0];
 #pragma unroll
-    for (int i = 1; i < kLpWaves; ++i) m = fmaxf(m, sh.m[i]);
+    for (int i = 1; i < (NT / kWave); ++i) m = fmaxf(m, sh.m[i]);
     LpSums all{m, 0.0f, 0.0f};
     above = 0;
 #pragma unroll
-    for (int i = 0; i < kLpWaves; ++i) {
+    for (int i = 0; i < (NT / kWave); ++i) {
         LpSums one{sh.m[i], sh.s[i], sh.t[i]};
         lp_rebase(one, m, c);
         all.s += one.s; all.t += one.t;
@@ -259,35 +260,35 @@ __device__ __forceinline__ void lp_block(LpSums &a, uint32_t &above, float c, Lp
 // the range of the bound until it does.  That ends: the orders are distinct.  (Cutting lists of more than 128 as well made rows of
 // 131072 uniform bfloat16 logits slower, 26 us in the place of 18.)  Where there are more such stretches than can be noted, the
 // whole row is read in their place: one of 131072 equal logits takes 69 us, 64 of them 84.
-template <int DT>
+template <int DT, int NT>
 struct LpRow {
     using E = Elem<DT>;
     const typename E::T *row;
     uint32_t V, full, J, seg_log, segs;  // logits; whole windows; windows of a thread in a slice, stretches in a slice
 
     // A list that has outgrown its room is made again: the rest of the row need not be looked at for it.
-    static __device__ __forceinline__ bool full_list(const LpShared &sh) { return *(const volatile uint32_t *)&sh.n > (uint32_t)kLpCap; }
+    static __device__ __forceinline__ bool full_list(const LpShared<NT> &sh) { return *(const volatile uint32_t *)&sh.n > (uint32_t)kLpCap<NT>; }
     template <typename F> __device__ __forceinline__ void tail(F f) const
     {
         const uint32_t i = full * E::kVec + threadIdx.x;
         if (i < V) f(E::one(row[i]), i);
     }
     // f(logit, index) for the windows of the stretches in sh.unit and the row's last few logits
-    template <typename F> __device__ __forceinline__ void units(const LpShared &sh, uint32_t n_units, float least, bool listing, F f) const
+    template <typename F> __device__ __forceinline__ void units(const LpShared<NT> &sh, uint32_t n_units, float least, bool listing, F f) const
     {
         constexpr int U = 4;
         const uint32_t items = n_units << seg_log, mask = (1u << seg_log) - 1u;
-        for (uint32_t i = threadIdx.x; i < items; i += U * kLpThreads) {
+        for (uint32_t i = threadIdx.x; i < items; i += U * NT) {
             if (listing && full_list(sh)) break;
             uint4 raw[U];
             uint32_t n[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const uint32_t at = i + u * kLpThreads;
+                const uint32_t at = i + u * NT;
                 n[u] = full;
                 if (at < items) {
                     const uint32_t unit = sh.unit[at >> seg_log], slice = (unit >> 8) / segs, j = (((unit >> 8) - slice * segs) << seg_log) + (at & mask);
-                    if (j < J) n[u] = (slice * J + j) * kLpThreads + (unit & 255u);
+                    if (j < J) n[u] = (slice * J + j) * NT + (unit & 255u);
                 }
                 if (n[u] < full) raw[u] = load_window<DT>(row, n[u]);
             }
@@ -307,17 +308,17 @@ struct LpRow {
         tail(f);
     }
     // ... for the whole row
-    template <typename F> __device__ __forceinline__ void all(const LpShared &sh, bool listing, F f) const
+    template <typename F> __device__ __forceinline__ void all(const LpShared<NT> &sh, bool listing, F f) const
     {
         constexpr int U = 4;
-        for (uint32_t n0 = threadIdx.x; n0 < full; n0 += U * kLpThreads) {
+        for (uint32_t n0 = threadIdx.x; n0 < full; n0 += U * NT) {
             if (listing && full_list(sh)) break;
             uint4 raw[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) if (n0 + u * kLpThreads < full) raw[u] = load_window<DT>(row, n0 + u * kLpThreads);
+            for (int u = 0; u < U; ++u) if (n0 + u * NT < full) raw[u] = load_window<DT>(row, n0 + u * NT);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const uint32_t n = n0 + u * kLpThreads;
+                const uint32_t n = n0 + u * NT;
                 if (n >= full) continue;
                 float x[E::kVec];
                 E::wide(raw[u], x);
@@ -331,20 +332,20 @@ struct LpRow {
 
 // A t with at least `k` and, unless keys are equal, at most k + spare of the workgroup's keys >= t; only the upper BITS bits matter.
 // No key is larger than `most`.
-template <int BITS, typename K>
+template <int BITS, int NT, typename K>
 __device__ __forceinline__ K lp_kth(const K *key, uint32_t k, uint32_t spare, K most)
 {
     constexpr int kAll = (int)sizeof(K) * 8;
-    K mine[kLpWaves];
+    K mine[NT / kWave];
 #pragma unroll
-    for (int i = 0; i < kLpWaves; ++i) mine[i] = key[i * kWave + threadIdx.x % kWave];
+    for (int i = 0; i < (NT / kWave); ++i) mine[i] = key[i * kWave + threadIdx.x % kWave];
     K t = 0;
     for (int bit = kAll - 1; bit >= kAll - BITS; --bit) {
         const K c = t | (K)1 << bit;
         if (c > most) continue;
         uint32_t n = 0;
 #pragma unroll
-        for (int i = 0; i < kLpWaves; ++i) n += (uint32_t)__popcll(__ballot(mine[i] >= c));
+        for (int i = 0; i < (NT / kWave); ++i) n += (uint32_t)__popcll(__ballot(mine[i] >= c));
         if (n >= k) t = c;
         if (n >= k && n <= k + spare) break;
     }
@@ -352,15 +353,15 @@ __device__ __forceinline__ K lp_kth(const K *key, uint32_t k, uint32_t spare, K 
 }
 
 // seg[s] is the thread's largest logit of stretch s of the row, `largest` the largest of those.
-template <int DT, int N>
-__device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float largest, const float (&seg)[N], const LpSums &a, float log_s, float inv_t,
-                                                uint32_t top, float *out_logprobs, int32_t *out_tokens, LpShared &sh)
+template <int DT, int NT, int N>
+__device__ __forceinline__ void lp_alternatives(const LpRow<DT, NT> &row, float largest, const float (&seg)[N], const LpSums &a, float log_s, float inv_t,
+                                                uint32_t top, float *out_logprobs, int32_t *out_tokens, LpShared<NT> &sh)
 {
     const uint32_t tid = threadIdx.x, lane = tid % kWave, w = tid / kWave;
     sh.key[tid] = lp_key(largest);
     if (tid == 0) sh.n = sh.n_units = 0;
     __syncthreads();
-    uint32_t tau = lp_kth<Elem<DT>::kBits>(sh.key, top, top / 4u, uniform(lp_key(a.m)));
+    uint32_t tau = lp_kth<Elem<DT>::kBits, NT>(sh.key, top, top / 4u, uniform(lp_key(a.m)));
     if (tau <= fkey(-__builtin_inff())) tau = 1u;        // fewer numbers than are wanted, perhaps: NaN too
     const float least = fkey_inv(tau);
     if (tau != 1u) {
@@ -368,7 +369,7 @@ __device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float larg
         for (int i = 0; i < N; ++i)
             if (seg[i] >= least) {
                 const uint32_t at = atomicAdd(&sh.n_units, 1u);
-                if (at < kLpUnits) sh.unit[at] = (uint32_t)i << 8 | tid;
+                if (at < kLpUnits<NT>) sh.unit[at] = (uint32_t)i << 8 | tid;
             }
         __syncthreads();
     }
@@ -377,32 +378,32 @@ __device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float larg
             const uint64_t k = lp_token(x, i);
             if (k >= from) {
                 const uint32_t at = atomicAdd(&sh.n, 1u);
-                if (at < kLpCap) sh.cand[at] = k;
+                if (at < kLpCap<NT>) sh.cand[at] = k;
             }
         };
     };
     const uint64_t from = (uint64_t)tau << 32;
     const uint32_t n_units = sh.n_units;
     auto walk = [&](bool listing, auto f) {
-        if (tau != 1u && n_units <= (uint32_t)kLpUnits) row.units(sh, n_units, least, listing, f);
+        if (tau != 1u && n_units <= (uint32_t)kLpUnits<NT>) row.units(sh, n_units, least, listing, f);
         else row.all(sh, listing, f);
     };
     walk(true, list(from));
     __syncthreads();
-    if (sh.n > (uint32_t)kLpCap) {
+    if (sh.n > (uint32_t)kLpCap<NT>) {
         uint64_t best = 0;
         walk(false, [&](float x, uint32_t i) { best = max(best, lp_token(x, i)); });
         __syncthreads();                                 // (the stretches' room is used again)
         sh.lane_top[tid] = best;
         __syncthreads();
-        uint64_t lo = max(lp_kth<64>(sh.lane_top, top, 0u, (uint64_t)~0ull), from), hi = ~0ull;
+        uint64_t lo = max(lp_kth<64, NT>(sh.lane_top, top, 0u, (uint64_t)~0ull), from), hi = ~0ull;
         for (uint64_t t = lo;; t = lo + (hi - lo) / 2) {
             __syncthreads();
             if (tid == 0) sh.n = 0;
             __syncthreads();
             walk(true, list(t));
             __syncthreads();
-            if (sh.n > (uint32_t)kLpCap) lo = t;
+            if (sh.n > (uint32_t)kLpCap<NT>) lo = t;
             else if (sh.n < top) hi = t;
             else break;
         }
@@ -422,7 +423,7 @@ __device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float larg
         if (lane < n) put(mine, place);
         return;
     }
-    for (uint32_t i = tid; i < n; i += kLpThreads) {
+    for (uint32_t i = tid; i < n; i += NT) {
         const uint64_t k = sh.cand[i];
         uint32_t place = 0;
 #pragma unroll 8
@@ -433,18 +434,18 @@ __device__ __forceinline__ void lp_alternatives(const LpRow<DT> &row, float larg
 
 // ------------------------------------------------------------------- forward --
 // U windows of each thread, whole ones below `full` only.  A batch is asked for before the one before it is worked on.
-template <int DT, int U>
+template <int DT, int NT, int U>
 __device__ __forceinline__ void lp_ask(const typename Elem<DT>::T *row, uint32_t n0, uint32_t full, uint4 (&raw)[U])
 {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t n = n0 + u * kLpThreads;
+        const uint32_t n = n0 + u * NT;
         if (n < full) raw[u] = load_window<DT>(row, n);
     }
 }
 
 // Returns the largest logit of the batch.  GUARD: lanes whose window is not below `full` have none.
-template <int DT, int U, bool GUARD>
+template <int DT, int NT, int U, bool GUARD>
 __device__ __forceinline__ float lp_batch(const uint4 *raw, uint32_t n0, uint32_t full, uint32_t token_window, float before, float after,
                                           float c, LpSums &a, uint32_t &above)
 {
@@ -452,7 +453,7 @@ __device__ __forceinline__ float lp_batch(const uint4 *raw, uint32_t n0, uint32_
     float x[U * E::kVec], edge[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t n = n0 + u * kLpThreads;
+        const uint32_t n = n0 + u * NT;
         float v[E::kVec];
         E::wide(raw[u], v);
         edge[u] = n < token_window ? before : after;
@@ -472,21 +473,25 @@ __device__ __forceinline__ float lp_stretch(const LpSlice *slices, uint32_t segs
     return a_load(&slices[slice].seg[s - slice * segs][tid]);
 }
 
-// One workgroup per row, or S of them (SPLIT), each on a stretch of the row, of which the last to arrive finishes the row.
-// Nothing waits.
-template <int DT, bool SPLIT>
-__global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
+// One workgroup of NT threads per row, or S of them (SPLIT), each on a stretch of the row, of which the last to arrive finishes the
+// row.  Nothing waits.  One pass over the logits with each thread's running maximum and sums, two batches of 64 bytes a thread
+// under way.  Bound by the memory where there are rows enough: 8192 x 131072 bfloat16 logits with 20 alternatives 382 us,
+// 5.6 TB/s; a call of one row by its chain of loads: the token, its logit, the slices' sums, the stretches, their windows
+// (1 x 65536 float32 with 5 alternatives 9.3 us, without any 4.8).
+template <int DT, int NT, bool SPLIT>
+__global__ __launch_bounds__(NT) void logprobs_kernel(LpParams p)
 {
     using E = Elem<DT>;
     constexpr int U = 4;
-    __shared__ LpShared sh;
+    static_assert(!SPLIT || NT == kLpThreads, "what the slices leave is of that many threads");
+    __shared__ LpShared<NT> sh;
     const uint32_t r = SPLIT ? blockIdx.x / p.S : blockIdx.x, slice = SPLIT ? blockIdx.x - r * p.S : 0;
     const uint32_t b = r / (uint32_t)p.T, pos = r - b * (uint32_t)p.T;
     const uint32_t V = (uint32_t)p.V, full = V / E::kVec, tid = threadIdx.x;
     const typename E::T *row = (const typename E::T *)p.logits + (int64_t)b * p.stride_b + (int64_t)pos * p.stride_t;
-    const uint32_t first = slice * p.J * kLpThreads, end = min(full, first + p.J * kLpThreads);
+    const uint32_t first = slice * p.J * NT, end = min(full, first + p.J * NT);
     uint4 raw[U];
-    lp_ask<DT, U>(row, first + tid, end, raw);
+    lp_ask<DT, NT, U>(row, first + tid, end, raw);
     const uint32_t last = full * E::kVec + tid;          // the row's last few logits
     const bool has_last = (!SPLIT || slice == p.S - 1u) && last < V;
     const float x_last = has_last ? E::one(row[last]) : -__builtin_inff();
@@ -510,14 +515,14 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
     LpSums a{-__builtin_inff(), 0.0f, 0.0f};
     uint32_t above = 0, n = first;
     float seg = -__builtin_inff();
-    for (; n + U * kLpThreads <= end; ) {
+    for (; n + U * NT <= end; ) {
         uint4 now[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) now[u] = raw[u];
-        lp_ask<DT, U>(row, n + U * kLpThreads + tid, end, raw);
-        seg = fmaxf(seg, lp_batch<DT, U, false>(now, n + tid, end, token_window, before, after, p.c, a, above));
-        n += U * kLpThreads;
-        const uint32_t j = (n - first) / kLpThreads;
+        lp_ask<DT, NT, U>(row, n + U * NT + tid, end, raw);
+        seg = fmaxf(seg, lp_batch<DT, NT, U, false>(now, n + tid, end, token_window, before, after, p.c, a, above));
+        n += U * NT;
+        const uint32_t j = (n - first) / NT;
         if (!(j & ((1u << p.seg_log) - 1u))) {
             if (p.top) sh.seg[(j >> p.seg_log) - 1u][tid] = seg;
             seg = -__builtin_inff();
@@ -525,11 +530,11 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-        if (n + u * kLpThreads < end) seg = fmaxf(seg, lp_batch<DT, 1, true>(raw + u, n + u * kLpThreads + tid, end, token_window, before, after, p.c, a, above));
+        if (n + u * NT < end) seg = fmaxf(seg, lp_batch<DT, NT, 1, true>(raw + u, n + u * NT + tid, end, token_window, before, after, p.c, a, above));
     const uint32_t segs = (p.J + (1u << p.seg_log) - 1u) >> p.seg_log;
     if (p.top) {
         // the stretch that the slice ends in, and those behind it
-        for (uint32_t g = end > first ? (end - first) / kLpThreads >> p.seg_log : 0u; g < segs; ++g) {
+        for (uint32_t g = end > first ? (end - first) / NT >> p.seg_log : 0u; g < segs; ++g) {
             sh.seg[g][tid] = seg;
             seg = -__builtin_inff();
         }
@@ -598,33 +603,37 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LpParams p)
         }
     }
     if (p.top) {
-        const LpRow<DT> whole{row, V, full, p.J, p.seg_log, segs};
+        const LpRow<DT, NT> whole{row, V, full, p.J, p.seg_log, segs};
         float *const lps = p.top_logprobs + (size_t)r * p.top;
         int32_t *const ids = p.top_tokens + (size_t)r * p.top;
         if constexpr (!SPLIT)
 #pragma unroll
             for (int s = 0; s < kLpSegs; ++s) seg_of[s] = s < (int)segs ? sh.seg[s][tid] : -__builtin_inff();
-        lp_alternatives<DT>(whole, mine, seg_of, a, log_s, p.inv_t, (uint32_t)p.top, lps, ids, sh);
+        lp_alternatives<DT, NT>(whole, mine, seg_of, a, log_s, p.inv_t, (uint32_t)p.top, lps, ids, sh);
     }
 }
 
 // ------------------------------------------------------------------ gradient --
-// dx_i = p_i (alpha + beta ln2 (z_i - ..)): one exponential and a product per logit; the few tokens that were named are then
-// written once more, whole, by the workgroup that wrote them first.
+// dx_i = p_i (alpha + beta log2 p_i), with alpha = -(g + sum a + h H) / T and beta = -h ln2 / T: one exponential and a few products
+// per logit, read once and written once, a wave for 256 windows.  The few tokens that were named are then written once more,
+// whole, by the wave that wrote them first.  Bound by the memory: 8192 x 131072 bfloat16 logits 724 us, 5.9 TB/s.  (Workgroups of
+// four waves were up to 4 % slower on long rows, and 275 us in the place of 93 on 262144 x 256.)
+constexpr uint32_t kLpGradWindows = 4 * kWave;
+
 template <int DT>
-__global__ __launch_bounds__(kLpThreads) void logprobs_grad_kernel(LpGradParams p)
+__global__ __launch_bounds__(kWave) void logprobs_grad_kernel(LpGradParams p)
 {
     using E = Elem<DT>;
     constexpr int U = 4;
     const uint32_t r = blockIdx.x / p.chunks, chunk = blockIdx.x - r * p.chunks;
     const uint32_t b = r / (uint32_t)p.T, pos = r - b * (uint32_t)p.T;
-    const uint32_t V = (uint32_t)p.V, full = V / E::kVec, tid = threadIdx.x, lane = tid % kWave;
+    const uint32_t V = (uint32_t)p.V, full = V / E::kVec, lane = threadIdx.x;
     const typename E::T *row = (const typename E::T *)p.logits + (int64_t)b * p.stride_b + (int64_t)pos * p.stride_t;
     typename E::T *out = (typename E::T *)p.grad + (size_t)r * V;
-    const uint32_t n0 = chunk * (U * kLpThreads) + tid;
+    const uint32_t n0 = chunk * (U * kWave) + lane;
     uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) if (n0 + u * kLpThreads < full) raw[u] = load_window<DT>(row, n0 + u * kLpThreads);
+    for (int u = 0; u < U; ++u) if (n0 + u * kWave < full) raw[u] = load_window<DT>(row, n0 + u * kWave);
 
     const float4 st = p.stats[r];
     const int64_t at = (int64_t)b * p.token_b + (int64_t)pos * p.token_t;
@@ -647,7 +656,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_grad_kernel(LpGradParams 
     };
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t n = n0 + u * kLpThreads;
+        const uint32_t n = n0 + u * kWave;
         if (n < full) {
             float x[E::kVec];
             E::wide(raw[u], x);
@@ -659,19 +668,17 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_grad_kernel(LpGradParams 
     }
     const bool last = chunk == p.chunks - 1u;
     if (last) {
-        const uint32_t i = full * E::kVec + tid;
+        const uint32_t i = full * E::kVec + lane;
         if (i < V) out[i] = E::round(grad(E::one(row[i])));
     }
     // the named tokens of this chunk
-    const int64_t begin = (int64_t)chunk * (U * kLpThreads * E::kVec);
-    const int64_t end = last ? (int64_t)V : begin + U * kLpThreads * E::kVec;
+    const int64_t begin = (int64_t)chunk * (U * kWave * E::kVec);
+    const int64_t end = last ? (int64_t)V : begin + U * kWave * E::kVec;
     const bool token_here = token >= begin && token < end;
     const bool id_here = id >= begin && id < end;
     const uint64_t any = __ballot(id_here || token_here);
     if (any == 0 || log2_s == __builtin_inff()) return;
     wait_vmem();
-    __syncthreads();
-    if (tid >= (uint32_t)kWave) return;
     const uint64_t both = __ballot(id_here && id == token);
     if (id_here) out[id] = E::round(grad(E::one(row[id])) + (a + (id == token ? g : 0.0f)) * p.inv_t);
     if (token_here && !both && lane == 0) out[token] = E::round(grad(E::one(row[token])) + g * p.inv_t);

@@ -243,3 +243,17 @@ def test_refusals_of_the_c_abi():
         return L.rs_linear_rows(x, dtype, K, w, ws, sw, M, N, K, y, y_dtype, ys, None)
     assert rows(x=None) == rows(w=None) == rows(sw=None) == rows(y=None) == -4 and rows(dtype=3) == rows(y_dtype=-1) == -7
     assert rows(M=0) == rows(M=5) == rows(K=8193, ws=8208) == rows(ws=16) == rows(ys=19) == -12 and rows(x=258) == rows(w=260) == rows(ws=40) == -6
+
+
+@gpu
+def test_example():
+    """The example runs, and its parts agree: what is scored again is what was answered, up to the logits' rounding to bfloat16
+    (2^-9 of logits below 16, twice over: 2^-4 / 0.8 in a log probability), and a row's gradient sums to nothing."""
+    import runpy
+
+    from tests.conftest import ROOT
+    answers, scored, grad = runpy.run_path(ROOT + "/examples/head_and_logprobs.py")["main"]()
+    for step, answer in enumerate(answers):
+        assert (answer.logprobs - scored.logprobs[:, step]).abs().max() < 0.1
+        assert (answer.top_logprobs[:, :1] >= answer.logprobs[:, None]).all() and (answer.rank <= 50).all()
+    assert grad.float().abs().sum() > 0 and grad.float().sum(-1).abs().max() < 1e-3

@@ -105,6 +105,29 @@ def test_rows_split_and_whole(rows):
 
 @gpu
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("V", [1, 7, 64, 300, 2049, 5000])
+def test_many_short_rows(V, dtype):
+    """Rows that a wave does by itself, masked ones among them."""
+    print("short rows", V, dtype, flush=True)
+    x, t = make(2300, V, dtype, V, scale=2.0)
+    if V > 60:
+        x[::7, V // 3:] = -INF
+        x[::11] = torch.finfo(x.dtype).min
+        x[::13] = -INF
+        x[5, :] = 1.0
+    pick = torch.cat([torch.arange(40), torch.arange(2260, 2300)]).cuda()
+    import rapid_sampling_amd as sample
+    for top in (0, min(V, 3), min(V, 64)):
+        out = sample.token_logprobs(x, t, 0.9, top=top)
+        some = check(x[pick], t[pick], 0.9, top)                      # (fewer rows: by workgroups)
+        want = formulas(x[pick], t[pick], 0.9, top)
+        assert out.rank[pick].tolist() == want[2].tolist() and out.top_tokens[pick].tolist() == want[4].tolist()
+        for a, b in zip((out.logprobs, out.entropy, out.top_logprobs), (some.logprobs, some.entropy, some.top_logprobs)):
+            near(a[pick], b.cpu(), b.cpu().double().nan_to_num(0, 0, 0), V, "short rows")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
 def test_long_rows(dtype):
     x, t = make(2, 131072 + 5, dtype, 1)
     check(x, t, 1.0, 20)
@@ -181,7 +204,7 @@ def test_tokens_that_are_none():
 
 @gpu
 @pytest.mark.parametrize("dtype", list(DTYPES))
-@pytest.mark.parametrize("rows", [2, 1030])
+@pytest.mark.parametrize("rows", [2, 1030, 2100])
 def test_rows_whose_alternatives_are_hard_to_find(rows, dtype):
     """Equal logits by the thousand, sorted rows, and large logits that all fall to one thread of the pass."""
     V = 20000 if rows == 2 else 2100
