@@ -181,6 +181,28 @@ def test_head_sampler_and_logprobs_together():
         assert all(torch.equal(a, b) for a, b in zip(held, step(fresh))), seed
 
 
+@gpu
+def test_more_elements_than_32_bits_count():
+    """The last rows of more than 2^31 outputs, and the last columns of more than 2^31 weights, against parts by themselves."""
+    import rapid_sampling_amd as sample
+    x, w = make(34000, 128, "bf16", 1), make(65536, 128, "f32", 2)
+    qw, sw = sample.quantize_fp8(w, block_rows=128)
+    y = sample.linear_fp8(x, qw, sw, out_dtype=torch.bfloat16)
+    assert torch.equal(y[-200:], sample.linear_fp8(x[-200:], qw, sw, out_dtype=torch.bfloat16))
+    del y
+    K, N = 4096, 540000
+    store = torch.zeros((N, K), dtype=torch.uint8, device="cuda").view(F8)
+    sw = torch.ones(((N + 127) // 128, K // 128), device="cuda")
+    x = make(40, K, "bf16", 3)
+    store[-256:] = sample.quantize_fp8(make(256, K, "f32", 4), block_rows=128)[0]
+    for M in (1, 10, 40):
+        y = sample.linear_fp8(x[:M], store, sw)
+        qx, sx = sample.quantize_fp8(x[:M])
+        part = store[-(256 + N % 128):]
+        check(y[:, -part.shape[0]:], qx, sx, part, sw[-3:], torch.float32)
+        assert (y[:, :1000] == 0).all()
+
+
 def test_refusals():
     import rapid_sampling_amd as sample
     x, w, s = torch.zeros((2, 32)), torch.zeros((16, 32), dtype=F8), torch.ones((1, 1))

@@ -361,6 +361,26 @@ def test_streams_and_graphs():
         assert all(torch.equal(a, b) for a, b in zip(held, want)), seed
 
 
+@gpu
+def test_more_elements_than_32_bits_count():
+    """The last rows of more than 2^31 logits, against the same rows by themselves; their gradient too."""
+    import rapid_sampling_amd as sample
+    V, rows = 1048576, 2060
+    x = torch.zeros((rows, V), dtype=torch.bfloat16, device="cuda")
+    last = slice(rows - 3, rows)
+    x[last] = make(3, V, "bf16", 77)[0]
+    t = torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(1)).cuda()
+    want = check(x[last], t[last], 1.0, 5)
+    got = sample.token_logprobs(x, t, top=5)
+    for a, b in zip(got, want):
+        assert torch.equal(a[last], b) if not a.is_floating_point() else torch.allclose(a[last], b, rtol=0, atol=EPS * (64 + V / 1024) * 20)
+    part = x[last].clone().requires_grad_()
+    sample.token_logprobs(part, t[last]).logprobs.sum().backward()
+    x.requires_grad_()
+    sample.token_logprobs(x, t).logprobs.sum().backward()
+    assert torch.equal(x.grad[last], part.grad)
+
+
 def test_refusals():
     import rapid_sampling_amd as sample
     x, t = torch.zeros((2, 8)), torch.zeros(2, dtype=torch.long)
