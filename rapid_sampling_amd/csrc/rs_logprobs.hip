@@ -9,8 +9,8 @@ namespace rs {
 constexpr uint32_t kLpSplitMost = 512;   // workgroups of a call whose rows are split
 
 // Workgroups per row: one, or enough for about two to a compute unit, each with at least four windows per thread.  (With four to a
-// compute unit 64 rows of 152064 bfloat16 logits and 20 alternatives take 18.5 us in the place of 17.0, 385 of 50257 23.1 in the
-// place of 19.6, with one 16.8 and 19.6, but 48 of 32768 float32 are as fast either way.)
+// compute unit 64 rows of 152064 bfloat16 logits and 20 alternatives took 18.5 us in the place of 17.0, 385 of 50257 23.1 in the
+// place of 19.6, with one 16.8 and 19.6; 48 of 32768 float32 are as fast either way.)
 static uint32_t lp_split(uint32_t rows, uint32_t windows)
 {
     const uint32_t most = kLpSplitMost / rows, per = (windows + 4u * kLpThreads - 1u) / (4u * kLpThreads);
@@ -38,9 +38,9 @@ static void lp_launch(const LpParams &p, uint32_t rows, bool one_wave, hipStream
     else hipLaunchKernelGGL((logprobs_kernel<DT, kLpThreads, false>), dim3(rows), dim3(kLpThreads), 0, st, p);
 }
 
-// Many short rows: a wave each, without a barrier.  262144 x 256 bfloat16 logits and 20 alternatives take 426 us in the place of
-// 1098, 30000 x 8192 127 in the place of 190, 8192 x 16384 67 in the place of 75; but 8192 x 32768 131 in the place of 115, and
-// 1024 x 8192 14.9 in the place of 13.8.
+// Many short rows: a wave each, without a barrier.  When this was chosen 262144 x 256 bfloat16 logits and 20 alternatives took 426 us
+// in the place of 1098 by workgroups (now 383), 30000 x 8192 127 in the place of 190, 8192 x 16384 67 in the place of 75; but
+// 8192 x 32768 131 in the place of 115, and 1024 x 8192 14.9 in the place of 13.8.
 static bool lp_one_wave(uint32_t rows, uint32_t windows) { return windows <= 2048u && rows >= 2048u; }
 
 }  // namespace rs
