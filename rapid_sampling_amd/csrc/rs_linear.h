@@ -3,8 +3,8 @@
 //   scale = max(max |x| over the block * r, 2^-126), r = 1/448 in float32        q = e4m3(x / scale), to nearest, ties to even
 //   y[m, n] = sum over blocks kb of sx[m, kb] sw[n / 128, kb] sum_{k in kb} qx[m, k] qw[n, k]
 //
-// The inner sums are the matrix cores' (products of two such values are exact in float32, the sum over a block is held in
-// float32); the scales are applied to them in float32, and so is the outer sum.  One rounding to y's type at the end.
+// The inner sums are the matrix cores' (see block_product for what they hold); the scales are applied to them in float32, and the
+// outer sum is of float32.  One rounding to y's type at the end.
 #pragma once
 
 #include "rs_common.h"
@@ -372,7 +372,6 @@ __global__ __launch_bounds__(512) void linear_few_kernel(LinearParams p)
 // STAGES - 1 blocks ahead of the one that is multiplied.  The eight 16-byte pieces of a row are stored in an order that depends on
 // the row (place = piece ^ turn(row)), so that the eight rows read at once lie in different banks.  The first operand's rows are
 // dealt so that a lane's sums are 4 NU consecutive columns of y.
-typedef __attribute__((address_space(1))) const void *GlobalPtr;
 typedef __attribute__((address_space(3))) void *LdsPtr;
 
 constexpr int64_t kTileStride = (1ll << 32) / 256 - kFpBlock;   // a tile's rows are reached with 32 bits

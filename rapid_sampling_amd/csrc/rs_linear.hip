@@ -82,9 +82,11 @@ static hipError_t launch_linear(const LinearParams &p, hipStream_t st)
 static LinearParams linear_params(const void *x, int64_t x_stride, const float *x_scale, const void *w, int64_t w_stride, const float *w_scale,
                                   int32_t M, int32_t N, int32_t K, void *y, int64_t y_stride, void *workspace)
 {
+    // (the distance to the next row of a single one is not looked at by the checks, and a tile's other rows must lie behind it)
+    const int64_t alone = ((int64_t)K + 15) / 16 * 16;
     LinearParams p;
-    p.x = (const uint8_t *)x; p.x_stride = x_stride; p.x_scale = x_scale;
-    p.w = (const uint8_t *)w; p.w_stride = w_stride; p.w_scale = w_scale;
+    p.x = (const uint8_t *)x; p.x_stride = M > 1 ? x_stride : alone; p.x_scale = x_scale;
+    p.w = (const uint8_t *)w; p.w_stride = N > 1 ? w_stride : alone; p.w_scale = w_scale;
     p.y = y; p.y_stride = y_stride;
     p.M = (uint32_t)M; p.N = (uint32_t)N; p.K = (uint32_t)K; p.blocks = ((uint32_t)K + kFpBlock - 1) / kFpBlock;
     p.split = 1;
