@@ -40,8 +40,10 @@ static void lp_launch(const LpParams &p, uint32_t rows, bool one_wave, hipStream
 
 // Many short rows: a wave each, without a barrier.  When this was chosen 262144 x 256 bfloat16 logits and 20 alternatives took 426 us
 // in the place of 1098 by workgroups (now 383), 30000 x 8192 127 in the place of 190, 8192 x 16384 67 in the place of 75; but
-// 8192 x 32768 131 in the place of 115, and 1024 x 8192 14.9 in the place of 13.8.
-static bool lp_one_wave(uint32_t rows, uint32_t windows) { return windows <= 2048u && rows >= 2048u; }
+// 8192 x 32768 131 in the place of 115, and 1024 x 8192 14.9 in the place of 13.8.  Up to 32 alternatives: the bound of as many as there
+// are lanes is a low one (30000 x 8192 with 32 138 in the place of 196, with 48 226 in the place of 204, with 64 1147 in the place of
+// 230).
+static bool lp_one_wave(uint32_t rows, uint32_t windows, int32_t top) { return windows <= 2048u && rows >= 2048u && top <= 32; }
 
 }  // namespace rs
 
@@ -72,7 +74,7 @@ int rs_token_logprobs(const void *logits, int32_t dtype, int64_t stride_b, int64
     p.logprobs = logprobs; p.entropy = entropy; p.rank = rank; p.top_logprobs = top_logprobs; p.top_tokens = top_tokens;
     p.stats = (float4 *)stats;
     // (a thread's windows are worked on four at a time)
-    const bool one_wave = lp_one_wave(rows, windows);
+    const bool one_wave = lp_one_wave(rows, windows, top);
     const uint32_t threads = one_wave ? kWave : kLpThreads;
     const uint32_t per_row = (windows + threads - 1) / threads, split = one_wave ? 1 : lp_split(rows, windows);
     p.J = split > 1 ? ((per_row + split - 1) / split + 3) / 4 * 4 : per_row;

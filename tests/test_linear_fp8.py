@@ -146,6 +146,20 @@ def test_values_that_are_no_numbers_stay_in_their_row(M):
 
 
 @gpu
+def test_gradient_of_x_by_the_transposed_weight():
+    """d/dx of sum g y is g W, the same product with W's blocks transposed."""
+    import rapid_sampling_amd as sample
+    w = make(640, 384, "f32", 1)
+    qw, sw = sample.quantize_fp8(w, block_rows=128)
+    g = make(30, 640, "f32", 2)
+    qt, st = qw.t().contiguous(), sw.t().contiguous()
+    back = sample.linear_fp8(g, qt, st)
+    qg, sg = sample.quantize_fp8(g)
+    check(back, qg, sg, qt, st, torch.float32)
+    assert torch.equal(values(qt, st, 128), values(qw, sw, 128).T)
+
+
+@gpu
 def test_head_sampler_and_logprobs_together():
     """hidden states -> logits -> a token each -> its log probability, on another stream and from a graph."""
     import rapid_sampling_amd as sample
