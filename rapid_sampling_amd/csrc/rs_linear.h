@@ -8,10 +8,9 @@
 #pragma once
 
 #include "rs_common.h"
+#include "rs_tile.h"
 
 namespace rs {
-
-constexpr int kFpBlock = 128;
 
 typedef int   v8i __attribute__((ext_vector_type(8)));
 typedef int   v4i __attribute__((ext_vector_type(4)));
@@ -374,8 +373,6 @@ __global__ __launch_bounds__(512) void linear_few_kernel(LinearParams p)
 // dealt so that a lane's sums are 4 NU consecutive columns of y.
 typedef __attribute__((address_space(3))) void *LdsPtr;
 
-constexpr int64_t kTileStride = (1ll << 32) / 256 - kFpBlock;   // a tile's rows are reached with 32 bits
-
 template <int NU> __device__ __forceinline__ uint32_t w_turn(uint32_t row) { return (row & 3u) | ((row / NU) & 4u); }
 __device__ __forceinline__ uint32_t x_turn(uint32_t row) { return row & 7u; }
 
@@ -399,26 +396,32 @@ struct LinearTile {
     static constexpr bool kWhole = kWaves == 8;                  // K has to be a whole number of blocks: no registers to spare for anything else
 
     // A wave fills eight rows of a stage with one load: the thread's row of load i, w's rows first.
-    static __device__ __forceinline__ uint32_t row_of(uint32_t i) { return (i * kWaves + wave_id()) * 8u + threadIdx.x % 64u / 8u; }
+    static __device__ __forceinline__ uint32_t row_of(uint32_t i) { return tile_row(i, kWaves, wave_id(), threadIdx.x % 64u); }
 
-    // The tile's rows as two buffers; what lies behind their last row reads as 0.
+    // The tile's rows as two buffers; rows behind the last read as 0.
     struct Source {
         __amdgpu_buffer_rsrc_t w, x;
-        uint32_t w_stride, x_stride;
-        uint32_t w_at[2], x_at;          // the thread's piece of the first block of its row of an even, of an odd load
+        uint32_t w_stride, x_stride, w_rows, x_rows;
+        uint32_t w_piece[2], x_piece;    // byte of a block of the thread's piece of its row of an even, of an odd load
+
+        // The thread's byte of load i, of the block that begins at column k
+        __device__ __forceinline__ uint32_t at(uint32_t i, uint32_t k) const
+        {
+            return i < kLoadsW ? tile_at(row_of(i), w_rows, w_stride, w_piece[kWaves % 8 ? i % 2 : 0] + k)
+                               : tile_at(row_of(i) - kTileN, x_rows, x_stride, x_piece + k);
+        }
     };
     static __device__ __forceinline__ Source source(const LinearParams &p, uint32_t n0, uint32_t m0)
     {
         Source s;
         s.w_stride = (uint32_t)p.w_stride;
         s.x_stride = (uint32_t)p.x_stride;
-        const uint32_t rows_w = min(p.N - n0, kTileN), rows_x = min(p.M - m0, kTileM);
-        const uint32_t bytes = (p.K + 3u) & ~3u;       // of the last row, in whole words: a word is read or it is not
-        s.w = __builtin_amdgcn_make_buffer_rsrc((void *)(p.w + (int64_t)n0 * p.w_stride), 0, (int)((rows_w - 1u) * s.w_stride + bytes), kBufferFlags);
-        s.x = __builtin_amdgcn_make_buffer_rsrc((void *)(p.x + (int64_t)m0 * p.x_stride), 0, (int)((rows_x - 1u) * s.x_stride + bytes), kBufferFlags);
-        const uint32_t r = row_of(0);
-        for (uint32_t i = 0; i < 2; ++i) s.w_at[i] = r * s.w_stride + ((threadIdx.x & 7u) ^ w_turn<NU>(r + i * 8u * kWaves)) * 16u;
-        s.x_at = r * s.x_stride + ((threadIdx.x & 7u) ^ x_turn(r)) * 16u;
+        s.w_rows = min(p.N - n0, kTileN);
+        s.x_rows = min(p.M - m0, kTileM);
+        s.w = __builtin_amdgcn_make_buffer_rsrc((void *)(p.w + (int64_t)n0 * p.w_stride), 0, (int)tile_bytes(s.w_rows, s.w_stride, p.K), kBufferFlags);
+        s.x = __builtin_amdgcn_make_buffer_rsrc((void *)(p.x + (int64_t)m0 * p.x_stride), 0, (int)tile_bytes(s.x_rows, s.x_stride, p.K), kBufferFlags);
+        for (uint32_t i = 0; i < 2; ++i) s.w_piece[i] = ((threadIdx.x & 7u) ^ w_turn<NU>(row_of(i))) * 16u;
+        s.x_piece = ((threadIdx.x & 7u) ^ x_turn(row_of(0))) * 16u;
         return s;
     }
     static __device__ __forceinline__ void fill(const LinearParams &p, const Source &s, uint32_t n0, uint32_t m0, uint32_t kb, uint8_t *lds)
@@ -428,8 +431,7 @@ struct LinearTile {
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
                 const LdsPtr to = (LdsPtr)(lds + (i * kWaves + wave_id()) * 1024u);
-                if (i < kLoadsW) __builtin_amdgcn_raw_ptr_buffer_load_lds(s.w, to, 16, s.w_at[kWaves % 8 ? i % 2 : 0], k + i * 8u * kWaves * s.w_stride, 0, 0);
-                else __builtin_amdgcn_raw_ptr_buffer_load_lds(s.x, to, 16, s.x_at, k + (i - kLoadsW) * 8u * kWaves * s.x_stride, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kLoadsW ? s.w : s.x, to, 16, s.at(i, 0), k, 0, 0);
             }
             return;
         }
@@ -437,10 +439,7 @@ struct LinearTile {
         if constexpr (kWhole) return;
         v4i v[kLoads];
 #pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i) {
-            if (i < kLoadsW) v[i] = __builtin_amdgcn_raw_buffer_load_b128(s.w, kWaves % 8 && i % 2 ? s.w_at[1] : s.w_at[0], k + i * 8u * kWaves * s.w_stride, 0);
-            else v[i] = __builtin_amdgcn_raw_buffer_load_b128(s.x, s.x_at, k + (i - kLoadsW) * 8u * kWaves * s.x_stride, 0);
-        }
+        for (uint32_t i = 0; i < kLoads; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(i < kLoadsW ? s.w : s.x, s.at(i, k), 0, 0);
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
             const uint32_t r = row_of(i) - (i < kLoadsW ? 0u : kTileN);
@@ -530,11 +529,10 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearPara
     const uint32_t wave = wave_id(), lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
     const uint32_t wn = wave % WN * (16u * NU), wm = wave / WN * (16u * MT);
     const float *sw = p.w_scale + (size_t)min((n0 + wn) / kFpBlock, (p.N - 1u) / kFpBlock) * p.blocks;
-    // x's scales as a buffer as well: one address register for all rows, and 0 behind the last
-    const __amdgpu_buffer_rsrc_t sx = __builtin_amdgcn_make_buffer_rsrc((void *)(p.x_scale + (size_t)m0 * p.blocks), 0,
-                                                                        (int)(min(p.M - m0, L::kTileM) * p.blocks * 4u), L::kBufferFlags);
-    const uint32_t sx_at = (wm + i) * p.blocks * 4u;
-    auto x_scale = [&](int t, uint32_t kb) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sx, sx_at, (t * 16u * p.blocks + kb) * 4u, 0)); };
+    // x's scales as a buffer as well: addressed with 32 bits, and 0 for rows that are not there
+    const uint32_t sx_rows = min(p.M - m0, L::kTileM);
+    const __amdgpu_buffer_rsrc_t sx = __builtin_amdgcn_make_buffer_rsrc((void *)(p.x_scale + (size_t)m0 * p.blocks), 0, (int)(sx_rows * p.blocks * 4u), L::kBufferFlags);
+    auto x_scale = [&](int t, uint32_t kb) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sx, tile_at(wm + t * 16u + i, sx_rows, p.blocks * 4u, 0u), kb * 4u, 0)); };
     v4f acc[NU][MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
