@@ -16,17 +16,17 @@ constexpr uint32_t kPartTiles = 256;                 // tiles of partial sums th
 constexpr size_t   kPartBytes = 128 * 64 * 4;        // ... of 128 x 64
 
 // SPLIT: where there are few tiles their blocks of columns are shared out, for up to one workgroup to a compute unit.  Leaving and
-// adding up the parts costs about 2 us, a block 0.5 us, 0.9 on bfloat16 cores: eight blocks or four to each at least (64 x 1024 x
-// 4096: 24 us whole, 12 in eight; 64 x 4096 x 512: 4.7 whole, 6.6 in two).
-template <int DT, int WN, int WM, int NU, int MT, int STAGES, bool EXACT, bool SPLIT>
+// adding up the parts costs about 2 us, a block 0.9: four blocks to each at least (64 x 1024 x 4096: 24 us whole, 12 in eight;
+// 64 x 4096 x 512: 4.7 whole, 6.6 in two).
+template <int DT, int WN, int WM, int NU, int MT, int STAGES, bool SPLIT>
 static hipError_t launch_tiles(LinearParams p, hipStream_t st)
 {
-    using L = LinearTile<WN, WM, NU, MT, STAGES, EXACT>;
+    using L = LinearTile<WN, WM, NU, MT, STAGES>;
     static_assert(!SPLIT || L::kTileN * L::kTileM * 4 <= kPartBytes, "a tile's sums fit the workspace");
     const uint64_t tiles = (uint64_t)((p.M + L::kTileM - 1) / L::kTileM) * ((p.N + L::kTileN - 1) / L::kTileN);
     if (tiles > 0x7FFFFFFF) return hipErrorInvalidValue;
-    p.split = SPLIT ? (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({kPartTiles / tiles, p.blocks / (EXACT ? 4 : 8), 8})) : 1;
-    hipLaunchKernelGGL((linear_tile_kernel<DT, WN, WM, NU, MT, STAGES, EXACT, SPLIT>), dim3((uint32_t)tiles * p.split), dim3(L::kThreads), L::kLds, st, p);
+    p.split = SPLIT ? (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({kPartTiles / tiles, p.blocks / 4, 8})) : 1;
+    hipLaunchKernelGGL((linear_tile_kernel<DT, WN, WM, NU, MT, STAGES, SPLIT>), dim3((uint32_t)tiles * p.split), dim3(L::kThreads), L::kLds, st, p);
     return hipGetLastError();
 }
 
@@ -60,23 +60,12 @@ static hipError_t launch_linear(const LinearParams &p, hipStream_t st)
     // (The tiles' kernel reaches its rows with 32 bits.)
     if (p.M <= 16 || p.x_stride > kTileStride || p.w_stride > kTileStride) return launch_few<DT, -1>(p, st);
     // Tiles of 128 x 64 (rows of w x rows of x) for up to 64 rows, and wherever those of 128 x 128 would not give every compute unit
-    // its own (1000 x 4096 x 4096 into bfloat16: 28.0 against 29.8; 300 x 8192 x 1440: 12.9 against 14.0).  On bfloat16 cores two
-    // waves share w's rows and two x's, since both have to be widened (64 x 50256 x 2000: 25.7 against 29.0 with four and one).
+    // its own.  Two waves share w's rows and two x's, since both have to be widened (64 x 50256 x 2000: 25.7 against 29.0 with four and
+    // one).
     const uint64_t n128 = (p.N + 127) / 128, m128 = (p.M + 127) / 128;
-    const bool few_tiles = n128 * m128 <= 256;
-    if (DT == RS_DTYPE_F32 || p.M <= 64) {
-        if (p.M <= 64 || few_tiles) return launch_tiles<DT, 2, 2, 4, 2, 3, true, true>(p, st);
-        // 128 x 128: 4096 x 32768 x 4096 in 1076 (1.02 PFLOP/s), bound by the widening; 1278 in tiles of 128 x 64
-        if constexpr (DT == RS_DTYPE_F32) return launch_tiles<DT, 1, 4, 8, 2, 2, true, false>(p, st);
-    }
-    if constexpr (DT != RS_DTYPE_F32) {
-        if (few_tiles) return launch_tiles<DT, 1, 4, 8, 1, 3, false, true>(p, st);
-        // 256 x 256 where that fills the card and wastes little: 8192^3 536 against 612 in tiles of 128 x 128, 2048 x 16384 x 2048 85
-        // against 92; but 128 x 131072 x 4096 143 against 129
-        const uint64_t n256 = (p.N + 255) / 256, m256 = (p.M + 255) / 256;
-        if (p.K % kFpBlock == 0 && n256 * m256 >= 256 && 20 * m256 <= 11 * m128) return launch_tiles<DT, 2, 4, 8, 4, 2, false, false>(p, st);
-        return launch_tiles<DT, 1, 4, 8, 2, 2, false, false>(p, st);
-    }
+    if (p.M <= 64 || n128 * m128 <= 256) return launch_tiles<DT, 2, 2, 4, 2, 3, true>(p, st);
+    // 128 x 128: 4096 x 32768 x 4096 in 1076 (1.02 PFLOP/s); 1278 in tiles of 128 x 64
+    return launch_tiles<DT, 1, 4, 8, 2, 2, false>(p, st);
 }
 
 static LinearParams linear_params(const void *x, int64_t x_stride, const float *x_scale, const void *w, int64_t w_stride, const float *w_scale,
