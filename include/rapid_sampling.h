@@ -498,7 +498,9 @@ int rs_token_logprobs(const void *logits_device, int32_t logits_dtype, int64_t s
  * rounded once to the logits' type.  logits, tokens, temperature and top as in the
  * call whose `stats` and `top_tokens` are passed.  A gradient's stride is 1
  * (contiguous) or 0 (one number for all).  grad_logits: contiguous rows.  A row
- * with a negative token has no g; one of nothing but -inf has gradient 0.
+ * with a negative token has no g; one whose token is V or more has NaN for its
+ * gradient if there is a g (its log probability is NaN), and what h and a make of it if
+ * there is none; one of nothing but -inf has gradient 0.
  * One launch, no workspace.
  */
 int rs_token_logprobs_backward(const void *logits_device, int32_t logits_dtype, int64_t stride_b, int64_t stride_t,

@@ -661,7 +661,7 @@ __global__ __launch_bounds__(kWave) void logprobs_grad_kernel(LpGradParams p)
     const int64_t at = (int64_t)b * p.token_b + (int64_t)pos * p.token_t;
     const int64_t token = p.tokens_64 ? ((const int64_t *)p.tokens)[at] : (int64_t)((const int32_t *)p.tokens)[at];
     float g = p.g && token >= 0 ? p.g[(int64_t)r * p.g_stride] : 0.0f;
-    if (token >= (int64_t)V) g = __builtin_nanf("");
+    if (p.g && token >= (int64_t)V) g = __builtin_nanf("");      // (the entropy and the alternatives do not know the token)
     const float h = p.h ? p.h[(int64_t)r * p.h_stride] : 0.0f;
     float a = 0.0f;
     int64_t id = -1;

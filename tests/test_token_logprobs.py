@@ -335,6 +335,36 @@ def test_gradient_of_what_is_used():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_gradient_of_a_row_whose_token_is_outside(dtype):
+    """The entropy and the alternatives of a row do not depend on its token, and neither do their gradients; the log probability of a
+    token that is outside the vocabulary is NaN, and its gradient with it."""
+    import rapid_sampling_amd as sample
+    V, T = 3001, 0.8
+    x, t = make(4, V, dtype, 21)
+    t[1], t[2] = V, 1 << 40
+    keep = [0, 3]
+    z = torch.zeros(4, dtype=torch.float64)
+    h, a = torch.tensor([0.5, -1.0, 2.0, 1.0]), torch.randn((4, 5), generator=torch.Generator().manual_seed(2))
+
+    def grad(f):
+        y = x.detach().requires_grad_()
+        out = sample.token_logprobs(y, t, T, top=5)
+        f(out).backward()
+        return y.grad.cpu().double(), out.top_tokens.cpu().long()
+    within = t.clamp(max=V - 1)
+    got, ids = grad(lambda o: (o.entropy * h.cuda()).sum())
+    want = gradient(x, within, T, z, h.double(), torch.zeros((4, 5), dtype=torch.float64), ids)
+    limit = lambda want: EPS * 400 * 20 + UNIT[x.dtype] * want.abs() * 1.01 + LEAST[x.dtype]
+    assert ((got - want).abs() <= limit(want)).all()
+    got, ids = grad(lambda o: (o.top_logprobs * a.cuda()).sum())
+    want = gradient(x, within, T, z, z, a.double(), ids)
+    assert ((got - want).abs() <= limit(want)).all()
+    got, ids = grad(lambda o: o.logprobs[keep].sum() + (o.entropy * h.cuda()).sum())
+    assert got[1:3].isnan().all() and not got[keep].isnan().any()
+
+
+@gpu
 def test_streams_and_graphs():
     import rapid_sampling_amd as sample
     x, t = make(3, 50001, "f32", 30)
