@@ -56,13 +56,17 @@ template <int DT> __device__ __forceinline__ void put(void *p, int64_t i, float 
 
 __device__ __forceinline__ float block_scale(float peak) { return fmaxf(peak * (1.0f / 448.0f), 0x1p-126f); }
 
-// x / scale, rounded once: the quotient by way of the reciprocal, and what it is off by divided once more.  (Compared with the
-// division on 4e8 pairs of a block's largest value and another: the same.)
+// x / scale, rounded once: the quotient by way of the reciprocal, and what it is off by divided once more.  Of small blocks both
+// are taken 2^64 times as large, which is exact: what the quotient is off by, some 2^-24 of x, would be below float32's range.
+// (Compared with the division on the CPU, for every significand of the scale and the five numbers about each point halfway between two
+// 8-bit values, 6.7e8 pairs: the same.  Without the larger numbers 1.8 % of them are not at a scale of 2^-126, none from 2^-94 on.)
 struct Divisor {
-    float s, r;
-    __device__ __forceinline__ explicit Divisor(float scale) : s(scale < __builtin_inff() ? scale : 0.0f), r(1.0f / scale) {}
+    float up, s, r;
+    __device__ __forceinline__ explicit Divisor(float scale)
+        : up(scale < 0x1p-60f ? 0x1p64f : 1.0f), s(scale < __builtin_inff() ? scale * up : 0.0f), r(1.0f / (scale * up)) {}
     __device__ __forceinline__ float operator()(float x) const
     {
+        x *= up;
         const float q = x * r;
         // (-0 stays one; an infinite scale gives 0 for a finite x, NaN for an infinite one)
         return __builtin_copysignf(__builtin_fmaf(__builtin_fmaf(-q, s, x), r, q), x);

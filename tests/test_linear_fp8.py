@@ -90,6 +90,31 @@ def test_quantize_extremes_and_strides():
 
 
 @gpu
+@pytest.mark.parametrize("exponent", [-149, -130, -126, -122, -117, -110, -104, -100, -96, -70, -61, -60, -59, 0, 110])
+@pytest.mark.parametrize("rows", [1, 128])
+def test_quantize_halfway_between_two_values(exponent, rows):
+    """Numbers at, just below and just above a point halfway between two 8-bit values, in blocks of every size: the division's rounding."""
+    import rapid_sampling_amd as sample
+    gen = torch.Generator().manual_seed(exponent + 200)
+    R = 512
+    most = (448.0 * (1.0 + torch.rand((R if rows == 1 else R // 128, 1), generator=gen, dtype=torch.float64)) * 2.0 ** exponent).float()
+    most = most.repeat_interleave(rows, 0)
+    scale = (most * torch.tensor(1.0 / 448.0)).clamp(min=2.0 ** -126)
+    eighths = torch.randint(0, 8, (R, 128), generator=gen).double()
+    binade = torch.randint(-6, 8, (R, 128), generator=gen).double()
+    half = torch.where(torch.rand((R, 128), generator=gen) < 0.2, (2 * eighths + 1) * 2.0 ** -10, (1 + (2 * eighths + 1) / 16) * 2.0 ** binade)
+    x = (half * scale.double()).float()
+    x = (x.view(torch.int32) + torch.randint(-2, 3, (R, 128), generator=gen, dtype=torch.int32)).clamp(min=0).view(torch.float32)
+    x = torch.minimum(x, most) * torch.where(torch.rand((R, 128), generator=gen) < 0.5, 1.0, -1.0)
+    x[:, 0] = most[:, 0]
+    q, got_scale = sample.quantize_fp8(x.cuda(), block_rows=rows)
+    want, want_scale = quantized(x, rows)
+    assert torch.equal(got_scale.cpu(), want_scale)
+    off = q.view(torch.uint8).cpu() != want
+    assert not off.any(), (off.float().mean().item(), x[off][:4].tolist())
+
+
+@gpu
 @pytest.mark.parametrize("M,K,N", [(1, 16, 1), (1, 100, 50), (2, 128, 16), (1, 4096, 1000), (4, 8192, 70), (3, 8200, 40), (4, 1999, 9000), (5, 1000, 257), (16, 512, 384), (17, 256, 129), (33, 2000, 515),
                                    (64, 144, 640), (77, 2000, 1037), (128, 1024, 256), (129, 128, 128), (257, 300, 700), (512, 2048, 1024), (300, 1, 5)])
 @pytest.mark.parametrize("out", list(DTYPES))
