@@ -30,7 +30,7 @@ Next to the sampler:
 `token_logprobs` gives, for each row of (V,), (B, V) or (B, T, V) logits (float32, bfloat16 or float16; any V up
 to 1048576, rows at any stride) and its token, the token's log probability at that temperature, the row's entropy,
 the token's rank (1: the likeliest) and the `top` (up to 64) likeliest alternatives, equal logits by the lower token.
-A negative token is none (padding): log probability 0, rank 0.  It can be differentiated (once) by its logits.
+A negative token is none (padding): log probability 0, rank 0.  It can be differentiated (once, in reverse mode) by its logits.
 `linear_fp8(x, weight, weight_scale)` is x @ weight.T for a float8_e4m3fn weight with a float32 scale for each block of
 128 x 128; x in float32, bfloat16 or float16 is rounded to 8 bits within the call, with a scale for each 128 values of a
 row, or is given so with x_scale=.  `quantize_fp8(x)` makes such values and scales, `quantize_fp8(w, block_rows=128)`

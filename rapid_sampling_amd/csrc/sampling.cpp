@@ -282,6 +282,15 @@ int32_t float_dtype(const at::Tensor &t, const char *what)
                                 std::string(t.dtype().name()) + " !\n");
 }
 
+// The operators carry no forward-mode tangent on, and an output without one would be taken for a constant.
+void refuse_tangent(const char *what, std::initializer_list<at::Tensor> inputs)
+{
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const at::Tensor &t : inputs)
+        if (t.defined() && t._fw_grad(0).defined())
+            throw std::invalid_argument(std::string(what) + " has no forward-mode derivative: call it on tensors without a tangent !\n");
+}
+
 // Rows of logits and their tokens, as the kernels walk them.
 struct TokenRows {
     int64_t B, T, V, stride_b, stride_t, token_b, token_t;
@@ -456,6 +465,7 @@ std::tuple<at::Tensor, at::Tensor> quantize(const at::Tensor &x, int64_t block_r
 {
     if (block_rows != 1 && block_rows != 128)
         throw std::invalid_argument("block_rows must be 1 or 128, got " + std::to_string(block_rows) + " !\n");
+    refuse_tangent("quantize_fp8", {x});
     check_floats(x, block_rows);
     if (x.requires_grad() && at::GradMode::is_enabled())
         throw std::invalid_argument("quantize_fp8 has no gradient: call it under torch.no_grad(), or on x.detach() !\n");
@@ -501,6 +511,7 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const at::Tenso
     if (weight.dtype() != at::kFloat8_e4m3fn || weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1)
         throw std::invalid_argument("weight must be of type float8_e4m3fn and shape (N, K) !\n");
     if (x.dim() < 1 || x.size(-1) != weight.size(1)) throw std::invalid_argument("x must have shape (..., K), with the weight's K !\n");
+    refuse_tangent("linear_fp8", {x, weight, weight_scale, x_scale.value_or(at::Tensor())});
     if (!x.is_cuda() || weight.device() != x.device()) throw std::invalid_argument("x and weight must live on the same GPU !\n");
     const bool given = x.dtype() == at::kFloat8_e4m3fn;
     if (given != x_scale.has_value()) throw std::invalid_argument("x_scale goes with an x of type float8_e4m3fn, and only with one !\n");
@@ -557,6 +568,7 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const at::Tenso
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(const at::Tensor &logits, const at::Tensor &tokens,
                                                                                      double temperature, int64_t top)
 {
+    refuse_tangent("token_logprobs", {logits});
     if (logits.requires_grad() && at::GradMode::is_enabled()) {
         variable_list o = Logprobs::apply(logits, tokens, temperature, top);
         return {o[0], o[1], o[2], o[3], o[4]};

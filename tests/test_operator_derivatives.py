@@ -1,0 +1,42 @@
+"""Derivatives that the operators next to the sampler do not have are refused where they are asked for, not dropped."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+F8 = torch.float8_e4m3fn
+
+
+def inputs(device):
+    gen = torch.Generator().manual_seed(1)
+    x, w, s = torch.randn((2, 32), generator=gen), torch.zeros((16, 32), dtype=torch.uint8).view(F8), torch.ones((1, 1))
+    return x.to(device), w.to(device), s.to(device), torch.zeros(2, dtype=torch.long, device=device)
+
+
+def tangents(device):
+    import rapid_sampling_amd as sample
+    x, w, s, t = inputs(device)
+    with fwd.dual_level():
+        dual, dual_scale = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(s, torch.ones_like(s))
+        for call in (lambda: sample.token_logprobs(dual, t), lambda: sample.token_logprobs(dual.detach().requires_grad_() * dual, t),
+                     lambda: sample.linear_fp8(dual, w, s), lambda: sample.linear_fp8(x, w, dual_scale), lambda: sample.quantize_fp8(dual)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):         # (which does not turn these off)
+                call()
+        return dual, fwd.unpack_dual(dual).primal
+
+
+def test_forward_mode_is_refused():
+    tangents("cpu")
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused_on_the_gpu():
+    import rapid_sampling_amd as sample
+    x, w, s, t = inputs("cuda")
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        primal = fwd.unpack_dual(dual).primal
+        assert torch.equal(sample.token_logprobs(primal, t).logprobs, sample.token_logprobs(x, t).logprobs)
+    tangents("cuda")
+    assert torch.equal(sample.token_logprobs(dual, t).logprobs, sample.token_logprobs(x, t).logprobs)          # its level is over
