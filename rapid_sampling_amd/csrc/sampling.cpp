@@ -423,6 +423,7 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
         const double temperature = ctx->saved_data["temperature"].toDouble();
         const int64_t top = ctx->saved_data["top"].toInt();
         if (!grads[0].defined() && !grads[1].defined() && !grads[3].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        refuse_tangent("token_logprobs' gradient", {grads[0], grads[1], grads[3]});
         auto given = [&](int i) { return grads[i].defined() ? std::optional<at::Tensor>(grads[i]) : std::nullopt; };
         const at::Tensor grad = at::GradMode::is_enabled()
             ? LogprobsBackward::apply(saved[0], saved[1], saved[2], saved[3], temperature, top, given(0), given(1), given(3))

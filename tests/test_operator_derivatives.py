@@ -40,3 +40,20 @@ def test_forward_mode_is_refused_on_the_gpu():
         assert torch.equal(sample.token_logprobs(primal, t).logprobs, sample.token_logprobs(x, t).logprobs)
     tangents("cuda")
     assert torch.equal(sample.token_logprobs(dual, t).logprobs, sample.token_logprobs(x, t).logprobs)          # its level is over
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("again", [False, True])
+def test_forward_mode_over_the_gradient_is_refused(again):
+    """A tangent that comes in with the outputs' gradients, by a factor of the loss."""
+    import rapid_sampling_amd as sample
+    x, _, _, t = inputs("cuda")
+    x.requires_grad_()
+    out = sample.token_logprobs(x, t, top=3)
+    with fwd.dual_level():
+        for value in (out.logprobs, out.entropy, out.top_logprobs):
+            factor = fwd.make_dual(torch.ones_like(value), torch.ones_like(value))
+            with pytest.raises((RuntimeError, ValueError), match="forward-mode"):
+                torch.autograd.grad((value * factor).sum(), x, retain_graph=True, create_graph=again)
+    grad, = torch.autograd.grad(out.entropy.sum(), x)
+    assert grad.abs().sum() > 0
