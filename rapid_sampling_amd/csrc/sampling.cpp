@@ -512,12 +512,13 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const at::Tenso
     if (weight.dtype() != at::kFloat8_e4m3fn || weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1)
         throw std::invalid_argument("weight must be of type float8_e4m3fn and shape (N, K) !\n");
     if (x.dim() < 1 || x.size(-1) != weight.size(1)) throw std::invalid_argument("x must have shape (..., K), with the weight's K !\n");
+    if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || weight_scale.requires_grad() || (x_scale && x_scale->requires_grad())))
+        throw std::invalid_argument("linear_fp8 has no gradient: call it under torch.no_grad(), or on tensors that ask for none "
+                                    "(x.detach(), a weight that is no Parameter or one with requires_grad=False) !\n");
     refuse_tangent("linear_fp8", {x, weight, weight_scale, x_scale.value_or(at::Tensor())});
     if (!x.is_cuda() || weight.device() != x.device()) throw std::invalid_argument("x and weight must live on the same GPU !\n");
     const bool given = x.dtype() == at::kFloat8_e4m3fn;
     if (given != x_scale.has_value()) throw std::invalid_argument("x_scale goes with an x of type float8_e4m3fn, and only with one !\n");
-    if (at::GradMode::is_enabled() && (x.requires_grad() || weight_scale.requires_grad() || (x_scale && x_scale->requires_grad())))
-        throw std::invalid_argument("linear_fp8 has no gradient: call it under torch.no_grad(), or on x.detach() !\n");
     const int64_t K = weight.size(1), N = weight.size(0), blocks = (K + 127) / 128, M = x.numel() / K;
     if (M > RS_LINEAR_MAX || N > RS_LINEAR_MAX || K > RS_LINEAR_MAX) throw std::invalid_argument("x or weight is too large !\n");
     if (!given) check_floats(x, 1);

@@ -57,3 +57,31 @@ def test_forward_mode_over_the_gradient_is_refused(again):
                 torch.autograd.grad((value * factor).sum(), x, retain_graph=True, create_graph=again)
     grad, = torch.autograd.grad(out.entropy.sum(), x)
     assert grad.abs().sum() > 0
+
+
+def test_weights_that_ask_for_a_gradient_are_refused():
+    """A Parameter of any floating type asks for one unless it is told not to."""
+    import rapid_sampling_amd as sample
+    x, w, s, _ = inputs("cpu")
+    learnt, scale = torch.nn.Parameter(w), torch.nn.Parameter(s)
+    assert learnt.requires_grad
+    for args in ((x, learnt, s), (x, w, scale), (x.clone().requires_grad_(), w, s)):
+        with pytest.raises(ValueError, match="no gradient"):
+            sample.linear_fp8(*args)
+        with torch.no_grad(), pytest.raises(ValueError, match="GPU"):                       # (asked for none: the next check)
+            sample.linear_fp8(*args)
+    with pytest.raises(ValueError, match="GPU"):
+        sample.linear_fp8(x, torch.nn.Parameter(w, requires_grad=False), s)
+
+
+@pytest.mark.gpu
+def test_a_frozen_parameter_is_a_weight():
+    import rapid_sampling_amd as sample
+    x, w, s, _ = inputs("cuda")
+    w = torch.randn((16, 32), device="cuda").to(F8)
+    y = sample.linear_fp8(x, w, s)
+    assert torch.equal(sample.linear_fp8(x, torch.nn.Parameter(w, requires_grad=False), s), y)
+    with torch.no_grad():
+        assert torch.equal(sample.linear_fp8(x, torch.nn.Parameter(w), s), y)
+    with pytest.raises(ValueError, match="no gradient"):
+        sample.linear_fp8(x, torch.nn.Parameter(w), s)
