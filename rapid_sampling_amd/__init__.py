@@ -34,8 +34,14 @@ A negative token is none (padding): log probability 0, rank 0.  It can be differ
 `linear_fp8(x, weight, weight_scale)` is x @ weight.T for a float8_e4m3fn weight with a float32 scale for each block of
 128 x 128; x in float32, bfloat16 or float16 is rounded to 8 bits within the call, with a scale for each 128 values of a
 row, or is given so with x_scale=.  `quantize_fp8(x)` makes such values and scales, `quantize_fp8(w, block_rows=128)`
-those of a weight.  Neither has a gradient; that of x, in 8 bits as well, is the same product with the transposed weight, whose
-blocks are the weight's own: linear_fp8(grad, weight.t().contiguous(), weight_scale.t().contiguous()).
+those of a weight.  Neither has a gradient, and what asks for one is refused; that of x, in 8 bits as well, is the same product with the
+transposed weight, whose blocks are the weight's own, in rows that begin at multiples of 16 bytes whatever N is:
+
+    N, K = weight.shape
+    transposed = torch.zeros((K, N + -N % 16), dtype=torch.uint8, device=weight.device)
+    transposed[:, :N] = weight.view(torch.uint8).t()
+    transposed = transposed.view(torch.float8_e4m3fn)[:, :N]
+    grad_x = sample.linear_fp8(grad, transposed, weight_scale.t().contiguous())
 
 The functions live in the compiled extension `_sample` (host layer in
 csrc/sampling.cpp, kernels in csrc/rs_*.hip and csrc/rs_*.h behind the C ABI of

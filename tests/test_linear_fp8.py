@@ -185,6 +185,26 @@ def test_gradient_of_x_by_the_transposed_weight():
 
 
 @gpu
+@pytest.mark.parametrize("N,K", [(515, 384), (1037, 200), (640, 7)])
+def test_gradient_of_x_as_it_is_documented(N, K):
+    """The module's own lines, for numbers of columns that are no multiples of 16 among others, against g W in 64 bits of the rounded g."""
+    import re
+    import textwrap
+
+    import rapid_sampling_amd as sample
+    lines = re.search(r"\n((?:    .*\n)+?    grad_x = .*\n)", sample.__doc__).group(1)
+    weight, weight_scale = sample.quantize_fp8(make(N, K, "f32", 1), block_rows=128)
+    grad = make(30, N, "bf16", 2)
+    names = {"torch": torch, "sample": sample, "weight": weight, "weight_scale": weight_scale, "grad": grad}
+    exec(textwrap.dedent(lines), names)
+    qg, sg = sample.quantize_fp8(grad)
+    a, b = values(qg, sg, 1), values(weight, weight_scale, 128)
+    want, size = a @ b, a.abs() @ b.abs()
+    off = (names["grad_x"].cpu().double() - want).abs()
+    assert (off <= EPS * (128 + 2 * sg.shape[-1] + 8) * size + 2.0 ** -25).all()
+
+
+@gpu
 def test_head_sampler_and_logprobs_together():
     """hidden states -> logits -> a token each -> its log probability, on another stream and from a graph."""
     import rapid_sampling_amd as sample
