@@ -37,7 +37,7 @@ extern "C" {
 #define RS_ERR_DEVICE      -9   /* a kernel gave up waiting for its peer workgroups           */
 #define RS_ERR_SCRATCH     -10  /* rs_sample_static: the call needs more than RS_STATIC_SCRATCH_BYTES */
 #define RS_ERR_UNSUPPORTED -11  /* the current device is not a whole MI355X (256 compute units)     */
-#define RS_ERR_SHAPE       -12  /* rs_quantize_blocks, rs_linear_blocks: a size or a row stride out of range */
+#define RS_ERR_SHAPE       -12  /* rs_quantize_blocks, rs_linear_*: a size or a row stride out of range */
 
 /* Bytes of RNG state per row.  Same size as the reference's
  * curandStatePhilox4_32_10_t record (sampling.cu:9,141) so that the opaque
@@ -449,7 +449,8 @@ int rs_exp_error(int32_t below, int64_t *out_device, void *stream);
 
 /*
  * Log probabilities of given tokens, with the entropy of their rows, their ranks
- * and the likeliest alternatives.  No counterpart in the reference.  One launch.
+ * and the likeliest alternatives.  No counterpart in the reference.  One launch, or
+ * several one after the other from 2^24 rows on.
  *
  * With z = x / temperature, m = max z and S = sum e^(z - m) over the V logits x
  * of a row, for the row's token t:
@@ -501,7 +502,8 @@ int rs_token_logprobs(const void *logits_device, int32_t logits_dtype, int64_t s
  * with a negative token has no g; one whose token is V or more has NaN for its
  * gradient if there is a g (its log probability is NaN), and what h and a make of it if
  * there is none; one of nothing but -inf has gradient 0.
- * One launch, no workspace.
+ * One launch, or several one after the other from 65536 rows on (2^26 short ones);
+ * no workspace.
  */
 int rs_token_logprobs_backward(const void *logits_device, int32_t logits_dtype, int64_t stride_b, int64_t stride_t,
                                const void *tokens_device, int32_t tokens_64, int64_t token_stride_b, int64_t token_stride_t,
@@ -523,7 +525,8 @@ int rs_token_logprobs_backward(const void *logits_device, int32_t logits_dtype, 
  * rounded up to one, 16-byte aligned; bytes behind column K are cleared up to the
  * stride, or to a multiple of 128 if that is less.  scale: ceil(R / block_rows) x
  * ceil(K / 128), contiguous.  A NaN or an infinity gives NaN in its place.
- * One launch.  No counterpart in the reference.
+ * One launch, or several one after the other from 2^28 blocks on (2^24 of 128 x 128).
+ * No counterpart in the reference.
  */
 #define RS_LINEAR_MAX (1 << 24)
 int rs_quantize_blocks(const void *x_device, int32_t x_dtype, int64_t x_row_stride, int32_t block_rows,
@@ -539,8 +542,9 @@ int rs_quantize_blocks(const void *x_device, int32_t x_dtype, int64_t x_row_stri
  * row's last bits can change with how many rows stand beside it.
  * workspace: rs_linear_workspace_bytes() bytes of device memory, 256-byte aligned,
  * cleared once with rs_workspace_init and not shared with other entry points;
- * calls that share it are ordered on one stream.  One launch.  No counterpart in
- * the reference.
+ * calls that share it are ordered on one stream.  M, N and K at most RS_LINEAR_MAX,
+ * and ceil(M / 128) ceil(N / 128) below 2^24.  One launch.  No counterpart in the
+ * reference.
  */
 size_t rs_linear_workspace_bytes(void);
 int rs_linear_blocks(const void *x_device, int64_t x_row_stride, const float *x_scale_device,

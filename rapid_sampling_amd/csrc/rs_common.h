@@ -14,6 +14,7 @@
 namespace rs {
 
 
+constexpr uint32_t kGridThreads = 0xFFFFFFFFu; // threads of a launch, at most, in one dimension
 constexpr int      kThreads   = 256;          // 4 waves, one per SIMD
 constexpr int      kWaves     = kThreads / kWave;
 constexpr int      kMaxParts  = 256;          // workgroups per row, at most

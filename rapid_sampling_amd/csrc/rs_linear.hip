@@ -5,11 +5,20 @@
 
 namespace rs {
 
+// As many rows at a time as a launch holds: a workgroup of 256 makes a block of 128 x 128, or 16 of 1 x 128.
 template <int DT>
-static void launch_quantize(const QuantParams &p, bool tiles, hipStream_t st)
+static void launch_quantize(QuantParams p, bool tiles, hipStream_t st)
 {
-    if (tiles) hipLaunchKernelGGL(quantize_tiles_kernel<DT>, dim3((p.R + kFpBlock - 1) / kFpBlock * p.blocks), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL(quantize_rows_kernel<DT>, dim3((uint32_t)(((uint64_t)p.R * p.blocks + 15) / 16)), dim3(256), 0, st, p);
+    constexpr uint32_t kGroups = kGridThreads / 256u;
+    const uint32_t R = p.R, most = std::min<uint64_t>(R, (uint64_t)kGroups * (tiles ? 1 : 16) / p.blocks * (tiles ? kFpBlock : 1));
+    for (uint32_t done = 0; done < R; done += p.R) {
+        p.R = std::min(most, R - done);
+        if (tiles) hipLaunchKernelGGL(quantize_tiles_kernel<DT>, dim3((uint32_t)(((uint64_t)p.R + kFpBlock - 1) / kFpBlock) * p.blocks), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL(quantize_rows_kernel<DT>, dim3((uint32_t)(((uint64_t)p.R * p.blocks + 15) / 16)), dim3(256), 0, st, p);
+        p.x = (const char *)p.x + (int64_t)p.R * p.x_stride * (DT == RS_DTYPE_F32 ? 4 : 2);
+        p.q += (int64_t)p.R * p.q_stride;
+        p.scale += (size_t)(tiles ? p.R / kFpBlock : p.R) * p.blocks;
+    }
 }
 
 constexpr uint32_t kPartTiles = 256;                 // tiles of partial sums that the workspace holds ...
@@ -24,7 +33,6 @@ static hipError_t launch_tiles(LinearParams p, hipStream_t st)
     using L = LinearTile<WN, WM, NU, MT, STAGES>;
     static_assert(!SPLIT || L::kTileN * L::kTileM * 4 <= kPartBytes, "a tile's sums fit the workspace");
     const uint64_t tiles = (uint64_t)((p.M + L::kTileM - 1) / L::kTileM) * ((p.N + L::kTileN - 1) / L::kTileN);
-    if (tiles > 0x7FFFFFFF) return hipErrorInvalidValue;
     p.split = SPLIT ? (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({kPartTiles / tiles, p.blocks / 4, 8})) : 1;
     hipLaunchKernelGGL((linear_tile_kernel<DT, WN, WM, NU, MT, STAGES, SPLIT>), dim3((uint32_t)tiles * p.split), dim3(L::kThreads), L::kLds, st, p);
     return hipGetLastError();
@@ -124,6 +132,7 @@ int rs_linear_blocks(const void *x, int64_t x_row_stride, const float *x_scale,
     if (!known(y_dtype)) return RS_ERR_ARG;
     if (M <= 0 || N <= 0 || K <= 0 || M > RS_LINEAR_MAX || N > RS_LINEAR_MAX || K > RS_LINEAR_MAX) return RS_ERR_SHAPE;
     if ((M > 1 && x_row_stride < K) || (N > 1 && w_row_stride < K) || (M > 1 && y_row_stride < N)) return RS_ERR_SHAPE;
+    if (((int64_t)M + 127) / 128 * (((int64_t)N + 127) / 128) > (int64_t)(kGridThreads / 256u)) return RS_ERR_SHAPE;    // workgroups of a launch
     if (((uintptr_t)x & 15) || (M > 1 && (x_row_stride & 15)) || ((uintptr_t)w & 15) || (N > 1 && (w_row_stride & 15)) ||
         ((uintptr_t)x_scale & 3) || ((uintptr_t)w_scale & 3) || ((uintptr_t)y & (y_dtype == RS_DTYPE_F32 ? 3 : 1)))
         return RS_ERR_ALIGN;

@@ -44,6 +44,7 @@ struct LpParams {
     float      *top_logprobs;
     int32_t    *top_tokens;
     float4     *stats;                   // for the gradient: max, log2 of the sum, entropy; or null
+    uint32_t    row0;                    // the launch's first row
     uint32_t    S, J;                    // workgroups per row (at most kLpStretches); windows per thread and slice
     uint32_t    seg_log;                 // a stretch is 2^seg_log windows, four at least
     LpSlice    *slices;                  // split rows: what the workgroups of a row leave for the last of them
@@ -64,6 +65,7 @@ struct LpGradParams {
     const float  *g, *h, *a;             // gradients of logprob, entropy, alternatives; any may be null
     int32_t       g_stride, h_stride, a_stride;
     void         *grad;                  // contiguous rows of the logits' type
+    uint32_t      row0;                  // the launch's first row
     uint32_t      chunks;                // workgroups per row
 };
 
@@ -507,7 +509,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LpParams p)
     constexpr int U = 4;
     static_assert(!SPLIT || NT == kLpThreads, "what the slices leave is of that many threads");
     __shared__ LpShared<NT> sh;
-    const uint32_t r = SPLIT ? blockIdx.x / p.S : blockIdx.x, slice = SPLIT ? blockIdx.x - r * p.S : 0;
+    const uint32_t r = SPLIT ? blockIdx.x / p.S : p.row0 + blockIdx.x, slice = SPLIT ? blockIdx.x - r * p.S : 0;
     const uint32_t b = r / (uint32_t)p.T, pos = r - b * (uint32_t)p.T;
     const uint32_t V = (uint32_t)p.V, full = V / E::kVec, tid = threadIdx.x;
     const typename E::T *row = (const typename E::T *)p.logits + (int64_t)b * p.stride_b + (int64_t)pos * p.stride_t;
@@ -647,7 +649,7 @@ __global__ __launch_bounds__(kWave) void logprobs_grad_kernel(LpGradParams p)
 {
     using E = Elem<DT>;
     constexpr int U = 4;
-    const uint32_t r = blockIdx.x / p.chunks, chunk = blockIdx.x - r * p.chunks;
+    const uint32_t in = blockIdx.x / p.chunks, chunk = blockIdx.x - in * p.chunks, r = p.row0 + in;
     const uint32_t b = r / (uint32_t)p.T, pos = r - b * (uint32_t)p.T;
     const uint32_t V = (uint32_t)p.V, full = V / E::kVec, lane = threadIdx.x;
     const typename E::T *row = (const typename E::T *)p.logits + (int64_t)b * p.stride_b + (int64_t)pos * p.stride_t;

@@ -30,12 +30,24 @@ static int lp_check(const void *logits, int32_t dtype, const void *tokens, int32
     return RS_OK;
 }
 
-template <int DT>
-static void lp_launch(const LpParams &p, uint32_t rows, bool one_wave, hipStream_t st)
+// f(first row, rows) for as many rows at a time as a launch of `threads` to a row holds.
+template <typename F>
+static void lp_rows(uint32_t rows, uint32_t threads, F f)
 {
-    if (one_wave) hipLaunchKernelGGL((logprobs_kernel<DT, kWave, false>), dim3(rows), dim3(kWave), 0, st, p);
-    else if (p.S > 1) hipLaunchKernelGGL((logprobs_kernel<DT, kLpThreads, true>), dim3(rows * p.S), dim3(kLpThreads), 0, st, p);
-    else hipLaunchKernelGGL((logprobs_kernel<DT, kLpThreads, false>), dim3(rows), dim3(kLpThreads), 0, st, p);
+    const uint32_t most = kGridThreads / threads;
+    for (uint32_t done = 0; done < rows; done += std::min(most, rows - done)) f(done, std::min(most, rows - done));
+}
+
+template <int DT>
+static void lp_launch(LpParams p, uint32_t rows, bool one_wave, hipStream_t st)
+{
+    p.row0 = 0;
+    if (p.S > 1) hipLaunchKernelGGL((logprobs_kernel<DT, kLpThreads, true>), dim3(rows * p.S), dim3(kLpThreads), 0, st, p);
+    else lp_rows(rows, one_wave ? kWave : kLpThreads, [&](uint32_t first, uint32_t n) {
+        p.row0 = first;
+        if (one_wave) hipLaunchKernelGGL((logprobs_kernel<DT, kWave, false>), dim3(n), dim3(kWave), 0, st, p);
+        else hipLaunchKernelGGL((logprobs_kernel<DT, kLpThreads, false>), dim3(n), dim3(kLpThreads), 0, st, p);
+    });
 }
 
 // Many short rows: a wave each, without a barrier.  When this was chosen 262144 x 256 bfloat16 logits and 20 alternatives took 426 us
@@ -117,12 +129,14 @@ int rs_token_logprobs_backward(const void *logits, int32_t dtype, int64_t stride
     p.g_stride = grad_logprobs_stride; p.h_stride = grad_entropy_stride; p.a_stride = grad_top_stride;
     p.grad = grad_logits;
     p.chunks = std::max(1u, (windows + kLpGradWindows - 1) / kLpGradWindows);
-    if ((uint64_t)rows * p.chunks > 0x7FFFFFFFull) return RS_ERR_BATCH;
-    const dim3 grid(rows * p.chunks), block(kWave);
     const hipStream_t st = (hipStream_t)stream;
-    if (dtype == RS_DTYPE_F32) hipLaunchKernelGGL(logprobs_grad_kernel<RS_DTYPE_F32>, grid, block, 0, st, p);
-    else if (dtype == RS_DTYPE_BF16) hipLaunchKernelGGL(logprobs_grad_kernel<RS_DTYPE_BF16>, grid, block, 0, st, p);
-    else hipLaunchKernelGGL(logprobs_grad_kernel<RS_DTYPE_F16>, grid, block, 0, st, p);
+    lp_rows(rows, p.chunks * kWave, [&](uint32_t first, uint32_t n) {
+        const dim3 grid(n * p.chunks), block(kWave);
+        p.row0 = first;
+        if (dtype == RS_DTYPE_F32) hipLaunchKernelGGL(logprobs_grad_kernel<RS_DTYPE_F32>, grid, block, 0, st, p);
+        else if (dtype == RS_DTYPE_BF16) hipLaunchKernelGGL(logprobs_grad_kernel<RS_DTYPE_BF16>, grid, block, 0, st, p);
+        else hipLaunchKernelGGL(logprobs_grad_kernel<RS_DTYPE_F16>, grid, block, 0, st, p);
+    });
     return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
 }
 

@@ -449,8 +449,8 @@ void check_floats(const at::Tensor &x, int64_t block_rows)
         throw std::invalid_argument("x must have shape (..., K), or (N, K) for blocks of 128 x 128 !\n");
     if (!x.is_cuda()) throw std::invalid_argument("x must live on the GPU !\n");
     const int64_t K = x.size(-1);
-    if (K < 1 || K > RS_LINEAR_MAX || x.numel() / K > 0x7FFFFFFF / ((K + 127) / 128))
-        throw std::invalid_argument("x has no columns, or too many elements !\n");
+    if (K < 1 || K > RS_LINEAR_MAX || x.numel() / K > 0x7FFFFFFF)
+        throw std::invalid_argument("x has no columns, or too many columns or rows !\n");
     if (x.stride(-1) != 1 && K > 1) throw std::invalid_argument("x must be contiguous along its last axis !\n");
 }
 void quantize_into(const at::Tensor &x, int64_t block_rows, void *q, float *scale, void *stream)
@@ -520,7 +520,7 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const at::Tenso
     const bool given = x.dtype() == at::kFloat8_e4m3fn;
     if (given != x_scale.has_value()) throw std::invalid_argument("x_scale goes with an x of type float8_e4m3fn, and only with one !\n");
     const int64_t K = weight.size(1), N = weight.size(0), blocks = (K + 127) / 128, M = x.numel() / K;
-    if (M > RS_LINEAR_MAX || N > RS_LINEAR_MAX || K > RS_LINEAR_MAX) throw std::invalid_argument("x or weight is too large !\n");
+    if (M > RS_LINEAR_MAX || N > RS_LINEAR_MAX || K > RS_LINEAR_MAX || (M + 127) / 128 * ((N + 127) / 128) >= 1 << 24) throw std::invalid_argument("x or weight is too large !\n");
     if (!given) check_floats(x, 1);
     const at::Tensor w = fp8_rows(weight, "weight");
     check_scale(weight_scale, weight, (N + 127) / 128, blocks, "weight_scale");
