@@ -14,8 +14,9 @@ Drop-in for the Python API of the reference module (`sample` in
 Beyond the reference: keyword names, `uniforms=` (injected draws, for tests),
 `accept_half=True` (bfloat16 / float16 logits read as they are; by default any
 type but float32 raises the reference's error), `reserve_workspace(B, V)`
-(allocates the current stream's workspace ahead of time: required before the
-calls are captured into a HIP graph), `workspace_status()` (synchronises and
+(allocates the current stream's workspaces ahead of time: required before the
+calls are captured into a HIP graph; any V, and `operators=False` leaves out the
+12.6 MB of the functions next to the sampler), `workspace_status()` (synchronises and
 returns the error word of the current stream's workspace), `set_wait_limit` and
 `reset_routing()` (forgets what the stream's calls have learnt about which
 kernel suits the workload; for measurements that change workload on one stream).

@@ -637,17 +637,20 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> batch_sampling_debug(
     return {out, dbg.diag, dbg.e_bits};
 }
 
-// Allocates and clears the workspace of the current stream of `device` for calls of up to B rows
-// of up to V tokens.  Needed before a stream capture (nothing may be allocated while capturing);
-// otherwise optional: the first call of a shape does the same.
-void reserve_workspace(int64_t B, int64_t V, std::optional<int64_t> device)
+// Allocates and clears the workspaces of the current stream of `device`: the sampler's, for calls of up to B rows of up to V tokens (a V
+// that the sampler does not take, for the next that it does), and, unless `operators` is false, those of token_logprobs and linear_fp8
+// (12.6 MB, whatever the sizes).  Needed before a stream capture (nothing may be allocated while capturing); otherwise
+// optional: the first call of a shape does the same.
+void reserve_workspace(int64_t B, int64_t V, std::optional<int64_t> device, bool operators)
 {
     size_t bytes = 0;
+    if (V > 0 && V <= 1048576) V = (V + 3) / 4 * 4;
     throw_for(rs_workspace_bytes((int32_t)B, (int32_t)V, &bytes), B, 1, V, 1.0);
     const auto dev = at::Device(at::kCUDA, (c10::DeviceIndex)(device ? *device : c10::hip::current_device()));
     c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
     auto like = at::empty({1}, at::TensorOptions().dtype(at::kChar).device(dev));
     workspace_for(like, current_stream(like), B, V);
+    if (!operators) return;
     logprobs_workspace(like, current_stream(like));
     linear_workspace(like, current_stream(like));
 }
@@ -781,7 +784,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           py::arg("temperature"), py::arg("top_k"), py::arg("top_p"), py::kw_only(),
           py::arg("uniforms") = py::none(), py::arg("accept_half") = false);
     m.def("floor_read", &floor_read, py::arg("logits"), py::arg("variant") = 1);
-    m.def("reserve_workspace", &reserve_workspace, py::arg("B"), py::arg("V"), py::arg("device") = py::none());
+    m.def("reserve_workspace", &reserve_workspace, py::arg("B"), py::arg("V"), py::arg("device") = py::none(), py::kw_only(),
+          py::arg("operators") = true);
     m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("tokens"), py::arg("temperature") = 1.0, py::kw_only(),
           py::arg("top") = 0);
     m.def("quantize_fp8", &quantize_fp8, py::arg("x"), py::kw_only(), py::arg("block_rows") = 1);
