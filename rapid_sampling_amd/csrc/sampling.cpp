@@ -498,7 +498,7 @@ at::Tensor fp8_rows(const at::Tensor &t, const char *what)
 
 void check_scale(const at::Tensor &scale, const at::Tensor &like, int64_t rows, int64_t blocks, const char *what)
 {
-    if (scale.dtype() != at::kFloat || scale.device() != like.device() || !scale.is_contiguous() || scale.size(-1) != blocks ||
+    if (scale.dtype() != at::kFloat || scale.device() != like.device() || !scale.is_contiguous() || scale.dim() < 1 || scale.size(-1) != blocks ||
         scale.numel() != rows * blocks)
         throw std::invalid_argument(std::string(what) + " must be a contiguous float32 GPU tensor of " + std::to_string(rows) + " x " +
                                     std::to_string(blocks) + " scales !\n");

@@ -295,6 +295,20 @@ def test_refusals_on_the_gpu():
         assert sample.linear_fp8(learnt, w, s).shape == (2, 20)
 
 
+@gpu
+def test_scales_without_a_dimension_are_refused():
+    """One number for all blocks is no scale for each, not even where there is one block."""
+    import rapid_sampling_amd as sample
+    x, w = make(1, 100, "f32", 1), make(20, 100, "f32", 2)
+    w, s = sample.quantize_fp8(w, block_rows=128)
+    qx, sx = sample.quantize_fp8(x)
+    with pytest.raises(ValueError, match="weight_scale"):
+        sample.linear_fp8(x, w, s[0, 0])
+    with pytest.raises(ValueError, match="x_scale"):
+        sample.linear_fp8(qx, w, s, x_scale=sx[0, 0])
+    assert torch.equal(sample.linear_fp8(qx, w, s, x_scale=sx), sample.linear_fp8(x, w, s))
+
+
 def test_refusals_of_the_c_abi():
     import ctypes as C
 
