@@ -400,6 +400,7 @@ struct LinearTile {
         __amdgpu_buffer_rsrc_t w, x;
         uint32_t w_stride, x_stride, w_rows, x_rows;
         uint32_t w_piece[2], x_piece;    // byte of a block of the thread's piece of its row of an even, of an odd load
+        uint32_t first[kLoads];          // at(i, 0)
 
         // The thread's byte of load i, of the block that begins at column k
         __device__ __forceinline__ uint32_t at(uint32_t i, uint32_t k) const
@@ -419,6 +420,11 @@ struct LinearTile {
         s.x = __builtin_amdgcn_make_buffer_rsrc((void *)(p.x + (int64_t)m0 * p.x_stride), 0, (int)tile_bytes(s.x_rows, s.x_stride, p.K), kBufferFlags);
         for (uint32_t i = 0; i < 2; ++i) s.w_piece[i] = ((threadIdx.x & 7u) ^ w_turn<NU>(row_of(i))) * 16u;
         s.x_piece = ((threadIdx.x & 7u) ^ x_turn(row_of(0))) * 16u;
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            s.first[i] = s.at(i, 0);
+            asm volatile("" : "+v"(s.first[i]));      // once, and not for every block (2 to 4 % of 256 x 4096 x 4096)
+        }
         return s;
     }
     static __device__ __forceinline__ void fill(const LinearParams &p, const Source &s, uint32_t n0, uint32_t m0, uint32_t kb, uint8_t *lds)
@@ -428,7 +434,7 @@ struct LinearTile {
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
                 const LdsPtr to = (LdsPtr)(lds + (i * kWaves + wave_id()) * 1024u);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kLoadsW ? s.w : s.x, to, 16, s.at(i, 0), k, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kLoadsW ? s.w : s.x, to, 16, s.first[i], k, 0, 0);
             }
             return;
         }
