@@ -729,7 +729,7 @@ using namespace rs;
 
 extern "C" {
 
-int rs_version(void) { return 500; }
+int rs_version(void) { return 510; }
 
 const char *rs_error_string(int code)
 {

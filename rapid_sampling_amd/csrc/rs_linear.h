@@ -213,7 +213,7 @@ __device__ __forceinline__ v4f block_product(const v8bf (&w)[4], const v8bf (&x)
 }
 
 // Four consecutive values, or eight of 16 bits, in one store.  y's rows begin at any multiple of a value's size (an odd number of
-// columns): the hardware stores at any address, 77 x 50257 x 2000 into bfloat16 took 45 us in single values.
+// columns), and the hardware stores at any address: 128 x 50257 x 2048 into bfloat16 41 us, 65 in single values.
 template <int DT> __device__ __forceinline__ void put_four(void *p, int64_t i, v4f a)
 {
     if constexpr (DT == RS_DTYPE_F32) __builtin_memcpy((float *)p + i, &a, 16);

@@ -25,8 +25,8 @@ constexpr uint32_t kPartTiles = 256;                 // tiles of partial sums th
 constexpr size_t   kPartBytes = 128 * 64 * 4;        // ... of 128 x 64
 
 // SPLIT: where there are few tiles their blocks of columns are shared out, for up to one workgroup to a compute unit.  Leaving and
-// adding up the parts costs about 2 us, a block 0.9: four blocks to each at least (64 x 1024 x 4096: 24 us whole, 12 in eight;
-// 64 x 4096 x 512: 4.7 whole, 6.6 in two).
+// adding up the parts costs about 2 us, a block 0.9: four blocks to each at least (64 x 1024 x 4096: 30.7 us whole, 12.9 in eight;
+// 64 x 4096 x 512: 6.5 whole, 8.0 in two).
 template <int DT, int WN, int WM, int NU, int MT, int STAGES, bool SPLIT>
 static hipError_t launch_tiles(LinearParams p, hipStream_t st)
 {
@@ -47,7 +47,8 @@ static hipError_t launch_few(const LinearParams &p, hipStream_t st)
     return hipGetLastError();
 }
 
-// 32 rows of w to a workgroup, 16 where there are few (1 x 1024 x 8192: 7.7 us against 10.5; 1 x 65536 x 4096: 55.6 against 48.5).
+// 32 rows of w to a workgroup, 16 where there are few (x in 8 bits, 1 x 1024 x 8192: 13.9 us against 10.1; 1 x 8192 x 4096: 9.6
+// against 9.4; 1 x 16384 x 4096: 15.3 against 16.5; 1 x 65536 x 4096: 50.8 against 59.1).
 template <int DT, int XT>
 static hipError_t launch_few(const LinearParams &p, hipStream_t st)
 {
@@ -64,15 +65,16 @@ static hipError_t launch_rows(const LinearParams &p, int32_t x_dtype, hipStream_
 template <int DT>
 static hipError_t launch_linear(const LinearParams &p, hipStream_t st)
 {
-    // Up to 16 rows one 16 x 16 product holds them all, and nothing but w is worth staging (1 x 131072 x 4096: 93, 5.8 TB/s).
+    // Up to 16 rows one 16 x 16 product holds them all, and nothing but w is worth staging (1 x 131072 x 4096: 98, 5.5 TB/s).
     // (The tiles' kernel reaches its rows with 32 bits.)
     if (p.M <= 16 || p.x_stride > kTileStride || p.w_stride > kTileStride) return launch_few<DT, -1>(p, st);
     // Tiles of 128 x 64 (rows of w x rows of x) for up to 64 rows, and wherever those of 128 x 128 would not give every compute unit
-    // its own.  Two waves share w's rows and two x's, since both have to be widened (64 x 50256 x 2000: 25.7 against 29.0 with four and
-    // one).
+    // its own (100 x 8192 x 4096: 21.8 against 40.6; 1000 x 4096 x 4096: 46.6 against 47.3).  Two waves share w's rows and two x's,
+    // since both have to be widened (64 x 131072 x 4096: 118.6 against 121.5 with four and one).
     const uint64_t n128 = (p.N + 127) / 128, m128 = (p.M + 127) / 128;
     if (p.M <= 64 || n128 * m128 <= 256) return launch_tiles<DT, 2, 2, 4, 2, 3, true>(p, st);
-    // 128 x 128: 4096 x 32768 x 4096 in 1076 (1.02 PFLOP/s); 1278 in tiles of 128 x 64
+    // 128 x 128: 4096 x 32768 x 4096 in 1105, 1055 into bfloat16 (1.0 PFLOP/s), against 1329 and 1257 in tiles of 128 x 64; 300 x 16384
+    // x 4096 in 69.6 against 72.5
     return launch_tiles<DT, 1, 4, 8, 2, 2, false>(p, st);
 }
 

@@ -530,8 +530,8 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const at::Tenso
     at::Tensor y = at::empty(sizes, at::TensorOptions().dtype(to).device(x.device()));
     if (!M) return y;
     // One launch for a few rows, where the launch that it saves (2 to 5 us) is more than what the workgroups spend on rounding the same
-    // rows each for itself: 1 x 8192 x 4096 7.7 us against 12.5, 1 x 65536 x 4096 52.8 either way, 4 x 16384 x 4096 16.3
-    // against 18.0, 4 x 65536 x 4096 59.4 against 55.7.
+    // rows each for itself: 1 x 8192 x 4096 8.7 us against 11.4, 1 x 65536 x 4096 51.7 against 52.6, 4 x 16384 x 4096 17.0
+    // against 18.1, 4 x 65536 x 4096 60.0 against 55.7.
     if (!given && M <= RS_LINEAR_ROWS_MAX && M * N <= 65536 && K <= RS_LINEAR_ROWS_COLUMNS_MAX) {
         const at::Tensor flat = x.dim() == 2 ? x : x.reshape({M, K});
         const int rc = rs_linear_rows(flat.data_ptr(), float_dtype(x, "x"), flat.stride(0), w.data_ptr(), w.stride(0), weight_scale.data_ptr<float>(),
