@@ -37,7 +37,7 @@ extern "C" {
 #define RS_ERR_DEVICE      -9   /* a kernel gave up waiting for its peer workgroups           */
 #define RS_ERR_SCRATCH     -10  /* rs_sample_static: the call needs more than RS_STATIC_SCRATCH_BYTES */
 #define RS_ERR_UNSUPPORTED -11  /* the current device is not a whole MI355X (256 compute units)     */
-#define RS_ERR_SHAPE       -12  /* rs_quantize_blocks, rs_linear_*: a size or a row stride out of range */
+#define RS_ERR_SHAPE       -12  /* the operators next to the sampler: a size or a row stride out of range */
 
 /* Bytes of RNG state per row.  Same size as the reference's
  * curandStatePhilox4_32_10_t record (sampling.cu:9,141) so that the opaque
@@ -564,6 +564,125 @@ int rs_linear_blocks(const void *x_device, int64_t x_row_stride, const float *x_
 int rs_linear_rows(const void *x_device, int32_t x_dtype, int64_t x_row_stride,
                    const void *w_device, int64_t w_row_stride, const float *w_scale_device,
                    int32_t M, int32_t N, int32_t K, void *y_device, int32_t y_dtype, int64_t y_row_stride, void *stream);
+
+/*
+ * R rows of K values of `size` bytes each (2 or 4), x_row_stride elements apart (0 or
+ * more), laid out y_row_stride elements apart in multiples of 16 bytes, 16-byte
+ * aligned, with zeros behind column K.  No counterpart in the reference.
+ */
+int rs_lay_out_rows(const void *x_device, int64_t x_row_stride, int32_t size, int64_t R, int32_t K, void *y_device, int64_t y_row_stride, void *stream);
+
+/*
+ * Cross entropy of tokens under softmax(x w^T / temperature), without the logits.
+ * x (M, K) and w (V, K) of one type (RS_DTYPE_*), rows x_row_stride and w_row_stride
+ * elements apart, at least K, in multiples of 16 bytes below 16 MB, 16-byte aligned
+ * (rs_lay_out_rows makes such rows of others).  What lies behind column K is not
+ * looked at.
+ *   lse    ln sum_v e^(x_m . w_v / temperature), of every row
+ *   loss   lse - x_m . w_t / temperature for the row's token t; 0 for a negative
+ *          one, which is none; NaN for one of V or more
+ * float32 sums, whatever the type, in an order that does not depend on chance.
+ * Tokens are int32 or (tokens_64 = 1) int64, token_stride elements apart.  stats:
+ * NULL, or (M, 2) floats, 8-byte aligned, for the gradient.  A row whose logits are
+ * all -inf has lse -inf and loss +inf; one with a NaN or +inf among them NaN.
+ * M up to RS_LINEAR_MAX, V up to 1048576, K up to RS_LOSS_COLUMNS_MAX, and
+ * ceil(M / 64) ceil(V / 128) below 2^24.
+ * workspace: rs_linear_cross_entropy_workspace_bytes() bytes of device memory,
+ * 256-byte aligned, of any contents; calls that share it are ordered on one stream.
+ * No counterpart in the reference.
+ */
+#define RS_LOSS_COLUMNS_MAX (1 << 20)
+size_t rs_linear_cross_entropy_workspace_bytes(int32_t M, int32_t V, int32_t K, int32_t dtype, int32_t backward);
+int rs_linear_cross_entropy(const void *x_device, int64_t x_row_stride, const void *w_device, int64_t w_row_stride, int32_t dtype,
+                            const void *tokens_device, int32_t tokens_64, int64_t token_stride, int32_t M, int32_t V, int32_t K,
+                            double temperature, float *loss_device, float *lse_device, float *stats_device,
+                            void *workspace_device, size_t workspace_bytes, void *stream);
+
+/*
+ * Gradients of x (M, K) and w (V, K), contiguous, of their type; either may be NULL.
+ * With g the gradient of the losses and h that of lse (either may be NULL: none; a
+ * stride of 1, or of 0: one number for all rows), p the probabilities:
+ *   G = ((g + h) p - g [v = t]) / temperature     grad_x = G w     grad_w = G^T x
+ * G is rounded to the inputs' type; sums are float32, and rounded once.  A negative
+ * token has no g, one of V or more has NaN for it.  The other arguments as in the
+ * call whose stats are passed.
+ */
+int rs_linear_cross_entropy_backward(const void *x_device, int64_t x_row_stride, const void *w_device, int64_t w_row_stride, int32_t dtype,
+                                     const void *tokens_device, int32_t tokens_64, int64_t token_stride, int32_t M, int32_t V, int32_t K,
+                                     double temperature, const float *stats_device,
+                                     const float *grad_loss_device, int32_t grad_loss_stride, const float *grad_lse_device, int32_t grad_lse_stride,
+                                     void *grad_x_device, void *grad_w_device, void *workspace_device, size_t workspace_bytes, void *stream);
+
+/*
+ * Values as 8-bit integers with a float32 scale for each row:
+ *   scale = max(max |x| * r, 2^-126), r = 1/127 in float32
+ *   q     = x / scale, to the nearest integer, ties to even: -127 to 127
+ * x: R rows of K values, x_row_stride elements apart (0 or more), at any address.
+ * q: rows q_row_stride bytes apart, a multiple of 16, 16-byte aligned; the bytes behind
+ * column K are cleared.  A row with a NaN or an infinity has the scale NaN and
+ * integers of 0.  One launch, or several one after the other from 2^24 rows on.  No
+ * counterpart in the reference.
+ */
+int rs_quantize_rows(const void *x_device, int32_t x_dtype, int64_t x_row_stride, int32_t R, int32_t K,
+                     int8_t *q_device, int64_t q_row_stride, float *scale_device, void *stream);
+
+/*
+ * y[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] for such values: x (M, K), w
+ * (N, K), one scale for each row of either, y (M, N) float32, bfloat16 or float16.
+ * The sums are exact, for any integers of 8 bits (-128 among them) and K up to
+ * RS_LINEAR_INT8_COLUMNS_MAX; a result is float32(sum) * (x_scale * w_scale) in
+ * float32, rounded to y's type, and is the same whatever rows stand beside it.  Rows of x and
+ * w 16-byte aligned; bytes behind column K are not looked at.  workspace: as
+ * rs_linear_blocks', and calls of either may share it on one stream.  M and N at most
+ * RS_LINEAR_MAX, and ceil(M / 64) ceil(N / 128) below 2^24.  One launch.  No counterpart
+ * in the reference.
+ */
+#define RS_LINEAR_INT8_COLUMNS_MAX 131071
+int rs_linear_int8(const int8_t *x_device, int64_t x_row_stride, const float *x_scale_device,
+                   const int8_t *w_device, int64_t w_row_stride, const float *w_scale_device,
+                   int32_t M, int32_t N, int32_t K, void *y_device, int32_t y_dtype, int64_t y_row_stride,
+                   void *workspace_device, size_t workspace_bytes, void *stream);
+
+/*
+ * rs_quantize_rows and rs_linear_int8 in one launch, without anything in between, for
+ * up to RS_LINEAR_ROWS_MAX rows of up to RS_LINEAR_ROWS_COLUMNS_MAX columns of x in
+ * float32, bfloat16 or float16 (rows x_row_stride elements apart, at any
+ * address).  The same y.  No workspace.  No counterpart in the reference.
+ */
+int rs_linear_int8_rows(const void *x_device, int32_t x_dtype, int64_t x_row_stride,
+                        const int8_t *w_device, int64_t w_row_stride, const float *w_scale_device,
+                        int32_t M, int32_t N, int32_t K, void *y_device, int32_t y_dtype, int64_t y_row_stride, void *stream);
+
+/*
+ * Rows of a table by token: y[i] = scale w[token i], rounded once to y's type.
+ *   tokens        M of them, int32 or (tokens_64 = 1) int64, token_stride elements
+ *                 apart.  A negative one is none: its row is 0.  One of V or more has
+ *                 a row of NaN.
+ *   w             V rows of K, w_row_stride elements apart: float32, bfloat16 or
+ *                 float16 at any address (w_scale is not looked at), or RS_TABLE_INT8 with
+ *                 one scale for each row (rs_quantize_rows), or RS_TABLE_FP8 with
+ *                 ceil(V / 128) x ceil(K / 128) (rs_quantize_blocks), in rows of
+ *                 multiples of 16 bytes, 16-byte aligned.
+ *   y             (M, K), contiguous, float32, bfloat16 or float16
+ * V and K up to RS_LINEAR_MAX, M below it.  One launch.  No counterpart in the reference.
+ */
+#define RS_TABLE_INT8 3
+#define RS_TABLE_FP8  4
+int rs_embedding(const void *tokens_device, int32_t tokens_64, int64_t token_stride, const void *w_device, int32_t w_dtype, int64_t w_row_stride,
+                 const float *w_scale_device, double scale, int32_t M, int32_t V, int32_t K, void *y_device, int32_t y_dtype, void *stream);
+
+/*
+ * The table's gradient from y's, g (M, K), rows g_row_stride elements apart (0 or more):
+ * dw[v] = scale times the sum of g's rows whose token is v, (V, K), contiguous;
+ * 0 in rows without one.  float32 sums in the order of the rows, which does not
+ * depend on chance (up to a few dozen tokens one after the other, more of them in
+ * chunks), rounded once.  Tokens outside the vocabulary have none.
+ * workspace: rs_embedding_workspace_bytes() bytes of device memory, 256-byte aligned,
+ * of any contents; calls that share it are ordered on one stream.
+ */
+size_t rs_embedding_workspace_bytes(int32_t M, int32_t V, int32_t K);
+int rs_embedding_backward(const void *tokens_device, int32_t tokens_64, int64_t token_stride, const void *g_device, int32_t g_dtype,
+                          int64_t g_row_stride, double scale, int32_t M, int32_t V, int32_t K, void *dw_device, int32_t dw_dtype, void *workspace_device, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

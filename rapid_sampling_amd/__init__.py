@@ -75,6 +75,9 @@ set_wait_limit = _sample.set_wait_limit
 reset_routing = _sample.reset_routing
 quantize_fp8 = _sample.quantize_fp8
 linear_fp8 = _sample.linear_fp8
+quantize_int8 = _sample.quantize_int8
+linear_int8 = _sample.linear_int8
+embedding = _sample.embedding
 LOGPROBS_TOP_MAX = _sample.LOGPROBS_TOP_MAX
 STATE_BYTES_PER_ROW = _sample.STATE_BYTES_PER_ROW
 DIAG_BYTES = _sample.DIAG_BYTES
@@ -95,6 +98,18 @@ def token_logprobs(logits, tokens, temperature=1.0, *, top=0):
     return TokenLogprobs(*_sample.token_logprobs(logits, tokens, temperature, top=top))
 
 
+class LinearCrossEntropy(_NamedTuple):
+    """What linear_cross_entropy returns, both float32 and of the tokens' shape."""
+    loss: _torch.Tensor
+    logsumexp: _torch.Tensor
+
+
+def linear_cross_entropy(x, weight, tokens, temperature=1.0):
+    """Cross entropy of `tokens` (int32 or int64) under softmax(x @ weight.T / temperature) without the logits: a
+    LinearCrossEntropy.  See the module's docstring."""
+    return LinearCrossEntropy(*_sample.linear_cross_entropy(x, weight, tokens, temperature))
+
+
 KERNEL_LIBRARY = _os.path.join(_HERE, "librapid_sampling_hip.so")
 
 __all__ = [
@@ -106,6 +121,11 @@ __all__ = [
     "TokenLogprobs",
     "quantize_fp8",
     "linear_fp8",
+    "quantize_int8",
+    "linear_int8",
+    "embedding",
+    "linear_cross_entropy",
+    "LinearCrossEntropy",
     "floor_read",
     "reserve_workspace",
     "workspace_status",

@@ -37,7 +37,7 @@ def _run(cmd, verbose):
 
 
 KERNEL_SOURCES = ["rs_api.hip", "rs_cluster.hip", "rs_stream.hip", "rs_wide.hip", "rs_row.hip", "rs_short.hip", "rs_sieve.hip",
-                  "rs_logprobs.hip", "rs_linear.hip"]
+                  "rs_logprobs.hip", "rs_linear.hip", "rs_int8.hip", "rs_loss.hip", "rs_embedding.hip"]
 
 
 def build_kernels(verbose=False):

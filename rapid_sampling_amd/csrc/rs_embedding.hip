@@ -1,0 +1,138 @@
+// Instantiations, launchers and C entry points of the embedding and its gradient.
+#include "rs_embedding.h"
+
+#include <algorithm>
+
+namespace rs {
+
+static uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+
+// Threads of a row: one for each eight columns, in powers of two up to a workgroup.
+static uint32_t row_width(uint32_t K)
+{
+    uint32_t w = 0;
+    while (w < 8 && (8u << w) < K) ++w;
+    return w;
+}
+
+template <int WT, int DT> static void launch_embedding(const EmbeddingParams &p, hipStream_t st)
+{
+    const uint32_t rows = 256u >> p.width;
+    hipLaunchKernelGGL((embedding_kernel<WT, DT>), dim3((p.M + rows - 1) / rows), dim3(256), 0, st, p);
+}
+template <int WT> static void launch_embedding(const EmbeddingParams &p, int32_t dtype, hipStream_t st)
+{
+    if (dtype == RS_DTYPE_F32) launch_embedding<WT, RS_DTYPE_F32>(p, st);
+    else if (dtype == RS_DTYPE_BF16) launch_embedding<WT, RS_DTYPE_BF16>(p, st);
+    else launch_embedding<WT, RS_DTYPE_F16>(p, st);
+}
+
+// Where a gradient's scratch lies.
+struct TableSpace {
+    uint64_t keys[2], at[2], counts, parts, bytes = 0;
+    uint32_t digits, bits, chunk, groups;
+    uint64_t take(uint64_t n) { const uint64_t a = bytes; bytes += up(n, 256); return a; }
+};
+static TableSpace table_space(uint32_t N, uint32_t V, uint32_t K)
+{
+    TableSpace s;
+    uint32_t bits = 1;
+    while (bits < 32 && (V >> bits)) ++bits;             // of a token, or of V itself
+    s.digits = (bits + kSortBits - 1) / kSortBits;
+    s.bits = (bits + s.digits - 1) / s.digits;
+    s.groups = N <= kSortAlone ? 1 : (N + kSortTile - 1) / kSortTile;
+    // chunks of about the square root of the tokens: a token that makes up all of them has as many chunks to add as each has rows
+    s.chunk = 5;
+    while (s.chunk < 12 && (1ull << (2 * s.chunk + 2)) <= N) ++s.chunk;
+    for (int i = 0; i < 2; ++i) { s.keys[i] = s.take(4ull * N); s.at[i] = s.take(4ull * N); }
+    s.counts = s.take(N <= kSortAlone ? 0 : 4ull * s.groups << s.bits);
+    s.parts = s.take((uint64_t)(N >> s.chunk) * K * 4);
+    return s;
+}
+
+template <int GT> static void launch_sums(const TableGradParams &p, int32_t dtype, hipStream_t st)
+{
+    if (p.N >> p.chunk)
+        hipLaunchKernelGGL(table_chunk_kernel<GT>, dim3(p.N >> p.chunk, (p.K + 2047) / 2048), dim3(256), 0, st, p);
+    const dim3 groups((p.V + kTableRows - 1) / kTableRows), threads(256);
+    if (dtype == RS_DTYPE_F32) hipLaunchKernelGGL((table_grad_kernel<GT, RS_DTYPE_F32>), groups, threads, 0, st, p);
+    else if (dtype == RS_DTYPE_BF16) hipLaunchKernelGGL((table_grad_kernel<GT, RS_DTYPE_BF16>), groups, threads, 0, st, p);
+    else hipLaunchKernelGGL((table_grad_kernel<GT, RS_DTYPE_F16>), groups, threads, 0, st, p);
+}
+
+static bool known(int32_t dtype) { return dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16 || dtype == RS_DTYPE_F16; }
+static uint32_t size_of(int32_t dtype) { return dtype == RS_DTYPE_F32 ? 4 : 2; }
+
+}  // namespace rs
+
+using namespace rs;
+
+extern "C" {
+
+int rs_embedding(const void *tokens, int32_t tokens_64, int64_t token_stride, const void *w, int32_t w_dtype, int64_t w_stride, const float *w_scale,
+                 double scale, int32_t M, int32_t V, int32_t K, void *y, int32_t y_dtype, void *stream)
+{
+    const bool eight = w_dtype == RS_TABLE_INT8 || w_dtype == RS_TABLE_FP8;
+    if (!tokens || !w || !y || (eight && !w_scale)) return RS_ERR_NULL;
+    if ((!known(w_dtype) && !eight) || !known(y_dtype) || (tokens_64 != 0 && tokens_64 != 1)) return RS_ERR_ARG;
+    if (M <= 0 || V <= 0 || K <= 0 || M >= RS_LINEAR_MAX || V > RS_LINEAR_MAX || K > RS_LINEAR_MAX || (V > 1 && w_stride < (eight ? K : 0))) return RS_ERR_SHAPE;
+    if (((uintptr_t)tokens & (tokens_64 ? 7 : 3)) || ((uintptr_t)y & (size_of(y_dtype) - 1))) return RS_ERR_ALIGN;
+    if (eight ? ((uintptr_t)w & 15) || (V > 1 && (w_stride & 15)) || ((uintptr_t)w_scale & 3) : ((uintptr_t)w & (size_of(w_dtype) - 1)) != 0) return RS_ERR_ALIGN;
+    EmbeddingParams p;
+    p.tokens = TokenList{tokens, token_stride, tokens_64};
+    p.w = w; p.w_stride = w_stride; p.w_scale = w_scale; p.y = y; p.scale = (float)scale;
+    p.M = (uint32_t)M; p.V = (uint32_t)V; p.K = (uint32_t)K; p.width = row_width(p.K);
+    const hipStream_t st = (hipStream_t)stream;
+    if (w_dtype == RS_DTYPE_F32) launch_embedding<RS_DTYPE_F32>(p, y_dtype, st);
+    else if (w_dtype == RS_DTYPE_BF16) launch_embedding<RS_DTYPE_BF16>(p, y_dtype, st);
+    else if (w_dtype == RS_DTYPE_F16) launch_embedding<RS_DTYPE_F16>(p, y_dtype, st);
+    else if (w_dtype == RS_TABLE_INT8) launch_embedding<kTableInt8>(p, y_dtype, st);
+    else launch_embedding<kTableFp8>(p, y_dtype, st);
+    return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
+}
+
+size_t rs_embedding_workspace_bytes(int32_t M, int32_t V, int32_t K)
+{
+    return M > 0 && V > 0 && K > 0 ? table_space((uint32_t)M, (uint32_t)V, (uint32_t)K).bytes : 0;
+}
+
+int rs_embedding_backward(const void *tokens, int32_t tokens_64, int64_t token_stride, const void *g, int32_t g_dtype, int64_t g_stride, double scale,
+                          int32_t M, int32_t V, int32_t K, void *dw, int32_t dw_dtype, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!tokens || !g || !dw || !workspace) return RS_ERR_NULL;
+    if (!known(g_dtype) || !known(dw_dtype) || (tokens_64 != 0 && tokens_64 != 1)) return RS_ERR_ARG;
+    if (M <= 0 || V <= 0 || K <= 0 || M >= RS_LINEAR_MAX || V > RS_LINEAR_MAX || K > RS_LINEAR_MAX || (M > 1 && g_stride < 0)) return RS_ERR_SHAPE;
+    if (((uintptr_t)tokens & (tokens_64 ? 7 : 3)) || ((uintptr_t)g & (size_of(g_dtype) - 1)) || ((uintptr_t)dw & (size_of(dw_dtype) - 1))) return RS_ERR_ALIGN;
+    const TableSpace s = table_space((uint32_t)M, (uint32_t)V, (uint32_t)K);
+    if (workspace_bytes < s.bytes || ((uintptr_t)workspace & 255)) return RS_ERR_WORKSPACE;
+    char *ws = (char *)workspace;
+    const hipStream_t st = (hipStream_t)stream;
+    auto keys = [&](uint32_t i) { return (uint32_t *)(ws + s.keys[i]); };
+    auto at = [&](uint32_t i) { return (uint32_t *)(ws + s.at[i]); };
+    SortParams p = {};
+    p.tokens = TokenList{tokens, token_stride, tokens_64};
+    p.N = (uint32_t)M; p.V = (uint32_t)V; p.bits = s.bits; p.first = 1; p.digits = s.digits;
+    p.counts = (uint32_t *)(ws + s.counts);
+    const uint32_t lds = (kSortWaves << s.bits) * 4;
+    if (p.N <= kSortAlone) {
+        p.keys = keys(0); p.at = at(0); p.keys_b = keys(1); p.at_b = at(1);
+        hipLaunchKernelGGL(sort_alone_kernel, dim3(1), dim3(kSortThreads), lds, st, p);
+    } else
+        for (uint32_t d = 0; d < s.digits; ++d) {
+            p.keys = keys(d & 1); p.at = at(d & 1);
+            hipLaunchKernelGGL(sort_count_kernel, dim3(s.groups), dim3(kSortThreads), lds, st, p);
+            hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(kSortThreads), 0, st, p.counts, s.groups << s.bits);
+            hipLaunchKernelGGL(sort_place_kernel, dim3(s.groups), dim3(kSortThreads), lds, st, p);
+            p.first = 0; p.shift += s.bits; p.keys_in = p.keys; p.at_in = p.at;
+        }
+    TableGradParams t;
+    t.keys = keys((s.digits - 1) & 1); t.at = at((s.digits - 1) & 1);
+    t.g = g; t.g_stride = M > 1 ? g_stride : 0; t.parts = (float *)(ws + s.parts); t.dw = dw; t.scale = (float)scale;
+    t.N = p.N; t.V = p.V; t.K = (uint32_t)K; t.chunk = s.chunk; t.width = row_width(t.K);
+    if (g_dtype == RS_DTYPE_F32) launch_sums<RS_DTYPE_F32>(t, dw_dtype, st);
+    else if (g_dtype == RS_DTYPE_BF16) launch_sums<RS_DTYPE_BF16>(t, dw_dtype, st);
+    else launch_sums<RS_DTYPE_F16>(t, dw_dtype, st);
+    return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -1,0 +1,268 @@
+// Values as 8-bit integers with a float32 scale for each row, and their matrix product:
+//
+//   scale = max(max |x| * r, 2^-126), r = 1/127 in float32        q = x / scale, to the nearest integer, ties to even
+//   y[m, n] = sx[m] sw[n] sum_k qx[m, k] qw[n, k]
+//
+// The sums are whole numbers of 32 bits, which no K up to 131071 leaves (128^2 K < 2^31): exact, in any order.  They are
+// rounded to float32 once, multiplied with the product of the two scales, and rounded to y's type.
+#pragma once
+
+#include "rs_product.h"
+
+namespace rs {
+
+struct Int8Rows {                    // of the quantiser
+    const void *x;
+    int64_t     x_stride;            // elements
+    int8_t     *q;
+    int64_t     q_stride;            // bytes; those behind column K are cleared
+    float      *scale;
+    uint32_t    R, K;
+};
+
+struct Int8Params {
+    Product      a;                  // P: w, Q: x
+    const float *x_scale, *w_scale;
+    void        *y;
+    int64_t      y_stride;
+    const void  *x;                  // few rows: x and w with 64-bit strides
+    int64_t      x_stride, w_stride; // elements of x, bytes of w
+    const int8_t *w;
+    uint32_t     M, N, K;
+    int         *parts;              // sums of workgroups that share a tile's reduction, and how many have left theirs; zero between calls
+    uint32_t    *arrived;
+};
+
+// A row's largest magnitude as the bits of a float without its sign: NaN is larger than infinity, infinity than any number.
+__device__ __forceinline__ uint32_t largest_bits(const float (&x)[8])
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+    return m;
+}
+// A row with an infinity or a NaN has the scale NaN, and so have its results, and integers of 0.
+__device__ __forceinline__ float row_scale(uint32_t peak)
+{
+    return peak < 0x7F800000u ? fmaxf(__uint_as_float(peak) * (1.0f / 127.0f), 0x1p-126f) : __builtin_nanf("");
+}
+__device__ __forceinline__ uint2 quantize8_int8(const float (&x)[8], float scale)
+{
+    if (!(scale < __builtin_inff())) return make_uint2(0u, 0u);
+    const Divisor d(scale);
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j / 4] |= ((uint32_t)(int)__builtin_rintf(d(x[j])) & 0xFFu) << (8 * (j % 4));
+    return make_uint2(w[0], w[1]);
+}
+
+// LANES threads to a row (64 or 256), eight values at a time; the first PIECES of a thread's are kept in registers, the others read again.
+template <int DT, int LANES, int PIECES>
+__global__ __launch_bounds__(256) void int8_rows_kernel(Int8Rows p)
+{
+    __shared__ uint32_t peaks[4];
+    const uint32_t r = blockIdx.x * (256u / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const bool live = r < p.R;
+    const int64_t at = (int64_t)min(r, p.R - 1u) * p.x_stride;
+    float x[PIECES][8];
+    uint32_t peak = 0;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) load8<DT>(p.x, at, (i * LANES + lane) * 8u, p.K, x[i]);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) peak = max(peak, largest_bits(x[i]));
+    for (uint32_t k = (PIECES * LANES + lane) * 8u; k < p.K; k += LANES * 8u) {
+        float more[8];
+        load8<DT>(p.x, at, k, p.K, more);
+        peak = max(peak, largest_bits(more));
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) peak = max(peak, (uint32_t)__shfl_xor((int)peak, d));
+    if (LANES > 64) {
+        if (threadIdx.x % 64u == 0) peaks[threadIdx.x / 64u] = peak;
+        __syncthreads();
+        peak = max(max(peaks[0], peaks[1]), max(peaks[2], peaks[3]));
+    }
+    if (!live) return;
+    const float scale = row_scale(peak);
+    if (lane == 0) p.scale[r] = scale;
+    int8_t *q = p.q + (int64_t)r * p.q_stride;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const uint32_t k = (i * LANES + lane) * 8u;
+        if (k < (uint32_t)p.q_stride) *(uint2 *)(q + k) = quantize8_int8(x[i], scale);
+    }
+    for (uint32_t k = (PIECES * LANES + lane) * 8u; k < (uint32_t)p.q_stride; k += LANES * 8u) {
+        float more[8];
+        load8<DT>(p.x, at, k, p.K, more);
+        *(uint2 *)(q + k) = quantize8_int8(more, scale);
+    }
+}
+
+// --------------------------------------------------------------- few rows --
+// Bound by reading w once.  A workgroup makes 16 NT rows of w x up to 16 rows of x; its waves take the blocks of 128 columns in turn, and
+// their sums go through LDS once, at the end.  A wave asks for its next block before it multiplies the one it has.
+//
+// XT < 0: x is in 8 bits.  Else it is of that type, and every workgroup rounds all of it (a few rows) into LDS while its first rows of w
+// are on their way: one launch in the place of two.
+template <int DT, int XT, int NT>
+__global__ __launch_bounds__(512) void int8_few_kernel(Int8Params p)
+{
+    __shared__ v4i sums[8][NT][64];
+    __shared__ uint32_t peaks[8][4];
+    extern __shared__ char lds[];
+    const uint32_t lane = threadIdx.x % 64u, wave = wave_id(), waves = blockDim.x / 64u, i = lane % 16u, part = lane / 16u;
+    const uint32_t n0 = blockIdx.x * (16u * NT), m0 = blockIdx.y * 16u, blocks = (p.K + 127u) / 128u;
+    const uint32_t m = min(m0 + i, p.M - 1u);
+    const uint8_t *w[NT], *x = XT < 0 ? (const uint8_t *)p.x + (int64_t)m * p.x_stride : (const uint8_t *)lds + m * (blocks * 128u);
+#pragma unroll
+    for (int u = 0; u < NT; ++u) w[u] = (const uint8_t *)p.w + (int64_t)min(n0 + u * 16u + i, p.N - 1u) * p.w_stride;
+    struct Block { v4i w[NT][2], x[2]; };
+    // (w is read once and need not stay in the caches; x is read by every workgroup)
+    auto load = [&](uint32_t kb, Block &b) {
+        const uint32_t k = kb * 128u + part * 16u;
+        const bool whole = kb * 128u + 128u <= p.K;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u) b.w[u][h] = whole ? __builtin_nontemporal_load((const v4i *)(w[u] + k + 64 * h)) : load16(w[u], k + 64u * h, p.K);
+            if constexpr (XT < 0) b.x[h] = whole ? *(const v4i *)(x + k + 64 * h) : load16(x, k + 64u * h, p.K);
+        }
+    };
+    // (every workgroup begins at another block: rows are usually a power of two of bytes apart, and workgroups in step would ask the same
+    // memory channels at a time)
+    const uint32_t turn = blockIdx.x % blocks;
+    auto turned = [&](uint32_t kb) { kb += turn; return kb < blocks ? kb : kb - blocks; };
+    Block now, next;
+    if (wave < blocks) load(turned(wave), now);
+    if constexpr (XT >= 0) {
+        float held[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t r = 0; r < 4; ++r) {
+            if (r >= p.M) break;
+            uint32_t peak = 0;
+            for (uint32_t k = threadIdx.x * 8u; k < p.K; k += blockDim.x * 8u) {
+                float v[8];
+                load8<XT < 0 ? 0 : XT>(p.x, (int64_t)r * p.x_stride, k, p.K, v);
+                peak = max(peak, largest_bits(v));
+            }
+#pragma unroll
+            for (int d = 32; d; d >>= 1) peak = max(peak, (uint32_t)__shfl_xor((int)peak, d));
+            if (lane == 0) peaks[wave][r] = peak;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t r = 0; r < 4; ++r) {
+            if (r >= p.M) break;
+            uint32_t peak = 0;
+            for (uint32_t o = 0; o < waves; ++o) peak = max(peak, peaks[o][r]);
+            held[r] = row_scale(peak);
+            for (uint32_t k = threadIdx.x * 8u; k < blocks * 128u; k += blockDim.x * 8u) {
+                float v[8];
+                load8<XT < 0 ? 0 : XT>(p.x, (int64_t)r * p.x_stride, k, p.K, v);
+                *(uint2 *)(lds + r * (blocks * 128u) + k) = quantize8_int8(v, held[r]);
+            }
+            if (threadIdx.x == 0) ((float *)(lds + p.M * (blocks * 128u)))[r] = held[r];
+        }
+        __syncthreads();
+    }
+    v4i acc[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) acc[u] = v4i{0, 0, 0, 0};
+    auto take = [&](Block &b, uint32_t kb) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (XT >= 0) b.x[h] = *(const v4i *)(x + kb * 128u + part * 16u + 64 * h);
+#pragma unroll
+            for (int u = 0; u < NT; ++u) acc[u] = multiply<kInt8>(b.w[u][h], b.x[h], acc[u]);
+        }
+    };
+    if (wave < blocks) {
+        uint32_t kb = turned(wave);
+        for (uint32_t j = wave + waves; j < blocks; j += waves) {
+            const uint32_t following = turned(j);
+            load(following, next);
+            take(now, kb);
+            now = next;
+            kb = following;
+        }
+        take(now, kb);
+    }
+#pragma unroll
+    for (int u = 0; u < NT; ++u) sums[wave][u][lane] = acc[u];
+    __syncthreads();
+    for (uint32_t u = wave; u < (uint32_t)NT; u += waves) {
+        v4i s = sums[0][u][lane];
+        for (uint32_t o = 1; o < waves; ++o) s += sums[o][u][lane];
+        const uint32_t row = m0 + i, n = n0 + u * 16u + part * 4u;
+        if (row >= p.M) continue;
+        const float f = XT < 0 ? p.x_scale[row] : ((const float *)(lds + p.M * (blocks * 128u)))[row];
+        v4f y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = (float)s[j] * (f * p.w_scale[min(n + j, p.N - 1u)]);
+        store_row<DT>(p.y, (int64_t)row * p.y_stride, n, p.N, y);
+    }
+}
+
+// -------------------------------------------------------------- many rows --
+template <int DT, class T, bool SPLIT>
+__global__ __launch_bounds__(T::kThreads, 2) void int8_tile_kernel(Int8Params p)
+{
+    extern __shared__ char lds[];
+    T tile;
+    const uint32_t part = tile.choose(p.a, blockIdx.x);
+    typename T::Acc acc;
+    tile.make(p.a, part, lds, acc);
+    if (SPLIT && p.a.split > 1u) {
+        // every workgroup leaves its sums; the last of the tile's adds them up
+        constexpr uint32_t kPart = T::kThreads * T::NU * T::MT * 2;
+        const uint32_t tiles = gridDim.x / p.a.split, id = blockIdx.x % tiles;
+        uint64_t *parts = (uint64_t *)p.parts + (size_t)id * p.a.split * kPart + threadIdx.x;
+#pragma unroll
+        for (int u = 0; u < T::NU; ++u)
+#pragma unroll
+            for (int t = 0; t < T::MT; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    a_store(&parts[part * kPart + ((u * T::MT + t) * 2 + h) * T::kThreads], (uint64_t)(uint32_t)acc[u][t][2 * h + 1] << 32 | (uint32_t)acc[u][t][2 * h]);
+        uint32_t *last = (uint32_t *)lds;
+        wait_vmem();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            *last = __hip_atomic_fetch_add(&p.arrived[id], 1u, __ATOMIC_RELAXED, RS_AGENT) == p.a.split - 1u;
+            if (*last) a_store(&p.arrived[id], 0u);
+        }
+        __syncthreads();
+        if (!*last) return;
+#pragma unroll
+        for (int u = 0; u < T::NU; ++u)
+#pragma unroll
+            for (int t = 0; t < T::MT; ++t) acc[u][t] = v4i{0, 0, 0, 0};
+#pragma unroll 2
+        for (uint32_t s = 0; s < p.a.split; ++s) {
+            uint64_t v[2 * T::NU * T::MT];
+#pragma unroll
+            for (int o = 0; o < 2 * T::NU * T::MT; ++o) v[o] = a_load(&parts[s * kPart + o * T::kThreads]);
+#pragma unroll
+            for (int o = 0; o < 2 * T::NU * T::MT; ++o) {
+                acc[o / 2 / T::MT][o / 2 % T::MT][o % 2 * 2] += (int)(uint32_t)v[o];
+                acc[o / 2 / T::MT][o / 2 % T::MT][o % 2 * 2 + 1] += (int)(uint32_t)(v[o] >> 32);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < T::MT; ++t) {
+        const uint32_t m = tile.m(t);
+        if (m >= p.M) continue;
+        const float f = p.x_scale[m];
+#pragma unroll
+        for (int u = 0; u < T::NU; ++u) {
+            const uint32_t n = tile.n(u);
+            v4f y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = (float)acc[u][t][j] * (f * p.w_scale[min(n + j, p.N - 1u)]);
+            store_row<DT>(p.y, (int64_t)m * p.y_stride, n, p.N, y);
+        }
+    }
+}
+
+}  // namespace rs

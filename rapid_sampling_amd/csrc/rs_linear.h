@@ -21,6 +21,9 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
+constexpr uint32_t kPartTiles = 256;                 // tiles of partial sums that the workspace holds ...
+constexpr size_t   kPartBytes = 128 * 64 * 4;        // ... of 128 x 64
+
 struct QuantParams {
     const void *x;
     int64_t     x_stride;                // elements from a row to the next

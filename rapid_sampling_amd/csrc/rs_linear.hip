@@ -21,9 +21,6 @@ static void launch_quantize(QuantParams p, bool tiles, hipStream_t st)
     }
 }
 
-constexpr uint32_t kPartTiles = 256;                 // tiles of partial sums that the workspace holds ...
-constexpr size_t   kPartBytes = 128 * 64 * 4;        // ... of 128 x 64
-
 // SPLIT: where there are few tiles their blocks of columns are shared out, for up to one workgroup to a compute unit.  Leaving and
 // adding up the parts costs about 2 us, a block 0.9: four blocks to each at least (64 x 1024 x 4096: 30.7 us whole, 12.9 in eight;
 // 64 x 4096 x 512: 6.5 whole, 8.0 in two).

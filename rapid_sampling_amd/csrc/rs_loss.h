@@ -1,0 +1,283 @@
+// Cross entropy of tokens under softmax(x w^T / T) without the logits, and its gradients.
+//
+//   z[m, v] = c x_m . w_v, c = log2(e) / T       lse_m = ln 2 (M_m + log2 S_m), S_m = sum_v 2^(z[m, v] - M_m)       loss_m = lse_m - ln 2 z[m, t_m]
+//   G[m, v] = ((g_m + h_m) 2^(z[m, v] - M_m) / S_m - g_m [v = t_m]) / T           dx = G w           dw = G^T x
+//
+// with g the gradient of the losses and h that of the lse.  Forward: a product whose tiles leave a maximum and a sum of each row in
+// the place of their logits, and a pass that joins these.  Backward, for a piece of the vocabulary at a time: the piece's product once
+// more, with G in the place of the logits, and the two products with it.  Three products are what the gradients cannot do without,
+// the fourth is the price of the logits that are not kept.
+#pragma once
+
+#include "rs_product.h"
+
+namespace rs {
+
+struct LossRow {                     // of one row, for G
+    float   max, a, b;               // M, (g + h) / (S T), g / T
+    int32_t token;
+};
+
+struct LossParams {
+    Product     a;                   // P: weights, Q: x
+    const void *tokens;
+    int64_t     token_stride;
+    int32_t     tokens_64;
+    uint32_t    V, M;                // of the whole call
+    uint32_t    v0;                  // the piece's first token
+    float       c, inv_t;
+    float2     *parts;               // [stretches of the vocabulary][M]: maximum, sum
+    uint32_t    n_parts;
+    float      *target;              // z of the row's token
+    float      *loss, *lse;
+    float2     *stats;               // maximum, sum; kept for the gradient
+    const float *g, *h;
+    int32_t     g_stride, h_stride;
+    LossRow    *rows;
+    float      *scale;               // [0] what G is multiplied with, [1] what the products are
+    void       *grad;                // G: rows of grad_stride bytes
+    uint32_t    grad_stride;
+};
+
+__device__ __forceinline__ int64_t loss_token(const LossParams &p, uint32_t m)
+{
+    return p.tokens_64 ? ((const int64_t *)p.tokens)[(int64_t)m * p.token_stride] : ((const int32_t *)p.tokens)[(int64_t)m * p.token_stride];
+}
+
+template <class T>
+__global__ __launch_bounds__(T::kThreads, 2) void loss_tile_kernel(LossParams p)
+{
+    extern __shared__ char lds[];
+    T tile;
+    tile.choose(p.a, blockIdx.x);
+    typename T::Acc acc;
+    tile.make(p.a, 0, lds, acc);
+    const uint32_t V = p.V, stretch = tile.n0 / (16u * T::NU) + wave_id() % T::WN;
+    const bool whole = (stretch + 1u) * (16u * T::NU) <= V;
+#pragma unroll
+    for (int t = 0; t < T::MT; ++t) {
+        const uint32_t m = tile.m(t);
+        const int64_t token = m < p.M ? loss_token(p, m) : -1;
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < T::NU; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float z = whole || tile.n(u) + j < V ? acc[u][t][j] * p.c : -__builtin_inff();
+                acc[u][t][j] = z;
+                if ((int64_t)(tile.n(u) + j) == token) p.target[m] = z;
+                top = fmaxf(top, z);
+            }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float from = top == -__builtin_inff() ? 0.0f : top;
+        float s = 0.0f;
+#pragma unroll
+        for (int u = 0; u < T::NU; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s += __builtin_amdgcn_exp2f(acc[u][t][j] - from);
+        s += __shfl_xor(s, 16);
+        s += __shfl_xor(s, 32);
+        if (m < p.M && threadIdx.x % 64u < 16u && stretch < p.n_parts) p.parts[(size_t)stretch * p.M + m] = make_float2(top, s);
+    }
+}
+
+__device__ __forceinline__ float2 join_sums(float2 a, float2 b)
+{
+    const float top = fmaxf(a.x, b.x), from = top == -__builtin_inff() ? 0.0f : top;
+    return make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - from) + b.y * __builtin_amdgcn_exp2f(b.x - from));
+}
+
+// 2^WIDTH rows to a workgroup, 256 / 2^WIDTH threads to a row.
+__global__ __launch_bounds__(256) void loss_join_kernel(LossParams p, uint32_t width)
+{
+    __shared__ float2 held[256];
+    const uint32_t m = (blockIdx.x << width) + (threadIdx.x & ((1u << width) - 1u)), k = threadIdx.x >> width, many = 256u >> width;
+    float2 sum = make_float2(-__builtin_inff(), 0.0f);
+    if (m < p.M)
+        for (uint32_t s = k; s < p.n_parts; s += many) sum = join_sums(sum, p.parts[(size_t)s * p.M + m]);
+    held[threadIdx.x] = sum;
+    for (uint32_t d = 128u; d >= 1u << width; d >>= 1) {
+        __syncthreads();
+        if (threadIdx.x < d) held[threadIdx.x] = join_sums(held[threadIdx.x], held[threadIdx.x + d]);
+    }
+    if (k || m >= p.M) return;
+    sum = held[threadIdx.x];
+    const bool none = sum.x == -__builtin_inff() && sum.y == 0.0f;             // no logit above -inf
+    const float ln2 = 0.693147180559945309f;
+    const float log2_s = none ? 0.0f : __builtin_log2f(sum.y);
+    const int64_t token = loss_token(p, m);
+    p.lse[m] = none ? -__builtin_inff() : ln2 * (sum.x + log2_s);
+    float loss = 0.0f;
+    if (token >= (int64_t)p.V) loss = __builtin_nanf("");
+    else if (token >= 0) loss = none ? __builtin_inff() : ln2 * ((sum.x - p.target[m]) + log2_s);
+    p.loss[m] = loss;
+    if (p.stats) p.stats[m] = none ? make_float2(0.0f, __builtin_inff()) : sum;
+}
+
+// ---------------------------------------------------------------- gradients --
+// G in 16 bits is rounded, to bfloat16 with 8 bits of its own size; in float16 it is made so large first (by a power of two, the same
+// for the whole call) that the largest possible is below 2^15, and a probability's share of it is lost from 2^-39 on.
+__global__ __launch_bounds__(1024) void loss_scale_kernel(LossParams p, int32_t half)
+{
+    __shared__ float tops[16];
+    float top = 0.0f;
+    if (half)
+        for (uint32_t m = threadIdx.x; m < p.M; m += 1024u) {
+            const float g = p.g ? fabsf(p.g[(int64_t)m * p.g_stride]) : 0.0f, h = p.h ? fabsf(p.h[(int64_t)m * p.h_stride]) : 0.0f;
+            const float v = (g + h) * p.inv_t;
+            if (v < __builtin_inff()) top = fmaxf(top, v);
+        }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (threadIdx.x % 64u == 0) tops[threadIdx.x / 64u] = top;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, tops[i]);
+    const int e = top > 0.0f ? min(max(14 - ((int)(__float_as_uint(top) >> 23) - 127), -100), 100) : 0;
+    p.scale[0] = __builtin_ldexpf(1.0f, e);
+    p.scale[1] = __builtin_ldexpf(1.0f, -e);
+}
+
+__global__ __launch_bounds__(256) void loss_rows_kernel(LossParams p)
+{
+    const uint32_t m = blockIdx.x * 256u + threadIdx.x;
+    if (m >= p.M) return;
+    const float2 st = p.stats[m];
+    const int64_t token = loss_token(p, m);
+    const float f = p.inv_t * p.scale[0], h = p.h ? p.h[(int64_t)m * p.h_stride] : 0.0f;
+    float g = p.g && token >= 0 ? p.g[(int64_t)m * p.g_stride] : 0.0f;
+    if (p.g && token >= (int64_t)p.V) g = __builtin_nanf("");                  // its loss is NaN
+    LossRow r;
+    r.max = st.x;
+    r.a = (g + h) * f / st.y;
+    r.b = st.y == __builtin_inff() ? 0.0f : g * f;
+    r.token = token >= 0 && token < (int64_t)p.V ? (int32_t)token : -1;
+    p.rows[m] = r;
+}
+
+template <class T>
+__global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
+{
+    extern __shared__ char lds[];
+    T tile;
+    tile.choose(p.a, blockIdx.x);
+    typename T::Acc acc;
+    tile.make(p.a, 0, lds, acc);
+#pragma unroll
+    for (int t = 0; t < T::MT; ++t) {
+        const uint32_t m = tile.m(t);
+        if (m >= p.M) continue;
+        const LossRow r = p.rows[m];
+        char *row = (char *)p.grad + (int64_t)m * p.grad_stride;
+#pragma unroll
+        for (int u = 0; u < T::NU; ++u) {
+            const uint32_t n = tile.n(u);
+            v4f v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = r.a * __builtin_amdgcn_exp2f(acc[u][t][j] * p.c - r.max);
+                if ((int32_t)(n + p.v0 + j) == r.token) v[j] -= r.b;
+            }
+            store_row<T::DT>(row, 0, n, p.a.p.rows, v);
+        }
+    }
+}
+
+struct GradParams {
+    Product      a;                  // P: the output's columns, Q: its rows
+    void        *y;                  // (rows, columns)
+    int64_t      y_stride;           // elements
+    const float *scale;              // [1]: factor of the result
+    int32_t      add;                // to what is there
+    int64_t      part_stride;        // elements between the sums of the workgroups that share the reduction
+};
+
+// dx's sums of one piece of the vocabulary, in float32; every share of the reduction has sums of its own
+template <class T>
+__global__ __launch_bounds__(T::kThreads, 2) void loss_dx_kernel(GradParams p)
+{
+    extern __shared__ char lds[];
+    T tile;
+    const uint32_t part = tile.choose(p.a, blockIdx.x);
+    typename T::Acc acc;
+    tile.make(p.a, part, lds, acc);
+    float *y = (float *)p.y + (int64_t)part * p.part_stride;
+#pragma unroll
+    for (int t = 0; t < T::MT; ++t) {
+        const uint32_t m = tile.m(t);
+        if (m >= p.a.q.rows) continue;
+#pragma unroll
+        for (int u = 0; u < T::NU; ++u) {
+            const uint32_t n = tile.n(u);
+            v4f v = acc[u][t];
+            float *at = y + (int64_t)m * p.y_stride;
+            if (p.add) {
+                if (n + 4u <= p.a.p.rows) { v4f old; __builtin_memcpy(&old, at + n, 16); v += old; }
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) if (n + j < p.a.p.rows) v[j] += at[n + j];
+            }
+            store_row<RS_DTYPE_F32>(at, 0, n, p.a.p.rows, v);
+        }
+    }
+}
+
+// dw of one piece, whole
+template <class T>
+__global__ __launch_bounds__(T::kThreads, 2) void loss_dw_kernel(GradParams p)
+{
+    extern __shared__ char lds[];
+    T tile;
+    tile.choose(p.a, blockIdx.x);
+    typename T::Acc acc;
+    tile.make(p.a, 0, lds, acc);
+    const float f = p.scale[1];
+#pragma unroll
+    for (int t = 0; t < T::MT; ++t) {
+        const uint32_t m = tile.m(t);
+        if (m >= p.a.q.rows) continue;
+#pragma unroll
+        for (int u = 0; u < T::NU; ++u) store_row<T::DT>(p.y, (int64_t)m * p.y_stride, tile.n(u), p.a.p.rows, acc[u][t] * f);
+    }
+}
+
+// dx from the sums of the shares, rounded once
+template <int DT>
+__global__ __launch_bounds__(256) void loss_round_kernel(const float *sums, int64_t part_stride, uint32_t parts, void *y, int64_t count, const float *scale)
+{
+    const float f = scale[1];
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (int64_t)gridDim.x * 1024) {
+        v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (i + 4 <= count) {
+            for (uint32_t k = 0; k < parts; ++k) s += *(const v4f *)(sums + k * part_stride + i);
+            put_four<DT>(y, i, s * f);
+        } else
+            for (int64_t j = i; j < count; ++j) {
+                float one = 0.0f;
+                for (uint32_t k = 0; k < parts; ++k) one += sums[k * part_stride + j];
+                put<DT>(y, j, one * f);
+            }
+    }
+}
+
+// Rows laid out in multiples of 16 bytes, for those that are not: 16 bytes to a thread.
+__global__ __launch_bounds__(256) void lay_out_rows_kernel(const char *x, int64_t x_stride, char *y, int64_t y_stride, int64_t rows, uint32_t bytes)
+{
+    const uint32_t pieces = (uint32_t)(y_stride / 16);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * pieces; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / pieces;
+        const uint32_t at = (uint32_t)(i - r * pieces) * 16u;
+        v4i v = {0, 0, 0, 0};
+        if (at + 16u <= bytes) __builtin_memcpy(&v, x + r * x_stride + at, 16);
+        else {
+            uint16_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) if (at + 2u * j < bytes) w[j] = *(const uint16_t *)(x + r * x_stride + at + 2u * j);
+            __builtin_memcpy(&v, w, 16);
+        }
+        *(v4i *)(y + r * y_stride + at) = v;
+    }
+}
+
+}  // namespace rs

@@ -1,0 +1,229 @@
+// Instantiations, launchers and C entry points of the cross entropy over a vocabulary without its logits.
+#include "rs_loss.h"
+
+#include <algorithm>
+
+namespace rs {
+
+static uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+static uint32_t size_of(int32_t dtype) { return dtype == RS_DTYPE_F32 ? 4 : 2; }
+
+// Where a call's scratch lies.  The same sizes give the same places.
+struct LossSpace {
+    uint64_t parts = 0, target = 0;                     // forward
+    uint64_t scale = 0, rows = 0, grad = 0, dx = 0;     // backward
+    uint64_t bytes = 0;
+    uint32_t piece = 0, split = 1;                      // tokens of a piece; shares of dx's reduction
+    uint64_t grad_stride = 0;
+    uint64_t take(uint64_t n) { const uint64_t at = bytes; bytes += up(n, 256); return at; }
+};
+
+// Large tiles where there are more than enough to go round.
+static bool large(uint64_t rows, uint64_t columns) { return rows > 128 && up(rows, 256) / 256 * (up(columns, 256) / 256) >= 192; }
+
+// A piece of the vocabulary: G of the piece stays within the last cache (256 MB) with the piece's weights, in steps of 256 tokens and
+// at least 8192, so that the sums of dx that each piece reads and writes again (8 bytes) are little next to its products.
+static LossSpace loss_space(int32_t M, int32_t V, int32_t K, int32_t dtype, bool backward)
+{
+    LossSpace s;
+    const uint64_t size = size_of(dtype);
+    if (!backward) {
+        s.parts = s.take((up(V, 64) / 64) * (uint64_t)M * sizeof(float2));
+        s.target = s.take((uint64_t)M * 4);
+        return s;
+    }
+    s.scale = s.take(8);
+    s.rows = s.take((uint64_t)M * sizeof(LossRow));
+    s.piece = (uint32_t)std::min<uint64_t>(up(V, 256), std::max<uint64_t>(8192, ((1ull << 27) / (M * size)) / 256 * 256));
+    s.grad_stride = s.piece * size + 256;              // (not a power of two: rows would share their memory channels)
+    s.grad = s.take((uint64_t)M * s.grad_stride);
+    const bool big = large(M, K);
+    const uint64_t tiles = big ? up(M, 256) / 256 * (up(K, 256) / 256) : up(M, 64) / 64 * (up(K, 128) / 128);
+    const uint64_t stages = s.piece * size / kRowBytes;
+    s.split = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(big ? 256 : 512) / tiles, stages / 8, 32}));
+    s.dx = s.take((uint64_t)s.split * M * K * 4);
+    return s;
+}
+
+template <int DT, bool TP, bool TQ> using LargeTile = Tile<DT, TP, TQ, 2, 4, 8, 4, 2>;       // 256 x 256, eight waves
+template <int DT, bool TP, bool TQ> using SmallTile = Tile<DT, TP, TQ, 2, 2, 4, 2, 3>;       // 128 x 64, four waves
+
+template <class T, class K, class A> static void launch_tiles(K kernel, const A &p, const Product &a, hipStream_t st)
+{
+    const uint64_t tiles = (uint64_t)((a.q.rows + T::kTileM - 1) / T::kTileM) * ((a.p.rows + T::kTileN - 1) / T::kTileN);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles * a.split)), dim3(T::kThreads), T::kLds, st, p);
+}
+
+template <int DT> static void launch_forward(const LossParams &p, hipStream_t st)
+{
+    if (large(p.M, p.V)) launch_tiles<LargeTile<DT, false, false>>(loss_tile_kernel<LargeTile<DT, false, false>>, p, p.a, st);
+    else launch_tiles<SmallTile<DT, false, false>>(loss_tile_kernel<SmallTile<DT, false, false>>, p, p.a, st);
+}
+
+template <int DT> static void launch_grad(const LossParams &p, hipStream_t st)
+{
+    if (large(p.M, p.a.p.rows)) launch_tiles<LargeTile<DT, false, false>>(loss_grad_kernel<LargeTile<DT, false, false>>, p, p.a, st);
+    else launch_tiles<SmallTile<DT, false, false>>(loss_grad_kernel<SmallTile<DT, false, false>>, p, p.a, st);
+}
+
+template <int DT> static void launch_dx(const GradParams &p, hipStream_t st)
+{
+    if (large(p.a.q.rows, p.a.p.rows)) launch_tiles<LargeTile<DT, true, false>>(loss_dx_kernel<LargeTile<DT, true, false>>, p, p.a, st);
+    else launch_tiles<SmallTile<DT, true, false>>(loss_dx_kernel<SmallTile<DT, true, false>>, p, p.a, st);
+}
+
+template <int DT> static void launch_dw(const GradParams &p, hipStream_t st)
+{
+    if (large(p.a.q.rows, p.a.p.rows)) launch_tiles<LargeTile<DT, true, true>>(loss_dw_kernel<LargeTile<DT, true, true>>, p, p.a, st);
+    else launch_tiles<SmallTile<DT, true, true>>(loss_dw_kernel<SmallTile<DT, true, true>>, p, p.a, st);
+}
+
+static bool known(int32_t dtype) { return dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16 || dtype == RS_DTYPE_F16; }
+
+static int check(const void *x, int64_t x_stride, const void *w, int64_t w_stride, int32_t dtype, const void *tokens, int32_t tokens_64, int32_t M, int32_t V,
+                 int32_t K, double temperature, const void *workspace)
+{
+    if (!x || !w || !tokens || !workspace) return RS_ERR_NULL;
+    if (!known(dtype) || (tokens_64 != 0 && tokens_64 != 1)) return RS_ERR_ARG;
+    if (M <= 0 || V <= 0 || K <= 0 || M > RS_LINEAR_MAX || V > 1048576 || K > RS_LOSS_COLUMNS_MAX) return RS_ERR_SHAPE;
+    if (((int64_t)M + 63) / 64 * (((int64_t)V + 127) / 128) > (int64_t)(kGridThreads / 256u)) return RS_ERR_SHAPE;       // workgroups of a launch
+    if (!(temperature >= 0.001 && temperature <= 1000)) return RS_ERR_TEMPERATURE;
+    const int64_t size = size_of(dtype), most = kTileStride / size;
+    if ((M > 1 && (x_stride < K || x_stride > most)) || (V > 1 && (w_stride < K || w_stride > most))) return RS_ERR_SHAPE;
+    if (((uintptr_t)x & 15) || ((uintptr_t)w & 15) || (M > 1 && (x_stride * size & 15)) || (V > 1 && (w_stride * size & 15)) ||
+        ((uintptr_t)tokens & (tokens_64 ? 7 : 3)))
+        return RS_ERR_ALIGN;
+    return RS_OK;
+}
+
+// (the distance to the next row of a single one is not looked at by the checks)
+static Operand rows_of(const void *x, int64_t stride, int32_t rows, int32_t K, uint32_t size)
+{
+    return Operand{(const char *)x, (uint32_t)(rows > 1 ? stride * size : up((uint64_t)K * size, 16)), (uint32_t)rows};
+}
+
+template <int DT>
+static void backward(LossParams p, const LossSpace &s, Operand x, Operand w, uint32_t K, void *grad_x, void *grad_w, char *ws, hipStream_t st)
+{
+    constexpr uint32_t size = kSize<DT>;
+    hipLaunchKernelGGL(loss_scale_kernel, dim3(1), dim3(1024), 0, st, p, (int32_t)(DT == RS_DTYPE_F16));
+    hipLaunchKernelGGL(loss_rows_kernel, dim3((p.M + 255) / 256), dim3(256), 0, st, p);
+    for (uint32_t v0 = 0; v0 < p.V; v0 += s.piece) {
+        const uint32_t n = std::min(s.piece, p.V - v0);
+        const char *piece = w.at + (int64_t)v0 * w.stride;
+        p.v0 = v0;
+        p.a = Product{Operand{piece, w.stride, n}, x, K, 1};
+        launch_grad<DT>(p, st);
+        GradParams g;
+        g.scale = p.scale;
+        if (grad_x) {
+            g.a = Product{Operand{piece, w.stride, K}, Operand{(const char *)p.grad, p.grad_stride, p.M}, n, s.split};
+            g.y = ws + s.dx;
+            g.y_stride = K;
+            g.part_stride = (int64_t)p.M * K;
+            g.add = v0 > 0;
+            launch_dx<DT>(g, st);
+        }
+        if (grad_w) {
+            g.a = Product{Operand{x.at, x.stride, K}, Operand{(const char *)p.grad, p.grad_stride, n}, p.M, 1};
+            g.y = (char *)grad_w + (int64_t)v0 * K * size;
+            g.y_stride = K;
+            g.part_stride = 0;
+            g.add = 0;
+            launch_dw<DT>(g, st);
+        }
+    }
+    if (grad_x) {
+        const int64_t count = (int64_t)p.M * K;
+        hipLaunchKernelGGL(loss_round_kernel<DT>, dim3((uint32_t)std::min<int64_t>((count + 1023) / 1024, 1 << 16)), dim3(256), 0, st, (const float *)(ws + s.dx),
+                           count, s.split, grad_x, count, p.scale);
+    }
+}
+
+}  // namespace rs
+
+using namespace rs;
+
+extern "C" {
+
+int rs_lay_out_rows(const void *x, int64_t x_row_stride, int32_t size, int64_t R, int32_t K, void *y, int64_t y_row_stride, void *stream)
+{
+    if (!x || !y) return RS_ERR_NULL;
+    if (size != 2 && size != 4) return RS_ERR_ARG;
+    if (R <= 0 || K <= 0 || K > RS_LINEAR_MAX || x_row_stride < 0 || y_row_stride < K || R > (1ll << 40) / y_row_stride) return RS_ERR_SHAPE;
+    if (((uintptr_t)x & (size - 1)) || ((uintptr_t)y & 15) || (y_row_stride * size & 15)) return RS_ERR_ALIGN;
+    const uint64_t groups = ((uint64_t)R * (y_row_stride * size / 16) + 255) / 256;
+    hipLaunchKernelGGL(lay_out_rows_kernel, dim3((uint32_t)std::min<uint64_t>(groups, 1u << 16)), dim3(256), 0, (hipStream_t)stream, (const char *)x,
+                       x_row_stride * size, (char *)y, y_row_stride * size, R, (uint32_t)(K * size));
+    return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
+}
+
+size_t rs_linear_cross_entropy_workspace_bytes(int32_t M, int32_t V, int32_t K, int32_t dtype, int32_t backward)
+{
+    if (M <= 0 || V <= 0 || K <= 0 || !known(dtype)) return 0;
+    return loss_space(M, V, K, dtype, backward != 0).bytes;
+}
+
+int rs_linear_cross_entropy(const void *x, int64_t x_stride, const void *w, int64_t w_stride, int32_t dtype, const void *tokens, int32_t tokens_64,
+                            int64_t token_stride, int32_t M, int32_t V, int32_t K, double temperature, float *loss, float *lse, float *stats, void *workspace,
+                            size_t workspace_bytes, void *stream)
+{
+    const int rc = check(x, x_stride, w, w_stride, dtype, tokens, tokens_64, M, V, K, temperature, workspace);
+    if (rc != RS_OK) return rc;
+    if (!loss || !lse) return RS_ERR_NULL;
+    if (((uintptr_t)loss & 3) || ((uintptr_t)lse & 3) || ((uintptr_t)stats & 7)) return RS_ERR_ALIGN;
+    const uint32_t size = size_of(dtype);
+    const LossSpace s = loss_space(M, V, K, dtype, false);
+    if (workspace_bytes < s.bytes || ((uintptr_t)workspace & 255)) return RS_ERR_WORKSPACE;
+    char *ws = (char *)workspace;
+    const hipStream_t st = (hipStream_t)stream;
+    LossParams p = {};
+    p.a = Product{rows_of(w, w_stride, V, K, size), rows_of(x, x_stride, M, K, size), (uint32_t)K, 1};
+    p.tokens = tokens; p.token_stride = token_stride; p.tokens_64 = tokens_64;
+    p.V = (uint32_t)V; p.M = (uint32_t)M;
+    p.c = (float)(1.4426950408889634 / temperature); p.inv_t = (float)(1.0 / temperature);
+    p.parts = (float2 *)(ws + s.parts); p.target = (float *)(ws + s.target);
+    p.loss = loss; p.lse = lse; p.stats = (float2 *)stats;
+    const uint32_t stretch = large(M, V) ? 128 : 64;
+    p.n_parts = (p.V + stretch - 1) / stretch;
+    if (dtype == RS_DTYPE_F32) launch_forward<RS_DTYPE_F32>(p, st);
+    else if (dtype == RS_DTYPE_BF16) launch_forward<RS_DTYPE_BF16>(p, st);
+    else launch_forward<RS_DTYPE_F16>(p, st);
+    uint32_t width = 0;                                  // rows of a workgroup: as many as leave every compute unit one
+    while (width < 6 && ((uint32_t)M >> (width + 1)) >= 256) ++width;
+    hipLaunchKernelGGL(loss_join_kernel, dim3(((uint32_t)M + (1u << width) - 1) >> width), dim3(256), 0, st, p, width);
+    return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
+}
+
+int rs_linear_cross_entropy_backward(const void *x, int64_t x_stride, const void *w, int64_t w_stride, int32_t dtype, const void *tokens, int32_t tokens_64,
+                                     int64_t token_stride, int32_t M, int32_t V, int32_t K, double temperature, const float *stats,
+                                     const float *grad_loss, int32_t grad_loss_stride, const float *grad_lse, int32_t grad_lse_stride,
+                                     void *grad_x, void *grad_w, void *workspace, size_t workspace_bytes, void *stream)
+{
+    const int rc = check(x, x_stride, w, w_stride, dtype, tokens, tokens_64, M, V, K, temperature, workspace);
+    if (rc != RS_OK) return rc;
+    if (!stats || (!grad_x && !grad_w)) return RS_ERR_NULL;
+    if ((grad_loss_stride | grad_lse_stride) & ~1) return RS_ERR_ARG;
+    const uint32_t size = size_of(dtype);
+    if (((uintptr_t)stats & 7) || ((uintptr_t)grad_loss & 3) || ((uintptr_t)grad_lse & 3) || ((uintptr_t)grad_x & (size - 1)) || ((uintptr_t)grad_w & (size - 1)))
+        return RS_ERR_ALIGN;
+    const LossSpace s = loss_space(M, V, K, dtype, true);
+    if (workspace_bytes < s.bytes || ((uintptr_t)workspace & 255)) return RS_ERR_WORKSPACE;
+    char *ws = (char *)workspace;
+    const hipStream_t st = (hipStream_t)stream;
+    const Operand q = rows_of(x, x_stride, M, K, size), r = rows_of(w, w_stride, V, K, size);
+    LossParams p = {};
+    p.tokens = tokens; p.token_stride = token_stride; p.tokens_64 = tokens_64;
+    p.V = (uint32_t)V; p.M = (uint32_t)M;
+    p.c = (float)(1.4426950408889634 / temperature); p.inv_t = (float)(1.0 / temperature);
+    p.stats = (float2 *)stats;
+    p.g = grad_loss; p.g_stride = grad_loss_stride; p.h = grad_lse; p.h_stride = grad_lse_stride;
+    p.scale = (float *)(ws + s.scale); p.rows = (LossRow *)(ws + s.rows);
+    p.grad = ws + s.grad; p.grad_stride = (uint32_t)s.grad_stride;
+    if (dtype == RS_DTYPE_F32) backward<RS_DTYPE_F32>(p, s, q, r, (uint32_t)K, grad_x, grad_w, ws, st);
+    else if (dtype == RS_DTYPE_BF16) backward<RS_DTYPE_BF16>(p, s, q, r, (uint32_t)K, grad_x, grad_w, ws, st);
+    else backward<RS_DTYPE_F16>(p, s, q, r, (uint32_t)K, grad_x, grad_w, ws, st);
+    return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
+}
+
+}  // extern "C"

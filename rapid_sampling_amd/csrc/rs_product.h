@@ -1,0 +1,274 @@
+// Tiles of a matrix product on the matrix cores, for the operators that make one and do something with its sums:
+//
+//   sum[m, n] = sum over r of P[n, r] Q[m, r]
+//
+// of bfloat16, float16 or float32 values with float32 sums, or of 8-bit integers with whole sums.  Either operand lies in memory with
+// the values of one row n (or m) side by side, as activations and weights do in y = x w^T, or (transposed) with those of one r
+// side by side, as both do in the products that make gradients.
+#pragma once
+
+#include "rs_linear.h"
+
+namespace rs {
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+constexpr int kInt8 = 100;                       // next to RS_DTYPE_*
+template <int DT> constexpr uint32_t kSize = DT == kInt8 ? 1 : DT == RS_DTYPE_F32 ? 4 : 2;
+template <int DT> struct SumOf { typedef v4f type; };
+template <> struct SumOf<kInt8> { typedef v4i type; };
+template <int DT> using Sum = typename SumOf<DT>::type;
+
+constexpr uint32_t kRowBytes = 128;              // of the reduction that a stage holds
+
+// 16 x 16 sums of 16 bytes of each row.  Lane l gives 16 bytes of row l % 16 of either side, the same part of the reduction on both, and has
+// the sums of the first side's rows 4 (l / 16) + 0..3 with the second side's row l % 16.
+template <int DT> __device__ __forceinline__ Sum<DT> multiply(v4i p, v4i q, Sum<DT> s)
+{
+    if constexpr (DT == kInt8) return __builtin_amdgcn_mfma_i32_16x16x64_i8(p, q, s, 0, 0, 0);
+    else if constexpr (DT == RS_DTYPE_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, p), __builtin_bit_cast(v8bf, q), s, 0, 0, 0);
+    else if constexpr (DT == RS_DTYPE_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, p), __builtin_bit_cast(v8h, q), s, 0, 0, 0);
+    else {
+        const v4f a = __builtin_bit_cast(v4f, p), b = __builtin_bit_cast(v4f, q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], s, 0, 0, 0);
+        return s;
+    }
+}
+
+// One operand of a product: `rows` rows (n or m) of `red` values, `stride` bytes from a row (transposed: from one r) to the next.  16-byte
+// aligned, as is the stride; at most kTileStride.
+struct Operand {
+    const char *at;
+    uint32_t    stride, rows;
+};
+
+struct Product {
+    Operand  p, q;
+    uint32_t red;                    // values of the reduction
+    uint32_t split;                  // workgroups that share a tile's reduction
+};
+
+// COUNT rows of one operand in LDS, STAGE after stage of the reduction, and how they get there.
+//
+// Rows from memory go to LDS without passing through registers.  As they are: a stage is 128 bytes of every row, its eight 16-byte
+// pieces in an order that depends on the row (place = piece ^ turn), so that the rows read at once lie in different banks.
+// Transposed: a stage is 128 / size values of r, the COUNT values of each side by side; those of 16 bits are turned by the reads from
+// LDS (ds_read_b64_tr_b16: four r of a row to a lane), whose 32-byte pieces are stored in such an order too.
+//
+// FIRST (the product's first operand, untransposed): the rows are dealt to the matrix instructions so that a lane's sums belong to 4 F
+// consecutive rows, F fragments of 16 rows to a wave.
+template <int DT, bool TR, bool FIRST, int COUNT, int F, int WAVES>
+struct Side {
+    static constexpr uint32_t kBytes = COUNT * kRowBytes, kLoads = kBytes / (1024 * WAVES), kRed = kRowBytes / kSize<DT>;
+    static constexpr uint32_t kWide = COUNT * kSize<DT>;                     // bytes of one r, transposed
+    static_assert(kBytes % (1024 * WAVES) == 0, "whole loads");
+    static_assert(!TR || (kWide <= 1024 && 1024 % kWide == 0 && DT != kInt8), "a wave's load is whole values of r");
+    static constexpr int kBufferFlags = 0x00027000;                          // untyped, offsets in bytes
+
+    const char *base;
+    uint32_t    stride, rows, bytes;       // transposed: bytes of one r from the tile's first row on
+    uint32_t    off[kLoads];
+
+    // the order of pieces: depends on the row and is the same for all the fragments of a lane
+    static __device__ __forceinline__ uint32_t turn(uint32_t row)
+    {
+        if (!TR) return FIRST ? (row & 3u) | ((row / F) & 4u) : row & 7u;
+        return kWide == 128 ? ((row >> 1) & 1u) | ((row >> 2) & 2u) : (row & 3u) | ((row >> 1) & 4u);
+    }
+    // byte of the source's row (or r) that a byte of the stage holds
+    static __device__ __forceinline__ void source_of(uint32_t at, uint32_t &row, uint32_t &byte)
+    {
+        if (!TR) { row = at / kRowBytes; byte = ((at / 16u % 8u) ^ turn(row)) * 16u; return; }
+        row = at / kWide;
+        byte = at % kWide;
+        if (kSize<DT> == 2) byte = ((byte / 32u) ^ turn(row)) * 32u + byte % 32u;
+    }
+    __device__ __forceinline__ uint32_t place(uint32_t i) const { return (i * WAVES + wave_id()) * 1024u + threadIdx.x % 64u * 16u; }
+
+    __device__ __forceinline__ Side(const Operand &o, uint32_t first)
+    {
+        stride = o.stride;
+        rows = min(o.rows - first, (uint32_t)COUNT);
+        base = o.at + (TR ? (int64_t)first * kSize<DT> : (int64_t)first * o.stride);
+        bytes = (o.rows - first) * kSize<DT>;
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            uint32_t row, byte;
+            source_of(place(i), row, byte);
+            off[i] = TR ? row * stride + byte : tile_at(row, rows, stride, byte);
+            asm volatile("" : "+v"(off[i]));               // once, and not for every stage
+        }
+    }
+    // Asks for the stage that begins at r.
+    __device__ __forceinline__ void fill(uint32_t r, uint32_t red, char *lds) const
+    {
+        const uint32_t left = red - r;
+        if constexpr (TR) {
+            // what lies behind the last r reads as 0; what lies behind a row's end belongs to sums that nobody asks for
+            const uint32_t size = (min(left, kRed) - 1u) * stride + ((bytes + 3u) & ~3u);
+            const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc((void *)(base + (int64_t)r * stride), 0, (int)size, kBufferFlags);
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (LdsPtr)(lds + (i * WAVES + wave_id()) * 1024u), 16, off[i], 0, 0, 0);
+        } else {
+            const uint32_t size = tile_bytes(rows, stride, left * kSize<DT>);
+            const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc((void *)(base + (int64_t)r * kSize<DT>), 0, (int)size, kBufferFlags);
+            if (left >= kRed) {
+#pragma unroll
+                for (uint32_t i = 0; i < kLoads; ++i)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (LdsPtr)(lds + (i * WAVES + wave_id()) * 1024u), 16, off[i], 0, 0, 0);
+                return;
+            }
+            // the last stage of a reduction that is no whole number of them: through registers, with the bytes behind its end cleared
+            v4i v[kLoads];
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(src, off[i], 0, 0);
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i) {
+                uint32_t row, byte;
+                source_of(place(i), row, byte);
+                const int32_t there = (int32_t)(left * kSize<DT>) - (int32_t)byte;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) v[i][d] &= there >= 4 * d + 4 ? -1 : there <= 4 * d ? 0 : (1 << 8 * (there - 4 * d)) - 1;
+                *(v4i *)(lds + place(i)) = v[i];
+            }
+            wait_vmem();
+        }
+    }
+
+    // The lane's 16 bytes of fragment f (16 rows from `first` + 16 f on; dealt, if they are) of half `sub` of the stage.
+    struct Reader {
+        uint32_t at[TR && kSize<DT> == 2 ? F : 1];
+        __device__ __forceinline__ explicit Reader(uint32_t first)
+        {
+            const uint32_t lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
+            if constexpr (!TR) {
+                const uint32_t row = first + (FIRST ? i / 4u * (4u * F) + i % 4u : i);
+                at[0] = row * kRowBytes + (part ^ turn(row)) * 16u;
+            } else if constexpr (kSize<DT> == 2) {
+                const uint32_t row = 8u * part + i / 4u;
+#pragma unroll
+                for (int f = 0; f < F; ++f) at[f] = row * kWide + ((first / 16u + f) ^ turn(row)) * 32u + i % 4u * 8u;
+            } else at[0] = 4u * part * kWide + (first + i) * 4u;
+        }
+        __device__ __forceinline__ v4i operator()(const char *lds, int f, int sub) const
+        {
+            if constexpr (!TR) return *(const v4i *)(lds + (at[0] ^ (sub ? 64u : 0u)) + f * (FIRST ? 4 : 16) * kRowBytes);
+            else if constexpr (kSize<DT> == 2) {
+                typedef __attribute__((address_space(3))) v4s *P;
+                const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lds + at[f] + sub * 32 * kWide));
+                const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lds + at[f] + (sub * 32 + 4) * kWide));
+                return __builtin_bit_cast(v4i, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+            } else {
+                v4i v;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = *(const int *)(lds + at[0] + (sub * 16 + j) * kWide + f * 64);
+                return v;
+            }
+        }
+    };
+};
+
+// A workgroup of WN x WM waves makes 16 NU WN rows of P x 16 MT WM rows of Q, a wave 16 NU x 16 MT of it.
+template <int DT_, bool TP_, bool TQ_, int WN_, int WM_, int NU_, int MT_, int STAGES_>
+struct Tile {
+    static constexpr int DT = DT_, WN = WN_, WM = WM_, NU = NU_, MT = MT_, STAGES = STAGES_;
+    static constexpr bool TP = TP_, TQ = TQ_;
+    static constexpr uint32_t kWaves = WN * WM, kThreads = 64 * kWaves, kTileN = 16 * NU * WN, kTileM = 16 * MT * WM;
+    typedef Side<DT, TP, true, kTileN, NU, kWaves> P;
+    typedef Side<DT, TQ, false, kTileM, MT, kWaves> Q;
+    static constexpr uint32_t kStage = P::kBytes + Q::kBytes, kLds = STAGES * kStage, kLoads = P::kLoads + Q::kLoads, kRed = P::kRed;
+    typedef Sum<DT> Acc[NU][MT];
+
+    // Sums of the lane: row m of Q and, for fragment u, the rows n(u) + 0..3 of P.
+    uint32_t n0, m0;
+    __device__ __forceinline__ uint32_t n(int u) const
+    {
+        const uint32_t part = threadIdx.x % 64u / 16u;
+        return n0 + wave_id() % WN * (16u * NU) + (TP ? u * 16u + part * 4u : part * (4u * NU) + u * 4u);
+    }
+    __device__ __forceinline__ uint32_t m(int t) const { return m0 + wave_id() / WN * (16u * MT) + t * 16u + threadIdx.x % 16u; }
+
+    // Which tile: workgroup b runs on XCD b % 8; each XCD takes a stretch of the tiles, in panels of eight rows of tiles, so that the 32
+    // tiles it works on at a time share their rows in its L2.
+    __device__ __forceinline__ uint32_t choose(const Product &a, uint32_t id)
+    {
+        const uint32_t tm = (a.q.rows + kTileM - 1u) / kTileM, tn = (a.p.rows + kTileN - 1u) / kTileN, tiles = tm * tn;
+        uint32_t part = 0;
+        if (a.split > 1u) { part = id / tiles; id -= part * tiles; }
+        const uint32_t each = tiles / 8u, rest = tiles % 8u, xcd = id % 8u;
+        id = xcd * each + min(xcd, rest) + id / 8u;
+        const uint32_t panel = id / (8u * tn), high = min(8u, tm - panel * 8u), in = id - panel * 8u * tn;
+        n0 = in / high * kTileN;
+        m0 = (panel * 8u + in % high) * kTileM;
+        return part;
+    }
+
+    __device__ __forceinline__ void make(const Product &a, uint32_t part, char *lds, Acc &acc) const
+    {
+        const P p(a.p, n0);
+        const Q q(a.q, m0);
+        const typename P::Reader rp(wave_id() % WN * (16u * NU));
+        const typename Q::Reader rq(wave_id() / WN * (16u * MT));
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[u][t] = Sum<DT>{0, 0, 0, 0};
+        const uint32_t stages = (a.red + kRed - 1u) / kRed;
+        const uint32_t s0 = (uint32_t)((uint64_t)stages * part / a.split), count = (uint32_t)((uint64_t)stages * (part + 1u) / a.split) - s0;
+        // Where P is read once, by one row of tiles, every workgroup begins at another stage: rows are usually a power of two of bytes
+        // apart, and workgroups in step would ask the same memory channels at a time.
+        uint32_t to_fill = s0;
+        if (!TP && a.q.rows <= kTileM && count) to_fill = s0 + n0 / kTileN % count;
+        auto fill = [&](char *to) {
+            p.fill(to_fill * kRed, a.red, to);
+            q.fill(to_fill * kRed, a.red, to + P::kBytes);
+            to_fill = to_fill + 1u == s0 + count ? s0 : to_fill + 1u;
+        };
+#pragma unroll
+        for (int b = 0; b < STAGES - 1; ++b)
+            if (b < (int)count) fill(lds + b * kStage);
+        uint32_t now = 0, next = (STAGES - 1) * kStage;
+        for (uint32_t j = 0; j < count; ++j) {
+            // (towards the end there are no newer stages to leave under way)
+            if (STAGES == 2 || j + STAGES - 1 > count) stage_barrier<0>();
+            else stage_barrier<(STAGES - 2) * kLoads>();
+            if (j + STAGES - 1u < count) fill(lds + next);
+            step(lds + now, rp, rq, acc);
+            now = now == (STAGES - 1) * kStage ? 0u : now + kStage;
+            next = next == (STAGES - 1) * kStage ? 0u : next + kStage;
+        }
+    }
+
+    static __device__ __forceinline__ void step(const char *lds, const typename P::Reader &rp, const typename Q::Reader &rq, Acc &acc)
+    {
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            v4i q[MT];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) q[t] = rq(lds + P::kBytes, t, sub);
+            v4i p = rp(lds, 0, sub);
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                const v4i ahead = u + 1 < NU ? rp(lds, u + 1, sub) : p;
+#pragma unroll
+                for (int t = 0; t < MT; ++t) acc[u][t] = multiply<DT>(p, q[t], acc[u][t]);
+                p = ahead;
+            }
+        }
+    }
+};
+
+// The columns n + 0..3 of a row that begins at element `at`, as far as there are any.
+template <int DT> __device__ __forceinline__ void store_row(void *y, int64_t at, uint32_t n, uint32_t N, v4f a)
+{
+    if (n + 4u <= N) put_four<DT>(y, at + n, a);
+    else
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (n + j < N) put<DT>(y, at + n + j, a[j]);
+}
+
+}  // namespace rs

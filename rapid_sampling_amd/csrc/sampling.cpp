@@ -13,6 +13,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/hip/HIPFunctions.h>
 
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <optional>
@@ -45,7 +46,7 @@ struct Entry {
     at::Tensor ws;
     int64_t B = 0, V = 0;
     rs_policy *policy = nullptr;
-    at::Tensor logprobs_ws, linear_ws;      // workspaces of token_logprobs and linear_fp8: of one size, so never replaced
+    at::Tensor logprobs_ws, linear_ws;      // workspaces of token_logprobs and of the 8-bit products: of one size, so never replaced
     bool captured = false;                  // a stream capture has recorded calls that point into ws
     std::vector<at::Tensor> retired;        // outgrown workspaces a captured graph may still point into
     std::vector<rs_policy *> retired_policies;   // replaced policies whose pinned words a captured graph's kernels may still write
@@ -268,9 +269,9 @@ at::Tensor &logprobs_workspace(const at::Tensor &like, void *stream)
 {
     return operator_workspace(&Entry::logprobs_ws, rs_logprobs_workspace_bytes(), "token_logprobs", like, stream);
 }
-at::Tensor &linear_workspace(const at::Tensor &like, void *stream)
+at::Tensor &linear_workspace(const at::Tensor &like, void *stream, const char *what = "linear_fp8")
 {
-    return operator_workspace(&Entry::linear_ws, rs_linear_workspace_bytes(), "linear_fp8", like, stream);
+    return operator_workspace(&Entry::linear_ws, rs_linear_workspace_bytes(), what, like, stream);
 }
 
 int32_t float_dtype(const at::Tensor &t, const char *what)
@@ -434,11 +435,11 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
 
 // ------------------------------------------------------- values and products in 8 bits --
 
-at::Tensor rows_of_16_bytes(std::vector<int64_t> sizes, const at::Device &device)
+at::Tensor rows_of_16_bytes(std::vector<int64_t> sizes, const at::Device &device, at::ScalarType type = at::kFloat8_e4m3fn)
 {
     const int64_t K = sizes.back();
     sizes.back() = (K + 15) / 16 * 16;
-    return at::empty(sizes, at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(device)).narrow(-1, 0, K);
+    return at::empty(sizes, at::TensorOptions().dtype(type).device(device)).narrow(-1, 0, K);
 }
 
 // Values to be rounded to 8 bits, (..., K); the rows of the result lie (K + 15) / 16 * 16 bytes apart.
@@ -481,7 +482,7 @@ std::tuple<at::Tensor, at::Tensor> quantize(const at::Tensor &x, int64_t block_r
 }
 
 // (..., K) as rows a fixed number of bytes apart; what does not lie so, or is not aligned, is refused.
-at::Tensor fp8_rows(const at::Tensor &t, const char *what)
+at::Tensor fp8_rows(const at::Tensor &t, const char *what, const char *maker = "quantize_fp8")
 {
     const int64_t K = t.size(-1);
     at::Tensor flat;
@@ -492,7 +493,7 @@ at::Tensor fp8_rows(const at::Tensor &t, const char *what)
     }
     if ((flat.stride(1) != 1 && K > 1) || (flat.size(0) > 1 && (flat.stride(0) % 16 || flat.stride(0) < K)) || ((uintptr_t)flat.data_ptr() & 15))
         throw std::invalid_argument(std::string(what) + " must be contiguous along its last axis, with rows that begin at multiples of 16 bytes "
-                                    "(as quantize_fp8 returns them) !\n");
+                                    "(as " + maker + " returns them) !\n");
     return flat;
 }
 
@@ -564,6 +565,342 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const at::Tenso
     return y;
 }
 
+// ------------------------------------------------------- values and products in 8-bit integers --
+
+std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor &x)
+{
+    refuse_tangent("quantize_int8", {x});
+    check_floats(x, 1);
+    if (x.requires_grad() && at::GradMode::is_enabled())
+        throw std::invalid_argument("quantize_int8 has no gradient: call it under torch.no_grad(), or on x.detach() !\n");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    const int64_t K = x.size(-1), rows = x.numel() / K;
+    at::Tensor q = rows_of_16_bytes(x.sizes().vec(), x.device(), at::kChar);
+    at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), at::TensorOptions().dtype(at::kFloat).device(x.device()));
+    if (!rows) return {q, scale};
+    const at::Tensor flat = x.dim() == 2 ? x : x.reshape({rows, K});
+    const int rc = rs_quantize_rows(flat.data_ptr(), float_dtype(x, "x"), flat.stride(0), (int32_t)rows, (int32_t)K, (int8_t *)q.data_ptr(),
+                                    (K + 15) / 16 * 16, scale.data_ptr<float>(), current_stream(x));
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    return {q, scale};
+}
+
+// One scale for each row of (..., K): of the shape without K, or with one in its place.
+void check_row_scale(const at::Tensor &scale, const at::Tensor &of, const char *what)
+{
+    std::vector<int64_t> sizes = of.sizes().slice(0, of.dim() - 1).vec(), one = sizes;
+    one.push_back(1);
+    if (scale.dtype() != at::kFloat || scale.device() != of.device() || !scale.is_contiguous() || (scale.sizes() != at::IntArrayRef(sizes) && scale.sizes() != at::IntArrayRef(one)))
+        throw std::invalid_argument(std::string(what) + " must be a contiguous float32 GPU tensor of one scale for each row !\n");
+}
+
+at::Tensor linear_rows(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &weight_scale, const std::optional<at::Tensor> &x_scale,
+                       const std::optional<at::ScalarType> &out_dtype)
+{
+    const at::ScalarType to = out_dtype ? *out_dtype : at::kFloat;
+    if (to != at::kFloat && to != at::kBFloat16 && to != at::kHalf) throw std::invalid_argument("out_dtype must be float32, bfloat16 or float16 !\n");
+    if (weight.dtype() != at::kChar || weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1)
+        throw std::invalid_argument("weight must be of type int8 and shape (N, K) !\n");
+    if (x.dim() < 1 || x.size(-1) != weight.size(1)) throw std::invalid_argument("x must have shape (..., K), with the weight's K !\n");
+    if (at::GradMode::is_enabled() && (x.requires_grad() || weight_scale.requires_grad() || (x_scale && x_scale->requires_grad())))
+        throw std::invalid_argument("linear_int8 has no gradient: call it under torch.no_grad(), or on tensors that ask for none !\n");
+    refuse_tangent("linear_int8", {x, weight_scale, x_scale.value_or(at::Tensor())});
+    if (!x.is_cuda() || weight.device() != x.device()) throw std::invalid_argument("x and weight must live on the same GPU !\n");
+    const bool given = x.dtype() == at::kChar;
+    if (given != x_scale.has_value()) throw std::invalid_argument("x_scale goes with an x of type int8, and only with one !\n");
+    const int64_t K = weight.size(1), N = weight.size(0), M = x.numel() / K;
+    if (M > RS_LINEAR_MAX || N > RS_LINEAR_MAX || K > RS_LINEAR_INT8_COLUMNS_MAX || (M + 63) / 64 * ((N + 127) / 128) >= 1 << 24)
+        throw std::invalid_argument("x or weight is too large !\n");
+    if (!given) check_floats(x, 1);
+    const at::Tensor w = fp8_rows(weight, "weight", "quantize_int8");
+    check_row_scale(weight_scale, weight, "weight_scale");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    std::vector<int64_t> sizes = x.sizes().vec();
+    sizes.back() = N;
+    at::Tensor y = at::empty(sizes, at::TensorOptions().dtype(to).device(x.device()));
+    if (!M) return y;
+    void *stream = current_stream(x);
+    const int8_t *wq = (const int8_t *)w.data_ptr();
+    if (!given && M <= RS_LINEAR_ROWS_MAX && M * N <= 65536 && K <= RS_LINEAR_ROWS_COLUMNS_MAX) {
+        const at::Tensor flat = x.dim() == 2 ? x : x.reshape({M, K});
+        const int rc = rs_linear_int8_rows(flat.data_ptr(), float_dtype(x, "x"), flat.stride(0), wq, w.stride(0), weight_scale.data_ptr<float>(),
+                                           (int32_t)M, (int32_t)N, (int32_t)K, y.data_ptr(), float_dtype(y, "y"), N, stream);
+        if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+        return y;
+    }
+    // x's rows as integers and their scales: as given, or made here, side by side in one buffer
+    at::Tensor held;
+    const int8_t *q;
+    const float *scale;
+    int64_t q_stride = (K + 15) / 16 * 16;
+    if (given) {
+        check_row_scale(*x_scale, x, "x_scale");
+        held = fp8_rows(x, "x", "quantize_int8");
+        q = (const int8_t *)held.data_ptr();
+        q_stride = held.stride(0);
+        scale = x_scale->data_ptr<float>();
+    } else {
+        held = at::empty({M * (q_stride + 4)}, at::TensorOptions().dtype(at::kByte).device(x.device()));
+        q = (const int8_t *)held.data_ptr();
+        scale = (const float *)(q + M * q_stride);
+        const at::Tensor flat = x.dim() == 2 ? x : x.reshape({M, K});
+        const int rc = rs_quantize_rows(flat.data_ptr(), float_dtype(x, "x"), flat.stride(0), (int32_t)M, (int32_t)K, (int8_t *)q, q_stride, (float *)scale, stream);
+        if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    }
+    at::Tensor &ws = linear_workspace(x, stream, "linear_int8");
+    const int rc = rs_linear_int8(q, q_stride, scale, wq, w.stride(0), weight_scale.data_ptr<float>(), (int32_t)M, (int32_t)N, (int32_t)K,
+                                  y.data_ptr(), float_dtype(y, "y"), N, ws.data_ptr(), (size_t)ws.numel(), stream);
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    return y;
+}
+
+// ------------------------------------------------------- rows of a table by token --
+
+void check_tokens(const at::Tensor &tokens)
+{
+    if (tokens.dtype() != at::kInt && tokens.dtype() != at::kLong)
+        throw std::invalid_argument("tokens must be of type int32 or int64, got " + std::string(tokens.dtype().name()) + " !\n");
+}
+// Tokens of any shape as one list.
+at::Tensor token_list(const at::Tensor &tokens) { return tokens.dim() == 1 ? tokens : tokens.reshape({tokens.numel()}); }
+
+at::Tensor scratch(size_t bytes, const at::Tensor &like)
+{
+    return at::empty({(int64_t)std::max<size_t>(bytes, 1)}, at::TensorOptions().dtype(at::kByte).device(like.device()));
+}
+
+struct TableCall {
+    int64_t M, V, K;
+    int32_t table, out;              // RS_DTYPE_* or RS_TABLE_*
+    at::ScalarType to;
+};
+
+TableCall read_table(const at::Tensor &tokens, const at::Tensor &weight, double scale, const std::optional<at::Tensor> &weight_scale,
+                     const std::optional<at::ScalarType> &out_dtype)
+{
+    TableCall c;
+    check_tokens(tokens);
+    const bool int8 = weight.dtype() == at::kChar, fp8 = weight.dtype() == at::kFloat8_e4m3fn;
+    if (int8 || fp8) c.table = int8 ? RS_TABLE_INT8 : RS_TABLE_FP8;
+    else if (weight.dtype() == at::kFloat) c.table = RS_DTYPE_F32;
+    else if (weight.dtype() == at::kBFloat16) c.table = RS_DTYPE_BF16;
+    else if (weight.dtype() == at::kHalf) c.table = RS_DTYPE_F16;
+    else throw std::invalid_argument("weight must be of type float32, bfloat16, float16, int8 or float8_e4m3fn, got " + std::string(weight.dtype().name()) + " !\n");
+    c.to = out_dtype ? *out_dtype : int8 || fp8 ? at::kFloat : weight.scalar_type();
+    if (c.to == at::kFloat) c.out = RS_DTYPE_F32;
+    else if (c.to == at::kBFloat16) c.out = RS_DTYPE_BF16;
+    else if (c.to == at::kHalf) c.out = RS_DTYPE_F16;
+    else throw std::invalid_argument("out_dtype must be float32, bfloat16 or float16 !\n");
+    if (weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1) throw std::invalid_argument("weight must have shape (V, K) !\n");
+    if ((int8 || fp8) != weight_scale.has_value()) throw std::invalid_argument("weight_scale goes with a weight of type int8 or float8_e4m3fn, and only with one !\n");
+    if (!std::isfinite(scale)) throw std::invalid_argument("scale must be finite !\n");
+    c.M = tokens.numel(); c.V = weight.size(0); c.K = weight.size(1);
+    if (c.M >= RS_LINEAR_MAX || c.V > RS_LINEAR_MAX || c.K > RS_LINEAR_MAX) throw std::invalid_argument("tokens or weight is too large !\n");
+    refuse_tangent("embedding", {weight, weight_scale.value_or(at::Tensor())});
+    if (at::GradMode::is_enabled() && (int8 || fp8) && (weight.requires_grad() || weight_scale->requires_grad()))
+        throw std::invalid_argument("embedding has no gradient for a table in 8 bits: call it under torch.no_grad(), or on tensors that ask for none !\n");
+    if (!weight.is_cuda() || tokens.device() != weight.device()) throw std::invalid_argument("tokens and weight must live on the same GPU !\n");
+    if (weight.stride(1) != 1 && c.K > 1) throw std::invalid_argument("weight must be contiguous along its last axis !\n");
+    if (int8) { fp8_rows(weight, "weight", "quantize_int8"); check_row_scale(*weight_scale, weight, "weight_scale"); }
+    if (fp8) { fp8_rows(weight, "weight"); check_scale(*weight_scale, weight, (c.V + 127) / 128, (c.K + 127) / 128, "weight_scale"); }
+    return c;
+}
+
+at::Tensor embedding_forward(const at::Tensor &tokens, const at::Tensor &weight, double scale, const std::optional<at::Tensor> &weight_scale,
+                             const std::optional<at::ScalarType> &out_dtype)
+{
+    const TableCall c = read_table(tokens, weight, scale, weight_scale, out_dtype);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(weight.device());
+    std::vector<int64_t> sizes = tokens.sizes().vec();
+    sizes.push_back(c.K);
+    at::Tensor y = at::empty(sizes, at::TensorOptions().dtype(c.to).device(weight.device()));
+    if (!c.M) return y;
+    const at::Tensor list = token_list(tokens);
+    const int rc = rs_embedding(list.data_ptr(), list.dtype() == at::kLong, list.stride(0), weight.data_ptr(), c.table, weight.stride(0),
+                                weight_scale ? weight_scale->data_ptr<float>() : nullptr, scale, (int32_t)c.M, (int32_t)c.V, (int32_t)c.K,
+                                y.data_ptr(), c.out, current_stream(weight));
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    return y;
+}
+
+at::Tensor embedding_backward(const at::Tensor &g, const at::Tensor &tokens, int64_t V, at::ScalarType type, double scale)
+{
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(tokens.device());
+    const int64_t M = tokens.numel(), K = g.size(-1);
+    const auto options = at::TensorOptions().dtype(type).device(tokens.device());
+    if (!M) return at::zeros({V, K}, options);
+    at::Tensor grad = at::empty({V, K}, options);
+    at::Tensor rows = g.reshape({M, K});
+    if (rows.stride(1) != 1 && K > 1) rows = rows.contiguous();
+    const at::Tensor list = token_list(tokens);
+    const at::Tensor ws = scratch(rs_embedding_workspace_bytes((int32_t)M, (int32_t)V, (int32_t)K), tokens);
+    const int rc = rs_embedding_backward(list.data_ptr(), list.dtype() == at::kLong, list.stride(0), rows.data_ptr(), float_dtype(rows, "the gradient"), rows.stride(0),
+                                         scale, (int32_t)M, (int32_t)V, (int32_t)K, grad.data_ptr(), float_dtype(grad, "the gradient"), ws.data_ptr(),
+                                         (size_t)ws.numel(), current_stream(tokens));
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    return grad;
+}
+
+// (the gradient is linear in g, but it is differentiated once only, as the others are)
+struct EmbeddingBackward : torch::autograd::Function<EmbeddingBackward> {
+    static at::Tensor forward(AutogradContext *, at::Tensor g, at::Tensor tokens, int64_t V, int64_t type, double scale)
+    {
+        return embedding_backward(g, tokens, V, (at::ScalarType)type, scale);
+    }
+    static variable_list backward(AutogradContext *, variable_list)
+    {
+        throw std::runtime_error("rapid_sampling: embedding can be differentiated once only");
+    }
+};
+
+struct Embedding : torch::autograd::Function<Embedding> {
+    static at::Tensor forward(AutogradContext *ctx, at::Tensor weight, at::Tensor tokens, double scale, int64_t to)
+    {
+        at::Tensor y = embedding_forward(tokens, weight, scale, std::nullopt, (at::ScalarType)to);
+        ctx->save_for_backward({tokens});
+        ctx->saved_data["V"] = weight.size(0);
+        ctx->saved_data["type"] = (int64_t)weight.scalar_type();
+        ctx->saved_data["scale"] = scale;
+        ctx->set_materialize_grads(false);
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        refuse_tangent("embedding's gradient", {grads[0]});
+        const at::Tensor tokens = ctx->get_saved_variables()[0];
+        const int64_t V = ctx->saved_data["V"].toInt(), type = ctx->saved_data["type"].toInt();
+        const double scale = ctx->saved_data["scale"].toDouble();
+        const at::Tensor grad = at::GradMode::is_enabled() ? EmbeddingBackward::apply(grads[0], tokens, V, type, scale)
+                                                           : embedding_backward(grads[0], tokens, V, (at::ScalarType)type, scale);
+        return {grad, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+// ------------------------------------------------------- cross entropy without the logits --
+
+// (..., K) as rows that the tiles can read: 16-byte aligned, in multiples of 16 bytes below 16 MB; laid out anew where they are not.
+at::Tensor tile_rows(const at::Tensor &t, int64_t rows, int64_t K, void *stream)
+{
+    const int64_t size = t.element_size();
+    const at::Tensor flat = t.dim() == 2 ? t : t.reshape({rows, K});
+    const bool fits = rows == 1 || (flat.stride(0) >= K && flat.stride(0) * size % 16 == 0 && flat.stride(0) * size < (1 << 24) - 128);
+    if (((uintptr_t)flat.data_ptr() & 15) == 0 && fits) return flat;
+    const int64_t stride = (K * size + 15) / 16 * 16 / size;
+    at::Tensor held = at::empty({rows, stride}, t.options().requires_grad(false)).narrow(1, 0, K);
+    const int rc = rs_lay_out_rows(flat.data_ptr(), rows > 1 ? flat.stride(0) : 0, (int32_t)size, rows, (int32_t)K, held.data_ptr(), stride, stream);
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    return held;
+}
+
+struct LossCall {
+    int64_t M, V, K;
+    int32_t dtype;
+};
+
+LossCall read_loss(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &tokens, double temperature)
+{
+    LossCall c;
+    c.dtype = float_dtype(x, "x");
+    if (weight.dtype() != x.dtype()) throw std::invalid_argument("x and weight must be of one type !\n");
+    if (weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1) throw std::invalid_argument("weight must have shape (V, K) !\n");
+    if (x.dim() < 1 || x.size(-1) != weight.size(1)) throw std::invalid_argument("x must have shape (..., K), with the weight's K !\n");
+    check_tokens(tokens);
+    if (tokens.sizes() != x.sizes().slice(0, x.dim() - 1)) throw std::invalid_argument("tokens must have x's shape without its last axis !\n");
+    if (!(temperature >= 0.001 && temperature <= 1000.0)) throw_for(RS_ERR_TEMPERATURE, 1, 1, weight.size(0), temperature);
+    c.K = weight.size(1); c.V = weight.size(0); c.M = x.numel() / c.K;
+    if (c.V > 1048576) throw std::invalid_argument("Vocabulary size must be positive, and no larger than 1048576, got " + std::to_string(c.V) + " !\n");
+    if (c.M > RS_LINEAR_MAX || c.K > RS_LOSS_COLUMNS_MAX || (c.M + 63) / 64 * ((c.V + 127) / 128) >= 1 << 24) throw std::invalid_argument("x or weight is too large !\n");
+    if (!x.is_cuda() || weight.device() != x.device() || tokens.device() != x.device())
+        throw std::invalid_argument("x, weight and tokens must live on the same GPU !\n");
+    if ((x.stride(-1) != 1 || weight.stride(1) != 1) && c.K > 1) throw std::invalid_argument("x and weight must be contiguous along their last axis !\n");
+    return c;
+}
+
+struct LossResult {
+    at::Tensor loss, lse, stats;
+};
+
+LossResult loss_forward(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &tokens, double temperature, bool want_stats)
+{
+    const LossCall c = read_loss(x, weight, tokens, temperature);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    const auto f32 = at::TensorOptions().dtype(at::kFloat).device(x.device());
+    LossResult o{at::empty(tokens.sizes(), f32), at::empty(tokens.sizes(), f32), want_stats ? at::empty({c.M, 2}, f32) : at::Tensor()};
+    if (!c.M) return o;
+    void *stream = current_stream(x);
+    const at::Tensor xr = tile_rows(x, c.M, c.K, stream), w = tile_rows(weight, c.V, c.K, stream), list = token_list(tokens);
+    const at::Tensor ws = scratch(rs_linear_cross_entropy_workspace_bytes((int32_t)c.M, (int32_t)c.V, (int32_t)c.K, c.dtype, 0), x);
+    const int rc = rs_linear_cross_entropy(xr.data_ptr(), xr.stride(0), w.data_ptr(), w.stride(0), c.dtype, list.data_ptr(), list.dtype() == at::kLong, list.stride(0),
+                                           (int32_t)c.M, (int32_t)c.V, (int32_t)c.K, temperature, o.loss.data_ptr<float>(), o.lse.data_ptr<float>(),
+                                           want_stats ? o.stats.data_ptr<float>() : nullptr, ws.data_ptr(), (size_t)ws.numel(), stream);
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    return o;
+}
+
+std::tuple<at::Tensor, at::Tensor> loss_backward(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &tokens, const at::Tensor &stats, double temperature,
+                                                 bool want_x, bool want_w, const at::Tensor &g, const at::Tensor &h)
+{
+    const LossCall c = read_loss(x, weight, tokens, temperature);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    at::Tensor gx, gw;
+    if (want_x) gx = at::empty(x.sizes(), x.options().requires_grad(false));
+    if (want_w) gw = c.M ? at::empty(weight.sizes(), weight.options().requires_grad(false)) : at::zeros(weight.sizes(), weight.options().requires_grad(false));
+    if (!c.M || (!want_x && !want_w)) return {gx, gw};
+    void *stream = current_stream(x);
+    int32_t gs, hs;
+    const at::Tensor g1 = gradient_in(g, &gs), h1 = gradient_in(h, &hs);
+    const at::Tensor xr = tile_rows(x, c.M, c.K, stream), w = tile_rows(weight, c.V, c.K, stream), list = token_list(tokens);
+    const at::Tensor ws = scratch(rs_linear_cross_entropy_workspace_bytes((int32_t)c.M, (int32_t)c.V, (int32_t)c.K, c.dtype, 1), x);
+    auto ptr = [](const at::Tensor &t) { return t.defined() ? (const float *)t.data_ptr() : nullptr; };
+    const int rc = rs_linear_cross_entropy_backward(xr.data_ptr(), xr.stride(0), w.data_ptr(), w.stride(0), c.dtype, list.data_ptr(), list.dtype() == at::kLong,
+                                                    list.stride(0), (int32_t)c.M, (int32_t)c.V, (int32_t)c.K, temperature, stats.data_ptr<float>(), ptr(g1), gs,
+                                                    ptr(h1), hs, want_x ? gx.data_ptr() : nullptr, want_w ? gw.data_ptr() : nullptr, ws.data_ptr(),
+                                                    (size_t)ws.numel(), stream);
+    if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    return {gx, gw};
+}
+
+struct LossBackward : torch::autograd::Function<LossBackward> {
+    static variable_list forward(AutogradContext *ctx, at::Tensor x, at::Tensor weight, at::Tensor tokens, at::Tensor stats, double temperature, bool want_x,
+                                 bool want_w, std::optional<at::Tensor> g, std::optional<at::Tensor> h)
+    {
+        const auto [gx, gw] = loss_backward(x, weight, tokens, stats, temperature, want_x, want_w, g.value_or(at::Tensor()), h.value_or(at::Tensor()));
+        return {gx, gw};
+    }
+    static variable_list backward(AutogradContext *, variable_list)
+    {
+        throw std::runtime_error("rapid_sampling: linear_cross_entropy can be differentiated once only");
+    }
+};
+
+struct Loss : torch::autograd::Function<Loss> {
+    static variable_list forward(AutogradContext *ctx, at::Tensor x, at::Tensor weight, at::Tensor tokens, double temperature)
+    {
+        LossResult o = loss_forward(x, weight, tokens, temperature, true);
+        ctx->save_for_backward({x, weight, tokens, o.stats});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->set_materialize_grads(false);
+        return {o.loss, o.lse};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const at::Tensor none;
+        if (!grads[0].defined() && !grads[1].defined()) return {none, none, none, none};
+        refuse_tangent("linear_cross_entropy's gradient", {grads[0], grads[1]});
+        const auto saved = ctx->get_saved_variables();
+        const double temperature = ctx->saved_data["temperature"].toDouble();
+        const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+        if (at::GradMode::is_enabled()) {
+            auto given = [&](int i) { return grads[i].defined() ? std::optional<at::Tensor>(grads[i]) : std::nullopt; };
+            const variable_list o = LossBackward::apply(saved[0], saved[1], saved[2], saved[3], temperature, want_x, want_w, given(0), given(1));
+            return {o[0], o[1], none, none};
+        }
+        const auto [gx, gw] = loss_backward(saved[0], saved[1], saved[2], saved[3], temperature, want_x, want_w, grads[0], grads[1]);
+        return {gx, gw, none, none};
+    }
+};
+
 }  // namespace
 
 // (logprobs, entropy, rank, top_logprobs, top_tokens); under autograd where the logits ask for a gradient.
@@ -585,6 +922,33 @@ at::Tensor linear_fp8(const at::Tensor &x, const at::Tensor &weight, const at::T
                       std::optional<at::ScalarType> out_dtype)
 {
     return linear(x, weight, weight_scale, x_scale, out_dtype);
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_int8(const at::Tensor &x) { return quantize_rows(x); }
+
+at::Tensor linear_int8(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &weight_scale, std::optional<at::Tensor> x_scale,
+                       std::optional<at::ScalarType> out_dtype)
+{
+    return linear_rows(x, weight, weight_scale, x_scale, out_dtype);
+}
+
+at::Tensor embedding(const at::Tensor &tokens, const at::Tensor &weight, double scale, std::optional<at::Tensor> weight_scale, std::optional<at::ScalarType> out_dtype)
+{
+    if (!weight.requires_grad() || !at::GradMode::is_enabled()) return embedding_forward(tokens, weight, scale, weight_scale, out_dtype);
+    const TableCall c = read_table(tokens, weight, scale, weight_scale, out_dtype);
+    return Embedding::apply(weight, tokens, scale, (int64_t)c.to);
+}
+
+// (loss, logsumexp); under autograd where x or the weight asks for a gradient.
+std::tuple<at::Tensor, at::Tensor> linear_cross_entropy(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &tokens, double temperature)
+{
+    refuse_tangent("linear_cross_entropy", {x, weight});
+    if ((x.requires_grad() || weight.requires_grad()) && at::GradMode::is_enabled()) {
+        variable_list o = Loss::apply(x, weight, tokens, temperature);
+        return {o[0], o[1]};
+    }
+    LossResult o = loss_forward(x, weight, tokens, temperature, false);
+    return {o.loss, o.lse};
 }
 
 // sampling.cu:140-144.  State is 64 bytes per row, opaque to the caller.
@@ -791,6 +1155,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("quantize_fp8", &quantize_fp8, py::arg("x"), py::kw_only(), py::arg("block_rows") = 1);
     m.def("linear_fp8", &linear_fp8, py::arg("x"), py::arg("weight"), py::arg("weight_scale"), py::kw_only(), py::arg("x_scale") = py::none(),
           py::arg("out_dtype") = py::none());
+    m.def("quantize_int8", &quantize_int8, py::arg("x"));
+    m.def("linear_int8", &linear_int8, py::arg("x"), py::arg("weight"), py::arg("weight_scale"), py::kw_only(), py::arg("x_scale") = py::none(),
+          py::arg("out_dtype") = py::none());
+    m.def("embedding", &embedding, py::arg("tokens"), py::arg("weight"), py::arg("scale") = 1.0, py::kw_only(), py::arg("weight_scale") = py::none(),
+          py::arg("out_dtype") = py::none());
+    m.def("linear_cross_entropy", &linear_cross_entropy, py::arg("x"), py::arg("weight"), py::arg("tokens"), py::arg("temperature") = 1.0);
     m.attr("LOGPROBS_TOP_MAX") = RS_LOGPROBS_TOP_MAX;
     m.def("workspace_status", &workspace_status, py::arg("device") = py::none());
     m.def("policy_state", &policy_state, py::arg("device") = py::none());
