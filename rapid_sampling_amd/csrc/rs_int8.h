@@ -204,9 +204,14 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Params p)
 }
 
 // -------------------------------------------------------------- many rows --
-template <int DT, class T, bool SPLIT>
-__global__ __launch_bounds__(T::kThreads, 2) void int8_tile_kernel(Int8Params p)
+// Results of 16 bits are stored eight at a time.
+template <int DT, int WN, int WM, int NU, int MT, int STAGES>
+using Int8Tile = Tile<kInt8, false, false, DT != RS_DTYPE_F32, WN, WM, NU, MT, STAGES>;
+
+template <int DT, int WN, int WM, int NU, int MT, int STAGES, bool SPLIT>
+__global__ __launch_bounds__(64 * WN * WM, 2) void int8_tile_kernel(Int8Params p)
 {
+    using T = Int8Tile<DT, WN, WM, NU, MT, STAGES>;
     extern __shared__ char lds[];
     T tile;
     const uint32_t part = tile.choose(p.a, blockIdx.x);
@@ -254,14 +259,12 @@ __global__ __launch_bounds__(T::kThreads, 2) void int8_tile_kernel(Int8Params p)
         const uint32_t m = tile.m(t);
         if (m >= p.M) continue;
         const float f = p.x_scale[m];
+        v4f y[T::NU];
 #pragma unroll
-        for (int u = 0; u < T::NU; ++u) {
-            const uint32_t n = tile.n(u);
-            v4f y;
+        for (int u = 0; u < T::NU; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = (float)acc[u][t][j] * (f * p.w_scale[min(n + j, p.N - 1u)]);
-            store_row<DT>(p.y, (int64_t)m * p.y_stride, n, p.N, y);
-        }
+            for (int j = 0; j < 4; ++j) y[u][j] = (float)acc[u][t][j] * (f * p.w_scale[min(tile.n(u) + j, p.N - 1u)]);
+        store_tile_row<DT>(tile, p.y, (int64_t)m * p.y_stride, p.N, y);
     }
 }
 

@@ -43,11 +43,12 @@ template <int DT> static void launch_few(const Int8Params &p, int32_t x_dtype, h
     else launch_few<DT, RS_DTYPE_F16>(p, st);
 }
 
-template <int DT, class T, bool SPLIT> static void launch_tiles(Int8Params p, hipStream_t st)
+template <int DT, int WN, int WM, int NU, int MT, int STAGES, bool SPLIT> static void launch_tiles(Int8Params p, hipStream_t st)
 {
+    using T = Int8Tile<DT, WN, WM, NU, MT, STAGES>;
     const uint64_t tiles = (uint64_t)((p.M + T::kTileM - 1) / T::kTileM) * ((p.N + T::kTileN - 1) / T::kTileN);
     p.a.split = SPLIT ? (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({kPartTiles / tiles, (p.K + 127) / 128 / 4, 8})) : 1;
-    hipLaunchKernelGGL((int8_tile_kernel<DT, T, SPLIT>), dim3((uint32_t)(tiles * p.a.split)), dim3(T::kThreads), T::kLds, st, p);
+    hipLaunchKernelGGL((int8_tile_kernel<DT, WN, WM, NU, MT, STAGES, SPLIT>), dim3((uint32_t)(tiles * p.a.split)), dim3(T::kThreads), T::kLds, st, p);
 }
 
 template <int DT> static void launch_product(const Int8Params &p, hipStream_t st)
@@ -55,8 +56,8 @@ template <int DT> static void launch_product(const Int8Params &p, hipStream_t st
     // (the tiles' kernel reaches its rows with 32 bits)
     if (p.M <= 16 || p.x_stride > kTileStride || p.w_stride > kTileStride) return launch_few<DT, -1>(p, st);
     const uint64_t n256 = (p.N + 255) / 256, m256 = (p.M + 255) / 256;
-    if (p.M > 128 && n256 * m256 >= 192) return launch_tiles<DT, Tile<kInt8, false, false, 2, 4, 8, 4, 2>, false>(p, st);
-    launch_tiles<DT, Tile<kInt8, false, false, 2, 2, 4, 2, 3>, true>(p, st);
+    if (p.M > 128 && n256 * m256 >= 192) return launch_tiles<DT, 2, 4, 8, 4, 2, false>(p, st);
+    launch_tiles<DT, 2, 2, 4, 2, 3, true>(p, st);
 }
 
 static Int8Params int8_params(const void *x, int64_t x_stride, const float *x_scale, const int8_t *w, int64_t w_stride, const float *w_scale, int32_t M, int32_t N,
@@ -114,9 +115,10 @@ int rs_linear_int8(const int8_t *x, int64_t x_row_stride, const float *x_scale, 
         return RS_ERR_ALIGN;
     const Int8Params p = int8_params(x, x_row_stride, x_scale, w, w_row_stride, w_scale, M, N, K, y, y_row_stride, workspace);
     const hipStream_t st = (hipStream_t)stream;
-    if (y_dtype == RS_DTYPE_F32) launch_product<RS_DTYPE_F32>(p, st);
+    // (float16 first: the compiler leaves the last of them without its host side otherwise)
+    if (y_dtype == RS_DTYPE_F16) launch_product<RS_DTYPE_F16>(p, st);
     else if (y_dtype == RS_DTYPE_BF16) launch_product<RS_DTYPE_BF16>(p, st);
-    else launch_product<RS_DTYPE_F16>(p, st);
+    else launch_product<RS_DTYPE_F32>(p, st);
     return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
 }
 

@@ -170,17 +170,15 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
         if (m >= p.M) continue;
         const LossRow r = p.rows[m];
         char *row = (char *)p.grad + (int64_t)m * p.grad_stride;
+        v4f v[T::NU];
 #pragma unroll
-        for (int u = 0; u < T::NU; ++u) {
-            const uint32_t n = tile.n(u);
-            v4f v;
+        for (int u = 0; u < T::NU; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                v[j] = r.a * __builtin_amdgcn_exp2f(acc[u][t][j] * p.c - r.max);
-                if ((int32_t)(n + p.v0 + j) == r.token) v[j] -= r.b;
+                v[u][j] = r.a * __builtin_amdgcn_exp2f(acc[u][t][j] * p.c - r.max);
+                if ((int32_t)(tile.n(u) + p.v0 + j) == r.token) v[u][j] -= r.b;
             }
-            store_row<T::DT>(row, 0, n, p.a.p.rows, v);
-        }
+        store_tile_row<T::DT>(tile, row, 0, p.a.p.rows, v);
     }
 }
 
@@ -237,8 +235,10 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_dw_kernel(GradParams p)
     for (int t = 0; t < T::MT; ++t) {
         const uint32_t m = tile.m(t);
         if (m >= p.a.q.rows) continue;
+        v4f v[T::NU];
 #pragma unroll
-        for (int u = 0; u < T::NU; ++u) store_row<T::DT>(p.y, (int64_t)m * p.y_stride, tile.n(u), p.a.p.rows, acc[u][t] * f);
+        for (int u = 0; u < T::NU; ++u) v[u] = acc[u][t] * f;
+        store_tile_row<T::DT>(tile, p.y, (int64_t)m * p.y_stride, p.a.p.rows, v);
     }
 }
 

@@ -45,8 +45,8 @@ static LossSpace loss_space(int32_t M, int32_t V, int32_t K, int32_t dtype, bool
     return s;
 }
 
-template <int DT, bool TP, bool TQ> using LargeTile = Tile<DT, TP, TQ, 2, 4, 8, 4, 2>;       // 256 x 256, eight waves
-template <int DT, bool TP, bool TQ> using SmallTile = Tile<DT, TP, TQ, 2, 2, 4, 2, 3>;       // 128 x 64, four waves
+template <int DT, bool TP, bool TQ> using LargeTile = Tile<DT, TP, TQ, !TP && DT != RS_DTYPE_F32, 2, 4, 8, 4, 2>;       // 256 x 256, eight waves
+template <int DT, bool TP, bool TQ> using SmallTile = Tile<DT, TP, TQ, !TP && DT != RS_DTYPE_F32, 2, 2, 4, 2, 3>;       // 128 x 64, four waves
 
 template <class T, class K, class A> static void launch_tiles(K kernel, const A &p, const Product &a, hipStream_t st)
 {

@@ -58,9 +58,9 @@ struct Product {
 // Transposed: a stage is 128 / size values of r, the COUNT values of each side by side; those of 16 bits are turned by the reads from
 // LDS (ds_read_b64_tr_b16: four r of a row to a lane), whose 32-byte pieces are stored in such an order too.
 //
-// FIRST (the product's first operand, untransposed): the rows are dealt to the matrix instructions so that a lane's sums belong to 4 F
-// consecutive rows, F fragments of 16 rows to a wave.
-template <int DT, bool TR, bool FIRST, int COUNT, int F, int WAVES>
+// PAIRS (untransposed): the rows are dealt to the matrix instructions so that a lane's sums of two fragments (of 16 rows; F to a wave) belong
+// to eight consecutive rows: 16 bytes of a result in 16 bits.
+template <int DT, bool TR, bool PAIRS, int COUNT, int F, int WAVES>
 struct Side {
     static constexpr uint32_t kBytes = COUNT * kRowBytes, kLoads = kBytes / (1024 * WAVES), kRed = kRowBytes / kSize<DT>;
     static constexpr uint32_t kWide = COUNT * kSize<DT>;                     // bytes of one r, transposed
@@ -70,12 +70,14 @@ struct Side {
 
     const char *base;
     uint32_t    stride, rows, bytes;       // transposed: bytes of one r from the tile's first row on
+    uint32_t    byte;                      // as they are: of the row, of the thread's pieces, the same for all its loads
     uint32_t    off[kLoads];
+    static_assert(TR || WAVES % 2 == 0, "a thread's loads have one turn");
 
     // the order of pieces: depends on the row and is the same for all the fragments of a lane
     static __device__ __forceinline__ uint32_t turn(uint32_t row)
     {
-        if (!TR) return FIRST ? (row & 3u) | ((row / F) & 4u) : row & 7u;
+        if (!TR) return PAIRS ? (row & 3u) | ((row >> 1) & 4u) : row & 7u;
         return kWide == 128 ? ((row >> 1) & 1u) | ((row >> 2) & 2u) : (row & 3u) | ((row >> 1) & 4u);
     }
     // byte of the source's row (or r) that a byte of the stage holds
@@ -94,59 +96,52 @@ struct Side {
         rows = min(o.rows - first, (uint32_t)COUNT);
         base = o.at + (TR ? (int64_t)first * kSize<DT> : (int64_t)first * o.stride);
         bytes = (o.rows - first) * kSize<DT>;
+        byte = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
-            uint32_t row, byte;
+            uint32_t row;
             source_of(place(i), row, byte);
             off[i] = TR ? row * stride + byte : tile_at(row, rows, stride, byte);
             asm volatile("" : "+v"(off[i]));               // once, and not for every stage
         }
     }
-    // Asks for the stage that begins at r.
+    // Asks for the stage that begins at r.  What lies behind the reduction's end reads as 0: as they are, pieces from there on by an address
+    // behind every buffer, and the bytes of the one that it cuts by clear(); transposed, by the buffer's size.  (What a transposed
+    // load reads behind a row's end belongs to sums that nobody asks for.)
     __device__ __forceinline__ void fill(uint32_t r, uint32_t red, char *lds) const
     {
         const uint32_t left = red - r;
-        if constexpr (TR) {
-            // what lies behind the last r reads as 0; what lies behind a row's end belongs to sums that nobody asks for
-            const uint32_t size = (min(left, kRed) - 1u) * stride + ((bytes + 3u) & ~3u);
-            const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc((void *)(base + (int64_t)r * stride), 0, (int)size, kBufferFlags);
+        const uint32_t size = TR ? (min(left, kRed) - 1u) * stride + ((bytes + 3u) & ~3u) : tile_bytes(rows, stride, left * kSize<DT>);
+        const int64_t at = TR ? (int64_t)r * stride : (int64_t)r * kSize<DT>;
+        const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc((void *)(base + at), 0, (int)size, kBufferFlags);
+        const bool there = TR || byte < left * kSize<DT>;
 #pragma unroll
-            for (uint32_t i = 0; i < kLoads; ++i)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (LdsPtr)(lds + (i * WAVES + wave_id()) * 1024u), 16, off[i], 0, 0, 0);
-        } else {
-            const uint32_t size = tile_bytes(rows, stride, left * kSize<DT>);
-            const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc((void *)(base + (int64_t)r * kSize<DT>), 0, (int)size, kBufferFlags);
-            if (left >= kRed) {
+        for (uint32_t i = 0; i < kLoads; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (LdsPtr)(lds + (i * WAVES + wave_id()) * 1024u), 16, there ? off[i] : kTileNone, 0, 0, 0);
+    }
+    // The bytes behind the reduction's end of the piece that it cuts, of the stage that begins `left` values before it.
+    static __device__ __forceinline__ void clear(uint32_t left, char *lds)
+    {
+        for (uint32_t row = threadIdx.x; !TR && row < (uint32_t)COUNT; row += 64u * WAVES) {
+            const uint32_t end = left * kSize<DT>;
+            v4i *piece = (v4i *)(lds + row * kRowBytes + ((end / 16u) ^ turn(row)) * 16u);
+            v4i v = *piece;
+            const int32_t keep = (int32_t)(end % 16u);
 #pragma unroll
-                for (uint32_t i = 0; i < kLoads; ++i)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (LdsPtr)(lds + (i * WAVES + wave_id()) * 1024u), 16, off[i], 0, 0, 0);
-                return;
-            }
-            // the last stage of a reduction that is no whole number of them: through registers, with the bytes behind its end cleared
-            v4i v[kLoads];
-#pragma unroll
-            for (uint32_t i = 0; i < kLoads; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(src, off[i], 0, 0);
-#pragma unroll
-            for (uint32_t i = 0; i < kLoads; ++i) {
-                uint32_t row, byte;
-                source_of(place(i), row, byte);
-                const int32_t there = (int32_t)(left * kSize<DT>) - (int32_t)byte;
-#pragma unroll
-                for (int d = 0; d < 4; ++d) v[i][d] &= there >= 4 * d + 4 ? -1 : there <= 4 * d ? 0 : (1 << 8 * (there - 4 * d)) - 1;
-                *(v4i *)(lds + place(i)) = v[i];
-            }
-            wait_vmem();
+            for (int d = 0; d < 4; ++d) v[d] &= keep >= 4 * d + 4 ? -1 : keep <= 4 * d ? 0 : (1 << 8 * (keep - 4 * d)) - 1;
+            *piece = v;
         }
     }
 
     // The lane's 16 bytes of fragment f (16 rows from `first` + 16 f on; dealt, if they are) of half `sub` of the stage.
     struct Reader {
+        static constexpr int kReads = !TR ? 1 : kSize<DT> == 2 ? 2 : 4;
         uint32_t at[TR && kSize<DT> == 2 ? F : 1];
         __device__ __forceinline__ explicit Reader(uint32_t first)
         {
             const uint32_t lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
             if constexpr (!TR) {
-                const uint32_t row = first + (FIRST ? i / 4u * (4u * F) + i % 4u : i);
+                const uint32_t row = first + (PAIRS ? i / 4u * 8u + i % 4u : i);
                 at[0] = row * kRowBytes + (part ^ turn(row)) * 16u;
             } else if constexpr (kSize<DT> == 2) {
                 const uint32_t row = 8u * part + i / 4u;
@@ -156,7 +151,7 @@ struct Side {
         }
         __device__ __forceinline__ v4i operator()(const char *lds, int f, int sub) const
         {
-            if constexpr (!TR) return *(const v4i *)(lds + (at[0] ^ (sub ? 64u : 0u)) + f * (FIRST ? 4 : 16) * kRowBytes);
+            if constexpr (!TR) return *(const v4i *)(lds + (at[0] ^ (sub ? 64u : 0u)) + (PAIRS ? f / 2 * 32 + f % 2 * 4 : f * 16) * kRowBytes);
             else if constexpr (kSize<DT> == 2) {
                 typedef __attribute__((address_space(3))) v4s *P;
                 const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lds + at[f] + sub * 32 * kWide));
@@ -173,12 +168,12 @@ struct Side {
 };
 
 // A workgroup of WN x WM waves makes 16 NU WN rows of P x 16 MT WM rows of Q, a wave 16 NU x 16 MT of it.
-template <int DT_, bool TP_, bool TQ_, int WN_, int WM_, int NU_, int MT_, int STAGES_>
+template <int DT_, bool TP_, bool TQ_, bool PAIRS_, int WN_, int WM_, int NU_, int MT_, int STAGES_>
 struct Tile {
     static constexpr int DT = DT_, WN = WN_, WM = WM_, NU = NU_, MT = MT_, STAGES = STAGES_;
-    static constexpr bool TP = TP_, TQ = TQ_;
+    static constexpr bool TP = TP_, TQ = TQ_, PAIRS = PAIRS_;
     static constexpr uint32_t kWaves = WN * WM, kThreads = 64 * kWaves, kTileN = 16 * NU * WN, kTileM = 16 * MT * WM;
-    typedef Side<DT, TP, true, kTileN, NU, kWaves> P;
+    typedef Side<DT, TP, PAIRS, kTileN, NU, kWaves> P;
     typedef Side<DT, TQ, false, kTileM, MT, kWaves> Q;
     static constexpr uint32_t kStage = P::kBytes + Q::kBytes, kLds = STAGES * kStage, kLoads = P::kLoads + Q::kLoads, kRed = P::kRed;
     typedef Sum<DT> Acc[NU][MT];
@@ -188,7 +183,7 @@ struct Tile {
     __device__ __forceinline__ uint32_t n(int u) const
     {
         const uint32_t part = threadIdx.x % 64u / 16u;
-        return n0 + wave_id() % WN * (16u * NU) + (TP ? u * 16u + part * 4u : part * (4u * NU) + u * 4u);
+        return n0 + wave_id() % WN * (16u * NU) + (PAIRS ? u / 2 * 32u + part * 8u + u % 2 * 4u : u * 16u + part * 4u);
     }
     __device__ __forceinline__ uint32_t m(int t) const { return m0 + wave_id() / WN * (16u * MT) + t * 16u + threadIdx.x % 16u; }
 
@@ -221,8 +216,8 @@ struct Tile {
         const uint32_t s0 = (uint32_t)((uint64_t)stages * part / a.split), count = (uint32_t)((uint64_t)stages * (part + 1u) / a.split) - s0;
         // Where P is read once, by one row of tiles, every workgroup begins at another stage: rows are usually a power of two of bytes
         // apart, and workgroups in step would ask the same memory channels at a time.
-        uint32_t to_fill = s0;
-        if (!TP && a.q.rows <= kTileM && count) to_fill = s0 + n0 / kTileN % count;
+        const uint32_t first = !TP && a.q.rows <= kTileM && count ? s0 + n0 / kTileN % count : s0;
+        uint32_t to_fill = first;
         auto fill = [&](char *to) {
             p.fill(to_fill * kRed, a.red, to);
             q.fill(to_fill * kRed, a.red, to + P::kBytes);
@@ -231,33 +226,54 @@ struct Tile {
 #pragma unroll
         for (int b = 0; b < STAGES - 1; ++b)
             if (b < (int)count) fill(lds + b * kStage);
-        uint32_t now = 0, next = (STAGES - 1) * kStage;
+        // Two halves of a stage, in registers: while one is multiplied the other is read, and the second half of a stage is multiplied behind
+        // the barrier that the next stage is waited for at.
+        v4i p0[NU], q0[MT], p1[NU], q1[MT];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) p1[u] = v4i{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < MT; ++t) q1[t] = v4i{0, 0, 0, 0};
+        uint32_t now = 0, next = (STAGES - 1) * kStage, at = first;
         for (uint32_t j = 0; j < count; ++j) {
             // (towards the end there are no newer stages to leave under way)
             if (STAGES == 2 || j + STAGES - 1 > count) stage_barrier<0>();
             else stage_barrier<(STAGES - 2) * kLoads>();
+            if (a.red - at * kRed < kRed && (a.red * kSize<DT>) % 16u) {
+                P::clear(a.red - at * kRed, lds + now);
+                Q::clear(a.red - at * kRed, lds + now + P::kBytes);
+                stage_barrier<0>();
+            }
+            at = at + 1u == s0 + count ? s0 : at + 1u;
             if (j + STAGES - 1u < count) fill(lds + next);
-            step(lds + now, rp, rq, acc);
+            half(lds + now, rp, rq, 0, p0, q0, p1, q1, acc);
+            half(lds + now, rp, rq, 1, p1, q1, p0, q0, acc);
             now = now == (STAGES - 1) * kStage ? 0u : now + kStage;
             next = next == (STAGES - 1) * kStage ? 0u : next + kStage;
         }
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[u][t] = multiply<DT>(p1[u], q1[t], acc[u][t]);
     }
 
-    static __device__ __forceinline__ void step(const char *lds, const typename P::Reader &rp, const typename Q::Reader &rq, Acc &acc)
+    // Reads half `sub` of a stage into p and q and multiplies what was read before, one behind the other.
+    static __device__ __forceinline__ void half(const char *lds, const typename P::Reader &rp, const typename Q::Reader &rq, int sub, v4i (&p)[NU], v4i (&q)[MT],
+                                                const v4i (&before_p)[NU], const v4i (&before_q)[MT], Acc &acc)
     {
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            v4i q[MT];
+        for (int t = 0; t < MT; ++t) q[t] = rq(lds + P::kBytes, t, sub);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) q[t] = rq(lds + P::kBytes, t, sub);
-            v4i p = rp(lds, 0, sub);
+        for (int u = 0; u < NU; ++u) p[u] = rp(lds, u, sub);
 #pragma unroll
-            for (int u = 0; u < NU; ++u) {
-                const v4i ahead = u + 1 < NU ? rp(lds, u + 1, sub) : p;
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
-                for (int t = 0; t < MT; ++t) acc[u][t] = multiply<DT>(p, q[t], acc[u][t]);
-                p = ahead;
-            }
+            for (int t = 0; t < MT; ++t) acc[u][t] = multiply<DT>(before_p[u], before_q[t], acc[u][t]);
+        constexpr int kReads = NU * P::Reader::kReads + MT * Q::Reader::kReads, kProducts = NU * MT * (DT == RS_DTYPE_F32 ? 4 : 1);
+        constexpr int kGroups = NU + MT;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            __builtin_amdgcn_sched_group_barrier(0x100, kReads / kGroups, 0);           // reads of LDS
+            __builtin_amdgcn_sched_group_barrier(0x008, kProducts / kGroups, 0);        // products
         }
     }
 };
@@ -269,6 +285,21 @@ template <int DT> __device__ __forceinline__ void store_row(void *y, int64_t at,
     else
 #pragma unroll
         for (int j = 0; j < 4; ++j) if (n + j < N) put<DT>(y, at + n + j, a[j]);
+}
+
+// A lane's values of one row of a tile: v[u] are those of fragment u.
+template <int DT, class T> __device__ __forceinline__ void store_tile_row(const T &tile, void *y, int64_t at, uint32_t N, const v4f (&v)[T::NU])
+{
+    if constexpr (T::PAIRS && DT != RS_DTYPE_F32) {
+#pragma unroll
+        for (int u = 0; u < T::NU; u += 2) {
+            const uint32_t n = tile.n(u);
+            if (n + 8u <= N) put_wide<DT>(y, at + n, v[u], v[u + 1]);
+            else { store_row<DT>(y, at, n, N, v[u]); store_row<DT>(y, at, n + 4u, N, v[u + 1]); }
+        }
+    } else
+#pragma unroll
+        for (int u = 0; u < T::NU; ++u) store_row<DT>(y, at, tile.n(u), N, v[u]);
 }
 
 }  // namespace rs
