@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void embedding_kernel(EmbeddingParams p)
         if (token >= 0 && token < (int64_t)p.V) {
             table8<WT>(p, token, k, x);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] *= p.scale;
+            for (int j = 0; j < 8; ++j) x[j] = in_float32(x[j] * p.scale);
         } else
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = token < 0 ? 0.0f : __builtin_nanf("");

@@ -198,7 +198,7 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Params p)
         const float f = XT < 0 ? p.x_scale[row] : ((const float *)(lds + p.M * (blocks * 128u)))[row];
         v4f y;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = (float)s[j] * (f * p.w_scale[min(n + j, p.N - 1u)]);
+        for (int j = 0; j < 4; ++j) y[j] = in_float32((float)s[j] * (f * p.w_scale[min(n + j, p.N - 1u)]));
         store_row<DT>(p.y, (int64_t)row * p.y_stride, n, p.N, y);
     }
 }
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void int8_tile_kernel(Int8Params p
 #pragma unroll
         for (int u = 0; u < T::NU; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[u][j] = (float)acc[u][t][j] * (f * p.w_scale[min(tile.n(u) + j, p.N - 1u)]);
+            for (int j = 0; j < 4; ++j) y[u][j] = in_float32((float)acc[u][t][j] * (f * p.w_scale[min(tile.n(u) + j, p.N - 1u)]));
         store_tile_row<DT>(tile, p.y, (int64_t)m * p.y_stride, p.N, y);
     }
 }

@@ -59,6 +59,13 @@ template <int DT> __device__ __forceinline__ void put(void *p, int64_t i, float 
 
 __device__ __forceinline__ float block_scale(float peak) { return fmaxf(peak * (1.0f / 448.0f), 0x1p-126f); }
 
+// A product in float32, rounded to it also where the next step rounds to float16 (one instruction would do both at once, with one rounding).
+__device__ __forceinline__ float in_float32(float v)
+{
+    asm("" : "+v"(v));
+    return v;
+}
+
 // x / scale, rounded once: the quotient by way of the reciprocal, and what it is off by divided once more.  Of small blocks both
 // are taken 2^64 times as large, which is exact: what the quotient is off by, some 2^-24 of x, would be below float32's range.
 // (Compared with the division on the CPU, for every significand of the scale and the five numbers about each point halfway between two

@@ -861,12 +861,16 @@ std::tuple<at::Tensor, at::Tensor> loss_backward(const at::Tensor &x, const at::
     return {gx, gw};
 }
 
+// (what is not wanted is left out: a function has no undefined outputs)
 struct LossBackward : torch::autograd::Function<LossBackward> {
-    static variable_list forward(AutogradContext *ctx, at::Tensor x, at::Tensor weight, at::Tensor tokens, at::Tensor stats, double temperature, bool want_x,
+    static variable_list forward(AutogradContext *, at::Tensor x, at::Tensor weight, at::Tensor tokens, at::Tensor stats, double temperature, bool want_x,
                                  bool want_w, std::optional<at::Tensor> g, std::optional<at::Tensor> h)
     {
         const auto [gx, gw] = loss_backward(x, weight, tokens, stats, temperature, want_x, want_w, g.value_or(at::Tensor()), h.value_or(at::Tensor()));
-        return {gx, gw};
+        variable_list made;
+        if (want_x) made.push_back(gx);
+        if (want_w) made.push_back(gw);
+        return made;
     }
     static variable_list backward(AutogradContext *, variable_list)
     {
@@ -891,10 +895,11 @@ struct Loss : torch::autograd::Function<Loss> {
         const auto saved = ctx->get_saved_variables();
         const double temperature = ctx->saved_data["temperature"].toDouble();
         const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+        if (!want_x && !want_w) return {none, none, none, none};
         if (at::GradMode::is_enabled()) {
             auto given = [&](int i) { return grads[i].defined() ? std::optional<at::Tensor>(grads[i]) : std::nullopt; };
             const variable_list o = LossBackward::apply(saved[0], saved[1], saved[2], saved[3], temperature, want_x, want_w, given(0), given(1));
-            return {o[0], o[1], none, none};
+            return {want_x ? o[0] : none, want_w ? o[want_x] : none, none, none};
         }
         const auto [gx, gw] = loss_backward(saved[0], saved[1], saved[2], saved[3], temperature, want_x, want_w, grads[0], grads[1]);
         return {gx, gw, none, none};
