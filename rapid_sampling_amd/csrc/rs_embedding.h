@@ -3,8 +3,7 @@
 //   y[i] = s w[t_i]          dw[v] = s sum over i with t_i = v of g_i, in the order of i, in float32
 //
 // The gradient's positions are put in the order of their tokens first (a radix sort that keeps the order of equal ones), so that a row of
-// dw is one stretch of them: no floating-point atomics, and the same sums every time.  Rows without a token are written as zeros by
-// the same pass.  Bound by memory: y and g once, dw once.
+// dw is one stretch of them: no floating-point atomics, and the same sums every time.  Bound by memory: y and g once, dw once.
 #pragma once
 
 #include "rs_linear.h"
@@ -33,6 +32,38 @@ struct EmbeddingParams {
     uint32_t     M, V, K;
     uint32_t     width;              // log2 of the threads of a row
 };
+
+// Eight values of a row as they lie in memory, and widened.  Reading and widening are apart so that several reads are under way at a
+// time.  A thread has the columns from k on, the last of a row the last eight of it: what two threads have both is the same in both.
+template <int DT> struct Eight { v4i v[DT == RS_DTYPE_F32 ? 2 : 1]; };
+__device__ __forceinline__ uint32_t eight_from(uint32_t k, uint32_t K) { return K >= 8u ? min(k, K - 8u) : 0u; }
+template <int DT> __device__ __forceinline__ Eight<DT> read8(const void *base, int64_t at, uint32_t k, uint32_t K)
+{
+    Eight<DT> r;
+    const char *p = (const char *)base + (at + k) * (DT == RS_DTYPE_F32 ? 4 : 2);
+    if (K >= 8u) __builtin_memcpy(&r, p, sizeof(r));
+    else {
+        uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t j = 0; j < 7; ++j)
+            if (j < K) {
+                if constexpr (DT == RS_DTYPE_F32) w[j] = ((const uint32_t *)p)[j];
+                else w[j / 2] |= (uint32_t)((const uint16_t *)p)[j] << (16 * (j % 2));
+            }
+        __builtin_memcpy(&r, w, sizeof(r));
+    }
+    return r;
+}
+template <int DT> __device__ __forceinline__ void widen8(const Eight<DT> &r, float (&x)[8])
+{
+    if constexpr (DT == RS_DTYPE_F32) __builtin_memcpy(x, &r, 32);
+    else {
+        uint16_t v[8];
+        __builtin_memcpy(v, &r, 16);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = DT == RS_DTYPE_BF16 ? __uint_as_float((uint32_t)v[j] << 16) : (float)__builtin_bit_cast(_Float16, v[j]);
+    }
+}
 
 // Eight values of a row of the table from column k on.
 template <int WT>
@@ -90,7 +121,7 @@ __global__ __launch_bounds__(256) void embedding_kernel(EmbeddingParams p)
 // -------------------------------------------------------------------- order --
 // A digit of up to 11 bits at a time.  A workgroup of 16 waves takes a stretch of the list, each wave a part of it, 64 tokens at
 // a time; a counter for each digit and wave in LDS.
-constexpr uint32_t kSortWaves = 16, kSortThreads = 64 * kSortWaves, kSortBits = 11, kSortTile = 8192, kSortAlone = 16384;
+constexpr uint32_t kSortBatch = 8, kSortWaves = 16, kSortThreads = 64 * kSortWaves, kSortBits = 11, kSortTile = 8192, kSortAlone = 16384;
 
 struct SortParams {
     TokenList       tokens;          // of the first digit: what is sorted; a token that is none counts as V
@@ -123,20 +154,30 @@ template <bool PLACE>
 __device__ __forceinline__ void sort_part(const SortParams &p, uint32_t from, uint32_t to, uint32_t *counts)
 {
     const uint32_t lane = threadIdx.x % 64u, mask = (1u << p.bits) - 1u;
-    for (uint32_t i0 = from; i0 < to; i0 += 64u) {
-        const uint32_t i = i0 + lane;
-        const bool live = i < to;
-        const uint32_t key = live ? sort_key(p, i) : 0u, digit = key >> p.shift & mask;
-        const uint64_t same = same_digit(digit, p.bits, live);
-        const uint32_t before = __popcll(same & ((1ull << lane) - 1ull));
-        const uint32_t have = live ? counts[digit] : 0u;
-        if (PLACE && live) {
-            p.keys[have + before] = key;
-            p.at[have + before] = p.first ? i : p.at_in[i];
+    for (uint32_t i0 = from; i0 < to; i0 += 64u * kSortBatch) {
+        // (a batch's tokens are asked for at once: each would cost a trip to memory by itself)
+        uint32_t keys[kSortBatch], at[kSortBatch];
+#pragma unroll
+        for (uint32_t e = 0; e < kSortBatch; ++e) {
+            const uint32_t i = i0 + e * 64u + lane;
+            keys[e] = i < to ? sort_key(p, i) : 0u;
+            at[e] = PLACE && i < to ? (p.first ? i : p.at_in[i]) : 0u;
         }
-        __builtin_amdgcn_wave_barrier();
-        if (live && before == 0) counts[digit] = have + (uint32_t)__popcll(same);
-        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (uint32_t e = 0; e < kSortBatch; ++e) {
+            const bool live = i0 + e * 64u + lane < to;
+            const uint32_t digit = keys[e] >> p.shift & mask;
+            const uint64_t same = same_digit(digit, p.bits, live);
+            const uint32_t before = __popcll(same & ((1ull << lane) - 1ull));
+            const uint32_t have = live ? counts[digit] : 0u;
+            if (PLACE && live) {
+                p.keys[have + before] = keys[e];
+                p.at[have + before] = at[e];
+            }
+            __builtin_amdgcn_wave_barrier();
+            if (live && before == 0) counts[digit] = have + (uint32_t)__popcll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 }
 // The stretch of this wave.
@@ -176,11 +217,33 @@ __device__ __forceinline__ uint32_t sums_before(uint32_t v, uint32_t *held, uint
     return before + s - v;
 }
 
-// Up to kSortAlone tokens, by one workgroup, all digits.
-__global__ __launch_bounds__(1024) void sort_alone_kernel(SortParams p)
+// dw is cleared first, all of it, and the rows that have a token written once more: they are few next to a vocabulary.
+struct ClearParams {
+    char    *at;
+    uint64_t bytes;
+};
+__device__ __forceinline__ void clear_part(const ClearParams &c, uint32_t group, uint32_t groups)
+{
+    const uint32_t head = (uint32_t)min((uint64_t)(-(uintptr_t)c.at & 15u), c.bytes);
+    const uint64_t pieces = (c.bytes - head) / 16u;
+    for (uint64_t i = (uint64_t)group * kSortThreads + threadIdx.x; i < pieces; i += (uint64_t)groups * kSortThreads)
+        *(uint4 *)(c.at + head + i * 16u) = make_uint4(0u, 0u, 0u, 0u);
+    if (group == 0 && threadIdx.x < 32u) {
+        const uint64_t at = threadIdx.x < 16u ? threadIdx.x : head + pieces * 16u + threadIdx.x - 16u;
+        if (threadIdx.x < 16u ? at < head : at < c.bytes) c.at[at] = 0;
+    }
+}
+__global__ __launch_bounds__(1024) void clear_kernel(ClearParams c) { clear_part(c, blockIdx.x, gridDim.x); }
+
+// Up to kSortAlone tokens, by one workgroup, all digits; the others of the launch clear dw meanwhile.
+__global__ __launch_bounds__(1024) void sort_alone_kernel(SortParams p, ClearParams c)
 {
     extern __shared__ uint32_t counts[];
     __shared__ uint32_t held[kSortWaves];
+    if (blockIdx.x) {
+        clear_part(c, blockIdx.x - 1u, gridDim.x - 1u);
+        return;
+    }
     for (uint32_t d = 0; d < p.digits; ++d) {
         sort_count(p, 0, p.N, counts);
         uint32_t from, to, base = 0, total;
@@ -201,8 +264,8 @@ __global__ __launch_bounds__(1024) void sort_alone_kernel(SortParams p)
         __syncthreads();
         sort_stretch(0, p.N, from, to);
         sort_part<true>(p, from, to, counts + ((threadIdx.x / 64u) << p.bits));
-        // the next digit reads what the other waves have written
-        __threadfence();
+        // the next digit reads what the other waves of this workgroup have written
+        __threadfence_block();
         __syncthreads();
         p.first = 0;
         p.shift += p.bits;
@@ -261,90 +324,103 @@ __global__ __launch_bounds__(1024) void sort_place_kernel(SortParams p)
 }
 
 // --------------------------------------------------------------------- sums --
+// The sorted places are cut into chunks of one size, whatever their tokens; a workgroup sums those of one chunk, for 2048 columns.  A
+// token whose places lie within a chunk is written at once.  One that goes on into the next leaves a part, and so does every
+// chunk that it comes from another into; a second launch joins these in their order.
 struct TableGradParams {
     const uint32_t *keys, *at;       // sorted by token
     const void     *g;
     int64_t         g_stride;        // elements
-    float          *parts;           // sums of whole chunks of one token, [chunk][K]
+    float          *parts;           // [chunk][2][K]: of the token that comes from the chunk before; of the one that goes on
     void           *dw;
     float           scale;
-    uint32_t        N, V, K, chunk;  // log2 of a chunk's tokens
-    uint32_t        width;           // log2 of the threads of a row
+    uint32_t        N, V, K, chunk;  // chunk: log2 of a chunk's places
 };
 
-// The sum of g's rows at the sorted places a .. b - 1, eight columns from k on; loads of eight rows under way at a time.
-template <int GT>
-__device__ __forceinline__ void add_rows(const TableGradParams &p, uint32_t a, uint32_t b, uint32_t k, float (&s)[8])
+template <int DT>
+__device__ __forceinline__ void table_row(const TableGradParams &p, uint32_t token, uint32_t k, const float (&s)[8])
 {
-    for (; a < b; a += 8u) {
-        float x[8][8];
+    float y[8];
 #pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) load8<GT>(p.g, (int64_t)p.at[min(a + e, b - 1u)] * p.g_stride, k, a + e < b ? p.K : 0u, x[e]);
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] += x[e][j];
-    }
+    for (int j = 0; j < 8; ++j) y[j] = s[j] * p.scale;
+    store8<DT>(p.dw, (int64_t)token * p.K, k, p.K, y);
 }
 
-// A chunk of the sorted places that holds one token only: its sum, for a row that is much longer than the others.
-template <int GT>
+template <int GT, int DT>
 __global__ __launch_bounds__(256) void table_chunk_kernel(TableGradParams p)
 {
-    const uint32_t first = blockIdx.x << p.chunk, k = (blockIdx.y * 256u + threadIdx.x) * 8u;
-    const uint32_t token = p.keys[first];
-    if (token >= p.V || token != p.keys[first + (1u << p.chunk) - 1u] || k >= p.K) return;
+    const uint32_t first = blockIdx.x << p.chunk, last = min(first + (1u << p.chunk), p.N), own = (blockIdx.y * 256u + threadIdx.x) * 8u;
+    if (own >= p.K) return;
+    const uint32_t k = eight_from(own, p.K);
+    const bool goes_on = last < p.N && p.keys[last] == p.keys[last - 1u];
+    uint32_t token = p.keys[first];
+    bool from_before = first > 0u && p.keys[first - 1u] == token;
     float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    add_rows<GT>(p, first, first + (1u << p.chunk), k, s);
-    store8<RS_DTYPE_F32>(p.parts, (int64_t)blockIdx.x * p.K, k, p.K, s);
+    auto leave = [&](bool to_next) {
+        if (token >= p.V) return;
+        if (from_before || to_next) store8<RS_DTYPE_F32>(p.parts, ((int64_t)blockIdx.x * 2 + (from_before ? 0 : 1)) * p.K, k, p.K, s);
+        else table_row<DT>(p, token, k, s);
+    };
+    // (the keys and places are the same for the whole workgroup; behind the last place: its token once more, not added)
+    constexpr uint32_t kBatch = 16;
+    for (uint32_t i = first; i < last; i += kBatch) {
+        Eight<GT> x[kBatch];
+        uint32_t keys[kBatch], at[kBatch];
+#pragma unroll
+        for (uint32_t e = 0; e < kBatch; ++e) { keys[e] = p.keys[min(i + e, last - 1u)]; at[e] = p.at[min(i + e, last - 1u)]; }
+#pragma unroll
+        for (uint32_t e = 0; e < kBatch; ++e) x[e] = read8<GT>(p.g, (int64_t)at[e] * p.g_stride, k, p.K);
+#pragma unroll
+        for (uint32_t e = 0; e < kBatch; ++e) {
+            if (keys[e] != token) {
+                leave(false);
+                token = keys[e];
+                from_before = false;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[j] = 0.0f;
+            }
+            float v[8];
+            widen8<GT>(x[e], v);
+            if (i + e < last)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[j] += v[j];
+        }
+    }
+    leave(goes_on);
 }
 
-// Fifteen rows of dw: sixteen threads look for where each of them begins in the sorted tokens, and where the last ends.
-constexpr uint32_t kTableRows = 15;
-template <int GT, int DT>
-__global__ __launch_bounds__(256) void table_grad_kernel(TableGradParams p)
+// The chunk in which a token begins that goes on into the next joins its parts.
+template <int DT>
+__global__ __launch_bounds__(256) void table_join_kernel(TableGradParams p)
 {
-    __shared__ uint32_t begins[kTableRows + 1];
-    const uint32_t v0 = blockIdx.x * kTableRows;
-    {
-        // the first place whose token is `wanted` or more lies in lo .. hi; sixteen places between them are looked at at a time
-        const uint32_t wanted = v0 + threadIdx.x / 16u, lane = threadIdx.x % 16u, group = threadIdx.x % 64u / 16u;
-        uint32_t lo = 0, hi = p.N;
-        while (lo < hi) {
-            const uint32_t step = (hi - lo + 15u) / 16u, at = lo + lane * step;
-            const bool less = at < hi && p.keys[at] < wanted;
-            const uint32_t n = __popcll(__ballot(less) >> (16u * group) & 0xFFFFull);
-            // the first n of them are less: it lies behind the n-th, and not behind the one after it
-            if (n == 0) hi = lo;
-            else {
-                hi = min(hi, lo + n * step);
-                lo = lo + (n - 1u) * step + 1u;
-            }
-        }
-        if (lane == 0) begins[threadIdx.x / 16u] = lo;
-    }
-    __syncthreads();
-    const uint32_t C = 1u << p.chunk;
-    for (uint32_t r = threadIdx.x >> p.width; r < kTableRows && v0 + r < p.V; r += 256u >> p.width) {
-        const uint32_t a = begins[r], b = begins[r + 1u];
-        for (uint32_t k = (threadIdx.x & ((1u << p.width) - 1u)) * 8u; k < p.K; k += 8u << p.width) {
-            float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            const uint32_t c0 = (a + C - 1u) >> p.chunk, c1 = b >> p.chunk;        // the whole chunks in between
-            if (c0 < c1) {
-                add_rows<GT>(p, a, c0 << p.chunk, k, s);
-                for (uint32_t c = c0; c < c1; ++c) {
-                    float x[8];
-                    load8<RS_DTYPE_F32>(p.parts, (int64_t)c * p.K, k, p.K, x);
+    const uint32_t C = 1u << p.chunk, c0 = blockIdx.x, first = c0 << p.chunk, last = first + C, own = (blockIdx.y * 256u + threadIdx.x) * 8u;
+    if (last >= p.N) return;
+    const uint32_t token = p.keys[last - 1u];
+    if (token >= p.V || p.keys[last] != token || (first > 0u && p.keys[first - 1u] == token) || own >= p.K) return;
+    const uint32_t k = eight_from(own, p.K);
+    float s[8];
+    widen8<RS_DTYPE_F32>(read8<RS_DTYPE_F32>(p.parts, ((int64_t)c0 * 2 + 1) * p.K, k, p.K), s);
+    for (uint32_t c = c0 + 1u; ; c += 8u) {
+        Eight<RS_DTYPE_F32> x[8];
+        bool there[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) s[j] += x[j];
-                }
-                add_rows<GT>(p, c1 << p.chunk, b, k, s);
-            } else add_rows<GT>(p, a, b, k, s);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] *= p.scale;
-            store8<DT>(p.dw, (int64_t)(v0 + r) * p.K, k, p.K, s);
+        for (uint32_t e = 0; e < 8; ++e) {
+            const uint64_t at = (uint64_t)(c + e) << p.chunk;
+            there[e] = at < p.N && p.keys[min(at, (uint64_t)p.N - 1u)] == token;
         }
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) x[e] = read8<RS_DTYPE_F32>(p.parts, (int64_t)(there[e] ? c + e : c0) * 2 * p.K, k, p.K);
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            float v[8];
+            widen8<RS_DTYPE_F32>(x[e], v);
+            if (there[e])
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[j] += v[j];
+        }
+        if (!there[7]) break;
     }
+    table_row<DT>(p, token, k, s);
 }
 
 }  // namespace rs

@@ -30,7 +30,7 @@ template <int WT> static void launch_embedding(const EmbeddingParams &p, int32_t
 // Where a gradient's scratch lies.
 struct TableSpace {
     uint64_t keys[2], at[2], counts, parts, bytes = 0;
-    uint32_t digits, bits, chunk, groups;
+    uint32_t digits, bits, chunk, chunks, groups;
     uint64_t take(uint64_t n) { const uint64_t a = bytes; bytes += up(n, 256); return a; }
 };
 static TableSpace table_space(uint32_t N, uint32_t V, uint32_t K)
@@ -41,23 +41,27 @@ static TableSpace table_space(uint32_t N, uint32_t V, uint32_t K)
     s.digits = (bits + kSortBits - 1) / kSortBits;
     s.bits = (bits + s.digits - 1) / s.digits;
     s.groups = N <= kSortAlone ? 1 : (N + kSortTile - 1) / kSortTile;
-    // chunks of about the square root of the tokens: a token that makes up all of them has as many chunks to add as each has rows
-    s.chunk = 5;
-    while (s.chunk < 12 && (1ull << (2 * s.chunk + 2)) <= N) ++s.chunk;
+    // Chunks of up to about the square root of the tokens: a token that makes up all of them has as many chunks to join as each has places.
+    s.chunk = 4;
+    while (s.chunk < 12 && (1ull << (2 * s.chunk + 4)) <= N) ++s.chunk;
+    s.chunks = (N + (1u << s.chunk) - 1) >> s.chunk;
     for (int i = 0; i < 2; ++i) { s.keys[i] = s.take(4ull * N); s.at[i] = s.take(4ull * N); }
     s.counts = s.take(N <= kSortAlone ? 0 : 4ull * s.groups << s.bits);
-    s.parts = s.take((uint64_t)(N >> s.chunk) * K * 4);
+    s.parts = s.take((uint64_t)s.chunks * 2 * K * 4);
     return s;
 }
 
-template <int GT> static void launch_sums(const TableGradParams &p, int32_t dtype, hipStream_t st)
+template <int GT, int DT> static void launch_sums(const TableGradParams &p, uint32_t chunks, hipStream_t st)
 {
-    if (p.N >> p.chunk)
-        hipLaunchKernelGGL(table_chunk_kernel<GT>, dim3(p.N >> p.chunk, (p.K + 2047) / 2048), dim3(256), 0, st, p);
-    const dim3 groups((p.V + kTableRows - 1) / kTableRows), threads(256);
-    if (dtype == RS_DTYPE_F32) hipLaunchKernelGGL((table_grad_kernel<GT, RS_DTYPE_F32>), groups, threads, 0, st, p);
-    else if (dtype == RS_DTYPE_BF16) hipLaunchKernelGGL((table_grad_kernel<GT, RS_DTYPE_BF16>), groups, threads, 0, st, p);
-    else hipLaunchKernelGGL((table_grad_kernel<GT, RS_DTYPE_F16>), groups, threads, 0, st, p);
+    const dim3 groups(chunks, (p.K + 2047) / 2048);
+    hipLaunchKernelGGL((table_chunk_kernel<GT, DT>), groups, dim3(256), 0, st, p);
+    if (chunks > 1) hipLaunchKernelGGL(table_join_kernel<DT>, groups, dim3(256), 0, st, p);
+}
+template <int GT> static void launch_sums(const TableGradParams &p, uint32_t chunks, int32_t dtype, hipStream_t st)
+{
+    if (dtype == RS_DTYPE_F32) launch_sums<GT, RS_DTYPE_F32>(p, chunks, st);
+    else if (dtype == RS_DTYPE_BF16) launch_sums<GT, RS_DTYPE_BF16>(p, chunks, st);
+    else launch_sums<GT, RS_DTYPE_F16>(p, chunks, st);
 }
 
 static bool known(int32_t dtype) { return dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16 || dtype == RS_DTYPE_F16; }
@@ -114,10 +118,13 @@ int rs_embedding_backward(const void *tokens, int32_t tokens_64, int64_t token_s
     p.N = (uint32_t)M; p.V = (uint32_t)V; p.bits = s.bits; p.first = 1; p.digits = s.digits;
     p.counts = (uint32_t *)(ws + s.counts);
     const uint32_t lds = (kSortWaves << s.bits) * 4;
+    const ClearParams clear{(char *)dw, (uint64_t)V * K * size_of(dw_dtype)};
+    const uint32_t clears = (uint32_t)std::min<uint64_t>(1023, clear.bytes / 65536 + 1);
     if (p.N <= kSortAlone) {
         p.keys = keys(0); p.at = at(0); p.keys_b = keys(1); p.at_b = at(1);
-        hipLaunchKernelGGL(sort_alone_kernel, dim3(1), dim3(kSortThreads), lds, st, p);
-    } else
+        hipLaunchKernelGGL(sort_alone_kernel, dim3(1 + clears), dim3(kSortThreads), lds, st, p, clear);
+    } else {
+        hipLaunchKernelGGL(clear_kernel, dim3(clears), dim3(kSortThreads), 0, st, clear);
         for (uint32_t d = 0; d < s.digits; ++d) {
             p.keys = keys(d & 1); p.at = at(d & 1);
             hipLaunchKernelGGL(sort_count_kernel, dim3(s.groups), dim3(kSortThreads), lds, st, p);
@@ -125,13 +132,14 @@ int rs_embedding_backward(const void *tokens, int32_t tokens_64, int64_t token_s
             hipLaunchKernelGGL(sort_place_kernel, dim3(s.groups), dim3(kSortThreads), lds, st, p);
             p.first = 0; p.shift += s.bits; p.keys_in = p.keys; p.at_in = p.at;
         }
+    }
     TableGradParams t;
     t.keys = keys((s.digits - 1) & 1); t.at = at((s.digits - 1) & 1);
     t.g = g; t.g_stride = M > 1 ? g_stride : 0; t.parts = (float *)(ws + s.parts); t.dw = dw; t.scale = (float)scale;
-    t.N = p.N; t.V = p.V; t.K = (uint32_t)K; t.chunk = s.chunk; t.width = row_width(t.K);
-    if (g_dtype == RS_DTYPE_F32) launch_sums<RS_DTYPE_F32>(t, dw_dtype, st);
-    else if (g_dtype == RS_DTYPE_BF16) launch_sums<RS_DTYPE_BF16>(t, dw_dtype, st);
-    else launch_sums<RS_DTYPE_F16>(t, dw_dtype, st);
+    t.N = p.N; t.V = p.V; t.K = (uint32_t)K; t.chunk = s.chunk;
+    if (g_dtype == RS_DTYPE_F32) launch_sums<RS_DTYPE_F32>(t, s.chunks, dw_dtype, st);
+    else if (g_dtype == RS_DTYPE_BF16) launch_sums<RS_DTYPE_BF16>(t, s.chunks, dw_dtype, st);
+    else launch_sums<RS_DTYPE_F16>(t, s.chunks, dw_dtype, st);
     return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
 }
 
