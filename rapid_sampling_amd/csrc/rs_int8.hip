@@ -51,6 +51,14 @@ template <int DT, int WN, int WM, int NU, int MT, int STAGES, bool SPLIT> static
     hipLaunchKernelGGL((int8_tile_kernel<DT, WN, WM, NU, MT, STAGES, SPLIT>), dim3((uint32_t)(tiles * p.a.split)), dim3(T::kThreads), T::kLds, st, p);
 }
 
+// (instantiated by name: the compiler leaves some of those that are only launched without their host side)
+#define RS_KERNELS(DT)                                                                     \
+    template __global__ void int8_tile_kernel<DT, 2, 4, 8, 4, 2, false>(Int8Params);        \
+    template __global__ void int8_tile_kernel<DT, 2, 2, 4, 2, 3, true>(Int8Params);
+RS_KERNELS(RS_DTYPE_F32)
+RS_KERNELS(RS_DTYPE_BF16)
+RS_KERNELS(RS_DTYPE_F16)
+
 template <int DT> static void launch_product(const Int8Params &p, hipStream_t st)
 {
     // (the tiles' kernel reaches its rows with 32 bits)
@@ -115,10 +123,9 @@ int rs_linear_int8(const int8_t *x, int64_t x_row_stride, const float *x_scale, 
         return RS_ERR_ALIGN;
     const Int8Params p = int8_params(x, x_row_stride, x_scale, w, w_row_stride, w_scale, M, N, K, y, y_row_stride, workspace);
     const hipStream_t st = (hipStream_t)stream;
-    // (float16 first: the compiler leaves the last of them without its host side otherwise)
-    if (y_dtype == RS_DTYPE_F16) launch_product<RS_DTYPE_F16>(p, st);
+    if (y_dtype == RS_DTYPE_F32) launch_product<RS_DTYPE_F32>(p, st);
     else if (y_dtype == RS_DTYPE_BF16) launch_product<RS_DTYPE_BF16>(p, st);
-    else launch_product<RS_DTYPE_F32>(p, st);
+    else launch_product<RS_DTYPE_F16>(p, st);
     return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
 }
 

@@ -63,11 +63,24 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_tile_kernel(LossParams p)
         for (int u = 0; u < T::NU; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float z = whole || tile.n(u) + j < V ? acc[u][t][j] * p.c : -__builtin_inff();
-                acc[u][t][j] = z;
-                if ((int64_t)(tile.n(u) + j) == token) p.target[m] = z;
-                top = fmaxf(top, z);
+                acc[u][t][j] = whole || tile.n(u) + j < V ? acc[u][t][j] * p.c : -__builtin_inff();
+                top = fmaxf(top, acc[u][t][j]);
             }
+        // (few stretches hold the token of any of their rows)
+        const bool here = token >= 0 && token < (int64_t)V && (uint32_t)token / (16u * T::NU) == stretch;
+        if (__any(here)) {
+            float z = 0.0f;
+            bool mine = false;
+#pragma unroll
+            for (int u = 0; u < T::NU; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool it = here && tile.n(u) + j == (uint32_t)token;
+                    z = it ? acc[u][t][j] : z;
+                    mine = mine || it;
+                }
+            if (mine) p.target[m] = z;
+        }
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         const float from = top == -__builtin_inff() ? 0.0f : top;

@@ -18,8 +18,13 @@ struct LossSpace {
     uint64_t take(uint64_t n) { const uint64_t at = bytes; bytes += up(n, 256); return at; }
 };
 
-// Large tiles where there are more than enough to go round.
-static bool large(uint64_t rows, uint64_t columns) { return rows > 128 && up(rows, 256) / 256 * (up(columns, 256) / 256) >= 192; }
+// Which tiles: of 256 x 256 where there are enough of them to go round, of 128 x 128 for more than 64 rows, else of 128 x 64 (columns x rows).
+enum Size { kSmall, kMiddle, kLarge };
+static Size size_for(uint64_t rows, uint64_t columns)
+{
+    if (rows > 128 && up(rows, 256) / 256 * (up(columns, 256) / 256) >= 192) return kLarge;
+    return rows > 64 ? kMiddle : kSmall;
+}
 
 // A piece of the vocabulary: G of the piece stays within the last cache (256 MB) with the piece's weights, in steps of 256 tokens and
 // at least 8192, so that the sums of dx that each piece reads and writes again (8 bytes) are little next to its products.
@@ -37,10 +42,11 @@ static LossSpace loss_space(int32_t M, int32_t V, int32_t K, int32_t dtype, bool
     s.piece = (uint32_t)std::min<uint64_t>(up(V, 256), std::max<uint64_t>(8192, ((1ull << 27) / (M * size)) / 256 * 256));
     s.grad_stride = s.piece * size + 256;              // (not a power of two: rows would share their memory channels)
     s.grad = s.take((uint64_t)M * s.grad_stride);
-    const bool big = large(M, K);
-    const uint64_t tiles = big ? up(M, 256) / 256 * (up(K, 256) / 256) : up(M, 64) / 64 * (up(K, 128) / 128);
-    const uint64_t stages = s.piece * size / kRowBytes;
-    s.split = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(big ? 256 : 512) / tiles, stages / 8, 32}));
+    // dx has few tiles: their reduction over the piece is shared out among up to one (two) workgroups to a compute unit
+    const Size tile = size_for(M, K);
+    const uint64_t high = tile == kLarge ? 256 : tile == kMiddle ? 128 : 64, wide = tile == kLarge ? 256 : 128;
+    const uint64_t tiles = up(M, high) / high * (up(K, wide) / wide), stages = s.piece * size / kRowBytes;
+    s.split = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(tile == kLarge ? 256 : 512) / tiles, stages / 8, 32}));
     s.dx = s.take((uint64_t)s.split * M * K * 4);
     return s;
 }
@@ -48,37 +54,36 @@ static LossSpace loss_space(int32_t M, int32_t V, int32_t K, int32_t dtype, bool
 // 256 x 256 by eight waves (2 x 4 of them, and 4 x 2 in dx, whose first operand alone costs two reads from LDS for a fragment: 540 us for
 // a piece of 8192 tokens with 8192 rows of 4096, and 512), 128 x 64 by four.
 template <int DT, bool TP, bool TQ> using LargeTile = Tile<DT, TP, TQ, !TP && DT != RS_DTYPE_F32, TP && !TQ ? 4 : 2, TP && !TQ ? 2 : 4, TP && !TQ ? 4 : 8, TP && !TQ ? 8 : 4, 2>;
+template <int DT, bool TP, bool TQ> using MiddleTile = Tile<DT, TP, TQ, !TP && DT != RS_DTYPE_F32, 2, 2, 4, 4, 2>;
 template <int DT, bool TP, bool TQ> using SmallTile = Tile<DT, TP, TQ, !TP && DT != RS_DTYPE_F32, 2, 2, 4, 2, 3>;
 
-template <class T, class K, class A> static void launch_tiles(K kernel, const A &p, const Product &a, hipStream_t st)
+template <class T, class K, class A> static void launch_tiles(K kernel, const A &p, hipStream_t st)
 {
-    const uint64_t tiles = (uint64_t)((a.q.rows + T::kTileM - 1) / T::kTileM) * ((a.p.rows + T::kTileN - 1) / T::kTileN);
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles * a.split)), dim3(T::kThreads), T::kLds, st, p);
+    const uint64_t tiles = (uint64_t)((p.a.q.rows + T::kTileM - 1) / T::kTileM) * ((p.a.p.rows + T::kTileN - 1) / T::kTileN);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles * p.a.split)), dim3(T::kThreads), T::kLds, st, p);
 }
 
-template <int DT> static void launch_forward(const LossParams &p, hipStream_t st)
-{
-    if (large(p.M, p.V)) launch_tiles<LargeTile<DT, false, false>>(loss_tile_kernel<LargeTile<DT, false, false>>, p, p.a, st);
-    else launch_tiles<SmallTile<DT, false, false>>(loss_tile_kernel<SmallTile<DT, false, false>>, p, p.a, st);
-}
+// (instantiated by name: the compiler leaves some of those that are only launched without their host side)
+#define RS_KERNELS(DT, TILE)                                                                                            \
+    template __global__ void loss_tile_kernel<TILE<DT, false, false>>(LossParams);                                      \
+    template __global__ void loss_grad_kernel<TILE<DT, false, false>>(LossParams);                                      \
+    template __global__ void loss_dx_kernel<TILE<DT, true, false>>(GradParams);                                         \
+    template __global__ void loss_dw_kernel<TILE<DT, true, true>>(GradParams);
+#define RS_TYPES(TILE) RS_KERNELS(RS_DTYPE_F32, TILE) RS_KERNELS(RS_DTYPE_BF16, TILE) RS_KERNELS(RS_DTYPE_F16, TILE)
+RS_TYPES(SmallTile)
+RS_TYPES(MiddleTile)
+RS_TYPES(LargeTile)
 
-template <int DT> static void launch_grad(const LossParams &p, hipStream_t st)
-{
-    if (large(p.M, p.a.p.rows)) launch_tiles<LargeTile<DT, false, false>>(loss_grad_kernel<LargeTile<DT, false, false>>, p, p.a, st);
-    else launch_tiles<SmallTile<DT, false, false>>(loss_grad_kernel<SmallTile<DT, false, false>>, p, p.a, st);
-}
-
-template <int DT> static void launch_dx(const GradParams &p, hipStream_t st)
-{
-    if (large(p.a.q.rows, p.a.p.rows)) launch_tiles<LargeTile<DT, true, false>>(loss_dx_kernel<LargeTile<DT, true, false>>, p, p.a, st);
-    else launch_tiles<SmallTile<DT, true, false>>(loss_dx_kernel<SmallTile<DT, true, false>>, p, p.a, st);
-}
-
-template <int DT> static void launch_dw(const GradParams &p, hipStream_t st)
-{
-    if (large(p.a.q.rows, p.a.p.rows)) launch_tiles<LargeTile<DT, true, true>>(loss_dw_kernel<LargeTile<DT, true, true>>, p, p.a, st);
-    else launch_tiles<SmallTile<DT, true, true>>(loss_dw_kernel<SmallTile<DT, true, true>>, p, p.a, st);
-}
+#define RS_LAUNCH(kernel, TP, TQ)                                                                                       \
+    switch (size_for(p.a.q.rows, p.a.p.rows)) {                                                                         \
+    case kLarge:  launch_tiles<LargeTile<DT, TP, TQ>>(kernel<LargeTile<DT, TP, TQ>>, p, st); break;                     \
+    case kMiddle: launch_tiles<MiddleTile<DT, TP, TQ>>(kernel<MiddleTile<DT, TP, TQ>>, p, st); break;                   \
+    default:      launch_tiles<SmallTile<DT, TP, TQ>>(kernel<SmallTile<DT, TP, TQ>>, p, st); break;                     \
+    }
+template <int DT> static void launch_forward(const LossParams &p, hipStream_t st) { RS_LAUNCH(loss_tile_kernel, false, false) }
+template <int DT> static void launch_grad(const LossParams &p, hipStream_t st) { RS_LAUNCH(loss_grad_kernel, false, false) }
+template <int DT> static void launch_dx(const GradParams &p, hipStream_t st) { RS_LAUNCH(loss_dx_kernel, true, false) }
+template <int DT> static void launch_dw(const GradParams &p, hipStream_t st) { RS_LAUNCH(loss_dw_kernel, true, true) }
 
 static bool known(int32_t dtype) { return dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16 || dtype == RS_DTYPE_F16; }
 
@@ -186,7 +191,7 @@ int rs_linear_cross_entropy(const void *x, int64_t x_stride, const void *w, int6
     p.c = (float)(1.4426950408889634 / temperature); p.inv_t = (float)(1.0 / temperature);
     p.parts = (float2 *)(ws + s.parts); p.target = (float *)(ws + s.target);
     p.loss = loss; p.lse = lse; p.stats = (float2 *)stats;
-    const uint32_t stretch = large(M, V) ? 128 : 64;
+    const uint32_t stretch = size_for(M, V) == kLarge ? 128 : 64;
     p.n_parts = (p.V + stretch - 1) / stretch;
     if (dtype == RS_DTYPE_F32) launch_forward<RS_DTYPE_F32>(p, st);
     else if (dtype == RS_DTYPE_BF16) launch_forward<RS_DTYPE_BF16>(p, st);

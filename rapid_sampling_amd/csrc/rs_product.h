@@ -30,12 +30,18 @@ template <int DT> __device__ __forceinline__ Sum<DT> multiply(v4i p, v4i q, Sum<
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, p), __builtin_bit_cast(v8bf, q), s, 0, 0, 0);
     else if constexpr (DT == RS_DTYPE_F16)
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, p), __builtin_bit_cast(v8h, q), s, 0, 0, 0);
-    else {
-        const v4f a = __builtin_bit_cast(v4f, p), b = __builtin_bit_cast(v4f, q);
+    else return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, p[0]), __builtin_bit_cast(float, q[0]), s, 0, 0, 0);
+}
+// The products of all fragments of one half of a stage.  (float32: four values of 16 bytes, one product each; the four of one sum not
+// behind one another.)
+template <int DT, int NU, int MT> __device__ __forceinline__ void multiply_all(const v4i (&p)[NU], const v4i (&q)[MT], Sum<DT> (&acc)[NU][MT])
+{
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], s, 0, 0, 0);
-        return s;
-    }
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int j = 0; j < (DT == RS_DTYPE_F32 ? 4 : 1); ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[u][t] = multiply<DT>(DT == RS_DTYPE_F32 ? v4i{p[u][j], 0, 0, 0} : p[u], DT == RS_DTYPE_F32 ? v4i{q[t][j], 0, 0, 0} : q[t], acc[u][t]);
 }
 
 // One operand of a product: `rows` rows (n or m) of `red` values, `stride` bytes from a row (transposed: from one r) to the next.  16-byte
@@ -250,10 +256,7 @@ struct Tile {
             now = now == (STAGES - 1) * kStage ? 0u : now + kStage;
             next = next == (STAGES - 1) * kStage ? 0u : next + kStage;
         }
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-            for (int t = 0; t < MT; ++t) acc[u][t] = multiply<DT>(p1[u], q1[t], acc[u][t]);
+        multiply_all<DT>(p1, q1, acc);
     }
 
     // Reads half `sub` of a stage into p and q and multiplies what was read before, one behind the other.
@@ -264,10 +267,7 @@ struct Tile {
         for (int t = 0; t < MT; ++t) q[t] = rq(lds + P::kBytes, t, sub);
 #pragma unroll
         for (int u = 0; u < NU; ++u) p[u] = rp(lds, u, sub);
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-            for (int t = 0; t < MT; ++t) acc[u][t] = multiply<DT>(before_p[u], before_q[t], acc[u][t]);
+        multiply_all<DT>(before_p, before_q, acc);
         constexpr int kReads = NU * P::Reader::kReads + MT * Q::Reader::kReads, kProducts = NU * MT * (DT == RS_DTYPE_F32 ? 4 : 1);
         constexpr int kGroups = NU + MT;
 #pragma unroll
