@@ -193,17 +193,20 @@ struct Tile {
     }
     __device__ __forceinline__ uint32_t m(int t) const { return m0 + wave_id() / WN * (16u * MT) + t * 16u + threadIdx.x % 16u; }
 
-    // Which tile: workgroup b runs on XCD b % 8; each XCD takes a stretch of the tiles, in panels of eight rows of tiles, so that the 32
-    // tiles it works on at a time share their rows in its L2.
+    // Which tile.  Groups of 32 columns of tiles one after the other: their rows of P (64 MB of 8192 x 4096 in 16 bits) stay in the last cache for
+    // all rows of tiles.  Of a group each XCD (workgroup b runs on XCD b % 8) takes a stretch, in panels of eight rows of tiles, so that
+    // the 32 tiles it works on at a time share their rows in its L2.
     __device__ __forceinline__ uint32_t choose(const Product &a, uint32_t id)
     {
         const uint32_t tm = (a.q.rows + kTileM - 1u) / kTileM, tn = (a.p.rows + kTileN - 1u) / kTileN, tiles = tm * tn;
         uint32_t part = 0;
         if (a.split > 1u) { part = id / tiles; id -= part * tiles; }
-        const uint32_t each = tiles / 8u, rest = tiles % 8u, xcd = id % 8u;
+        const uint32_t group = id / (tm * 32u), wide = min(32u, tn - group * 32u);
+        id -= group * (tm * 32u);
+        const uint32_t each = tm * wide / 8u, rest = tm * wide % 8u, xcd = id % 8u;
         id = xcd * each + min(xcd, rest) + id / 8u;
-        const uint32_t panel = id / (8u * tn), high = min(8u, tm - panel * 8u), in = id - panel * 8u * tn;
-        n0 = in / high * kTileN;
+        const uint32_t panel = id / (8u * wide), high = min(8u, tm - panel * 8u), in = id - panel * 8u * wide;
+        n0 = (group * 32u + in / high) * kTileN;
         m0 = (panel * 8u + in % high) * kTileM;
         return part;
     }
