@@ -254,17 +254,32 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void int8_tile_kernel(Int8Params p
             }
         }
     }
-#pragma unroll
-    for (int t = 0; t < T::MT; ++t) {
-        const uint32_t m = tile.m(t);
-        if (m >= p.M) continue;
-        const float f = p.x_scale[m];
-        v4f y[T::NU];
+    auto row_of = [&](int t, v4f (&v)[T::NU]) {
+        const float f = p.x_scale[min(tile.m(t), p.M - 1u)];
 #pragma unroll
         for (int u = 0; u < T::NU; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[u][j] = in_float32((float)acc[u][t][j] * (f * p.w_scale[min(tile.n(u) + j, p.N - 1u)]));
-        store_tile_row<DT>(tile, p.y, (int64_t)m * p.y_stride, p.N, y);
+            for (int j = 0; j < 4; ++j) v[u][j] = in_float32((float)acc[u][t][j] * (f * p.w_scale[min(tile.n(u) + j, p.N - 1u)]));
+    };
+    if constexpr (DT == RS_DTYPE_F32) {
+#pragma unroll
+        for (int t = 0; t < T::MT; ++t) {
+            v4f v[T::NU];
+            row_of(t, v);
+            const uint32_t m = tile.m(t);
+            if (m < p.M)
+#pragma unroll
+                for (int u = 0; u < T::NU; ++u) store_row<DT>(p.y, (int64_t)m * p.y_stride, tile.n(u), p.N, v[u]);
+        }
+    } else {
+        const TileStore<DT, T> out(lds);
+#pragma unroll
+        for (int t = 0; t < T::MT; ++t) {
+            v4f v[T::NU];
+            row_of(t, v);
+            out.put(t, v);
+        }
+        out.flush(tile, p.y, p.y_stride, p.M, p.N);
     }
 }
 

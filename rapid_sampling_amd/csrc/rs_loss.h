@@ -177,13 +177,8 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
     tile.choose(p.a, blockIdx.x);
     typename T::Acc acc;
     tile.make(p.a, 0, lds, acc);
-#pragma unroll
-    for (int t = 0; t < T::MT; ++t) {
-        const uint32_t m = tile.m(t);
-        if (m >= p.M) continue;
-        const LossRow r = p.rows[m];
-        char *row = (char *)p.grad + (int64_t)m * p.grad_stride;
-        v4f v[T::NU];
+    auto row_of = [&](int t, v4f (&v)[T::NU]) {
+        const LossRow r = p.rows[min(tile.m(t), p.M - 1u)];
 #pragma unroll
         for (int u = 0; u < T::NU; ++u)
 #pragma unroll
@@ -191,7 +186,26 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
                 v[u][j] = r.a * __builtin_amdgcn_exp2f(acc[u][t][j] * p.c - r.max);
                 if ((int32_t)(tile.n(u) + p.v0 + j) == r.token) v[u][j] -= r.b;
             }
-        store_tile_row<T::DT>(tile, row, 0, p.a.p.rows, v);
+    };
+    if constexpr (T::DT == RS_DTYPE_F32) {
+#pragma unroll
+        for (int t = 0; t < T::MT; ++t) {
+            v4f v[T::NU];
+            row_of(t, v);
+            const uint32_t m = tile.m(t);
+            if (m < p.M)
+#pragma unroll
+                for (int u = 0; u < T::NU; ++u) store_row<T::DT>((char *)p.grad + (int64_t)m * p.grad_stride, 0, tile.n(u), p.a.p.rows, v[u]);
+        }
+    } else {
+        const TileStore<T::DT, T> out(lds);
+#pragma unroll
+        for (int t = 0; t < T::MT; ++t) {
+            v4f v[T::NU];
+            row_of(t, v);
+            out.put(t, v);
+        }
+        out.flush(tile, p.grad, p.grad_stride / 2u, p.M, p.a.p.rows);
     }
 }
 
@@ -244,14 +258,24 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_dw_kernel(GradParams p)
     typename T::Acc acc;
     tile.make(p.a, 0, lds, acc);
     const float f = p.scale[1];
+    if constexpr (T::DT == RS_DTYPE_F32) {
 #pragma unroll
-    for (int t = 0; t < T::MT; ++t) {
-        const uint32_t m = tile.m(t);
-        if (m >= p.a.q.rows) continue;
-        v4f v[T::NU];
+        for (int t = 0; t < T::MT; ++t) {
+            const uint32_t m = tile.m(t);
+            if (m < p.a.q.rows)
 #pragma unroll
-        for (int u = 0; u < T::NU; ++u) v[u] = acc[u][t] * f;
-        store_tile_row<T::DT>(tile, p.y, (int64_t)m * p.y_stride, p.a.p.rows, v);
+                for (int u = 0; u < T::NU; ++u) store_row<T::DT>(p.y, (int64_t)m * p.y_stride, tile.n(u), p.a.p.rows, acc[u][t] * f);
+        }
+    } else {
+        const TileStore<T::DT, T> out(lds);
+#pragma unroll
+        for (int t = 0; t < T::MT; ++t) {
+            v4f v[T::NU];
+#pragma unroll
+            for (int u = 0; u < T::NU; ++u) v[u] = acc[u][t] * f;
+            out.put(t, v);
+        }
+        out.flush(tile, p.y, p.y_stride, p.a.q.rows, p.a.p.rows);
     }
 }
 

@@ -21,27 +21,44 @@ template <> struct SumOf<kInt8> { typedef v4i type; };
 template <int DT> using Sum = typename SumOf<DT>::type;
 
 
-// 16 x 16 sums of 16 bytes of each row.  Lane l gives 16 bytes of row l % 16 of either side, the same part of the reduction on both, and has
-// the sums of the first side's rows 4 (l / 16) + 0..3 with the second side's row l % 16.
+// 16 x 16 sums of 64 bytes of each row.  Lane l gives 16 bytes of row l % 16 of either side, the same part of the reduction on both, and has
+// the sums of the first side's rows 4 (l / 16) + 0..3 with the second side's row l % 16.  (float32: of what is left of its values in bfloat16)
 template <int DT> __device__ __forceinline__ Sum<DT> multiply(v4i p, v4i q, Sum<DT> s)
 {
     if constexpr (DT == kInt8) return __builtin_amdgcn_mfma_i32_16x16x64_i8(p, q, s, 0, 0, 0);
-    else if constexpr (DT == RS_DTYPE_BF16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, p), __builtin_bit_cast(v8bf, q), s, 0, 0, 0);
     else if constexpr (DT == RS_DTYPE_F16)
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, p), __builtin_bit_cast(v8h, q), s, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, p[0]), __builtin_bit_cast(float, q[0]), s, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, p), __builtin_bit_cast(v8bf, q), s, 0, 0, 0);
 }
-// The products of all fragments of one half of a stage.  (float32: four values of 16 bytes, one product each; the four of one sum not
-// behind one another.)
+// The products of all fragments of one half of a stage.
 template <int DT, int NU, int MT> __device__ __forceinline__ void multiply_all(const v4i (&p)[NU], const v4i (&q)[MT], Sum<DT> (&acc)[NU][MT])
 {
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int j = 0; j < (DT == RS_DTYPE_F32 ? 4 : 1); ++j)
+        for (int t = 0; t < MT; ++t) acc[u][t] = multiply<DT>(p[u], q[t], acc[u][t]);
+}
+
+// Eight float32 values as three times eight of bfloat16, x = x0 + x1 + x2 exactly: eight bits of the significand each, cut off, not rounded.
+// Of the nine products of two such sums the six largest are made: what is left out is below 2^-23 of a product, and 2^-25 on
+// average.  Six matrix instructions of 16 cycles in the place of eight of 32.
+struct Thirds { v4i x[3]; };
+__device__ __forceinline__ Thirds thirds(v4i lo, v4i hi)
+{
+    Thirds r;
+    uint32_t v[8];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) acc[u][t] = multiply<DT>(DT == RS_DTYPE_F32 ? v4i{p[u][j], 0, 0, 0} : p[u], DT == RS_DTYPE_F32 ? v4i{q[t][j], 0, 0, 0} : q[t], acc[u][t]);
+    for (int j = 0; j < 4; ++j) { v[j] = (uint32_t)lo[j]; v[j + 4] = (uint32_t)hi[j]; }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            r.x[i][j / 2] = (int)__builtin_amdgcn_perm(v[j + 1], v[j], 0x07060302u);          // the upper halves of both
+            if (i < 2)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) v[j + h] = __float_as_uint(__uint_as_float(v[j + h]) - __uint_as_float(v[j + h] & 0xFFFF0000u));
+        }
+    return r;
 }
 
 // One operand of a product: `rows` rows (n or m) of `red` values, `stride` bytes from a row (transposed: from one r) to the next.  16-byte
@@ -62,7 +79,8 @@ struct Product {
 // Rows from memory go to LDS without passing through registers.  As they are: a stage is 128 bytes of every row, its eight 16-byte
 // pieces in an order that depends on the row (place = piece ^ turn), so that the eight rows read at once lie in different banks.
 // Transposed: a stage is 128 / size values of r, the COUNT values of each side by side; those of 16 bits are turned by the reads from
-// LDS (ds_read_b64_tr_b16: four r of a row to a lane), whose 32-byte pieces are stored in such an order too.
+// LDS (ds_read_b64_tr_b16: four r of a row to a lane), whose 32-byte pieces are stored in such an order too; those of 32 bits, 64-byte
+// pieces in an order of their own, are read one by one.
 //
 // PAIRS (untransposed): the rows are dealt to the matrix instructions so that a lane's sums of two fragments (of 16 rows; F to a wave) belong
 // to eight consecutive rows: 16 bytes of a result in 16 bits.
@@ -93,6 +111,7 @@ struct Side {
         row = at / kWide;
         byte = at % kWide;
         if (kSize<DT> == 2) byte = ((byte / 32u) ^ turn(row)) * 32u + byte % 32u;
+        else byte ^= (row / 8u & 3u) * 64u;
     }
     __device__ __forceinline__ uint32_t place(uint32_t i) const { return (i * WAVES + wave_id()) * 1024u + threadIdx.x % 64u * 16u; }
 
@@ -139,25 +158,28 @@ struct Side {
         }
     }
 
-    // The lane's 16 bytes of fragment f (16 rows from `first` + 16 f on; dealt, if they are) of half `sub` of the stage.
+    // The lane's 16 bytes of fragment f (16 rows from `first` + 16 f on; dealt, if they are) of half `sub` of the stage: its quarter of 64
+    // bytes of the row, or (float32) of 128 bytes the half `sub` of its quarter.
     struct Reader {
         static constexpr int kReads = !TR ? 1 : kSize<DT> == 2 ? 2 : 4;
-        uint32_t at[TR && kSize<DT> == 2 ? F : 1];
+        uint32_t at[TR ? F : 1];
         __device__ __forceinline__ explicit Reader(uint32_t first)
         {
             const uint32_t lane = threadIdx.x % 64u, i = lane % 16u, part = lane / 16u;
             if constexpr (!TR) {
                 const uint32_t row = first + (PAIRS ? i / 4u * 8u + i % 4u : i);
-                at[0] = row * kRowBytes + (part ^ turn(row)) * 16u;
+                at[0] = row * kRowBytes + ((kSize<DT> == 4 ? 2u * part : part) ^ turn(row)) * 16u;
             } else if constexpr (kSize<DT> == 2) {
                 const uint32_t row = 8u * part + i / 4u;
 #pragma unroll
                 for (int f = 0; f < F; ++f) at[f] = row * kWide + ((first / 16u + f) ^ turn(row)) * 32u + i % 4u * 8u;
-            } else at[0] = 4u * part * kWide + (first + i) * 4u;
+            } else
+#pragma unroll
+                for (int f = 0; f < F; ++f) at[f] = 8u * part * kWide + ((first / 16u + f) ^ part) * 64u + i * 4u;
         }
         __device__ __forceinline__ v4i operator()(const char *lds, int f, int sub) const
         {
-            if constexpr (!TR) return *(const v4i *)(lds + (at[0] ^ (sub ? 64u : 0u)) + (PAIRS ? f / 2 * 32 + f % 2 * 4 : f * 16) * kRowBytes);
+            if constexpr (!TR) return *(const v4i *)(lds + (at[0] ^ (sub ? (kSize<DT> == 4 ? 16u : 64u) : 0u)) + (PAIRS ? f / 2 * 32 + f % 2 * 4 : f * 16) * kRowBytes);
             else if constexpr (kSize<DT> == 2) {
                 typedef __attribute__((address_space(3))) v4s *P;
                 const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lds + at[f] + sub * 32 * kWide));
@@ -166,7 +188,7 @@ struct Side {
             } else {
                 v4i v;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = *(const int *)(lds + at[0] + (sub * 16 + j) * kWide + f * 64);
+                for (int j = 0; j < 4; ++j) v[j] = *(const int *)(lds + at[f] + (sub * 4 + j) * kWide);
                 return v;
             }
         }
@@ -235,15 +257,9 @@ struct Tile {
 #pragma unroll
         for (int b = 0; b < STAGES - 1; ++b)
             if (b < (int)count) fill(lds + b * kStage);
-        // Both halves of a stage in registers: while one is multiplied the other is read, and the second half of a stage is multiplied behind the
-        // barrier that the next stage is waited for at (8192 x 8192 x 4096 in bfloat16 476 us without, 413 with).
-        v4i p0[NU], q0[MT], p1[NU], q1[MT];
-#pragma unroll
-        for (int u = 0; u < NU; ++u) p1[u] = v4i{0, 0, 0, 0};
-#pragma unroll
-        for (int t = 0; t < MT; ++t) q1[t] = v4i{0, 0, 0, 0};
-        uint32_t now = 0, next = (STAGES - 1) * kStage, at = first;
-        for (uint32_t j = 0; j < count; ++j) {
+        uint32_t now = 0, next = (STAGES - 1) * kStage, at = first, j = 0;
+        // The next stage is there, and the one after the last that is under way is asked for.
+        auto arrive = [&]() {
             // (towards the end there are no newer stages to leave under way)
             if (STAGES == 2 || j + STAGES - 1 > count) stage_barrier<0>();
             else stage_barrier<(STAGES - 2) * kLoads>();
@@ -254,12 +270,97 @@ struct Tile {
             }
             at = at + 1u == s0 + count ? s0 : at + 1u;
             if (j + STAGES - 1u < count) fill(lds + next);
-            half(lds + now, rp, rq, 0, p0, q0, p1, q1, acc);
-            half(lds + now, rp, rq, 1, p1, q1, p0, q0, acc);
+        };
+        auto advance = [&]() {
+            ++j;
             now = now == (STAGES - 1) * kStage ? 0u : now + kStage;
             next = next == (STAGES - 1) * kStage ? 0u : next + kStage;
+        };
+        if constexpr (kAhead) {
+            Raw even, odd;
+            auto step = [&](Raw &fresh, const Raw &held) {
+                arrive();
+                read(lds + now, rp, rq, fresh);
+                multiply_raw(held, acc);
+                advance();
+            };
+            if (count) {
+                arrive();
+                read(lds + now, rp, rq, even);
+                advance();
+            }
+            while (j < count) {
+                step(odd, even);
+                if (j == count) {
+                    multiply_raw(odd, acc);
+                    return;
+                }
+                step(even, odd);
+            }
+            if (count) multiply_raw(even, acc);
+        } else if constexpr (DT == RS_DTYPE_F32) {
+            while (j < count) {
+                arrive();
+                whole(lds + now, rp, rq, acc);
+                advance();
+            }
+        } else {
+            // Both halves of a stage in registers: while one is multiplied the other is read, and the second half of a stage is multiplied behind
+            // the barrier that the next stage is waited for at (8192 x 8192 x 4096 in bfloat16 476 us without, 413 with).
+            v4i p0[NU], q0[MT], p1[NU], q1[MT];
+#pragma unroll
+            for (int u = 0; u < NU; ++u) p1[u] = v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < MT; ++t) q1[t] = v4i{0, 0, 0, 0};
+            while (j < count) {
+                arrive();
+                half(lds + now, rp, rq, 0, p0, q0, p1, q1, acc);
+                half(lds + now, rp, rq, 1, p1, q1, p0, q0, acc);
+                advance();
+            }
+            multiply_all<DT>(p1, q1, acc);
         }
-        multiply_all<DT>(p1, q1, acc);
+    }
+
+    // float32: a stage at a time, the first operand's fragments one by one.  Of the smallest tiles, which few waves share a compute unit
+    // with, a stage is read while the one before is multiplied.
+    static constexpr bool kAhead = DT == RS_DTYPE_F32 && NU * MT <= 8;
+    struct Raw { v4i p[NU][2], q[MT][2]; };
+    static __device__ __forceinline__ void read(const char *lds, const typename P::Reader &rp, const typename Q::Reader &rq, Raw &r)
+    {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) { r.q[t][0] = rq(lds + P::kBytes, t, 0); r.q[t][1] = rq(lds + P::kBytes, t, 1); }
+#pragma unroll
+        for (int u = 0; u < NU; ++u) { r.p[u][0] = rp(lds, u, 0); r.p[u][1] = rp(lds, u, 1); }
+    }
+    static __device__ __forceinline__ void products(const Thirds &p, const Thirds (&q)[MT], Sum<DT> (&acc)[MT])
+    {
+        constexpr int kFirst[6] = {0, 1, 2, 0, 1, 0}, kSecond[6] = {2, 1, 0, 1, 0, 0};           // the smallest first
+#pragma unroll
+        for (int i = 0; i < 6; ++i)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = multiply<DT>(p.x[kFirst[i]], q[t].x[kSecond[i]], acc[t]);
+    }
+    static __device__ __forceinline__ void multiply_raw(const Raw &r, Acc &acc)
+    {
+        Thirds q[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) q[t] = thirds(r.q[t][0], r.q[t][1]);
+#pragma unroll
+        for (int u = 0; u < NU; ++u) products(thirds(r.p[u][0], r.p[u][1]), q, acc[u]);
+    }
+    static __device__ __forceinline__ void whole(const char *lds, const typename P::Reader &rp, const typename Q::Reader &rq, Acc &acc)
+    {
+        Thirds q[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) q[t] = thirds(rq(lds + P::kBytes, t, 0), rq(lds + P::kBytes, t, 1));
+        v4i lo = rp(lds, 0, 0), hi = rp(lds, 0, 1);
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const Thirds p = thirds(lo, hi);
+            if (u + 1 < NU) { lo = rp(lds, u + 1, 0); hi = rp(lds, u + 1, 1); }
+            products(p, q, acc[u]);
+        }
     }
 
     // Reads half `sub` of a stage into p and q and multiplies what was read before, one behind the other.
@@ -271,7 +372,7 @@ struct Tile {
 #pragma unroll
         for (int u = 0; u < NU; ++u) p[u] = rp(lds, u, sub);
         multiply_all<DT>(before_p, before_q, acc);
-        constexpr int kReads = NU * P::Reader::kReads + MT * Q::Reader::kReads, kProducts = NU * MT * (DT == RS_DTYPE_F32 ? 4 : 1);
+        constexpr int kReads = NU * P::Reader::kReads + MT * Q::Reader::kReads, kProducts = NU * MT;
         constexpr int kGroups = NU + MT;
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
@@ -290,19 +391,53 @@ template <int DT> __device__ __forceinline__ void store_row(void *y, int64_t at,
         for (int j = 0; j < 4; ++j) if (n + j < N) put<DT>(y, at + n + j, a[j]);
 }
 
-// A lane's values of one row of a tile: v[u] are those of fragment u.
-template <int DT, class T> __device__ __forceinline__ void store_tile_row(const T &tile, void *y, int64_t at, uint32_t N, const v4f (&v)[T::NU])
-{
-    if constexpr (T::PAIRS && DT != RS_DTYPE_F32) {
+// A tile of results of 16 bits on its way to memory, by way of LDS, where a wave's lanes trade pieces: a wave's 16 MT rows of 16 NU columns, 16
+// bytes of a row to a lane in the end, and whole rows of the wave's to a store.  The pieces of a row lie in an order of its own, for
+// the banks.  put() for every row t of the lane, flush() once; a barrier first, since the tile's stages lay there.
+template <int DT, class T> struct TileStore {
+    static_assert(DT != RS_DTYPE_F32 && 16u * T::MT * 32u * T::NU * T::kWaves <= T::kLds, "16 bits; the tile fits where its stages were");
+    static constexpr uint32_t kPieces = 2u * T::NU, kRow = 16u * kPieces;
+    char *at;
+    __device__ __forceinline__ explicit TileStore(char *lds) : at(lds + wave_id() * (16u * T::MT * kRow)) { __syncthreads(); }
+    static __device__ __forceinline__ uint32_t two(float a, float b)
+    {
+        if constexpr (DT == RS_DTYPE_BF16) { const __bf16 v[2] = {(__bf16)a, (__bf16)b}; return __builtin_bit_cast(uint32_t, v); }
+        else { const _Float16 v[2] = {(_Float16)a, (_Float16)b}; return __builtin_bit_cast(uint32_t, v); }
+    }
+    __device__ __forceinline__ void put(int t, const v4f (&v)[T::NU]) const
+    {
+        const uint32_t i = threadIdx.x % 16u, part = threadIdx.x % 64u / 16u;
+        char *row = at + (t * 16u + i) * kRow;
+        if constexpr (T::PAIRS) {
 #pragma unroll
-        for (int u = 0; u < T::NU; u += 2) {
-            const uint32_t n = tile.n(u);
-            if (n + 8u <= N) put_wide<DT>(y, at + n, v[u], v[u + 1]);
-            else { store_row<DT>(y, at, n, N, v[u]); store_row<DT>(y, at, n + 4u, N, v[u + 1]); }
+            for (int u = 0; u < T::NU; u += 2)
+                *(uint4 *)(row + (((uint32_t)u * 2u + part) ^ (i % kPieces)) * 16u) =
+                    make_uint4(two(v[u][0], v[u][1]), two(v[u][2], v[u][3]), two(v[u + 1][0], v[u + 1][1]), two(v[u + 1][2], v[u + 1][3]));
+        } else {
+#pragma unroll
+            for (int u = 0; u < T::NU; ++u)
+                *(uint2 *)(row + (((uint32_t)u * 2u + part / 2u) ^ (i % kPieces)) * 16u + part % 2u * 8u) = make_uint2(two(v[u][0], v[u][1]), two(v[u][2], v[u][3]));
         }
-    } else
+    }
+    __device__ __forceinline__ void flush(const T &tile, void *y, int64_t y_stride, uint32_t M, uint32_t N) const
+    {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const uint32_t lane = threadIdx.x % 64u, piece = lane % kPieces, n = tile.n0 + wave_id() % T::WN * (16u * T::NU) + piece * 8u;
+        const uint32_t first = tile.m0 + wave_id() / T::WN * (16u * T::MT);
 #pragma unroll
-        for (int u = 0; u < T::NU; ++u) store_row<DT>(y, at, tile.n(u), N, v[u]);
-}
+        for (uint32_t r = lane / kPieces; r < 16u * T::MT; r += 64u / kPieces) {
+            const uint4 v = *(const uint4 *)(at + r * kRow + (piece ^ (r % 16u % kPieces)) * 16u);
+            const uint32_t m = first + r;
+            if (m >= M || n >= N) continue;
+            uint16_t *to = (uint16_t *)y + (int64_t)m * y_stride + n;
+            if (n + 8u <= N) __builtin_memcpy(to, &v, 16);
+            else {
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (uint32_t j = 0; j < 7; ++j) if (n + j < N) to[j] = (uint16_t)(w[j / 2] >> (16 * (j % 2)));
+            }
+        }
+    }
+};
 
 }  // namespace rs
