@@ -1,7 +1,8 @@
 // Cross entropy of tokens under softmax(x w^T / T) without the logits, and its gradients.
 //
-//   z[m, v] = c x_m . w_v, c = log2(e) / T       lse_m = ln 2 (M_m + log2 S_m), S_m = sum_v 2^(z[m, v] - M_m)       loss_m = lse_m - ln 2 z[m, t_m]
-//   G[m, v] = ((g_m + h_m) 2^(z[m, v] - M_m) / S_m - g_m [v = t_m]) / T           dx = G w           dw = G^T x
+//   z[m, v] = x_m . w_v     M_m = max_v z[m, v]     S_m = sum_v 2^(c (z[m, v] - M_m)), c = log2(e) / T
+//   lse_m = M_m / T + ln S_m                        loss_m = (M_m - z[m, t_m]) / T + ln S_m
+//   G[m, v] = ((g_m + h_m) 2^(c (z[m, v] - M_m)) / S_m - g_m [v = t_m]) / T        dx = G w        dw = G^T x
 //
 // with g the gradient of the losses and h that of the lse.  Forward: a product whose tiles leave a maximum and a sum of each row in
 // the place of their logits, and a pass that joins these.  Backward, for a piece of the vocabulary at a time: the piece's product once
@@ -12,6 +13,8 @@
 #include "rs_product.h"
 
 namespace rs {
+
+constexpr uint32_t kFewRows = 32;    // up to these what G's rounding leaves is kept
 
 struct LossRow {                     // of one row, for G
     float   max, a, b;               // M, (g + h) / (S T), g / T
@@ -34,9 +37,10 @@ struct LossParams {
     const float *g, *h;
     int32_t     g_stride, h_stride;
     LossRow    *rows;
-    float      *scale;               // [0] what G is multiplied with, [1] what the products are
+    float      *scale;               // null, or [0] what G is multiplied with, [1] what the products are
     void       *grad;                // G: rows of grad_stride bytes
     uint32_t    grad_stride;
+    uint32_t    rest;                // 0, or rows from one of G to what its rounding left, rounded too
 };
 
 __device__ __forceinline__ int64_t loss_token(const LossParams &p, uint32_t m)
@@ -63,7 +67,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_tile_kernel(LossParams p)
         for (int u = 0; u < T::NU; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                acc[u][t][j] = whole || tile.n(u) + j < V ? acc[u][t][j] * p.c : -__builtin_inff();
+                acc[u][t][j] = whole || tile.n(u) + j < V ? acc[u][t][j] : -__builtin_inff();
                 top = fmaxf(top, acc[u][t][j]);
             }
         // (few stretches hold the token of any of their rows)
@@ -88,17 +92,17 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_tile_kernel(LossParams p)
 #pragma unroll
         for (int u = 0; u < T::NU; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s += __builtin_amdgcn_exp2f(acc[u][t][j] - from);
+            for (int j = 0; j < 4; ++j) s += __builtin_amdgcn_exp2f((acc[u][t][j] - from) * p.c);
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
         if (m < p.M && threadIdx.x % 64u < 16u && stretch < p.n_parts) p.parts[(size_t)stretch * p.M + m] = make_float2(top, s);
     }
 }
 
-__device__ __forceinline__ float2 join_sums(float2 a, float2 b)
+__device__ __forceinline__ float2 join_sums(float2 a, float2 b, float c)
 {
     const float top = fmaxf(a.x, b.x), from = top == -__builtin_inff() ? 0.0f : top;
-    return make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - from) + b.y * __builtin_amdgcn_exp2f(b.x - from));
+    return make_float2(top, a.y * __builtin_amdgcn_exp2f((a.x - from) * c) + b.y * __builtin_amdgcn_exp2f((b.x - from) * c));
 }
 
 // 2^WIDTH rows to a workgroup, 256 / 2^WIDTH threads to a row.
@@ -108,39 +112,41 @@ __global__ __launch_bounds__(256) void loss_join_kernel(LossParams p, uint32_t w
     const uint32_t m = (blockIdx.x << width) + (threadIdx.x & ((1u << width) - 1u)), k = threadIdx.x >> width, many = 256u >> width;
     float2 sum = make_float2(-__builtin_inff(), 0.0f);
     if (m < p.M)
-        for (uint32_t s = k; s < p.n_parts; s += many) sum = join_sums(sum, p.parts[(size_t)s * p.M + m]);
+        for (uint32_t s = k; s < p.n_parts; s += many) sum = join_sums(sum, p.parts[(size_t)s * p.M + m], p.c);
     held[threadIdx.x] = sum;
     for (uint32_t d = 128u; d >= 1u << width; d >>= 1) {
         __syncthreads();
-        if (threadIdx.x < d) held[threadIdx.x] = join_sums(held[threadIdx.x], held[threadIdx.x + d]);
+        if (threadIdx.x < d) held[threadIdx.x] = join_sums(held[threadIdx.x], held[threadIdx.x + d], p.c);
     }
     if (k || m >= p.M) return;
     sum = held[threadIdx.x];
     const bool none = sum.x == -__builtin_inff() && sum.y == 0.0f;             // no logit above -inf
-    const float ln2 = 0.693147180559945309f;
-    const float log2_s = none ? 0.0f : __builtin_log2f(sum.y);
+    const float ln_s = none ? 0.0f : 0.693147180559945309f * __builtin_log2f(sum.y);
     const int64_t token = loss_token(p, m);
-    p.lse[m] = none ? -__builtin_inff() : ln2 * (sum.x + log2_s);
+    p.lse[m] = none ? -__builtin_inff() : sum.x * p.inv_t + ln_s;
     float loss = 0.0f;
     if (token >= (int64_t)p.V) loss = __builtin_nanf("");
-    else if (token >= 0) loss = none ? __builtin_inff() : ln2 * ((sum.x - p.target[m]) + log2_s);
+    else if (token >= 0) loss = none ? __builtin_inff() : (sum.x - p.target[m]) * p.inv_t + ln_s;
     p.loss[m] = loss;
     if (p.stats) p.stats[m] = none ? make_float2(0.0f, __builtin_inff()) : sum;
 }
 
 // ---------------------------------------------------------------- gradients --
 // G in 16 bits is rounded, to bfloat16 with 8 bits of its own size; in float16 it is made so large first (by a power of two, the same
-// for the whole call) that the largest possible is below 2^15, and a probability's share of it is lost from 2^-39 on.
-__global__ __launch_bounds__(1024) void loss_scale_kernel(LossParams p, int32_t half)
+// for the whole call) that the largest possible is below 2^15, and a probability's share of it is lost from 2^-39 on.  That adds to the
+// gradients' own rounding another of its size (a row's or a column's many are off in all directions: 1.4 times as much in all).  Of few
+// rows, where a gradient can hang on a few numbers of G, what the rounding left is kept as well, as rows of their own behind G's: the
+// products are then of twice as many rows, and wait for memory all the same (forward and gradients of 1 row of 4096 over 131072 in
+// bfloat16 876 us without, 890 with; of 48 rows it would be 907 and 1012).
+__global__ __launch_bounds__(1024) void loss_scale_kernel(LossParams p)
 {
     __shared__ float tops[16];
     float top = 0.0f;
-    if (half)
-        for (uint32_t m = threadIdx.x; m < p.M; m += 1024u) {
-            const float g = p.g ? fabsf(p.g[(int64_t)m * p.g_stride]) : 0.0f, h = p.h ? fabsf(p.h[(int64_t)m * p.h_stride]) : 0.0f;
-            const float v = (g + h) * p.inv_t;
-            if (v < __builtin_inff()) top = fmaxf(top, v);
-        }
+    for (uint32_t m = threadIdx.x; m < p.M; m += 1024u) {
+        const float g = p.g ? fabsf(p.g[(int64_t)m * p.g_stride]) : 0.0f, h = p.h ? fabsf(p.h[(int64_t)m * p.h_stride]) : 0.0f;
+        const float v = (g + h) * p.inv_t;
+        if (v < __builtin_inff()) top = fmaxf(top, v);
+    }
 #pragma unroll
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     if (threadIdx.x % 64u == 0) tops[threadIdx.x / 64u] = top;
@@ -158,7 +164,7 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossParams p)
     if (m >= p.M) return;
     const float2 st = p.stats[m];
     const int64_t token = loss_token(p, m);
-    const float f = p.inv_t * p.scale[0], h = p.h ? p.h[(int64_t)m * p.h_stride] : 0.0f;
+    const float f = p.scale ? p.inv_t * p.scale[0] : p.inv_t, h = p.h ? p.h[(int64_t)m * p.h_stride] : 0.0f;
     float g = p.g && token >= 0 ? p.g[(int64_t)m * p.g_stride] : 0.0f;
     if (p.g && token >= (int64_t)p.V) g = __builtin_nanf("");                  // its loss is NaN
     LossRow r;
@@ -183,7 +189,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
         for (int u = 0; u < T::NU; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                v[u][j] = r.a * __builtin_amdgcn_exp2f(acc[u][t][j] * p.c - r.max);
+                v[u][j] = r.a * __builtin_amdgcn_exp2f((acc[u][t][j] - r.max) * p.c);
                 if ((int32_t)(tile.n(u) + p.v0 + j) == r.token) v[u][j] -= r.b;
             }
     };
@@ -206,6 +212,23 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
             out.put(t, v);
         }
         out.flush(tile, p.grad, p.grad_stride / 2u, p.M, p.a.p.rows);
+        if constexpr (T::kTileM <= kFewRows * 2u) {
+            if (!p.rest) return;
+#pragma unroll
+            for (int t = 0; t < T::MT; ++t) {
+                v4f v[T::NU];
+                row_of(t, v);
+#pragma unroll
+                for (int u = 0; u < T::NU; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if constexpr (T::DT == RS_DTYPE_BF16) v[u][j] -= (float)(__bf16)v[u][j];
+                        else v[u][j] -= (float)(_Float16)v[u][j];
+                    }
+                out.put(t, v);
+            }
+            out.flush(tile, (char *)p.grad + (int64_t)p.rest * p.grad_stride, p.grad_stride / 2u, p.M, p.a.p.rows);
+        }
     }
 }
 
@@ -213,7 +236,7 @@ struct GradParams {
     Product      a;                  // P: the output's columns, Q: its rows
     void        *y;                  // (rows, columns)
     int64_t      y_stride;           // elements
-    const float *scale;              // [1]: factor of the result
+    const float *scale;              // null, or [1]: factor of the result
     int32_t      add;                // to what is there
     int64_t      part_stride;        // elements between the sums of the workgroups that share the reduction
 };
@@ -257,7 +280,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_dw_kernel(GradParams p)
     tile.choose(p.a, blockIdx.x);
     typename T::Acc acc;
     tile.make(p.a, 0, lds, acc);
-    const float f = p.scale[1];
+    const float f = p.scale ? p.scale[1] : 1.0f;
     if constexpr (T::DT == RS_DTYPE_F32) {
 #pragma unroll
         for (int t = 0; t < T::MT; ++t) {
@@ -283,10 +306,11 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_dw_kernel(GradParams p)
 template <int DT>
 __global__ __launch_bounds__(256) void loss_round_kernel(const float *sums, int64_t part_stride, uint32_t parts, void *y, int64_t count, const float *scale)
 {
-    const float f = scale[1];
+    const float f = scale ? scale[1] : 1.0f;
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (int64_t)gridDim.x * 1024) {
         v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
         if (i + 4 <= count) {
+#pragma unroll 8
             for (uint32_t k = 0; k < parts; ++k) s += *(const v4f *)(sums + k * part_stride + i);
             put_four<DT>(y, i, s * f);
         } else
@@ -298,19 +322,20 @@ __global__ __launch_bounds__(256) void loss_round_kernel(const float *sums, int6
     }
 }
 
-// Rows laid out in multiples of 16 bytes, for those that are not: 16 bytes to a thread.
-__global__ __launch_bounds__(256) void lay_out_rows_kernel(const char *x, int64_t x_stride, char *y, int64_t y_stride, int64_t rows, uint32_t bytes)
+// Rows laid out in multiples of 16 bytes, for those that are not (or, `source` of them, several times over): 16 bytes to a thread.
+__global__ __launch_bounds__(256) void lay_out_rows_kernel(const char *x, int64_t x_stride, char *y, int64_t y_stride, int64_t rows, int64_t source, uint32_t bytes)
 {
     const uint32_t pieces = (uint32_t)(y_stride / 16);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * pieces; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / pieces;
+        const char *from = x + (r < source ? r : r - source) * x_stride;
         const uint32_t at = (uint32_t)(i - r * pieces) * 16u;
         v4i v = {0, 0, 0, 0};
-        if (at + 16u <= bytes) __builtin_memcpy(&v, x + r * x_stride + at, 16);
+        if (at + 16u <= bytes) __builtin_memcpy(&v, from + at, 16);
         else {
             uint16_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) if (at + 2u * j < bytes) w[j] = *(const uint16_t *)(x + r * x_stride + at + 2u * j);
+            for (uint32_t j = 0; j < 8; ++j) if (at + 2u * j < bytes) w[j] = *(const uint16_t *)(from + at + 2u * j);
             __builtin_memcpy(&v, w, 16);
         }
         *(v4i *)(y + r * y_stride + at) = v;

@@ -12,6 +12,8 @@ static uint32_t size_of(int32_t dtype) { return dtype == RS_DTYPE_F32 ? 4 : 2; }
 struct LossSpace {
     uint64_t parts = 0, target = 0;                     // forward
     uint64_t scale = 0, rows = 0, grad = 0, dx = 0;     // backward
+    uint64_t twice = 0;                                 // x's rows two times over
+    uint32_t high = 0;                                  // rows of G: x's, or twice as many (see loss_scale_kernel)
     uint64_t bytes = 0;
     uint32_t piece = 0, split = 1;                      // tokens of a piece; shares of dx's reduction
     uint64_t grad_stride = 0;
@@ -37,17 +39,19 @@ static LossSpace loss_space(int32_t M, int32_t V, int32_t K, int32_t dtype, bool
         s.target = s.take((uint64_t)M * 4);
         return s;
     }
+    s.high = M <= (int32_t)kFewRows && dtype != RS_DTYPE_F32 ? 2 * M : M;
+    if (s.high > (uint32_t)M) s.twice = s.take(s.high * up((uint64_t)K * size, 16));
     s.scale = s.take(8);
     s.rows = s.take((uint64_t)M * sizeof(LossRow));
-    s.piece = (uint32_t)std::min<uint64_t>(up(V, 256), std::max<uint64_t>(8192, ((1ull << 27) / (M * size)) / 256 * 256));
+    s.piece = (uint32_t)std::min<uint64_t>(up(V, 256), std::max<uint64_t>(8192, ((1ull << 27) / (s.high * size)) / 256 * 256));
     s.grad_stride = s.piece * size + 256;              // (not a power of two: rows would share their memory channels)
-    s.grad = s.take((uint64_t)M * s.grad_stride);
+    s.grad = s.take((uint64_t)s.high * s.grad_stride);
     // dx has few tiles: their reduction over the piece is shared out among up to one (two) workgroups to a compute unit
-    const Size tile = size_for(M, K);
+    const Size tile = size_for(s.high, K);
     const uint64_t high = tile == kLarge ? 256 : tile == kMiddle ? 128 : 64, wide = tile == kLarge ? 256 : 128;
-    const uint64_t tiles = up(M, high) / high * (up(K, wide) / wide), stages = s.piece * size / kRowBytes;
+    const uint64_t tiles = up(s.high, high) / high * (up(K, wide) / wide), stages = s.piece * size / kRowBytes;
     s.split = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(tile == kLarge ? 256 : 512) / tiles, stages / 8, 32}));
-    s.dx = s.take((uint64_t)s.split * M * K * 4);
+    s.dx = s.take((uint64_t)s.split * s.high * K * 4);
     return s;
 }
 
@@ -117,12 +121,28 @@ static Operand rows_of(const void *x, int64_t stride, int32_t rows, int32_t K, u
     return Operand{(const char *)x, (uint32_t)(rows > 1 ? stride * size : up((uint64_t)K * size, 16)), (uint32_t)rows};
 }
 
+static void launch_lay_out(const void *x, int64_t x_bytes, void *y, int64_t y_bytes, int64_t rows, int64_t source, uint32_t bytes, hipStream_t st)
+{
+    const uint64_t groups = ((uint64_t)rows * (y_bytes / 16) + 255) / 256;
+    hipLaunchKernelGGL(lay_out_rows_kernel, dim3((uint32_t)std::min<uint64_t>(groups, 1u << 16)), dim3(256), 0, st, (const char *)x, x_bytes, (char *)y, y_bytes, rows,
+                       source, bytes);
+}
+
 template <int DT>
 static void backward(LossParams p, const LossSpace &s, Operand x, Operand w, uint32_t K, void *grad_x, void *grad_w, char *ws, hipStream_t st)
 {
     constexpr uint32_t size = kSize<DT>;
-    hipLaunchKernelGGL(loss_scale_kernel, dim3(1), dim3(1024), 0, st, p, (int32_t)(DT == RS_DTYPE_F16));
+    if (DT == RS_DTYPE_F16) hipLaunchKernelGGL(loss_scale_kernel, dim3(1), dim3(1024), 0, st, p);
+    else p.scale = nullptr;
     hipLaunchKernelGGL(loss_rows_kernel, dim3((p.M + 255) / 256), dim3(256), 0, st, p);
+    Operand xs = x;
+    if (s.high > p.M) {
+        p.rest = p.M;
+        if (grad_w) {
+            xs = Operand{ws + s.twice, (uint32_t)up((uint64_t)K * size, 16), s.high};
+            launch_lay_out(x.at, x.stride, (char *)ws + s.twice, xs.stride, s.high, p.M, K * size, st);
+        }
+    }
     for (uint32_t v0 = 0; v0 < p.V; v0 += s.piece) {
         const uint32_t n = std::min(s.piece, p.V - v0);
         const char *piece = w.at + (int64_t)v0 * w.stride;
@@ -132,15 +152,15 @@ static void backward(LossParams p, const LossSpace &s, Operand x, Operand w, uin
         GradParams g;
         g.scale = p.scale;
         if (grad_x) {
-            g.a = Product{Operand{piece, w.stride, K}, Operand{(const char *)p.grad, p.grad_stride, p.M}, n, s.split};
+            g.a = Product{Operand{piece, w.stride, K}, Operand{(const char *)p.grad, p.grad_stride, s.high}, n, s.split};
             g.y = ws + s.dx;
             g.y_stride = K;
-            g.part_stride = (int64_t)p.M * K;
+            g.part_stride = (int64_t)s.high * K;
             g.add = v0 > 0;
             launch_dx<DT>(g, st);
         }
         if (grad_w) {
-            g.a = Product{Operand{x.at, x.stride, K}, Operand{(const char *)p.grad, p.grad_stride, n}, p.M, 1};
+            g.a = Product{Operand{xs.at, xs.stride, K}, Operand{(const char *)p.grad, p.grad_stride, n}, s.high, 1};
             g.y = (char *)grad_w + (int64_t)v0 * K * size;
             g.y_stride = K;
             g.part_stride = 0;
@@ -151,7 +171,7 @@ static void backward(LossParams p, const LossSpace &s, Operand x, Operand w, uin
     if (grad_x) {
         const int64_t count = (int64_t)p.M * K;
         hipLaunchKernelGGL(loss_round_kernel<DT>, dim3((uint32_t)std::min<int64_t>((count + 1023) / 1024, 1 << 16)), dim3(256), 0, st, (const float *)(ws + s.dx),
-                           count, s.split, grad_x, count, p.scale);
+                           count, s.split * (s.high / p.M), grad_x, count, p.scale);
     }
 }
 
@@ -167,9 +187,7 @@ int rs_lay_out_rows(const void *x, int64_t x_row_stride, int32_t size, int64_t R
     if (size != 2 && size != 4) return RS_ERR_ARG;
     if (R <= 0 || K <= 0 || K > RS_LINEAR_MAX || x_row_stride < 0 || y_row_stride < K || R > (1ll << 40) / y_row_stride) return RS_ERR_SHAPE;
     if (((uintptr_t)x & (size - 1)) || ((uintptr_t)y & 15) || (y_row_stride * size & 15)) return RS_ERR_ALIGN;
-    const uint64_t groups = ((uint64_t)R * (y_row_stride * size / 16) + 255) / 256;
-    hipLaunchKernelGGL(lay_out_rows_kernel, dim3((uint32_t)std::min<uint64_t>(groups, 1u << 16)), dim3(256), 0, (hipStream_t)stream, (const char *)x,
-                       x_row_stride * size, (char *)y, y_row_stride * size, R, (uint32_t)(K * size));
+    launch_lay_out(x, x_row_stride * size, y, y_row_stride * size, R, R, (uint32_t)(K * size), (hipStream_t)stream);
     return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
 }
 
