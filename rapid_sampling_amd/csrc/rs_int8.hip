@@ -1,8 +1,6 @@
 // Instantiations, launchers and C entry points of the product in 8-bit integers.
 #include "rs_int8.h"
 
-#include <algorithm>
-
 namespace rs {
 
 // As many rows at a time as a launch holds; a wave to a row of up to 2048 columns, a workgroup to a longer one.
@@ -54,6 +52,7 @@ template <int DT, int WN, int WM, int NU, int MT, int STAGES, bool SPLIT> static
 // (instantiated by name: the compiler leaves some of those that are only launched without their host side)
 #define RS_KERNELS(DT)                                                                     \
     template __global__ void int8_tile_kernel<DT, 2, 4, 8, 4, 2, false>(Int8Params);        \
+    template __global__ void int8_tile_kernel<DT, 2, 2, 4, 4, 2, false>(Int8Params);        \
     template __global__ void int8_tile_kernel<DT, 2, 2, 4, 2, 3, true>(Int8Params);
 RS_KERNELS(RS_DTYPE_F32)
 RS_KERNELS(RS_DTYPE_BF16)
@@ -63,9 +62,11 @@ template <int DT> static void launch_product(const Int8Params &p, hipStream_t st
 {
     // (the tiles' kernel reaches its rows with 32 bits)
     if (p.M <= 16 || p.x_stride > kTileStride || p.w_stride > kTileStride) return launch_few<DT, -1>(p, st);
-    const uint64_t n256 = (p.N + 255) / 256, m256 = (p.M + 255) / 256;
-    if (p.M > 128 && n256 * m256 >= 192) return launch_tiles<DT, 2, 4, 8, 4, 2, false>(p, st);
-    launch_tiles<DT, 2, 2, 4, 2, 3, true>(p, st);
+    // Where there are few tiles they are small ones, and their columns are shared out.
+    const TileSize size = tiles_of(p.M, p.N, 128, 128) < 192 ? kSmall : tile_size(p.M, p.N);
+    if (size == kLarge) launch_tiles<DT, 2, 4, 8, 4, 2, false>(p, st);
+    else if (size == kMiddle) launch_tiles<DT, 2, 2, 4, 4, 2, false>(p, st);
+    else launch_tiles<DT, 2, 2, 4, 2, 3, true>(p, st);
 }
 
 static Int8Params int8_params(const void *x, int64_t x_stride, const float *x_scale, const int8_t *w, int64_t w_stride, const float *w_scale, int32_t M, int32_t N,

@@ -1,11 +1,8 @@
 // Instantiations, launchers and C entry points of the cross entropy over a vocabulary without its logits.
 #include "rs_loss.h"
 
-#include <algorithm>
-
 namespace rs {
 
-static uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 static uint32_t size_of(int32_t dtype) { return dtype == RS_DTYPE_F32 ? 4 : 2; }
 
 // Where a call's scratch lies.  The same sizes give the same places.
@@ -20,13 +17,9 @@ struct LossSpace {
     uint64_t take(uint64_t n) { const uint64_t at = bytes; bytes += up(n, 256); return at; }
 };
 
-// Which tiles: of 256 x 256 where there are enough of them to go round, of 128 x 128 for more than 64 rows, else of 128 x 64 (columns x rows).
-enum Size { kSmall, kMiddle, kLarge };
-static Size size_for(uint64_t rows, uint64_t columns)
-{
-    if (rows > 128 && up(rows, 256) / 256 * (up(columns, 256) / 256) >= 192) return kLarge;
-    return rows > 64 ? kMiddle : kSmall;
-}
+// dx has few tiles: where those of 256 x 256 do not go round, others, whose reduction over the piece is shared out among up to two workgroups
+// to a compute unit (385 rows of 2000 and a piece of 50257 in float16: 128 x 64 164 us, 128 x 128 111).
+static TileSize dx_size(uint64_t rows, uint64_t columns) { return rows <= 64 ? kSmall : tiles_of(rows, columns, 256, 256) >= 192 ? kLarge : kMiddle; }
 
 // A piece of the vocabulary: G of the piece stays within the last cache (256 MB) with the piece's weights, in steps of 256 tokens and
 // at least 8192, so that the sums of dx that each piece reads and writes again (8 bytes) are little next to its products.
@@ -46,10 +39,8 @@ static LossSpace loss_space(int32_t M, int32_t V, int32_t K, int32_t dtype, bool
     s.piece = (uint32_t)std::min<uint64_t>(up(V, 256), std::max<uint64_t>(8192, ((1ull << 27) / (s.high * size)) / 256 * 256));
     s.grad_stride = s.piece * size + 256;              // (not a power of two: rows would share their memory channels)
     s.grad = s.take((uint64_t)s.high * s.grad_stride);
-    // dx has few tiles: their reduction over the piece is shared out among up to one (two) workgroups to a compute unit
-    const Size tile = size_for(s.high, K);
-    const uint64_t high = tile == kLarge ? 256 : tile == kMiddle ? 128 : 64, wide = tile == kLarge ? 256 : 128;
-    const uint64_t tiles = up(s.high, high) / high * (up(K, wide) / wide), stages = s.piece * size / kRowBytes;
+    const TileSize tile = dx_size(s.high, K);
+    const uint64_t tiles = tile == kLarge ? tiles_of(s.high, K, 256, 256) : tiles_of(s.high, K, tile == kMiddle ? 128 : 64, 128), stages = s.piece * size / kRowBytes;
     s.split = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({(tile == kLarge ? 256 : 512) / tiles, stages / 8, 32}));
     s.dx = s.take((uint64_t)s.split * s.high * K * 4);
     return s;
@@ -80,21 +71,21 @@ RS_TYPES(SmallTile)
 RS_TYPES(MiddleTile)
 RS_TYPES(LargeTile)
 
-#define RS_LAUNCH(kernel, TP, TQ)                                                                                       \
-    switch (size_for(p.a.q.rows, p.a.p.rows)) {                                                                         \
+#define RS_LAUNCH(size, kernel, TP, TQ)                                                                                 \
+    switch (size(p.a.q.rows, p.a.p.rows)) {                                                                             \
     case kLarge:  launch_tiles<LargeTile<DT, TP, TQ>>(kernel<LargeTile<DT, TP, TQ>>, p, st); break;                     \
     case kMiddle: launch_tiles<MiddleTile<DT, TP, TQ>>(kernel<MiddleTile<DT, TP, TQ>>, p, st); break;                   \
     default:      launch_tiles<SmallTile<DT, TP, TQ>>(kernel<SmallTile<DT, TP, TQ>>, p, st); break;                     \
     }
-template <int DT> static void launch_forward(const LossParams &p, hipStream_t st) { RS_LAUNCH(loss_tile_kernel, false, false) }
-template <int DT> static void launch_grad(const LossParams &p, hipStream_t st) { RS_LAUNCH(loss_grad_kernel, false, false) }
-template <int DT> static void launch_dx(const GradParams &p, hipStream_t st) { RS_LAUNCH(loss_dx_kernel, true, false) }
+template <int DT> static void launch_forward(const LossParams &p, hipStream_t st) { RS_LAUNCH(tile_size, loss_tile_kernel, false, false) }
+template <int DT> static void launch_grad(const LossParams &p, hipStream_t st) { RS_LAUNCH(tile_size, loss_grad_kernel, false, false) }
+template <int DT> static void launch_dx(const GradParams &p, hipStream_t st) { RS_LAUNCH(dx_size, loss_dx_kernel, true, false) }
 // (for few rows dw is all stores, and two workgroups to a compute unit hide more of them: 48 rows of 4096 over 131072 in bfloat16 1083 us with
 // its forward pass, 966 so; 385 rows of 2000 over 50257 the same either way)
 template <int DT> static void launch_dw(const GradParams &p, hipStream_t st)
 {
     if (p.a.red <= 256) launch_tiles<MiddleTile<DT, true, true>>(loss_dw_kernel<MiddleTile<DT, true, true>>, p, st);
-    else RS_LAUNCH(loss_dw_kernel, true, true)
+    else RS_LAUNCH(tile_size, loss_dw_kernel, true, true)
 }
 
 static bool known(int32_t dtype) { return dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16 || dtype == RS_DTYPE_F16; }
@@ -217,7 +208,7 @@ int rs_linear_cross_entropy(const void *x, int64_t x_stride, const void *w, int6
     p.c = (float)(1.4426950408889634 / temperature); p.inv_t = (float)(1.0 / temperature);
     p.parts = (float2 *)(ws + s.parts); p.target = (float *)(ws + s.target);
     p.loss = loss; p.lse = lse; p.stats = (float2 *)stats;
-    const uint32_t stretch = size_for(M, V) == kLarge ? 128 : 64;
+    const uint32_t stretch = tile_size(M, V) == kLarge ? 128 : 64;
     p.n_parts = (p.V + stretch - 1) / stretch;
     if (dtype == RS_DTYPE_F32) launch_forward<RS_DTYPE_F32>(p, st);
     else if (dtype == RS_DTYPE_BF16) launch_forward<RS_DTYPE_BF16>(p, st);

@@ -9,6 +9,8 @@
 
 #include "rs_linear.h"
 
+#include <algorithm>
+
 namespace rs {
 
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -194,6 +196,21 @@ struct Side {
         }
     };
 };
+
+// Which tiles (columns x rows): 256 x 256, 128 x 128 or 128 x 64, by how many rounds of them the chip makes.  Of the large ones a compute
+// unit makes one at a time, of the others two, and those take 0.6 and 0.45 of the time, not half and a quarter: they read more for a
+// product.  (Forward pass over 50257 x 2048 in bfloat16, large and middle: 300 rows 109 and 90 us, 385 rows 108 and 120, 256 rows 63 and
+// 67, 1024 rows 217 and 215, with gradients 944 and 998.  int8, middle and small: 77 x 50257 x 2000 24.1 and 31.1 us, 128 x 32768 x 4096
+// 29.7 and 25.3.)
+enum TileSize { kSmall, kMiddle, kLarge };
+inline uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+inline uint64_t tiles_of(uint64_t rows, uint64_t columns, uint64_t high, uint64_t wide) { return up(rows, high) / high * (up(columns, wide) / wide); }
+inline TileSize tile_size(uint64_t rows, uint64_t columns)
+{
+    const uint64_t large = 20 * (up(tiles_of(rows, columns, 256, 256), 256) / 256), middle = 12 * (up(tiles_of(rows, columns, 128, 128), 512) / 512),
+                   small = 9 * (up(tiles_of(rows, columns, 64, 128), 512) / 512);
+    return large <= std::min(middle, small) ? kLarge : middle <= small ? kMiddle : kSmall;
+}
 
 // A workgroup of WN x WM waves makes 16 NU WN rows of P x 16 MT WM rows of Q, a wave 16 NU x 16 MT of it.
 template <int DT_, bool TP_, bool TQ_, bool PAIRS_, int WN_, int WM_, int NU_, int MT_, int STAGES_>
