@@ -546,6 +546,7 @@ int rs_quantize_blocks(const void *x_device, int32_t x_dtype, int64_t x_row_stri
  * and ceil(M / 128) ceil(N / 128) below 2^24.  One launch.  No counterpart in the
  * reference.
  */
+#define RS_LINEAR_COUNTER_BYTES 4096   /* of the workspace, its front: what has to be clear; calls leave it so */
 size_t rs_linear_workspace_bytes(void);
 int rs_linear_blocks(const void *x_device, int64_t x_row_stride, const float *x_scale_device,
                      const void *w_device, int64_t w_row_stride, const float *w_scale_device,
@@ -586,7 +587,8 @@ int rs_lay_out_rows(const void *x_device, int64_t x_row_stride, int32_t size, in
  * NULL, or (M, 2) floats, 8-byte aligned, for the gradient.  A row whose logits are
  * all -inf has lse -inf and loss +inf; one with a NaN or +inf among them NaN.
  * M up to RS_LINEAR_MAX, V up to 1048576, K up to RS_LOSS_COLUMNS_MAX, and
- * ceil(M / 64) ceil(V / 128) below 2^24.
+ * ceil(M / 64) ceil(V / 128), ceil(M / 64) ceil(K / 128) and ceil(V / 128) ceil(K / 128)
+ * below 2^24.
  * workspace: rs_linear_cross_entropy_workspace_bytes() bytes of device memory,
  * 256-byte aligned, of any contents; calls that share it are ordered on one stream.
  * No counterpart in the reference.

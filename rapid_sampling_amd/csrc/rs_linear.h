@@ -23,6 +23,7 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t kPartTiles = 256;                 // tiles of partial sums that the workspace holds ...
 constexpr size_t   kPartBytes = 128 * 64 * 4;        // ... of 128 x 64
+static_assert(RS_LINEAR_COUNTER_BYTES == 16 * kPartTiles, "the counters in front of them");
 
 struct QuantParams {
     const void *x;

@@ -311,7 +311,11 @@ __global__ __launch_bounds__(256) void loss_round_kernel(const float *sums, int6
         v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
         if (i + 4 <= count) {
 #pragma unroll 8
-            for (uint32_t k = 0; k < parts; ++k) s += *(const v4f *)(sums + k * part_stride + i);
+            for (uint32_t k = 0; k < parts; ++k) {
+                v4f v;
+                __builtin_memcpy(&v, sums + k * part_stride + i, 16);            // (part_stride is any number)
+                s += v;
+            }
             put_four<DT>(y, i, s * f);
         } else
             for (int64_t j = i; j < count; ++j) {

@@ -96,10 +96,12 @@ static int check(const void *x, int64_t x_stride, const void *w, int64_t w_strid
     if (!x || !w || !tokens || !workspace) return RS_ERR_NULL;
     if (!known(dtype) || (tokens_64 != 0 && tokens_64 != 1)) return RS_ERR_ARG;
     if (M <= 0 || V <= 0 || K <= 0 || M > RS_LINEAR_MAX || V > 1048576 || K > RS_LOSS_COLUMNS_MAX) return RS_ERR_SHAPE;
-    if (((int64_t)M + 63) / 64 * (((int64_t)V + 127) / 128) > (int64_t)(kGridThreads / 256u)) return RS_ERR_SHAPE;       // workgroups of a launch
+    // workgroups of a launch, of 256 threads (those of 512 make tiles four times as large)
+    const uint64_t most = kGridThreads / 256u;
+    if (tiles_of(M, V, 64, 128) > most || tiles_of(M, K, 64, 128) > most || tiles_of(V, K, 128, 128) > most) return RS_ERR_SHAPE;
     if (!(temperature >= 0.001 && temperature <= 1000)) return RS_ERR_TEMPERATURE;
-    const int64_t size = size_of(dtype), most = kTileStride / size;
-    if ((M > 1 && (x_stride < K || x_stride > most)) || (V > 1 && (w_stride < K || w_stride > most))) return RS_ERR_SHAPE;
+    const int64_t size = size_of(dtype), far = kTileStride / size;
+    if ((M > 1 && (x_stride < K || x_stride > far)) || (V > 1 && (w_stride < K || w_stride > far))) return RS_ERR_SHAPE;
     if (((uintptr_t)x & 15) || ((uintptr_t)w & 15) || (M > 1 && (x_stride * size & 15)) || (V > 1 && (w_stride * size & 15)) ||
         ((uintptr_t)tokens & (tokens_64 ? 7 : 3)))
         return RS_ERR_ALIGN;

@@ -567,6 +567,11 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const at::Tenso
 
 // ------------------------------------------------------- values and products in 8-bit integers --
 
+at::Tensor scratch(size_t bytes, const at::Tensor &like)
+{
+    return at::empty({(int64_t)std::max<size_t>(bytes, 1)}, at::TensorOptions().dtype(at::kByte).device(like.device()));
+}
+
 std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor &x)
 {
     refuse_tangent("quantize_int8", {x});
@@ -647,7 +652,13 @@ at::Tensor linear_rows(const at::Tensor &x, const at::Tensor &weight, const at::
         const int rc = rs_quantize_rows(flat.data_ptr(), float_dtype(x, "x"), flat.stride(0), (int32_t)M, (int32_t)K, (int8_t *)q, q_stride, (float *)scale, stream);
         if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
     }
-    at::Tensor &ws = linear_workspace(x, stream, "linear_int8");
+    // (a call that is captured has a workspace of its own, whose counters the graph clears: graphs captured on one stream can run side by side)
+    at::Tensor ws;
+    if (is_capturing(stream)) {
+        ws = scratch(rs_linear_workspace_bytes(), x);
+        const int rc = rs_workspace_init(ws.data_ptr(), RS_LINEAR_COUNTER_BYTES, stream);
+        if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    } else ws = linear_workspace(x, stream, "linear_int8");
     const int rc = rs_linear_int8(q, q_stride, scale, wq, w.stride(0), weight_scale.data_ptr<float>(), (int32_t)M, (int32_t)N, (int32_t)K,
                                   y.data_ptr(), float_dtype(y, "y"), N, ws.data_ptr(), (size_t)ws.numel(), stream);
     if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
@@ -663,11 +674,6 @@ void check_tokens(const at::Tensor &tokens)
 }
 // Tokens of any shape as one list.
 at::Tensor token_list(const at::Tensor &tokens) { return tokens.dim() == 1 ? tokens : tokens.reshape({tokens.numel()}); }
-
-at::Tensor scratch(size_t bytes, const at::Tensor &like)
-{
-    return at::empty({(int64_t)std::max<size_t>(bytes, 1)}, at::TensorOptions().dtype(at::kByte).device(like.device()));
-}
 
 struct TableCall {
     int64_t M, V, K;
@@ -693,7 +699,7 @@ TableCall read_table(const at::Tensor &tokens, const at::Tensor &weight, double 
     else throw std::invalid_argument("out_dtype must be float32, bfloat16 or float16 !\n");
     if (weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1) throw std::invalid_argument("weight must have shape (V, K) !\n");
     if ((int8 || fp8) != weight_scale.has_value()) throw std::invalid_argument("weight_scale goes with a weight of type int8 or float8_e4m3fn, and only with one !\n");
-    if (!std::isfinite(scale)) throw std::invalid_argument("scale must be finite !\n");
+    if (!std::isfinite((float)scale)) throw std::invalid_argument("scale must be finite, in float32 as well !\n");
     c.M = tokens.numel(); c.V = weight.size(0); c.K = weight.size(1);
     if (c.M >= RS_LINEAR_MAX || c.V > RS_LINEAR_MAX || c.K > RS_LINEAR_MAX) throw std::invalid_argument("tokens or weight is too large !\n");
     refuse_tangent("embedding", {weight, weight_scale.value_or(at::Tensor())});

@@ -90,7 +90,7 @@ def test_quantize_halfway_between_two_integers(exponent):
 
 # few rows (one and two rows of w's fragments to a wave), small tiles whole and shared, large tiles; odd sizes of everything
 SIZES = [(1, 16, 1), (1, 100, 50), (1, 4096, 9000), (2, 128, 16), (3, 127, 8193), (4, 8192, 70), (16, 1000, 257), (17, 1000, 257), (33, 2000, 515), (64, 144, 640),
-         (64, 4100, 130), (77, 2000, 1037), (129, 130, 700), (300, 65, 5), (2000, 200, 6200), (1025, 1029, 10007)]
+         (64, 4100, 130), (77, 2000, 1037), (129, 130, 700), (300, 65, 5), (2000, 200, 6200), (1025, 1029, 10007), (3, 100, 40001), (100, 300, 33000), (300, 77, 40000)]
 
 
 @gpu
@@ -184,31 +184,35 @@ def test_rows_that_lie_far_apart():
 
 @gpu
 def test_from_a_graph_and_on_other_streams():
+    """Captured without anything reserved; graphs captured on one stream run side by side on two, each with its own workspace."""
     import rapid_sampling_amd as sample
     from tests.test_operator_workspaces import fresh_stream
     w, sw = sample.quantize_int8(make(600, 1024, "f32", 1))
-    inputs = [make(M, 1024, "bf16", M) for M in (2, 40)]
+    inputs = [make(M, 1024, "bf16", M) for M in (2, 40, 100)]
     want = [sample.linear_int8(x, w, sw) for x in inputs]
     torch.cuda.synchronize()
-    side = fresh_stream()
+    side, sets = fresh_stream(), []
     with torch.cuda.stream(side):
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=side):
-            with pytest.raises(RuntimeError, match="reserve_workspace"):
-                sample.linear_int8(inputs[1], w, sw)
-            inputs[0].add_(0)
-        sample.reserve_workspace(2, 600)
-        held_in = [x.clone() for x in inputs]
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=side):
-            held = [sample.linear_int8(x, w, sw) for x in held_in]
-    for seed in range(3):
-        for x in held_in:
-            x.copy_(make(x.shape[0], 1024, "bf16", 90 + seed))
+        for _ in range(2):
+            held_in = [x.clone() for x in inputs]
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                held = [sample.linear_int8(x, w, sw) for x in held_in]
+            sets.append((graph, held_in, held))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for seed in range(4):
+        for n, (graph, held_in, held) in enumerate(sets):
+            for x in held_in:
+                x.copy_(make(x.shape[0], 1024, "bf16", 90 + 2 * seed + n))
         torch.cuda.synchronize()
-        graph.replay()
+        for stream, (graph, held_in, held) in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    graph.replay()
         torch.cuda.synchronize()
-        assert all(torch.equal(y, sample.linear_int8(x, w, sw)) for x, y in zip(held_in, held)), seed
+        for graph, held_in, held in sets:
+            assert all(torch.equal(y, sample.linear_int8(x, w, sw)) for x, y in zip(held_in, held)), seed
     # products of either kind take turns at one workspace
     w8, s8 = sample.quantize_fp8(make(600, 1024, "f32", 1), block_rows=128)
     fp8 = sample.linear_fp8(inputs[1], w8, s8)
