@@ -586,6 +586,8 @@ int rs_lay_out_rows(const void *x_device, int64_t x_row_stride, int32_t size, in
  * Tokens are int32 or (tokens_64 = 1) int64, token_stride elements apart.  stats:
  * NULL, or (M, 2) floats, 8-byte aligned, for the gradient.  A row whose logits are
  * all -inf has lse -inf and loss +inf; one with a NaN or +inf among them NaN.
+ * (Values of float32 are taken apart into three of bfloat16, exactly, and an
+ * infinity among x or w makes NaN.)
  * M up to RS_LINEAR_MAX, V up to 1048576, K up to RS_LOSS_COLUMNS_MAX, and
  * ceil(M / 64) ceil(V / 128), ceil(M / 64) ceil(K / 128) and ceil(V / 128) ceil(K / 128)
  * below 2^24.
@@ -605,7 +607,8 @@ int rs_linear_cross_entropy(const void *x_device, int64_t x_row_stride, const vo
  * With g the gradient of the losses and h that of lse (either may be NULL: none; a
  * stride of 1, or of 0: one number for all rows), p the probabilities:
  *   G = ((g + h) p - g [v = t]) / temperature     grad_x = G w     grad_w = G^T x
- * G is rounded to the inputs' type; sums are float32, and rounded once.  A negative
+ * G is rounded to the inputs' type (of up to 32 rows what that leaves, rounded so
+ * as well, is multiplied beside it); sums are float32, and rounded once.  A negative
  * token has no g, one of V or more has NaN for it.  The other arguments as in the
  * call whose stats are passed.
  */

@@ -44,6 +44,34 @@ transposed weight, whose blocks are the weight's own, in rows that begin at mult
     transposed = transposed.view(torch.float8_e4m3fn)[:, :N]
     grad_x = sample.linear_fp8(grad, transposed, weight_scale.t().contiguous())
 
+At the two ends of the vocabulary's table:
+
+    x = sample.embedding(tokens, table, scale)               # tokens -> hidden states
+    out = sample.linear_cross_entropy(hidden, table, tokens) # hidden states -> loss, without the logits
+    q, s = sample.quantize_int8(table)                       # once, for serving: 8-bit integers, a scale for each row
+    logits = sample.linear_int8(hidden, q, s)
+
+`embedding(tokens, weight, scale=1.0, *, weight_scale=None, out_dtype=None)` gives scale * weight[token] for int32 or int64
+tokens of any shape; a negative token's row is 0, that of a token outside the vocabulary NaN.  weight is (V, K) in float32,
+bfloat16 or float16, or in 8 bits with weight_scale= as `quantize_int8(w)` or `quantize_fp8(w, block_rows=128)` made them (float32 results by
+default).  The gradient of a table that is not in 8 bits is summed in float32 in the tokens' order, the same on every run, and
+written whole: rows that no token names are 0.
+
+`linear_cross_entropy(x, weight, tokens, temperature=1.0)`: x (..., K) and weight (V, K) of one type, tokens (...).  `logsumexp` is
+ln sum e^(x . w / temperature), `loss` that minus the token's own x . w / temperature; 0 for a negative token, NaN for one
+outside the vocabulary.  Both have gradients by x and weight (once, in reverse mode; logsumexp's for an auxiliary loss).  The
+logits are never kept: the vocabulary is worked through in pieces of up to 128 MB of what takes their place (8192 columns at least), and made
+again in the backward pass.  What multiplies the operands there is rounded to their type (up to 32 rows: and what the rounding leaves
+multiplies them as well), all sums are float32.  float32 operands are taken apart into three bfloat16 numbers each, whose products keep 24 bits.
+
+`quantize_int8(x)` gives integers from -127 to 127 with a float32 scale for each row (a row with a NaN or an infinity:
+scale NaN), and `linear_int8(x, weight, weight_scale, *, x_scale=None, out_dtype=torch.float32)` x @ weight.T for such a weight; x in float32, bfloat16 or
+float16 is rounded so within the call, or is given so with x_scale=.  The sums are exact (K up to 131071), so a row's results do
+not depend on what stands beside it.  No gradient, as linear_fp8.
+
+`linear_int8` shares linear_fp8's workspace of a stream, which its first call there or `reserve_workspace` makes; captured into a graph it has one of its own,
+as the others have their scratch memory: nothing needs to be reserved for any of these before a capture.
+
 The functions live in the compiled extension `_sample` (host layer in
 csrc/sampling.cpp, kernels in csrc/rs_*.hip and csrc/rs_*.h behind the C ABI of
 include/rapid_sampling.h).  There is no Python or CPU fallback: without the

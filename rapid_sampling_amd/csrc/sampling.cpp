@@ -1013,8 +1013,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> batch_sampling_debug(
 }
 
 // Allocates and clears the workspaces of the current stream of `device`: the sampler's, for calls of up to B rows of up to V tokens (a V
-// that the sampler does not take, for the next that it does), and, unless `operators` is false, those of token_logprobs and linear_fp8
-// (12.6 MB, whatever the sizes).  Needed before a stream capture (nothing may be allocated while capturing); otherwise
+// that the sampler does not take, for the next that it does), and, unless `operators` is false, those of token_logprobs and of linear_fp8
+// and linear_int8 (12.6 MB, whatever the sizes).  Needed before a stream capture (nothing may be allocated while capturing); otherwise
 // optional: the first call of a shape does the same.
 void reserve_workspace(int64_t B, int64_t V, std::optional<int64_t> device, bool operators)
 {
