@@ -639,8 +639,8 @@ int rs_quantize_rows(const void *x_device, int32_t x_dtype, int64_t x_row_stride
  * float32, rounded to y's type, and is the same whatever rows stand beside it.  Rows of x and
  * w 16-byte aligned; bytes behind column K are not looked at.  workspace: as
  * rs_linear_blocks', and calls of either may share it on one stream.  M and N at most
- * RS_LINEAR_MAX, and ceil(M / 64) ceil(N / 128) below 2^24.  One launch.  No counterpart
- * in the reference.
+ * RS_LINEAR_MAX, and ceil(M / 64) ceil(N / 128) below 2^24; with rows of x or w more
+ * than 16 MB apart M at most 524288.  One launch.  No counterpart in the reference.
  */
 #define RS_LINEAR_INT8_COLUMNS_MAX 131071
 int rs_linear_int8(const int8_t *x_device, int64_t x_row_stride, const float *x_scale_device,

@@ -58,12 +58,18 @@ RS_KERNELS(RS_DTYPE_F32)
 RS_KERNELS(RS_DTYPE_BF16)
 RS_KERNELS(RS_DTYPE_F16)
 
+static bool near(const Int8Params &p) { return p.x_stride <= kTileStride && p.w_stride <= kTileStride; }
+
 template <int DT> static void launch_product(const Int8Params &p, hipStream_t st)
 {
-    // Up to 16 rows one 16 x 16 product holds them all; of a large weight the tiles' loads, whole rows of 128 bytes, read faster (K = 4096, weights
-    // beyond the caches, 1 and 16 rows: N = 4096 6.8 and 7.3 us against 13.9 and 14.1, 16384 17.1 and 19.4 against 21.2 and 19.8, 65536 54.4
-    // and 67 against 52.8 and 52.6).  (The tiles' kernel reaches its rows with 32 bits.)
-    if ((p.M <= 16 && p.N <= 32768) || p.x_stride > kTileStride || p.w_stride > kTileStride) return launch_few<DT, -1>(p, st);
+    // Sixteen rows by sixteen of w, whose whole rows a workgroup reads and with nothing to join, where there are no more of them than the chip has
+    // places for and not many columns; up to 16 rows w is read once all the same, but the tiles' loads, whole lines of 128 bytes, read a large
+    // one faster.  (us, weights beyond the caches, few against tiles.  1, 16 rows, K = 4096: N = 4096 6.8, 7.3 and 13.9, 14.1; 16384 17.1, 19.4
+    // and 21.2, 19.8; 65536 54.4, 67 and 52.8, 52.6; 16 rows, K = 14336: N = 4096 18.6 and 21, 8192 37.6 and 28.  32, 64 rows, K = 1024: N = 4096
+    // 5.3, 7.0 and 8.3, 8.3; 8192 7.7, 12.2 and 8.9, 8.9; K = 4096: 1024 6.7, 6.7 and 12, 12; 4096 12.1, 21.2 and 14.7, 14.7; K = 14336, 17
+    // rows: 4096 32.8 and 21.)  (The tiles' kernel reaches its rows with 32 bits.)
+    const uint64_t blocks = tiles_of(p.M, p.N, 16, 16), most = blocks * p.K;
+    if ((p.M <= 16 ? most <= 96u << 16 : blocks <= 1024 && most <= 32u << 16) || !near(p)) return launch_few<DT, -1>(p, st);
     // Where there are few tiles they are small ones, and their columns are shared out.
     const TileSize size = tiles_of(p.M, p.N, 128, 128) < 192 ? kSmall : tile_size(p.M, p.N);
     if (size == kLarge) launch_tiles<DT, 2, 4, 8, 4, 2, false>(p, st);
@@ -125,6 +131,7 @@ int rs_linear_int8(const int8_t *x, int64_t x_row_stride, const float *x_scale, 
         ((uintptr_t)x_scale & 3) || ((uintptr_t)w_scale & 3) || ((uintptr_t)y & (y_dtype == RS_DTYPE_F32 ? 3 : 1)))
         return RS_ERR_ALIGN;
     const Int8Params p = int8_params(x, x_row_stride, x_scale, w, w_row_stride, w_scale, M, N, K, y, y_row_stride, workspace);
+    if (!near(p) && M > 1 << 19) return RS_ERR_SHAPE;                                // (the second axis of a launch)
     const hipStream_t st = (hipStream_t)stream;
     if (y_dtype == RS_DTYPE_F32) launch_product<RS_DTYPE_F32>(p, st);
     else if (y_dtype == RS_DTYPE_BF16) launch_product<RS_DTYPE_BF16>(p, st);

@@ -435,11 +435,11 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
 
 // ------------------------------------------------------- values and products in 8 bits --
 
-at::Tensor rows_of_16_bytes(std::vector<int64_t> sizes, const at::Device &device, at::ScalarType type = at::kFloat8_e4m3fn)
+at::Tensor rows_of_16_bytes(std::vector<int64_t> sizes, const at::Device &device)
 {
     const int64_t K = sizes.back();
     sizes.back() = (K + 15) / 16 * 16;
-    return at::empty(sizes, at::TensorOptions().dtype(type).device(device)).narrow(-1, 0, K);
+    return at::empty(sizes, at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(device)).narrow(-1, 0, K);
 }
 
 // Values to be rounded to 8 bits, (..., K); the rows of the result lie (K + 15) / 16 * 16 bytes apart.
@@ -572,6 +572,10 @@ at::Tensor scratch(size_t bytes, const at::Tensor &like)
     return at::empty({(int64_t)std::max<size_t>(bytes, 1)}, at::TensorOptions().dtype(at::kByte).device(like.device()));
 }
 
+// From a row of integers to the next: a multiple of 16 bytes, and of 128 where that is little more, so that no row shares its cache lines with others
+// (77 rows with 50257 x 2000 integers: 34.9 us, with 50257 x 2048 26.1).
+int64_t row_bytes(int64_t K) { return K < 1024 ? (K + 15) / 16 * 16 : (K + 127) / 128 * 128; }
+
 std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor &x)
 {
     refuse_tangent("quantize_int8", {x});
@@ -580,12 +584,14 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor &x)
         throw std::invalid_argument("quantize_int8 has no gradient: call it under torch.no_grad(), or on x.detach() !\n");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     const int64_t K = x.size(-1), rows = x.numel() / K;
-    at::Tensor q = rows_of_16_bytes(x.sizes().vec(), x.device(), at::kChar);
+    std::vector<int64_t> sizes = x.sizes().vec();
+    sizes.back() = row_bytes(K);
+    at::Tensor q = at::empty(sizes, at::TensorOptions().dtype(at::kChar).device(x.device())).narrow(-1, 0, K);
     at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), at::TensorOptions().dtype(at::kFloat).device(x.device()));
     if (!rows) return {q, scale};
     const at::Tensor flat = x.dim() == 2 ? x : x.reshape({rows, K});
     const int rc = rs_quantize_rows(flat.data_ptr(), float_dtype(x, "x"), flat.stride(0), (int32_t)rows, (int32_t)K, (int8_t *)q.data_ptr(),
-                                    (K + 15) / 16 * 16, scale.data_ptr<float>(), current_stream(x));
+                                    row_bytes(K), scale.data_ptr<float>(), current_stream(x));
     if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
     return {q, scale};
 }
@@ -637,7 +643,7 @@ at::Tensor linear_rows(const at::Tensor &x, const at::Tensor &weight, const at::
     at::Tensor held;
     const int8_t *q;
     const float *scale;
-    int64_t q_stride = (K + 15) / 16 * 16;
+    int64_t q_stride = row_bytes(K);
     if (given) {
         check_row_scale(*x_scale, x, "x_scale");
         held = fp8_rows(x, "x", "quantize_int8");

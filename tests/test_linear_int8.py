@@ -90,7 +90,8 @@ def test_quantize_halfway_between_two_integers(exponent):
 
 # few rows (one and two rows of w's fragments to a wave), small tiles whole and shared, large tiles; odd sizes of everything
 SIZES = [(1, 16, 1), (1, 100, 50), (1, 4096, 9000), (2, 128, 16), (3, 127, 8193), (4, 8192, 70), (16, 1000, 257), (17, 1000, 257), (33, 2000, 515), (64, 144, 640),
-         (64, 4100, 130), (77, 2000, 1037), (129, 130, 700), (300, 65, 5), (2000, 200, 6200), (1025, 1029, 10007), (3, 100, 40001), (100, 300, 33000), (300, 77, 40000)]
+         (64, 4100, 130), (77, 2000, 1037), (129, 130, 700), (300, 65, 5), (2000, 200, 6200), (1025, 1029, 10007), (3, 100, 40001), (100, 300, 33000), (300, 77, 40000),
+         (64, 8200, 1300), (77, 2000, 5037), (33, 515, 9001), (20, 40001, 1000), (129, 130, 3700), (16, 15000, 7000)]
 
 
 @gpu
@@ -187,8 +188,8 @@ def test_from_a_graph_and_on_other_streams():
     """Captured without anything reserved; graphs captured on one stream run side by side on two, each with its own workspace."""
     import rapid_sampling_amd as sample
     from tests.test_operator_workspaces import fresh_stream
-    w, sw = sample.quantize_int8(make(600, 1024, "f32", 1))
-    inputs = [make(M, 1024, "bf16", M) for M in (2, 40, 100)]
+    w, sw = sample.quantize_int8(make(1200, 16384, "f32", 1))               # (whose columns are shared out, from 17 rows on)
+    inputs = [make(M, 16384, "bf16", M) for M in (2, 40, 100)]
     want = [sample.linear_int8(x, w, sw) for x in inputs]
     torch.cuda.synchronize()
     side, sets = fresh_stream(), []
@@ -204,7 +205,7 @@ def test_from_a_graph_and_on_other_streams():
     for seed in range(4):
         for n, (graph, held_in, held) in enumerate(sets):
             for x in held_in:
-                x.copy_(make(x.shape[0], 1024, "bf16", 90 + 2 * seed + n))
+                x.copy_(make(x.shape[0], 16384, "bf16", 90 + 2 * seed + n))
         torch.cuda.synchronize()
         for stream, (graph, held_in, held) in zip(streams, sets):
             with torch.cuda.stream(stream):
@@ -214,7 +215,7 @@ def test_from_a_graph_and_on_other_streams():
         for graph, held_in, held in sets:
             assert all(torch.equal(y, sample.linear_int8(x, w, sw)) for x, y in zip(held_in, held)), seed
     # products of either kind take turns at one workspace
-    w8, s8 = sample.quantize_fp8(make(600, 1024, "f32", 1), block_rows=128)
+    w8, s8 = sample.quantize_fp8(make(1200, 16384, "f32", 1), block_rows=128)
     fp8 = sample.linear_fp8(inputs[1], w8, s8)
     for _ in range(5):
         assert torch.equal(sample.linear_int8(inputs[1], w, sw), want[1]) and torch.equal(sample.linear_fp8(inputs[1], w8, s8), fp8)
@@ -273,7 +274,7 @@ def test_refusals_of_the_c_abi():
     assert linear(x=None) == linear(w=None) == linear(y=None) == linear(sx=None) == linear(sw=None) == linear(ws_at=None) == -4 and linear(dtype=7) == -7
     assert linear(ws_at=264) == linear(ws_bytes=n - 1) == -5
     assert linear(M=0) == linear(N=0) == linear(K=0) == linear(xs=16) == linear(ws=16) == linear(ys=19) == linear(K=131072, xs=1 << 18, ws=1 << 18) == -12
-    assert linear(M=1 << 24, N=1 << 16, ys=1 << 16) == linear(M=1 << 25) == -12
+    assert linear(M=1 << 24, N=1 << 16, ys=1 << 16) == linear(M=1 << 25) == linear(M=(1 << 19) + 1, ws=1 << 25) == -12
     assert linear(x=264) == linear(w=260) == linear(xs=40) == linear(ws=40) == linear(y=258) == -6
 
     def rows(x=256, dtype=0, xs=20, w=256, ws=32, sw=256, M=2, N=20, K=20, y=256, y_dtype=0, ys=20):
