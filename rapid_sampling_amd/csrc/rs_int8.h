@@ -117,14 +117,13 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Params p)
 #pragma unroll
     for (int u = 0; u < NT; ++u) w[u] = (const uint8_t *)p.w + (int64_t)min(n0 + u * 16u + i, p.N - 1u) * p.w_stride;
     struct Block { v4i w[NT][2], x[2]; };
-    // (w is read once and need not stay in the caches; x is read by every workgroup)
     auto load = [&](uint32_t kb, Block &b) {
         const uint32_t k = kb * 128u + part * 16u;
         const bool whole = kb * 128u + 128u <= p.K;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int u = 0; u < NT; ++u) b.w[u][h] = whole ? __builtin_nontemporal_load((const v4i *)(w[u] + k + 64 * h)) : load16(w[u], k + 64u * h, p.K);
+            for (int u = 0; u < NT; ++u) b.w[u][h] = whole ? *(const v4i *)(w[u] + k + 64 * h) : load16(w[u], k + 64u * h, p.K);
             if constexpr (XT < 0) b.x[h] = whole ? *(const v4i *)(x + k + 64 * h) : load16(x, k + 64u * h, p.K);
         }
     };
