@@ -46,14 +46,21 @@ __device__ __forceinline__ float row_scale(uint32_t peak)
 {
     return peak < 0x7F800000u ? fmaxf(__uint_as_float(peak) * (1.0f / 127.0f), 0x1p-126f) : __builtin_nanf("");
 }
+// (with 1.5 2^23 added a number's integer, to the nearest and ties to even, is in the lowest bits of the sum)
 __device__ __forceinline__ uint2 quantize8_int8(const float (&x)[8], float scale)
 {
     if (!(scale < __builtin_inff())) return make_uint2(0u, 0u);
     const Divisor d(scale);
-    uint32_t w[2] = {0, 0};
+    uint32_t v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j / 4] |= ((uint32_t)(int)__builtin_rintf(d(x[j])) & 0xFFu) << (8 * (j % 4));
-    return make_uint2(w[0], w[1]);
+    for (int j = 0; j < 8; ++j) {
+        const float up = x[j] * d.up, q = up * d.r;                              // as Divisor, but for the sign of 0
+        v[j] = __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, d.s, up), d.r, q) + 12582912.0f);
+    }
+    auto four = [](uint32_t a, uint32_t b, uint32_t c, uint32_t e) {
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(e, c, 0x0C0C0400u), __builtin_amdgcn_perm(b, a, 0x0C0C0400u), 0x05040100u);
+    };
+    return make_uint2(four(v[0], v[1], v[2], v[3]), four(v[4], v[5], v[6], v[7]));
 }
 
 // LANES threads to a row (64 or 256), eight values at a time; the first PIECES of a thread's are kept in registers, the others read again.
@@ -103,19 +110,18 @@ __global__ __launch_bounds__(256) void int8_rows_kernel(Int8Rows p)
 // their sums go through LDS once, at the end.  A wave asks for its next block before it multiplies the one it has.
 //
 // XT < 0: x is in 8 bits.  Else it is of that type, and every workgroup rounds all of it (a few rows) into LDS while its first rows of w
-// are on their way: one launch in the place of two.
+// are on their way: one launch in the place of two.  Such workgroups are no more than the chip holds, and go from one stretch of w
+// to another.
 template <int DT, int XT, int NT>
 __global__ __launch_bounds__(512) void int8_few_kernel(Int8Params p)
 {
     __shared__ v4i sums[8][NT][64];
-    __shared__ uint32_t peaks[8][4];
+    __shared__ uint32_t peaks[4];
     extern __shared__ char lds[];
     const uint32_t lane = threadIdx.x % 64u, wave = wave_id(), waves = blockDim.x / 64u, i = lane % 16u, part = lane / 16u;
-    const uint32_t n0 = blockIdx.x * (16u * NT), m0 = blockIdx.y * 16u, blocks = (p.K + 127u) / 128u;
+    const uint32_t m0 = blockIdx.y * 16u, blocks = (p.K + 127u) / 128u, stretches = (p.N + 16u * NT - 1u) / (16u * NT);
     const uint32_t m = min(m0 + i, p.M - 1u);
     const uint8_t *w[NT], *x = XT < 0 ? (const uint8_t *)p.x + (int64_t)m * p.x_stride : (const uint8_t *)lds + m * (blocks * 128u);
-#pragma unroll
-    for (int u = 0; u < NT; ++u) w[u] = (const uint8_t *)p.w + (int64_t)min(n0 + u * 16u + i, p.N - 1u) * p.w_stride;
     struct Block { v4i w[NT][2], x[2]; };
     auto load = [&](uint32_t kb, Block &b) {
         const uint32_t k = kb * 128u + part * 16u;
@@ -127,47 +133,68 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Params p)
             if constexpr (XT < 0) b.x[h] = whole ? *(const v4i *)(x + k + 64 * h) : load16(x, k + 64u * h, p.K);
         }
     };
+    Block now, next;
+    uint32_t turn = 0;
+    auto turned = [&](uint32_t kb) { kb += turn; return kb < blocks ? kb : kb - blocks; };
     // (every workgroup begins at another block: rows are usually a power of two of bytes apart, and workgroups in step would ask the same
     // memory channels at a time)
-    const uint32_t turn = blockIdx.x % blocks;
-    auto turned = [&](uint32_t kb) { kb += turn; return kb < blocks ? kb : kb - blocks; };
-    Block now, next;
-    if (wave < blocks) load(turned(wave), now);
-    if constexpr (XT >= 0) {
-        float held[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto begin = [&](uint32_t stretch) {
+        turn = stretch % blocks;
 #pragma unroll
-        for (uint32_t r = 0; r < 4; ++r) {
-            if (r >= p.M) break;
-            uint32_t peak = 0;
-            for (uint32_t k = threadIdx.x * 8u; k < p.K; k += blockDim.x * 8u) {
-                float v[8];
-                load8<XT < 0 ? 0 : XT>(p.x, (int64_t)r * p.x_stride, k, p.K, v);
-                peak = max(peak, largest_bits(v));
-            }
+        for (int u = 0; u < NT; ++u) w[u] = (const uint8_t *)p.w + (int64_t)min((stretch * NT + u) * 16u + i, p.N - 1u) * p.w_stride;
+        if (wave < blocks) load(turned(wave), now);
+    };
+    begin(blockIdx.x);
+    if constexpr (XT >= 0) {
+        // The waves are shared out among the rows, and of its row a wave takes pieces of 512 values in turn, the first of which it keeps in
+        // registers; where there are more rows than waves (of up to 384 columns) it takes a piece, and all, of several.
+        constexpr uint32_t kHeld = 4;
+        const uint32_t high = p.M <= 2u ? p.M : 4u, each = max(waves / high, 1u), step = waves / each, pieces = (blocks + 3u) / 4u;
+        const uint32_t row = wave / each, sub = wave % each;
+        const bool several = waves < high;
+        const uint32_t count = row >= p.M ? 0u : several ? (p.M - row + step - 1u) / step : sub >= pieces ? 0u : (pieces - sub + each - 1u) / each;
+        auto row_of = [&](uint32_t e) { return several ? row + e * step : row; };
+        auto first_of = [&](uint32_t e) { return (several ? 0u : (sub + e * each) * 512u) + lane * 8u; };
+        float held[kHeld][8];
+        auto fetch = [&](uint32_t e, float (&v)[8]) { load8<XT>(p.x, (int64_t)row_of(e) * p.x_stride, first_of(e), p.K, v); };
+        uint32_t peak = 0;
+        auto note = [&](uint32_t e, const float (&v)[8]) {
+            peak = max(peak, largest_bits(v));
+            if (!several && e + 1u < count) return;
 #pragma unroll
             for (int d = 32; d; d >>= 1) peak = max(peak, (uint32_t)__shfl_xor((int)peak, d));
-            if (lane == 0) peaks[wave][r] = peak;
+            if (lane == 0) atomicMax(&peaks[row_of(e)], peak);
+            peak = 0;
+        };
+        auto put_piece = [&](uint32_t e, const float (&v)[8]) {
+            const uint32_t k = first_of(e);
+            if (k < blocks * 128u) *(uint2 *)(lds + row_of(e) * (blocks * 128u) + k) = quantize8_int8(v, row_scale(peaks[row_of(e)]));
+        };
+#pragma unroll
+        for (uint32_t h = 0; h < kHeld; ++h)
+            if (h < count) fetch(h, held[h]);
+        if (threadIdx.x < 4u) peaks[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t h = 0; h < kHeld; ++h)
+            if (h < count) note(h, held[h]);
+        for (uint32_t e = kHeld; e < count; ++e) {
+            float v[8];
+            fetch(e, v);
+            note(e, v);
         }
         __syncthreads();
 #pragma unroll
-        for (uint32_t r = 0; r < 4; ++r) {
-            if (r >= p.M) break;
-            uint32_t peak = 0;
-            for (uint32_t o = 0; o < waves; ++o) peak = max(peak, peaks[o][r]);
-            held[r] = row_scale(peak);
-            for (uint32_t k = threadIdx.x * 8u; k < blocks * 128u; k += blockDim.x * 8u) {
-                float v[8];
-                load8<XT < 0 ? 0 : XT>(p.x, (int64_t)r * p.x_stride, k, p.K, v);
-                *(uint2 *)(lds + r * (blocks * 128u) + k) = quantize8_int8(v, held[r]);
-            }
-            if (threadIdx.x == 0) ((float *)(lds + p.M * (blocks * 128u)))[r] = held[r];
+        for (uint32_t h = 0; h < kHeld; ++h)
+            if (h < count) put_piece(h, held[h]);
+        for (uint32_t e = kHeld; e < count; ++e) {
+            float v[8];
+            fetch(e, v);
+            put_piece(e, v);
         }
         __syncthreads();
     }
-    v4i acc[NT];
-#pragma unroll
-    for (int u = 0; u < NT; ++u) acc[u] = v4i{0, 0, 0, 0};
-    auto take = [&](Block &b, uint32_t kb) {
+    auto take = [&](Block &b, uint32_t kb, v4i (&acc)[NT]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if constexpr (XT >= 0) b.x[h] = *(const v4i *)(x + kb * 128u + part * 16u + 64 * h);
@@ -175,30 +202,41 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Params p)
             for (int u = 0; u < NT; ++u) acc[u] = multiply<kInt8>(b.w[u][h], b.x[h], acc[u]);
         }
     };
-    if (wave < blocks) {
-        uint32_t kb = turned(wave);
-        for (uint32_t j = wave + waves; j < blocks; j += waves) {
-            const uint32_t following = turned(j);
-            load(following, next);
-            take(now, kb);
-            now = next;
-            kb = following;
+    for (uint32_t stretch = blockIdx.x;;) {
+        v4i acc[NT];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) acc[u] = v4i{0, 0, 0, 0};
+        if (wave < blocks) {
+            uint32_t kb = turned(wave);
+            for (uint32_t j = wave + waves; j < blocks; j += waves) {
+                const uint32_t following = turned(j);
+                load(following, next);
+                take(now, kb, acc);
+                now = next;
+                kb = following;
+            }
+            take(now, kb, acc);
         }
-        take(now, kb);
-    }
 #pragma unroll
-    for (int u = 0; u < NT; ++u) sums[wave][u][lane] = acc[u];
-    __syncthreads();
-    for (uint32_t u = wave; u < (uint32_t)NT; u += waves) {
-        v4i s = sums[0][u][lane];
-        for (uint32_t o = 1; o < waves; ++o) s += sums[o][u][lane];
-        const uint32_t row = m0 + i, n = n0 + u * 16u + part * 4u;
-        if (row >= p.M) continue;
-        const float f = XT < 0 ? p.x_scale[row] : ((const float *)(lds + p.M * (blocks * 128u)))[row];
-        v4f y;
+        for (int u = 0; u < NT; ++u) sums[wave][u][lane] = acc[u];
+        const uint32_t n0 = stretch * (16u * NT);
+        stretch += gridDim.x;
+        const bool more = XT >= 0 && stretch < stretches;
+        if (more) begin(stretch);
+        __syncthreads();
+        for (uint32_t u = wave; u < (uint32_t)NT; u += waves) {
+            v4i s = sums[0][u][lane];
+            for (uint32_t o = 1; o < waves; ++o) s += sums[o][u][lane];
+            const uint32_t row = m0 + i, n = n0 + u * 16u + part * 4u;
+            if (row >= p.M) continue;
+            const float f = XT < 0 ? p.x_scale[row] : row_scale(peaks[row]);
+            v4f y;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = in_float32((float)s[j] * (f * p.w_scale[min(n + j, p.N - 1u)]));
-        store_row<DT>(p.y, (int64_t)row * p.y_stride, n, p.N, y);
+            for (int j = 0; j < 4; ++j) y[j] = in_float32((float)s[j] * (f * p.w_scale[min(n + j, p.N - 1u)]));
+            store_row<DT>(p.y, (int64_t)row * p.y_stride, n, p.N, y);
+        }
+        if (!more) return;
+        __syncthreads();
     }
 }
 

@@ -23,11 +23,15 @@ template <int DT> static void launch_rows(const Int8Rows &p, hipStream_t st)
     else launch_rows<DT, 256, 4>(p, st);
 }
 
+// Workgroups that round x for themselves: three to a compute unit at a time (1 row, weights beyond the caches: 65536 x 2048 33.7 us with one to
+// each stretch of w, 31.7 with two to a compute unit, 28.7 with three; 65536 x 4096 53.0, 48.8 and 48.1; 65536 x 8192 105, 104.7 and 104).
+constexpr uint32_t kAtATime = 768;
+
 template <int DT, int XT, int NT> static void launch_few(const Int8Params &p, hipStream_t st)
 {
     const uint32_t blocks = (p.K + 127) / 128, waves = blocks >= 8 ? 8 : blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
-    const uint32_t lds = XT < 0 ? 0 : p.M * (blocks * 128 + 4);
-    hipLaunchKernelGGL((int8_few_kernel<DT, XT, NT>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 15) / 16), dim3(64 * waves), lds, st, p);
+    const uint32_t lds = XT < 0 ? 0 : p.M * blocks * 128, stretches = (p.N + 16 * NT - 1) / (16 * NT);
+    hipLaunchKernelGGL((int8_few_kernel<DT, XT, NT>), dim3(XT < 0 ? stretches : std::min(stretches, kAtATime), (p.M + 15) / 16), dim3(64 * waves), lds, st, p);
 }
 template <int DT, int XT> static void launch_few(const Int8Params &p, hipStream_t st)
 {
