@@ -144,7 +144,10 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Params p)
         for (int u = 0; u < NT; ++u) w[u] = (const uint8_t *)p.w + (int64_t)min((stretch * NT + u) * 16u + i, p.N - 1u) * p.w_stride;
         if (wave < blocks) load(turned(wave), now);
     };
-    begin(blockIdx.x);
+    // (each XCD has a part of w of its own, see Tile::choose: 1 row, 65536 x 2048 29.9 us in plain order, 27.5 so; 65536 x 8192 104 and 100; 65536 x 1024
+    // 16.2 and 17.1)
+    auto place = [&](uint32_t id) { return id % 8u * (stretches / 8u) + min(id % 8u, stretches % 8u) + id / 8u; };
+    begin(place(blockIdx.x));
     if constexpr (XT >= 0) {
         // The waves are shared out among the rows, and of its row a wave takes pieces of 512 values in turn, the first of which it keeps in
         // registers; where there are more rows than waves (of up to 384 columns) it takes a piece, and all, of several.
@@ -202,7 +205,7 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Params p)
             for (int u = 0; u < NT; ++u) acc[u] = multiply<kInt8>(b.w[u][h], b.x[h], acc[u]);
         }
     };
-    for (uint32_t stretch = blockIdx.x;;) {
+    for (uint32_t id = blockIdx.x;;) {
         v4i acc[NT];
 #pragma unroll
         for (int u = 0; u < NT; ++u) acc[u] = v4i{0, 0, 0, 0};
@@ -219,10 +222,10 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Params p)
         }
 #pragma unroll
         for (int u = 0; u < NT; ++u) sums[wave][u][lane] = acc[u];
-        const uint32_t n0 = stretch * (16u * NT);
-        stretch += gridDim.x;
-        const bool more = XT >= 0 && stretch < stretches;
-        if (more) begin(stretch);
+        const uint32_t n0 = place(id) * (16u * NT);
+        id += gridDim.x;
+        const bool more = XT >= 0 && id < stretches;
+        if (more) begin(place(id));
         __syncthreads();
         for (uint32_t u = wave; u < (uint32_t)NT; u += waves) {
             v4i s = sums[0][u][lane];
@@ -298,26 +301,17 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void int8_tile_kernel(Int8Params p
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[u][j] = in_float32((float)acc[u][t][j] * (f * p.w_scale[min(tile.n(u) + j, p.N - 1u)]));
     };
-    if constexpr (DT == RS_DTYPE_F32) {
+    const TileStore<DT, T> out(lds);
 #pragma unroll
-        for (int t = 0; t < T::MT; ++t) {
-            v4f v[T::NU];
-            row_of(t, v);
-            const uint32_t m = tile.m(t);
-            if (m < p.M)
-#pragma unroll
-                for (int u = 0; u < T::NU; ++u) store_row<DT>(p.y, (int64_t)m * p.y_stride, tile.n(u), p.N, v[u]);
-        }
-    } else {
-        const TileStore<DT, T> out(lds);
-#pragma unroll
-        for (int t = 0; t < T::MT; ++t) {
-            v4f v[T::NU];
-            row_of(t, v);
-            out.put(t, v);
-        }
-        out.flush(tile, p.y, p.y_stride, p.M, p.N);
+    for (int t = 0; t < T::MT; ++t) {
+        v4f v[T::NU];
+        row_of(t, v);
+        if constexpr (DT == RS_DTYPE_F32) {
+            out.put(v);
+            out.flush(tile, t, (float *)p.y, p.y_stride, p.M, p.N);
+        } else out.put(t, v);
     }
+    if constexpr (DT != RS_DTYPE_F32) out.flush(tile, p.y, p.y_stride, p.M, p.N);
 }
 
 }  // namespace rs

@@ -632,9 +632,10 @@ at::Tensor linear_rows(const at::Tensor &x, const at::Tensor &weight, const at::
     if (!M) return y;
     void *stream = current_stream(x);
     const int8_t *wq = (const int8_t *)w.data_ptr();
-    // (rounded in the product's own launch, or in one before it: 1 and 4 rows with 16384 x 1024 7.5 and 8.1 us, 10.4 and 10.8; with 65536 x 4096 50.1
-    // and 51.8, 57.2 and 58.1; with 16384 x 8192 34.8 and 36.1, 34.6 and 35.0; with 65536 x 8192 104 and 111, 98 and 99)
-    if (!given && M <= RS_LINEAR_ROWS_MAX && K <= RS_LINEAR_ROWS_COLUMNS_MAX && (K <= 4096 || N <= 16384)) {
+    // (rounded in the product's own launch, or in one before it, us, 1 and 4 rows: with 16384 x 2048 10.1 and 11.4, 12.5 and 13.5; 65536 x 2048 27.5 and
+    // 28.2, 29.0 and 29.0; 65536 x 4096 50.1 and 51.5, 52.2 and 52.7; 131072 x 4096 98.8 and 99.0, 94.2 and 94.9; 4096 x 8192 11.9 and 16.7, 14.2
+    // and 14.9; 16384 x 8192 36.4 and 37.0, 32.7 and 32.4)
+    if (!given && M <= RS_LINEAR_ROWS_MAX && K <= RS_LINEAR_ROWS_COLUMNS_MAX && (K <= 4096 ? N <= 65536 : M * N <= 8192)) {
         const at::Tensor flat = x.dim() == 2 ? x : x.reshape({M, K});
         const int rc = rs_linear_int8_rows(flat.data_ptr(), float_dtype(x, "x"), flat.stride(0), wq, w.stride(0), weight_scale.data_ptr<float>(),
                                            (int32_t)M, (int32_t)N, (int32_t)K, y.data_ptr(), float_dtype(y, "y"), N, stream);
