@@ -60,3 +60,38 @@ def test_differences():
     # two distances cancel the third derivative: (8 (f(h) - f(-h)) - (f(2h) - f(-2h))) / 12 h, off by the fifth; 18 / 12 h of the loss's own error
     got = (8 * (ends[0] - ends[1]) - (wide[0] - wide[1])) / (12 * h)
     assert abs(got - slope) <= 18 / (12 * h) * 64 * 2 ** -24 * loss.item() + 1e-3 * abs(slope)
+
+
+@gpu
+def test_a_captured_step_beside_an_eager_graph():
+    """A training step is captured, and replayed, with both gradients of the table; while an eager graph of the table from another stream lives the
+    capture is refused, and goes through once that is gone."""
+    import rapid_sampling_amd as sample
+    from tests.test_operator_workspaces import fresh_stream
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    table = (torch.randn((3000, 64), generator=gen, device="cuda") * 0.1).requires_grad_()
+    tokens = torch.randint(3000, (700,), generator=gen, device="cuda")
+    eager = sample.embedding(tokens, table)
+    side = fresh_stream()
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            spare = torch.zeros(4, device="cuda")
+            for call in (lambda: sample.embedding(tokens, table), lambda: sample.linear_cross_entropy(table[:700].detach(), table, tokens)):
+                with pytest.raises(RuntimeError, match="another stream lives"):
+                    call()
+            spare.add_(1)
+        del eager
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            loss = sample.linear_cross_entropy(sample.embedding(tokens, table, 2.0), table, tokens).loss.sum()
+            loss.backward()
+    held = table.grad
+    for seed in range(4):
+        tokens.copy_(torch.randint(3000, (700,), generator=gen, device="cuda"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        fresh = table.detach().clone().requires_grad_()
+        sample.linear_cross_entropy(sample.embedding(tokens, fresh, 2.0), fresh, tokens).loss.sum().backward()
+        assert torch.equal(held, fresh.grad), seed
