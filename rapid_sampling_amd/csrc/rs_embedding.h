@@ -165,6 +165,7 @@ __device__ __forceinline__ void sort_part(const SortParams &p, uint32_t from, ui
         }
 #pragma unroll
         for (uint32_t e = 0; e < kSortBatch; ++e) {
+            if (i0 + e * 64u >= to) continue;
             const bool live = i0 + e * 64u + lane < to;
             const uint32_t digit = keys[e] >> p.shift & mask;
             const uint64_t same = same_digit(digit, p.bits, live);

@@ -119,7 +119,8 @@ int rs_embedding_backward(const void *tokens, int32_t tokens_64, int64_t token_s
     p.counts = (uint32_t *)(ws + s.counts);
     const uint32_t lds = (kSortWaves << s.bits) * 4;
     const ClearParams clear{(char *)dw, (uint64_t)V * K * size_of(dw_dtype)};
-    const uint32_t clears = (uint32_t)std::min<uint64_t>(1023, clear.bytes / 65536 + 1);
+    // (64 KB to a workgroup, one behind the other: 1 GiB in 168 us; in 1023 workgroups 189)
+    const uint32_t clears = (uint32_t)std::min<uint64_t>(32767, clear.bytes / 65536 + 1);
     if (p.N <= kSortAlone) {
         p.keys = keys(0); p.at = at(0); p.keys_b = keys(1); p.at_b = at(1);
         hipLaunchKernelGGL(sort_alone_kernel, dim3(1 + clears), dim3(kSortThreads), lds, st, p, clear);
