@@ -27,9 +27,14 @@ template <int WT> static void launch_embedding(const EmbeddingParams &p, int32_t
     else launch_embedding<WT, RS_DTYPE_F16>(p, st);
 }
 
+// Who sorts: one workgroup, while others clear dw, or stretches of the list in three launches for a digit, behind the clearing.  (Gradient of a table of
+// 131072 x 4096, 131072 x 8 and 2000 x 512 in bfloat16, us, one and stretches: 1024 tokens 205, 19, 20 and 227, 31, 27; 8192 230, 47, 35 and 267,
+// 53, 40; 16384 270, 80, 55 and 305, 63, 46; 32768 445, 157, 104 and 361, 68, 54.)
+static bool sorts_alone(uint32_t N, uint64_t clear) { return N <= kSortAlone / 2 || (N <= kSortAlone && clear >= 1ull << 28); }
+
 // Where a gradient's scratch lies.
 struct TableSpace {
-    uint64_t keys[2], at[2], counts, parts, bytes = 0;
+    uint64_t pairs[2], counts, parts, bytes = 0;
     uint32_t digits, bits, chunk, chunks, groups;
     uint64_t take(uint64_t n) { const uint64_t a = bytes; bytes += up(n, 256); return a; }
 };
@@ -40,13 +45,13 @@ static TableSpace table_space(uint32_t N, uint32_t V, uint32_t K)
     while (bits < 32 && (V >> bits)) ++bits;             // of a token, or of V itself
     s.digits = (bits + kSortBits - 1) / kSortBits;
     s.bits = (bits + s.digits - 1) / s.digits;
-    s.groups = N <= kSortAlone ? 1 : (N + kSortTile - 1) / kSortTile;
+    s.groups = (N + kSortTile - 1) / kSortTile;
     // Chunks of up to about the square root of the tokens: a token that makes up all of them has as many chunks to join as each has places.
     s.chunk = 4;
     while (s.chunk < 12 && (1ull << (2 * s.chunk + 4)) <= N) ++s.chunk;
     s.chunks = (N + (1u << s.chunk) - 1) >> s.chunk;
-    for (int i = 0; i < 2; ++i) { s.keys[i] = s.take(4ull * N); s.at[i] = s.take(4ull * N); }
-    s.counts = s.take(N <= kSortAlone ? 0 : 4ull * s.groups << s.bits);
+    for (int i = 0; i < 2; ++i) s.pairs[i] = s.take(8ull * N);
+    s.counts = s.take(N <= kSortAlone / 2 ? 0 : 4ull * s.groups << s.bits);
     s.parts = s.take((uint64_t)s.chunks * 2 * K * 4);
     return s;
 }
@@ -111,8 +116,7 @@ int rs_embedding_backward(const void *tokens, int32_t tokens_64, int64_t token_s
     if (workspace_bytes < s.bytes || ((uintptr_t)workspace & 255)) return RS_ERR_WORKSPACE;
     char *ws = (char *)workspace;
     const hipStream_t st = (hipStream_t)stream;
-    auto keys = [&](uint32_t i) { return (uint32_t *)(ws + s.keys[i]); };
-    auto at = [&](uint32_t i) { return (uint32_t *)(ws + s.at[i]); };
+    auto pairs = [&](uint32_t i) { return (uint2 *)(ws + s.pairs[i]); };
     SortParams p = {};
     p.tokens = TokenList{tokens, token_stride, tokens_64};
     p.N = (uint32_t)M; p.V = (uint32_t)V; p.bits = s.bits; p.first = 1; p.digits = s.digits;
@@ -121,21 +125,21 @@ int rs_embedding_backward(const void *tokens, int32_t tokens_64, int64_t token_s
     const ClearParams clear{(char *)dw, (uint64_t)V * K * size_of(dw_dtype)};
     // (64 KB to a workgroup, one behind the other: 1 GiB in 168 us; in 1023 workgroups 189)
     const uint32_t clears = (uint32_t)std::min<uint64_t>(32767, clear.bytes / 65536 + 1);
-    if (p.N <= kSortAlone) {
-        p.keys = keys(0); p.at = at(0); p.keys_b = keys(1); p.at_b = at(1);
+    if (sorts_alone(p.N, clear.bytes)) {
+        p.out = pairs(0); p.out_b = pairs(1);
         hipLaunchKernelGGL(sort_alone_kernel, dim3(1 + clears), dim3(kSortThreads), lds, st, p, clear);
     } else {
         hipLaunchKernelGGL(clear_kernel, dim3(clears), dim3(kSortThreads), 0, st, clear);
         for (uint32_t d = 0; d < s.digits; ++d) {
-            p.keys = keys(d & 1); p.at = at(d & 1);
+            p.out = pairs(d & 1);
             hipLaunchKernelGGL(sort_count_kernel, dim3(s.groups), dim3(kSortThreads), lds, st, p);
             hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(kSortThreads), 0, st, p.counts, s.groups << s.bits);
             hipLaunchKernelGGL(sort_place_kernel, dim3(s.groups), dim3(kSortThreads), lds, st, p);
-            p.first = 0; p.shift += s.bits; p.keys_in = p.keys; p.at_in = p.at;
+            p.first = 0; p.shift += s.bits; p.in = p.out;
         }
     }
     TableGradParams t;
-    t.keys = keys((s.digits - 1) & 1); t.at = at((s.digits - 1) & 1);
+    t.pairs = pairs((s.digits - 1) & 1);
     t.g = g; t.g_stride = M > 1 ? g_stride : 0; t.parts = (float *)(ws + s.parts); t.dw = dw; t.scale = (float)scale;
     t.N = p.N; t.V = p.V; t.K = (uint32_t)K; t.chunk = s.chunk;
     if (g_dtype == RS_DTYPE_F32) launch_sums<RS_DTYPE_F32>(t, s.chunks, dw_dtype, st);

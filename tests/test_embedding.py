@@ -111,7 +111,7 @@ def check_gradient(w, t, g, scale, got):
 @gpu
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("M,V,K", [(1, 1, 1), (2, 50, 7), (33, 15, 8), (100, 16, 129), (700, 5, 300), (5000, 3000, 64), (16384, 2047, 12), (16385, 2048, 12), (20000, 70000, 9),
-                                   (8193 * 2, 40, 2050)])
+                                   (8193 * 2, 40, 2050), (8192, 300, 5), (8193, 300, 5), (4097, 300, 5)])
 def test_gradient(M, V, K, dtype):
     gen = torch.Generator().manual_seed(M + V)
     w, t = table(V, K, dtype, 1), some_tokens((M,), V, M + 7)
@@ -138,6 +138,21 @@ def test_gradient_of_whole_numbers(M, kind):
     want = torch.zeros((V + 1, K), dtype=torch.float64)
     want.index_add_(0, torch.where(t < 0, V, t).cpu(), g.cpu().double())
     assert torch.equal(got.cpu().double(), want[:-1])
+
+
+@gpu
+@pytest.mark.parametrize("M", [8192, 8193, 16384, 16385])
+def test_gradient_of_whole_numbers_for_a_large_table(M):
+    """280 MB of gradient: one workgroup sorts more tokens.  Whole numbers are exact, in bfloat16 up to 256."""
+    V, K = 70000, 2000
+    gen = torch.Generator().manual_seed(M)
+    t = torch.randint(-1, V + 1, (M,), generator=gen)
+    t[::100] = 69999
+    t, g = t.cuda(), torch.randint(-1, 2, (M, K), generator=gen).bfloat16().cuda()
+    got = gradient(torch.zeros((V, K), dtype=torch.bfloat16, device="cuda"), t, g, 1.0)
+    there = (t >= 0) & (t < V)
+    want = torch.zeros((V, K), device="cuda").index_add_(0, t[there], g[there].float())
+    assert want.abs().max() <= 256 and torch.equal(got.float(), want)
 
 
 @gpu
