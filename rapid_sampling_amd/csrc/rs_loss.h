@@ -41,6 +41,8 @@ struct LossParams {
     void       *grad;                // G: rows of grad_stride bytes
     uint32_t    grad_stride;
     uint32_t    rest;                // 0, or rows from one of G to what its rounding left, rounded too
+    const float *sums;               // [share of the reduction][M][sum_stride] of the product, where it is shared out
+    uint32_t    sum_stride, shares;
 };
 
 __device__ __forceinline__ int64_t loss_token(const LossParams &p, uint32_t m)
@@ -106,6 +108,20 @@ __device__ __forceinline__ float2 join_sums(float2 a, float2 b, float c)
     return make_float2(top, a.y * __builtin_amdgcn_exp2f((a.x - from) * c) + b.y * __builtin_amdgcn_exp2f((b.x - from) * c));
 }
 
+// The row's results, from its maximum, its sum, and the logit of its token if it has one.
+__device__ __forceinline__ void finish_row(const LossParams &p, uint32_t m, float2 sum, float target)
+{
+    const bool none = sum.x == -__builtin_inff() && sum.y == 0.0f;             // no logit above -inf
+    const float ln_s = none ? 0.0f : 0.693147180559945309f * __builtin_log2f(sum.y);
+    const int64_t token = loss_token(p, m);
+    p.lse[m] = none ? -__builtin_inff() : sum.x * p.inv_t + ln_s;
+    float loss = 0.0f;
+    if (token >= (int64_t)p.V) loss = __builtin_nanf("");
+    else if (token >= 0) loss = none ? __builtin_inff() : (sum.x - target) * p.inv_t + ln_s;
+    p.loss[m] = loss;
+    if (p.stats) p.stats[m] = none ? make_float2(0.0f, __builtin_inff()) : sum;
+}
+
 // 2^WIDTH rows to a workgroup, 256 / 2^WIDTH threads to a row (8192 rows of 1024 stretches 62 us, one row 4).
 __global__ __launch_bounds__(256) void loss_join_kernel(LossParams p, uint32_t width)
 {
@@ -119,17 +135,45 @@ __global__ __launch_bounds__(256) void loss_join_kernel(LossParams p, uint32_t w
         __syncthreads();
         if (threadIdx.x < d) held[threadIdx.x] = join_sums(held[threadIdx.x], held[threadIdx.x + d], p.c);
     }
-    if (k || m >= p.M) return;
-    sum = held[threadIdx.x];
-    const bool none = sum.x == -__builtin_inff() && sum.y == 0.0f;             // no logit above -inf
-    const float ln_s = none ? 0.0f : 0.693147180559945309f * __builtin_log2f(sum.y);
+    if (!k && m < p.M) finish_row(p, m, held[threadIdx.x], p.target[m]);
+}
+
+// Where the product has few tiles and a long reduction, workgroups share it out and leave sums (loss_dx_kernel); there are few logits then, and
+// these take up where the tiles end otherwise.  The logits from column v on, a multiple of 4:
+__device__ __forceinline__ v4f shared_sums(const LossParams &p, uint32_t m, uint32_t v)
+{
+    const float *at = p.sums + (int64_t)m * p.sum_stride + v;
+    v4f z = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (uint32_t k = 0; k < p.shares; ++k) z += *(const v4f *)(at + (int64_t)k * p.M * p.sum_stride);
+    return z;
+}
+// Forward: a workgroup to kShared columns of a row (with the product, 64 x 1000 x 4096 in bfloat16, 11.4 us; by tiles alone 31.8).
+constexpr uint32_t kShared = 1024;
+__global__ __launch_bounds__(256) void loss_shares_kernel(LossParams p)
+{
+    __shared__ float2 held[256];
+    __shared__ float target;
+    const uint32_t m = blockIdx.y, v = blockIdx.x * kShared + threadIdx.x * 4u;
     const int64_t token = loss_token(p, m);
-    p.lse[m] = none ? -__builtin_inff() : sum.x * p.inv_t + ln_s;
-    float loss = 0.0f;
-    if (token >= (int64_t)p.V) loss = __builtin_nanf("");
-    else if (token >= 0) loss = none ? __builtin_inff() : (sum.x - p.target[m]) * p.inv_t + ln_s;
-    p.loss[m] = loss;
-    if (p.stats) p.stats[m] = none ? make_float2(0.0f, __builtin_inff()) : sum;
+    float2 sum = make_float2(-__builtin_inff(), 0.0f);
+    if (v < p.V) {
+        const v4f z = shared_sums(p, m, v);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            if (v + j >= p.V) break;
+            sum = join_sums(sum, make_float2(z[j], 1.0f), p.c);
+            if ((int64_t)(v + j) == token) p.target[m] = target = z[j];
+        }
+    }
+    held[threadIdx.x] = sum;
+    for (uint32_t d = 128u; d; d >>= 1) {
+        __syncthreads();
+        if (threadIdx.x < d) held[threadIdx.x] = join_sums(held[threadIdx.x], held[threadIdx.x + d], p.c);
+    }
+    if (threadIdx.x) return;
+    if (gridDim.x > 1u) p.parts[(size_t)blockIdx.x * p.M + m] = held[0];
+    else finish_row(p, m, held[0], target);
 }
 
 // ---------------------------------------------------------------- gradients --
@@ -231,6 +275,32 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
             }
             out.flush(tile, (char *)p.grad + (int64_t)p.rest * p.grad_stride, p.grad_stride / 2u, p.M, p.a.p.rows);
         }
+    }
+}
+
+// The same from shared-out sums: four columns to a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void loss_shares_grad_kernel(LossParams p)
+{
+    const uint32_t m = blockIdx.y, v = blockIdx.x * kShared + threadIdx.x * 4u;
+    if (v >= p.V) return;
+    const LossRow r = p.rows[m];
+    v4f g = shared_sums(p, m, v);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        g[j] = r.a * __builtin_amdgcn_exp2f((g[j] - r.max) * p.c);
+        if ((int32_t)(v + j) == r.token) g[j] -= r.b;
+    }
+    char *row = (char *)p.grad + (int64_t)m * p.grad_stride;
+    store_row<DT>(row, 0, v, p.V, g);
+    if constexpr (DT != RS_DTYPE_F32) {
+        if (!p.rest) return;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == RS_DTYPE_BF16) g[j] -= (float)(__bf16)g[j];
+            else g[j] -= (float)(_Float16)g[j];
+        }
+        store_row<DT>(row + (int64_t)p.rest * p.grad_stride, 0, v, p.V, g);
     }
 }
 

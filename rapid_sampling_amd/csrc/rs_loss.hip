@@ -14,6 +14,8 @@ struct LossSpace {
     uint64_t bytes = 0;
     uint32_t piece = 0, split = 1;                      // tokens of a piece; shares of dx's reduction
     uint64_t grad_stride = 0;
+    uint32_t shares = 1;                                // of the product's reduction
+    uint64_t sums = 0, sum_stride = 0;
     uint64_t take(uint64_t n) { const uint64_t at = bytes; bytes += up(n, 256); return at; }
 };
 
@@ -21,12 +23,29 @@ struct LossSpace {
 // to a compute unit (385 rows of 2000 and a piece of 50257 in float16: 128 x 64 164 us, 128 x 128 111).
 static TileSize dx_size(uint64_t rows, uint64_t columns) { return rows <= 64 ? kSmall : tiles_of(rows, columns, 256, 256) >= 192 ? kLarge : kMiddle; }
 
+// Workgroups that share a tile of x w^T: where the tiles leave much of the chip idle and a tile's columns take long.  (Forward, and with gradients, us, in
+// one and shared.  bfloat16: 64 x 1000 x 4096 31.8, 77.5 and 11.4, 39.0; 4 x 16000 x 4096 31.4, 120 and 29.6, 116; 64 x 1000 x 1024 14.7,
+// 40.2 and 10.4, 35.4; of 188 tiles, 64 x 24000 x 4096, 35.7, 172 and 43.2, 193.  float32, whose tiles take four times as long: 64 x 1000 x 4096 148, 321
+// and 18.8, 62.1; 64 x 8000 x 1024 44.5, 118 and 23.9, 77.8; of 188 tiles 156, 511 and 127, 483; of 243, 64 x 31000 x 1024, 45.7, 171 and
+// 44.1, 170.)
+static uint32_t product_shares(uint64_t M, uint64_t V, uint64_t K, int32_t dtype)
+{
+    const uint64_t tiles = tiles_of(M, V, 64, 128);
+    if (tiles >= (dtype == RS_DTYPE_F32 ? 256 : 128)) return 1;
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({512 / tiles, K * size_of(dtype) / kRowBytes / 8, 32}));
+}
+
 // A piece of the vocabulary: G of the piece stays within the last cache (256 MB) with the piece's weights, in steps of 256 tokens and
 // at least 8192, so that the sums of dx that each piece reads and writes again (8 bytes) are little next to its products.
 static LossSpace loss_space(int32_t M, int32_t V, int32_t K, int32_t dtype, bool backward)
 {
     LossSpace s;
     const uint64_t size = size_of(dtype);
+    s.shares = product_shares(M, V, K, dtype);
+    if (s.shares > 1) {
+        s.sum_stride = up(V, 4);
+        s.sums = s.take(s.shares * s.sum_stride * M * 4);
+    }
     if (!backward) {
         s.parts = s.take((up(V, 64) / 64) * (uint64_t)M * sizeof(float2));
         s.target = s.take((uint64_t)M * 4);
@@ -67,6 +86,10 @@ template <class T, class K, class A> static void launch_tiles(K kernel, const A 
     template __global__ void loss_dx_kernel<TILE<DT, true, false>>(GradParams);                                         \
     template __global__ void loss_dw_kernel<TILE<DT, true, true>>(GradParams);
 #define RS_TYPES(TILE) RS_KERNELS(RS_DTYPE_F32, TILE) RS_KERNELS(RS_DTYPE_BF16, TILE) RS_KERNELS(RS_DTYPE_F16, TILE)
+#define RS_SHARED(DT)                                                                                                   \
+    template __global__ void loss_dx_kernel<SmallTile<DT, false, false>>(GradParams);                                   \
+    template __global__ void loss_shares_grad_kernel<DT>(LossParams);
+RS_SHARED(RS_DTYPE_F32) RS_SHARED(RS_DTYPE_BF16) RS_SHARED(RS_DTYPE_F16)
 RS_TYPES(SmallTile)
 RS_TYPES(MiddleTile)
 RS_TYPES(LargeTile)
@@ -86,6 +109,21 @@ template <int DT> static void launch_dw(const GradParams &p, hipStream_t st)
 {
     if (p.a.red <= 256) launch_tiles<MiddleTile<DT, true, true>>(loss_dw_kernel<MiddleTile<DT, true, true>>, p, st);
     else RS_LAUNCH(tile_size, loss_dw_kernel, true, true)
+}
+
+// The product's sums by shares of its reduction.
+template <int DT> static void launch_shares(LossParams &p, const LossSpace &s, char *ws, hipStream_t st)
+{
+    GradParams g = {};
+    g.a = p.a;
+    g.a.split = s.shares;
+    g.y = ws + s.sums;
+    g.y_stride = (int64_t)s.sum_stride;
+    g.part_stride = (int64_t)s.sum_stride * p.M;
+    launch_tiles<SmallTile<DT, false, false>>(loss_dx_kernel<SmallTile<DT, false, false>>, g, st);
+    p.sums = (const float *)(ws + s.sums);
+    p.sum_stride = (uint32_t)s.sum_stride;
+    p.shares = s.shares;
 }
 
 static bool known(int32_t dtype) { return dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16 || dtype == RS_DTYPE_F16; }
@@ -141,7 +179,10 @@ static void backward(LossParams p, const LossSpace &s, Operand x, Operand w, uin
         const char *piece = w.at + (int64_t)v0 * w.stride;
         p.v0 = v0;
         p.a = Product{Operand{piece, w.stride, n}, x, K, 1};
-        launch_grad<DT>(p, st);
+        if (s.shares > 1) {
+            launch_shares<DT>(p, s, ws, st);
+            hipLaunchKernelGGL(loss_shares_grad_kernel<DT>, dim3((p.V + kShared - 1) / kShared, p.M), dim3(256), 0, st, p);
+        } else launch_grad<DT>(p, st);
         GradParams g;
         g.scale = p.scale;
         if (grad_x) {
@@ -210,11 +251,20 @@ int rs_linear_cross_entropy(const void *x, int64_t x_stride, const void *w, int6
     p.c = (float)(1.4426950408889634 / temperature); p.inv_t = (float)(1.0 / temperature);
     p.parts = (float2 *)(ws + s.parts); p.target = (float *)(ws + s.target);
     p.loss = loss; p.lse = lse; p.stats = (float2 *)stats;
-    const uint32_t stretch = tile_size(M, V) == kLarge ? 128 : 64;
-    p.n_parts = (p.V + stretch - 1) / stretch;
-    if (dtype == RS_DTYPE_F32) launch_forward<RS_DTYPE_F32>(p, st);
-    else if (dtype == RS_DTYPE_BF16) launch_forward<RS_DTYPE_BF16>(p, st);
-    else launch_forward<RS_DTYPE_F16>(p, st);
+    if (s.shares > 1) {
+        if (dtype == RS_DTYPE_F32) launch_shares<RS_DTYPE_F32>(p, s, ws, st);
+        else if (dtype == RS_DTYPE_BF16) launch_shares<RS_DTYPE_BF16>(p, s, ws, st);
+        else launch_shares<RS_DTYPE_F16>(p, s, ws, st);
+        p.n_parts = (p.V + kShared - 1) / kShared;
+        hipLaunchKernelGGL(loss_shares_kernel, dim3(p.n_parts, p.M), dim3(256), 0, st, p);
+        if (p.n_parts == 1) return hipGetLastError() == hipSuccess ? RS_OK : RS_ERR_LAUNCH;
+    } else {
+        const uint32_t stretch = tile_size(M, V) == kLarge ? 128 : 64;
+        p.n_parts = (p.V + stretch - 1) / stretch;
+        if (dtype == RS_DTYPE_F32) launch_forward<RS_DTYPE_F32>(p, st);
+        else if (dtype == RS_DTYPE_BF16) launch_forward<RS_DTYPE_BF16>(p, st);
+        else launch_forward<RS_DTYPE_F16>(p, st);
+    }
     uint32_t width = 0;                                  // rows of a workgroup: as many as leave every compute unit one
     while (width < 6 && ((uint32_t)M >> (width + 1)) >= 256) ++width;
     hipLaunchKernelGGL(loss_join_kernel, dim3(((uint32_t)M + (1u << width) - 1) >> width), dim3(256), 0, st, p, width);
