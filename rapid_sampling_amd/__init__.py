@@ -61,8 +61,8 @@ written whole: rows that no token names are 0.
 ln sum e^(x . w / temperature), `loss` that minus the token's own x . w / temperature; 0 for a negative token, NaN for one
 outside the vocabulary.  Both have gradients by x and weight (once, in reverse mode; logsumexp's for an auxiliary loss).  The
 logits are never kept: the vocabulary is worked through in pieces of up to 128 MB of what takes their place (8192 columns at least), and made
-again in the backward pass.  What multiplies the operands there is rounded to their type (up to 32 rows: and what the rounding leaves
-multiplies them as well), all sums are float32.  float32 operands are taken apart into three bfloat16 numbers each, whose products keep 24 bits.
+again in the backward pass.  What multiplies the operands there is rounded to their type (and what the rounding leaves as well, of up to
+32 rows, and at the rows' own tokens of up to 2048), all sums are float32.  float32 operands are taken apart into three bfloat16 numbers each, whose products keep 24 bits.
 
 `quantize_int8(x)` gives integers from -127 to 127 with a float32 scale for each row (a row with a NaN or an infinity:
 scale NaN), and `linear_int8(x, weight, weight_scale, *, x_scale=None, out_dtype=torch.float32)` x @ weight.T for such a weight; x in float32, bfloat16 or

@@ -14,7 +14,8 @@
 
 namespace rs {
 
-constexpr uint32_t kFewRows = 32;    // up to these what G's rounding leaves is kept
+constexpr uint32_t kFewRows = 32;    // up to these what G's rounding leaves is kept; up to kHitRows at the rows' tokens
+constexpr uint32_t kHitRows = 2048;
 
 struct LossRow {                     // of one row, for G
     float   max, a, b;               // M, (g + h) / (S T), g / T
@@ -43,7 +44,13 @@ struct LossParams {
     uint32_t    rest;                // 0, or rows from one of G to what its rounding left, rounded too
     const float *sums;               // [share of the reduction][M][sum_stride] of the product, where it is shared out
     uint32_t    sum_stride, shares;
+    uint2      *order;               // null, or (token, row), by token and row
+    uint32_t   *rank;                // ... and each row's place there
+    float      *hit;                 // ... and what G's rounding left at the token, for each place
+    uint32_t   *starts;              // ... and the first place of a token from kStretch s on, for every s
+    uint32_t    n_starts;
 };
+constexpr uint32_t kStretch = 64, kNoToken = 0x7FFFFFFFu;
 
 __device__ __forceinline__ int64_t loss_token(const LossParams &p, uint32_t m)
 {
@@ -179,10 +186,12 @@ __global__ __launch_bounds__(256) void loss_shares_kernel(LossParams p)
 // ---------------------------------------------------------------- gradients --
 // G in 16 bits is rounded, to bfloat16 with 8 bits of its own size; in float16 it is made so large first (by a power of two, the same
 // for the whole call) that the largest possible is below 2^15, and a probability's share of it is lost from 2^-39 on.  That adds to the
-// gradients' own rounding another of its size (a row's or a column's many are off in all directions: 1.4 times as much in all).  Of few
-// rows, where a gradient can hang on a few numbers of G, what the rounding left is kept as well, as rows of their own behind G's: the
+// gradients' own rounding another of its size (a row's or a column's many are off in all directions: 1.4 times as much in all).  What the
+// rounding left is made up for where few numbers of G make a gradient.  Of up to kFewRows rows it is kept as rows of their own behind G's: the
 // products are then of twice as many rows, and wait for memory all the same (forward and gradients of 1 row of 4096 over 131072 in
-// bfloat16 876 us without, 890 with; of 48 rows it would be 907 and 1012).
+// bfloat16 876 us without, 890 with; of 48 rows it would be 907 and 1012).  Of up to kHitRows that of each row at its own token, the largest of
+// the row as long as it is not learnt, is added to the two products' sums (385 x 50257 x 2000 in float16 498 us without, 520 with, and the
+// errors 1.3 times the result's own rounding and 1.0; of 8192 rows, off by 1.35 to 1.41 times it whatever the data, 28.8 ms and 29.9).
 __global__ __launch_bounds__(1024) void loss_scale_kernel(LossParams p)
 {
     __shared__ float tops[16];
@@ -203,8 +212,48 @@ __global__ __launch_bounds__(1024) void loss_scale_kernel(LossParams p)
     p.scale[1] = __builtin_ldexpf(1.0f, -e);
 }
 
+// Rows and then (with p.order) stretches of the vocabulary: a row's place in the order, and a stretch's start, is the number of tokens that come before it,
+// counted one by one.
+__device__ __forceinline__ void loss_order(const LossParams &p)
+{
+    __shared__ uint4 held[256];
+    const uint32_t row_groups = (p.M + 255u) / 256u, m = blockIdx.x * 256u + threadIdx.x;
+    const bool is_row = blockIdx.x < row_groups;
+    auto key_of = [&](uint32_t j) {
+        const int64_t t = j < p.M ? loss_token(p, j) : -1;
+        return t >= 0 && t < (int64_t)p.V ? (uint32_t)t : kNoToken;
+    };
+    const uint32_t key = is_row ? key_of(m) : (m - row_groups * 256u) * kStretch;
+    uint32_t before = 0;
+    for (uint32_t j0 = 0; j0 < p.M; j0 += 1024u) {
+        __syncthreads();
+        for (uint32_t e = 0; e < 4u; ++e) ((uint32_t *)held)[e * 256u + threadIdx.x] = key_of(j0 + e * 256u + threadIdx.x);
+        __syncthreads();
+        const uint32_t many = (min(p.M - j0, 1024u) + 3u) / 4u;
+        if (is_row && j0 / 1024u == blockIdx.x / 4u)
+#pragma unroll 4
+            for (uint32_t q = 0; q < many; ++q) {
+                const uint4 k = held[q];
+                const uint32_t j = j0 + q * 4u;
+                before += (k.x < key + (j < m)) + (k.y < key + (j + 1u < m)) + (k.z < key + (j + 2u < m)) + (k.w < key + (j + 3u < m));
+            }
+        else {
+            // (equal ones come before if their rows do; behind the last row there is nothing below any key)
+            const uint32_t to = key + (is_row && j0 < m);
+#pragma unroll 8
+            for (uint32_t q = 0; q < many; ++q) {
+                const uint4 k = held[q];
+                before += (k.x < to) + (k.y < to) + (k.z < to) + (k.w < to);
+            }
+        }
+    }
+    if (is_row) { if (m < p.M) { p.order[before] = make_uint2(key, m); p.rank[m] = before; } }
+    else if (m - row_groups * 256u < p.n_starts) p.starts[m - row_groups * 256u] = before;
+}
+
 __global__ __launch_bounds__(256) void loss_rows_kernel(LossParams p)
 {
+    if (p.order) loss_order(p);
     const uint32_t m = blockIdx.x * 256u + threadIdx.x;
     if (m >= p.M) return;
     const float2 st = p.stats[m];
@@ -221,6 +270,15 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossParams p)
 }
 
 // (8192 rows, a piece of 8192 tokens, 4096 columns in bfloat16: 408 us, 1.35 PFLOP/s)
+// What is left of a number when it is rounded to 16 bits; nothing of one that is none.
+template <int DT> __device__ __forceinline__ float rounding_left(float v)
+{
+    float d = 0.0f;
+    if constexpr (DT == RS_DTYPE_BF16) d = v - (float)(__bf16)v;
+    if constexpr (DT == RS_DTYPE_F16) d = v - (float)(_Float16)v;
+    return d == d ? d : 0.0f;
+}
+
 template <class T>
 __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
 {
@@ -236,7 +294,10 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 v[u][j] = r.a * __builtin_amdgcn_exp2f((acc[u][t][j] - r.max) * p.c);
-                if ((int32_t)(tile.n(u) + p.v0 + j) == r.token) v[u][j] -= r.b;
+                if ((int32_t)(tile.n(u) + p.v0 + j) == r.token) {
+                    v[u][j] -= r.b;
+                    if (T::DT != RS_DTYPE_F32 && p.hit && tile.m(t) < p.M) p.hit[p.rank[tile.m(t)]] = rounding_left<T::DT>(v[u][j]);
+                }
             }
     };
     if constexpr (T::DT == RS_DTYPE_F32) {
@@ -267,10 +328,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
 #pragma unroll
                 for (int u = 0; u < T::NU; ++u)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if constexpr (T::DT == RS_DTYPE_BF16) v[u][j] -= (float)(__bf16)v[u][j];
-                        else v[u][j] -= (float)(_Float16)v[u][j];
-                    }
+                    for (int j = 0; j < 4; ++j) v[u][j] = rounding_left<T::DT>(v[u][j]);
                 out.put(t, v);
             }
             out.flush(tile, (char *)p.grad + (int64_t)p.rest * p.grad_stride, p.grad_stride / 2u, p.M, p.a.p.rows);
@@ -289,17 +347,17 @@ __global__ __launch_bounds__(256) void loss_shares_grad_kernel(LossParams p)
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
         g[j] = r.a * __builtin_amdgcn_exp2f((g[j] - r.max) * p.c);
-        if ((int32_t)(v + j) == r.token) g[j] -= r.b;
+        if ((int32_t)(v + j) == r.token) {
+            g[j] -= r.b;
+            if (p.hit) p.hit[p.rank[m]] = rounding_left<DT>(g[j]);
+        }
     }
     char *row = (char *)p.grad + (int64_t)m * p.grad_stride;
     store_row<DT>(row, 0, v, p.V, g);
     if constexpr (DT != RS_DTYPE_F32) {
         if (!p.rest) return;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (DT == RS_DTYPE_BF16) g[j] -= (float)(__bf16)g[j];
-            else g[j] -= (float)(_Float16)g[j];
-        }
+        for (int j = 0; j < 4; ++j) g[j] = rounding_left<DT>(g[j]);
         store_row<DT>(row + (int64_t)p.rest * p.grad_stride, 0, v, p.V, g);
     }
 }
@@ -311,6 +369,11 @@ struct GradParams {
     const float *scale;              // null, or [1]: factor of the result
     int32_t      add;                // to what is there
     int64_t      part_stride;        // elements between the sums of the workgroups that share the reduction
+    const float *hit;                // dw: null, or as in LossParams, with x and the piece's first token
+    const uint2 *order;
+    const uint32_t *starts;
+    uint32_t     n_starts, v0;
+    Operand      x;
 };
 
 // dx's sums of one piece of the vocabulary, in float32; every share of the reduction has sums of its own.  (The same piece: 458 us, 1.2 PFLOP/s.  w's
@@ -344,6 +407,52 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_dx_kernel(GradParams p)
     }
 }
 
+template <int DT> __device__ __forceinline__ float widen16(uint32_t v)
+{
+    if constexpr (DT == RS_DTYPE_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)v);
+    else return __uint_as_float(v << 16);
+}
+
+// What G's rounding left at the tokens of a tile of dw: the rows' x, as much of them as the tile holds, by way of LDS.
+template <class T> __device__ __forceinline__ void add_hits(const GradParams &p, const T &tile, char *lds, typename T::Acc &acc)
+{
+    constexpr uint32_t kBatch = 32, kPieces = T::kTileN / 8u;
+    static_assert(kBatch * (T::kTileN * 2u + 8u) <= T::kLds, "where the stages were");
+    uint2 *list = (uint2 *)(lds + kBatch * T::kTileN * 2u);                      // (token, what is left)
+    const uint32_t s = (p.v0 + tile.m0) / kStretch, K = p.a.p.rows;
+    const uint32_t first = p.starts[s], last = p.starts[min(s + T::kTileM / kStretch, p.n_starts - 1u)];
+    for (uint32_t e0 = first; e0 < last; e0 += kBatch) {
+        const uint32_t many = min(last - e0, kBatch);
+        __syncthreads();
+        if (threadIdx.x < many) list[threadIdx.x] = make_uint2(p.order[e0 + threadIdx.x].x, __float_as_uint(p.hit[e0 + threadIdx.x]));
+        for (uint32_t i = threadIdx.x; i < many * kPieces; i += T::kThreads) {
+            const uint32_t k = tile.n0 + i % kPieces * 8u;
+            const uint16_t *row = (const uint16_t *)(p.x.at + (int64_t)p.order[e0 + i / kPieces].y * p.x.stride);
+            v4i v = {0, 0, 0, 0};
+            if (k + 8u <= K) v = *(const v4i *)(row + k);
+            else
+#pragma unroll
+                for (uint32_t j = 0; j < 7; ++j) if (k + j < K) v[j / 2] |= (int)((uint32_t)row[k + j] << (16 * (j % 2)));
+            *(v4i *)(lds + i * 16u) = v;
+        }
+        __syncthreads();
+        for (uint32_t e = 0; e < many; ++e) {
+            const uint2 at = list[e];
+#pragma unroll
+            for (int t = 0; t < T::MT; ++t) {
+                if (tile.m(t) + p.v0 != at.x) continue;
+#pragma unroll
+                for (int u = 0; u < T::NU; ++u) {
+                    const uint2 four = *(const uint2 *)(lds + (e * T::kTileN + tile.n(u) - tile.n0) * 2u);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[u][t][j] += __uint_as_float(at.y) * widen16<T::DT>((j < 2 ? four.x : four.y) >> (16 * (j % 2)) & 0xFFFFu);
+                }
+            }
+        }
+    }
+}
+
 // dw of one piece, whole.  (The same piece: 473 us; both operands are turned.)
 template <class T>
 __global__ __launch_bounds__(T::kThreads, 2) void loss_dw_kernel(GradParams p)
@@ -354,6 +463,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_dw_kernel(GradParams p)
     typename T::Acc acc;
     tile.make(p.a, 0, lds, acc);
     const float f = p.scale ? p.scale[1] : 1.0f;
+    if constexpr (T::DT != RS_DTYPE_F32) if (p.hit) add_hits(p, tile, lds, acc);
     if constexpr (T::DT == RS_DTYPE_F32) {
 #pragma unroll
         for (int t = 0; t < T::MT; ++t) {
@@ -375,27 +485,50 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_dw_kernel(GradParams p)
     }
 }
 
-// dx from the sums of the shares, rounded once
+// dx (rows, K) from the sums of the shares, and what G's rounding left at the token, rounded once
+struct RoundParams {
+    const float   *sums;
+    int64_t        part_stride, count;
+    void          *y;
+    const float   *scale, *hit;      // hit: null, or as in LossParams, with rank
+    const uint32_t *rank;
+    const LossRow *rows;
+    Operand        w;
+    uint32_t       parts, K;
+};
 template <int DT>
-__global__ __launch_bounds__(256) void loss_round_kernel(const float *sums, int64_t part_stride, uint32_t parts, void *y, int64_t count, const float *scale)
+__global__ __launch_bounds__(256) void loss_round_kernel(RoundParams p)
 {
-    const float f = scale ? scale[1] : 1.0f;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (int64_t)gridDim.x * 1024) {
+    const float f = p.scale ? p.scale[1] : 1.0f;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < p.count; i += (int64_t)gridDim.x * 1024) {
         v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (i + 4 <= count) {
+        const bool whole = i + 4 <= p.count;
+        if (whole) {
 #pragma unroll 8
-            for (uint32_t k = 0; k < parts; ++k) {
+            for (uint32_t k = 0; k < p.parts; ++k) {
                 v4f v;
-                __builtin_memcpy(&v, sums + k * part_stride + i, 16);            // (part_stride is any number)
+                __builtin_memcpy(&v, p.sums + k * p.part_stride + i, 16);        // (part_stride is any number)
                 s += v;
             }
-            put_four<DT>(y, i, s * f);
         } else
-            for (int64_t j = i; j < count; ++j) {
-                float one = 0.0f;
-                for (uint32_t k = 0; k < parts; ++k) one += sums[k * part_stride + j];
-                put<DT>(y, j, one * f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                for (uint32_t k = 0; i + j < p.count && k < p.parts; ++k) s[j] += p.sums[k * p.part_stride + i + j];
+        if (DT != RS_DTYPE_F32 && p.hit) {
+            int64_t m = i / p.K;
+            uint32_t k = (uint32_t)(i - m * p.K);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int32_t token = i + j < p.count ? p.rows[m].token : -1;
+                if (token >= 0) s[j] += p.hit[p.rank[m]] * widen16<DT>(((const uint16_t *)(p.w.at + (int64_t)token * p.w.stride))[k]);
+                if (++k == p.K) { k = 0; ++m; }
             }
+        }
+        s *= f;
+        if (whole) put_four<DT>(p.y, i, s);
+        else
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (i + j < p.count) put<DT>(p.y, i + j, s[j]);
     }
 }
 

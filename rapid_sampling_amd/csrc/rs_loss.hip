@@ -16,6 +16,8 @@ struct LossSpace {
     uint64_t grad_stride = 0;
     uint32_t shares = 1;                                // of the product's reduction
     uint64_t sums = 0, sum_stride = 0;
+    uint64_t hit = 0, order = 0, rank = 0, starts = 0;
+    uint32_t n_starts = 0;                              // 0: what G's rounding leaves at the tokens is not made up for
     uint64_t take(uint64_t n) { const uint64_t at = bytes; bytes += up(n, 256); return at; }
 };
 
@@ -53,6 +55,13 @@ static LossSpace loss_space(int32_t M, int32_t V, int32_t K, int32_t dtype, bool
     }
     s.high = M <= (int32_t)kFewRows && dtype != RS_DTYPE_F32 ? 2 * M : M;
     if (s.high > (uint32_t)M) s.twice = s.take(s.high * up((uint64_t)K * size, 16));
+    else if (dtype != RS_DTYPE_F32 && M <= (int32_t)kHitRows) {
+        s.n_starts = (uint32_t)(up(V, kStretch) / kStretch) + 1;
+        s.hit = s.take((uint64_t)M * 4);
+        s.order = s.take((uint64_t)M * 8);
+        s.rank = s.take((uint64_t)M * 4);
+        s.starts = s.take((uint64_t)s.n_starts * 4);
+    }
     s.scale = s.take(8);
     s.rows = s.take((uint64_t)M * sizeof(LossRow));
     s.piece = (uint32_t)std::min<uint64_t>(up(V, 256), std::max<uint64_t>(8192, ((1ull << 27) / (s.high * size)) / 256 * 256));
@@ -165,7 +174,10 @@ static void backward(LossParams p, const LossSpace &s, Operand x, Operand w, uin
     constexpr uint32_t size = kSize<DT>;
     if (DT == RS_DTYPE_F16) hipLaunchKernelGGL(loss_scale_kernel, dim3(1), dim3(1024), 0, st, p);
     else p.scale = nullptr;
-    hipLaunchKernelGGL(loss_rows_kernel, dim3((p.M + 255) / 256), dim3(256), 0, st, p);
+    if (s.n_starts) {
+        p.hit = (float *)(ws + s.hit); p.order = (uint2 *)(ws + s.order); p.rank = (uint32_t *)(ws + s.rank); p.starts = (uint32_t *)(ws + s.starts); p.n_starts = s.n_starts;
+    }
+    hipLaunchKernelGGL(loss_rows_kernel, dim3((p.M + 255) / 256 + (s.n_starts + 255) / 256), dim3(256), 0, st, p);
     Operand xs = x;
     if (s.high > p.M) {
         p.rest = p.M;
@@ -183,7 +195,7 @@ static void backward(LossParams p, const LossSpace &s, Operand x, Operand w, uin
             launch_shares<DT>(p, s, ws, st);
             hipLaunchKernelGGL(loss_shares_grad_kernel<DT>, dim3((p.V + kShared - 1) / kShared, p.M), dim3(256), 0, st, p);
         } else launch_grad<DT>(p, st);
-        GradParams g;
+        GradParams g = {};
         g.scale = p.scale;
         if (grad_x) {
             g.a = Product{Operand{piece, w.stride, K}, Operand{(const char *)p.grad, p.grad_stride, s.high}, n, s.split};
@@ -199,13 +211,16 @@ static void backward(LossParams p, const LossSpace &s, Operand x, Operand w, uin
             g.y_stride = K;
             g.part_stride = 0;
             g.add = 0;
+            g.hit = p.hit; g.order = p.order; g.starts = p.starts; g.n_starts = p.n_starts; g.v0 = v0; g.x = x;
             launch_dw<DT>(g, st);
         }
     }
     if (grad_x) {
-        const int64_t count = (int64_t)p.M * K;
-        hipLaunchKernelGGL(loss_round_kernel<DT>, dim3((uint32_t)std::min<int64_t>((count + 1023) / 1024, 1 << 16)), dim3(256), 0, st, (const float *)(ws + s.dx),
-                           count, s.split * (s.high / p.M), grad_x, count, p.scale);
+        RoundParams r = {};
+        r.count = (int64_t)p.M * K;
+        r.sums = (const float *)(ws + s.dx); r.part_stride = r.count; r.parts = s.split * (s.high / p.M);
+        r.y = grad_x; r.scale = p.scale; r.hit = p.hit; r.rank = p.rank; r.rows = p.rows; r.w = w; r.K = K;
+        hipLaunchKernelGGL(loss_round_kernel<DT>, dim3((uint32_t)std::min<int64_t>((r.count + 1023) / 1024, 1 << 16)), dim3(256), 0, st, r);
     }
 }
 

@@ -167,6 +167,34 @@ def test_one_gradient_at_a_time_and_broadcast_ones():
 
 @gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("M,V,K,tokens", [(33, 700, 64, 700), (33, 3001, 100, 5), (64, 900, 2100, 900), (300, 20011, 33, 20011), (1025, 5000, 130, 40), (2048, 520, 64, 520), (1500, 9000, 1040, 9000)])
+def test_what_a_row_gives_its_token_is_not_rounded(M, V, K, tokens, dtype):
+    """From 33 to 2048 rows G's numbers are rounded to 16 bits, but for those at the rows' tokens, which make most of a gradient: there the two
+    products hold what the rounding left as well.  (Tokens of few kinds: rows of dw to which many rows of x give.)"""
+    x, w, t = make(M, V, K, dtype, 4, spread=1.0)
+    t = torch.where(t >= 0, t * tokens // V * (V // tokens), t)
+    t[-1] = V - 1
+    gen = torch.Generator().manual_seed(M)
+    g, h = torch.randn(M, generator=gen).cuda(), torch.randn(M, generator=gen).cuda() * 0.01
+    _, gx, gw = gradients(x, w, t, 0.8, g, h)
+    f = Formula(x, w, t, 0.8)
+    rows = torch.arange(M, device="cuda")[f.there]
+    g = torch.where(f.there, g, 0.0).double()
+    hot = torch.zeros_like(f.p).scatter_(1, f.at[:, None], g[:, None])
+    G = ((g + h)[:, None] * f.p - hot) / 0.8
+    dG = ((g + h).abs()[:, None] * f.p * (2 * f.d + EPS * (V + 16))[:, None] + 4 * EPS * hot.abs()) / 0.8
+    rounded = f.unit * G.abs() * 1.01 + (g.abs().max() + h.abs().max()) / 0.8 * 2.0 ** -38
+    rounded[rows, f.at[rows]] = 0.0
+    dG = dG + rounded + EPS * G.abs() + LEAST[torch.bfloat16]
+    wide = G.abs() + dG
+    for got, want, bound in ((gx, G @ f.w, dG @ f.w.abs() + EPS * (V + 64) * (wide @ f.w.abs())),
+                             (gw, G.t().contiguous() @ f.x, dG.t().contiguous() @ f.x.abs() + EPS * (2 * M + 8) * (wide.t().contiguous() @ f.x.abs()))):
+        off, bound = (got.double() - want).abs(), bound + f.unit * want.abs() * 1.01 + f.least
+        assert (off <= bound).all(), (off / bound).max().item()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_gradients_of_sure_tokens_and_rare_ones(dtype):
     """Losses near 0, and tokens of probabilities down to 2^-30, whose rows of w have gradients of that size and no less exact ones."""
     x, w, t = make(64, 400, 128, dtype, 6, spread=1.0)
