@@ -177,7 +177,7 @@ static void backward(LossParams p, const LossSpace &s, Operand x, Operand w, uin
     if (s.n_starts) {
         p.hit = (float *)(ws + s.hit); p.order = (uint2 *)(ws + s.order); p.rank = (uint32_t *)(ws + s.rank); p.starts = (uint32_t *)(ws + s.starts); p.n_starts = s.n_starts;
     }
-    hipLaunchKernelGGL(loss_rows_kernel, dim3((p.M + 255) / 256 + (s.n_starts + 255) / 256), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(loss_rows_kernel, dim3(s.n_starts ? (p.M + 63) / 64 + (s.n_starts + 63) / 64 : (p.M + 255) / 256), dim3(256), 0, st, p);
     Operand xs = x;
     if (s.high > p.M) {
         p.rest = p.M;

@@ -269,9 +269,9 @@ at::Tensor &logprobs_workspace(const at::Tensor &like, void *stream)
 {
     return operator_workspace(&Entry::logprobs_ws, rs_logprobs_workspace_bytes(), "token_logprobs", like, stream);
 }
-at::Tensor &linear_workspace(const at::Tensor &like, void *stream, const char *what = "linear_fp8")
+at::Tensor &linear_workspace(const at::Tensor &like, void *stream)
 {
-    return operator_workspace(&Entry::linear_ws, rs_linear_workspace_bytes(), what, like, stream);
+    return operator_workspace(&Entry::linear_ws, rs_linear_workspace_bytes(), "linear_fp8", like, stream);
 }
 
 int32_t float_dtype(const at::Tensor &t, const char *what)
@@ -684,7 +684,7 @@ at::Tensor linear_rows(const at::Tensor &x, const at::Tensor &weight, const at::
         ws = scratch(rs_linear_workspace_bytes(), x);
         const int rc = rs_workspace_init(ws.data_ptr(), RS_LINEAR_COUNTER_BYTES, stream);
         if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
-    } else ws = linear_workspace(x, stream, "linear_int8");
+    } else ws = linear_workspace(x, stream);
     const int rc = rs_linear_int8(q, q_stride, scale, wq, w.stride(0), weight_scale.data_ptr<float>(), (int32_t)M, (int32_t)N, (int32_t)K,
                                   y.data_ptr(), float_dtype(y, "y"), N, ws.data_ptr(), (size_t)ws.numel(), stream);
     if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));

@@ -167,7 +167,7 @@ def test_one_gradient_at_a_time_and_broadcast_ones():
 
 @gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
-@pytest.mark.parametrize("M,V,K,tokens", [(33, 700, 64, 700), (33, 3001, 100, 5), (64, 900, 2100, 900), (300, 20011, 33, 20011), (1025, 5000, 130, 40), (2048, 520, 64, 520), (1500, 9000, 1040, 9000)])
+@pytest.mark.parametrize("M,V,K,tokens", [(33, 700, 64, 700), (33, 3001, 100, 5), (64, 900, 2100, 900), (300, 20011, 33, 20011), (1025, 5000, 130, 40), (2048, 520, 64, 520), (1500, 9000, 1040, 9000), (40, 1048576, 16, 1048576)])
 def test_what_a_row_gives_its_token_is_not_rounded(M, V, K, tokens, dtype):
     """From 33 to 2048 rows G's numbers are rounded to 16 bits, but for those at the rows' tokens, which make most of a gradient: there the two
     products hold what the rounding left as well.  (Tokens of few kinds: rows of dw to which many rows of x give.)"""
