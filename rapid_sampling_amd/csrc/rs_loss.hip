@@ -82,6 +82,13 @@ using LargeTile = Tile<DT, TP, TQ, !TP && DT != RS_DTYPE_F32, kTurned<DT, TP, TQ
 template <int DT, bool TP, bool TQ> using MiddleTile = Tile<DT, TP, TQ, !TP && DT != RS_DTYPE_F32, 2, 2, 4, 4, 2>;
 template <int DT, bool TP, bool TQ> using SmallTile = Tile<DT, TP, TQ, !TP && DT != RS_DTYPE_F32, 2, 2, 4, 2, 3>;
 
+// float32 and up to 16 rows: 128 x 16 by two waves, which take a row of x apart once for four of w's and make no products for rows that are not there.
+// (Forward, and with gradients, us, 128 x 64 and so: 1 x 50000 x 1024 57.6, 219 and 44.1, 183; 16 x 24000 x 4096 112, 414 and 93, 378; 16 x 100000 x 4096
+// 417, 1544 and 342, 1325.  128 x 32 for up to 32 rows would save 2 to 10 of 100 more.)
+constexpr uint32_t kNarrowRows = 16;
+template <int DT, bool TP, bool TQ> using NarrowTile = Tile<DT, TP, TQ, false, 2, 1, 4, 1, 4>;
+static bool narrow(int32_t dtype, uint32_t rows) { return dtype == RS_DTYPE_F32 && rows <= kNarrowRows; }
+
 template <class T, class K, class A> static void launch_tiles(K kernel, const A &p, hipStream_t st)
 {
     const uint64_t tiles = (uint64_t)((p.a.q.rows + T::kTileM - 1) / T::kTileM) * ((p.a.p.rows + T::kTileN - 1) / T::kTileN);
@@ -99,6 +106,10 @@ template <class T, class K, class A> static void launch_tiles(K kernel, const A 
     template __global__ void loss_dx_kernel<SmallTile<DT, false, false>>(GradParams);                                   \
     template __global__ void loss_shares_grad_kernel<DT>(LossParams);
 RS_SHARED(RS_DTYPE_F32) RS_SHARED(RS_DTYPE_BF16) RS_SHARED(RS_DTYPE_F16)
+template __global__ void loss_tile_kernel<NarrowTile<RS_DTYPE_F32, false, false>>(LossParams);
+template __global__ void loss_grad_kernel<NarrowTile<RS_DTYPE_F32, false, false>>(LossParams);
+template __global__ void loss_dx_kernel<NarrowTile<RS_DTYPE_F32, false, false>>(GradParams);
+template __global__ void loss_dx_kernel<NarrowTile<RS_DTYPE_F32, true, false>>(GradParams);
 RS_TYPES(SmallTile)
 RS_TYPES(MiddleTile)
 RS_TYPES(LargeTile)
@@ -109,15 +120,36 @@ RS_TYPES(LargeTile)
     case kMiddle: launch_tiles<MiddleTile<DT, TP, TQ>>(kernel<MiddleTile<DT, TP, TQ>>, p, st); break;                   \
     default:      launch_tiles<SmallTile<DT, TP, TQ>>(kernel<SmallTile<DT, TP, TQ>>, p, st); break;                     \
     }
-template <int DT> static void launch_forward(const LossParams &p, hipStream_t st) { RS_LAUNCH(tile_size, loss_tile_kernel, false, false) }
-template <int DT> static void launch_grad(const LossParams &p, hipStream_t st) { RS_LAUNCH(tile_size, loss_grad_kernel, false, false) }
-template <int DT> static void launch_dx(const GradParams &p, hipStream_t st) { RS_LAUNCH(dx_size, loss_dx_kernel, true, false) }
+#define RS_NARROW(kernel, TP, TQ)                                                                                       \
+    if constexpr (DT == RS_DTYPE_F32)                                                                                   \
+        if (narrow(DT, p.a.q.rows)) return launch_tiles<NarrowTile<DT, TP, TQ>>(kernel<NarrowTile<DT, TP, TQ>>, p, st);
+template <int DT> static void launch_forward(const LossParams &p, hipStream_t st)
+{
+    RS_NARROW(loss_tile_kernel, false, false)
+    RS_LAUNCH(tile_size, loss_tile_kernel, false, false)
+}
+template <int DT> static void launch_grad(const LossParams &p, hipStream_t st)
+{
+    RS_NARROW(loss_grad_kernel, false, false)
+    RS_LAUNCH(tile_size, loss_grad_kernel, false, false)
+}
+template <int DT> static void launch_dx(const GradParams &p, hipStream_t st)
+{
+    RS_NARROW(loss_dx_kernel, true, false)
+    RS_LAUNCH(dx_size, loss_dx_kernel, true, false)
+}
 // (for few rows dw is all stores, and two workgroups to a compute unit hide more of them: 48 rows of 4096 over 131072 in bfloat16 1083 us with
 // its forward pass, 966 so; 385 rows of 2000 over 50257 the same either way)
 template <int DT> static void launch_dw(const GradParams &p, hipStream_t st)
 {
     if (p.a.red <= 256) launch_tiles<MiddleTile<DT, true, true>>(loss_dw_kernel<MiddleTile<DT, true, true>>, p, st);
     else RS_LAUNCH(tile_size, loss_dw_kernel, true, true)
+}
+
+template <int DT> static void launch_product(const GradParams &p, hipStream_t st)
+{
+    RS_NARROW(loss_dx_kernel, false, false)
+    launch_tiles<SmallTile<DT, false, false>>(loss_dx_kernel<SmallTile<DT, false, false>>, p, st);
 }
 
 // The product's sums by shares of its reduction.
@@ -129,7 +161,7 @@ template <int DT> static void launch_shares(LossParams &p, const LossSpace &s, c
     g.y = ws + s.sums;
     g.y_stride = (int64_t)s.sum_stride;
     g.part_stride = (int64_t)s.sum_stride * p.M;
-    launch_tiles<SmallTile<DT, false, false>>(loss_dx_kernel<SmallTile<DT, false, false>>, g, st);
+    launch_product<DT>(g, st);
     p.sums = (const float *)(ws + s.sums);
     p.sum_stride = (uint32_t)s.sum_stride;
     p.shares = s.shares;

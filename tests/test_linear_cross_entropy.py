@@ -81,7 +81,7 @@ def gradients(x, w, t, T, g, h=None):
 
 # one row and few, small tiles and large ones, several pieces of the vocabulary, odd sizes of everything
 SIZES = [(1, 1, 1), (1, 100, 64), (2, 63, 7), (5, 300, 100), (64, 129, 65), (65, 1000, 33), (130, 700, 130), (200, 5003, 201), (257, 8200, 72), (40, 20011, 64), (1500, 8193, 96), (32, 500, 128), (33, 500, 128), (300, 30011, 24),
-         (27, 674, 2100), (155, 556, 1501), (2, 5000, 3000), (300, 65, 1030), (33, 129, 2056), (1, 1, 4000), (32, 1001, 9000)]
+         (27, 674, 2100), (155, 556, 1501), (2, 5000, 3000), (300, 65, 1030), (33, 129, 2056), (1, 1, 4000), (32, 1001, 9000), (16, 33001, 100), (9, 300, 5000)]
 
 
 @gpu
