@@ -851,6 +851,7 @@ LossCall read_loss(const at::Tensor &x, const at::Tensor &weight, const at::Tens
 
 struct LossResult {
     at::Tensor loss, lse, stats;
+    at::Tensor weight;               // laid out anew, if it was
 };
 
 LossResult loss_forward(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &tokens, double temperature, bool want_stats)
@@ -858,7 +859,7 @@ LossResult loss_forward(const at::Tensor &x, const at::Tensor &weight, const at:
     const LossCall c = read_loss(x, weight, tokens, temperature);
     c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     const auto f32 = at::TensorOptions().dtype(at::kFloat).device(x.device());
-    LossResult o{at::empty(tokens.sizes(), f32), at::empty(tokens.sizes(), f32), want_stats ? at::empty({c.M, 2}, f32) : at::Tensor()};
+    LossResult o{at::empty(tokens.sizes(), f32), at::empty(tokens.sizes(), f32), want_stats ? at::empty({c.M, 2}, f32) : at::Tensor(), at::Tensor()};
     if (!c.M) return o;
     void *stream = current_stream(x);
     const at::Tensor xr = tile_rows(x, c.M, c.K, stream), w = tile_rows(weight, c.V, c.K, stream), list = token_list(tokens);
@@ -867,6 +868,7 @@ LossResult loss_forward(const at::Tensor &x, const at::Tensor &weight, const at:
                                            (int32_t)c.M, (int32_t)c.V, (int32_t)c.K, temperature, o.loss.data_ptr<float>(), o.lse.data_ptr<float>(),
                                            want_stats ? o.stats.data_ptr<float>() : nullptr, ws.data_ptr(), (size_t)ws.numel(), stream);
     if (rc != RS_OK) throw std::runtime_error(std::string("rapid_sampling: ") + rs_error_string(rc));
+    if (w.data_ptr() != weight.data_ptr()) o.weight = w;
     return o;
 }
 
@@ -914,7 +916,8 @@ struct Loss : torch::autograd::Function<Loss> {
     static variable_list forward(AutogradContext *ctx, at::Tensor x, at::Tensor weight, at::Tensor tokens, double temperature)
     {
         LossResult o = loss_forward(x, weight, tokens, temperature, true);
-        ctx->save_for_backward({x, weight, tokens, o.stats});
+        // (a weight that had to be laid out anew is kept so until the gradients: making it again costs as much as a product of a few hundred rows)
+        ctx->save_for_backward({x, weight, tokens, o.stats, o.weight});
         ctx->saved_data["temperature"] = temperature;
         ctx->set_materialize_grads(false);
         return {o.loss, o.lse};
@@ -927,13 +930,14 @@ struct Loss : torch::autograd::Function<Loss> {
         const auto saved = ctx->get_saved_variables();
         const double temperature = ctx->saved_data["temperature"].toDouble();
         const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+        const at::Tensor weight = saved[4].defined() ? saved[4] : saved[1];
         if (!want_x && !want_w) return {none, none, none, none};
         if (at::GradMode::is_enabled()) {
             auto given = [&](int i) { return grads[i].defined() ? std::optional<at::Tensor>(grads[i]) : std::nullopt; };
-            const variable_list o = LossBackward::apply(saved[0], saved[1], saved[2], saved[3], temperature, want_x, want_w, given(0), given(1));
+            const variable_list o = LossBackward::apply(saved[0], weight, saved[2], saved[3], temperature, want_x, want_w, given(0), given(1));
             return {want_x ? o[0] : none, want_w ? o[want_x] : none, none, none};
         }
-        const auto [gx, gw] = loss_backward(saved[0], saved[1], saved[2], saved[3], temperature, want_x, want_w, grads[0], grads[1]);
+        const auto [gx, gw] = loss_backward(saved[0], weight, saved[2], saved[3], temperature, want_x, want_w, grads[0], grads[1]);
         return {gx, gw, none, none};
     }
 };
