@@ -14,8 +14,7 @@
 
 namespace rs {
 
-constexpr uint32_t kFewRows = 32;    // up to these what G's rounding leaves is kept; up to kHitRows at the rows' tokens
-constexpr uint32_t kHitRows = 2048;
+constexpr uint32_t kFewRows = 32, kHitRows = 2048;           // see G's rounding
 
 struct LossRow {                     // of one row, for G
     float   max, a, b;               // M, (g + h) / (S T), g / T
@@ -187,11 +186,12 @@ __global__ __launch_bounds__(256) void loss_shares_kernel(LossParams p)
 // G in 16 bits is rounded, to bfloat16 with 8 bits of its own size; in float16 it is made so large first (by a power of two, the same
 // for the whole call) that the largest possible is below 2^15, and a probability's share of it is lost from 2^-39 on.  That adds to the
 // gradients' own rounding another of its size (a row's or a column's many are off in all directions: 1.4 times as much in all).  What the
-// rounding left is made up for where few numbers of G make a gradient.  Of up to kFewRows rows it is kept as rows of their own behind G's: the
-// products are then of twice as many rows, and wait for memory all the same (forward and gradients of 1 row of 4096 over 131072 in
-// bfloat16 876 us without, 890 with; of 48 rows it would be 907 and 1012).  Of up to kHitRows that of each row at its own token, the largest of
-// the row as long as it is not learnt, is added to the two products' sums (385 x 50257 x 2000 in float16 498 us without, 520 with, and the
-// errors 1.3 times the result's own rounding and 1.0; of 8192 rows, off by 1.35 to 1.41 times it whatever the data, 28.8 ms and 29.9).
+// rounding left is made up for where few numbers of G make a gradient.  Of up to kFewRows rows (twice as many over small vocabularies) it is kept as
+// rows of their own behind G's: the products are then of twice as many rows, and wait for memory all the same (forward and gradients of 1 row
+// of 4096 over 131072 in bfloat16 876 us without, 890 with; of 48 rows it would be 907 and 1012).  Of up to kHitRows that of each row at its own
+// token, the largest of the row as long as it is not learnt, is added to the two products' sums (385 x 50257 x 2000 in float16 498 us without, 521
+// with, and the errors 1.3 times the result's own rounding and 1.0), as long as a tile of dw has few of them (2000 x 7900 x 4096 in bfloat16 473 and
+// 547).  More rows are off by 1.35 to 1.41 times it whatever the data (8192 x 131072 x 4096 28.8 ms, and 29.9 with it).
 __global__ __launch_bounds__(1024) void loss_scale_kernel(LossParams p)
 {
     __shared__ float tops[16];

@@ -53,9 +53,9 @@ static LossSpace loss_space(int32_t M, int32_t V, int32_t K, int32_t dtype, bool
         s.target = s.take((uint64_t)M * 4);
         return s;
     }
-    s.high = M <= (int32_t)kFewRows && dtype != RS_DTYPE_F32 ? 2 * M : M;
+    s.high = (M <= (int32_t)kFewRows || (M <= (int32_t)(2 * kFewRows) && 16 * M > V)) && dtype != RS_DTYPE_F32 ? 2 * M : M;
     if (s.high > (uint32_t)M) s.twice = s.take(s.high * up((uint64_t)K * size, 16));
-    else if (dtype != RS_DTYPE_F32 && M <= (int32_t)kHitRows) {
+    else if (dtype != RS_DTYPE_F32 && M <= (int32_t)kHitRows && 16 * M <= V) {
         s.n_starts = (uint32_t)(up(V, kStretch) / kStretch) + 1;
         s.hit = s.take((uint64_t)M * 4);
         s.order = s.take((uint64_t)M * 8);

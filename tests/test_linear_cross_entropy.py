@@ -167,10 +167,10 @@ def test_one_gradient_at_a_time_and_broadcast_ones():
 
 @gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
-@pytest.mark.parametrize("M,V,K,tokens", [(33, 700, 64, 700), (33, 3001, 100, 5), (64, 900, 2100, 900), (300, 20011, 33, 20011), (1025, 5000, 130, 40), (2048, 520, 64, 520), (1500, 9000, 1040, 9000), (40, 1048576, 16, 1048576)])
+@pytest.mark.parametrize("M,V,K,tokens", [(33, 528, 64, 528), (33, 3001, 100, 5), (64, 1024, 2100, 1024), (64, 900, 70, 900), (50, 130, 2100, 130), (300, 20011, 33, 20011), (300, 4800, 130, 40), (2048, 32768, 64, 32768), (1500, 24000, 1040, 24000), (40, 1048576, 16, 1048576)])
 def test_what_a_row_gives_its_token_is_not_rounded(M, V, K, tokens, dtype):
-    """From 33 to 2048 rows G's numbers are rounded to 16 bits, but for those at the rows' tokens, which make most of a gradient: there the two
-    products hold what the rounding left as well.  (Tokens of few kinds: rows of dw to which many rows of x give.)"""
+    """From 33 to 2048 rows, of up to a sixteenth of the vocabulary, G's numbers are rounded to 16 bits, but for those at the rows' tokens, which make
+    most of a gradient: there the two products hold what the rounding left as well.  (Up to 64 rows over less hold all of it.)  (Tokens of few kinds: rows of dw to which many rows of x give.)"""
     x, w, t = make(M, V, K, dtype, 4, spread=1.0)
     t = torch.where(t >= 0, t * tokens // V * (V // tokens), t)
     t[-1] = V - 1
