@@ -288,18 +288,23 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
     tile.choose(p.a, blockIdx.x);
     typename T::Acc acc;
     tile.make(p.a, 0, lds, acc);
+    const uint32_t from = p.v0 + tile.n0 + wave_id() % T::WN * (16u * T::NU);             // the wave's first token
     auto row_of = [&](int t, v4f (&v)[T::NU]) {
         const LossRow r = p.rows[min(tile.m(t), p.M - 1u)];
 #pragma unroll
         for (int u = 0; u < T::NU; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[u][j] = r.a * __builtin_amdgcn_exp2f((acc[u][t][j] - r.max) * p.c);
+            for (int j = 0; j < 4; ++j) v[u][j] = r.a * __builtin_amdgcn_exp2f((acc[u][t][j] - r.max) * p.c);
+        // (few waves have the token of any of their rows)
+        if (!__any((uint32_t)r.token - from < 16u * T::NU)) return;
+#pragma unroll
+        for (int u = 0; u < T::NU; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
                 if ((int32_t)(tile.n(u) + p.v0 + j) == r.token) {
                     v[u][j] -= r.b;
                     if (T::DT != RS_DTYPE_F32 && p.hit && tile.m(t) < p.M) p.hit[p.rank[tile.m(t)]] = rounding_left<T::DT>(v[u][j]);
                 }
-            }
     };
     if constexpr (T::DT == RS_DTYPE_F32) {
 #pragma unroll
