@@ -197,8 +197,11 @@ __global__ __launch_bounds__(1024) void loss_scale_kernel(LossParams p)
     __shared__ float tops[16];
     float top = 0.0f;
     for (uint32_t m = threadIdx.x; m < p.M; m += 1024u) {
-        const float g = p.g ? fabsf(p.g[(int64_t)m * p.g_stride]) : 0.0f, h = p.h ? fabsf(p.h[(int64_t)m * p.h_stride]) : 0.0f;
-        const float v = (g + h) * p.inv_t;
+        // (what loss_rows_kernel leaves out may not make the others small: the g of a row without a token, and both of one without a finite logit)
+        const int64_t token = loss_token(p, m);
+        const bool looked_at = token >= 0 && token < (int64_t)p.V;
+        const float g = p.g && looked_at ? fabsf(p.g[(int64_t)m * p.g_stride]) : 0.0f, h = p.h ? fabsf(p.h[(int64_t)m * p.h_stride]) : 0.0f;
+        const float v = p.stats[m].y < __builtin_inff() ? (g + h) * p.inv_t : 0.0f;
         if (v < __builtin_inff()) top = fmaxf(top, v);
     }
 #pragma unroll
