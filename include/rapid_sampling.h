@@ -587,7 +587,8 @@ int rs_lay_out_rows(const void *x_device, int64_t x_row_stride, int32_t size, in
  * NULL, or (M, 2) floats, 8-byte aligned, for the gradient.  A row whose logits are
  * all -inf has lse -inf and loss +inf; one with a NaN or +inf among them NaN.
  * (Values of float32 are taken apart into three of bfloat16, exactly, and an
- * infinity among x or w makes NaN.)
+ * infinity among x or w makes NaN.  Of their products what is below 2^-22 of each is
+ * rounded, in either direction.)
  * M up to RS_LINEAR_MAX, V up to 1048576, K up to RS_LOSS_COLUMNS_MAX, and
  * ceil(M / 64) ceil(V / 128), ceil(M / 64) ceil(K / 128) and ceil(V / 128) ceil(K / 128)
  * below 2^24.

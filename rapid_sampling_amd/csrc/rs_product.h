@@ -41,10 +41,13 @@ template <int DT, int NU, int MT> __device__ __forceinline__ void multiply_all(c
         for (int t = 0; t < MT; ++t) acc[u][t] = multiply<DT>(p[u], q[t], acc[u][t]);
 }
 
-// Eight float32 values as three times eight of bfloat16, x = x0 + x1 + x2 exactly: eight bits of the significand each, cut off, not rounded.
-// Of the nine products of two such sums the six largest are made: what is left out is below 2^-23 of a product, and 2^-25 on
-// average.  Six matrix instructions of 16 cycles in the place of eight of 32.
-struct Thirds { v4i x[3]; };
+// Eight float32 values as three times eight of bfloat16, x = x0 + x1 + x2 exactly: eight bits of the significand each, cut off, not rounded, so that they have x's
+// sign, and products that overflow the same infinity.  Of the nine products of two such sums the five with a first part are made, and of (x1 + x2)(y1 + y2) one, of
+// both rounded to bfloat16 (the fourth of a value's parts).  That is off by at most 2^-22 of x y, by 2^-26 on average and in either direction: half of what
+// the product's own rounding is.  (x1 y1 in its place, one of nine, is too small by up to 2^-21 and by 0.67 2^-24 on average; x0 and x1 rounded are off by 2^-24 at
+// most, but have parts of both signs, whose overflows make NaN.  Products that are left out as well, eight in all, take 19 % longer where M is large.)  Six
+// matrix instructions of 16 cycles in the place of eight of 32.
+struct Thirds { v4i x[4]; };
 __device__ __forceinline__ Thirds thirds(v4i lo, v4i hi)
 {
     Thirds r;
@@ -56,6 +59,10 @@ __device__ __forceinline__ Thirds thirds(v4i lo, v4i hi)
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
             r.x[i][j / 2] = (int)__builtin_amdgcn_perm(v[j + 1], v[j], 0x07060302u);          // the upper halves of both
+            if (i == 1) {                                             // v: x1 + x2
+                const v2bf two = {(__bf16)__uint_as_float(v[j]), (__bf16)__uint_as_float(v[j + 1])};
+                r.x[3][j / 2] = __builtin_bit_cast(int, two);
+            }
             if (i < 2)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) v[j + h] = __float_as_uint(__uint_as_float(v[j + h]) - __uint_as_float(v[j + h] & 0xFFFF0000u));
@@ -353,7 +360,7 @@ struct Tile {
     }
     static __device__ __forceinline__ void products(const Thirds &p, const Thirds (&q)[MT], Sum<DT> (&acc)[MT])
     {
-        constexpr int kFirst[6] = {0, 1, 2, 0, 1, 0}, kSecond[6] = {2, 1, 0, 1, 0, 0};           // the smallest first
+        constexpr int kFirst[6] = {0, 3, 2, 0, 1, 0}, kSecond[6] = {2, 3, 0, 1, 0, 0};           // the smallest first; 3: see thirds
 #pragma unroll
         for (int i = 0; i < 6; ++i)
 #pragma unroll
@@ -372,13 +379,8 @@ struct Tile {
         Thirds q[MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t) q[t] = thirds(rq(lds + P::kBytes, t, 0), rq(lds + P::kBytes, t, 1));
-        v4i lo = rp(lds, 0, 0), hi = rp(lds, 0, 1);
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            const Thirds p = thirds(lo, hi);
-            if (u + 1 < NU) { lo = rp(lds, u + 1, 0); hi = rp(lds, u + 1, 1); }
-            products(p, q, acc[u]);
-        }
+        for (int u = 0; u < NU; ++u) products(thirds(rp(lds, u, 0), rp(lds, u, 1)), q, acc[u]);
     }
 
     // Reads half `sub` of a stage into p and q and multiplies what was read before, one behind the other.
