@@ -608,9 +608,9 @@ int rs_linear_cross_entropy(const void *x_device, int64_t x_row_stride, const vo
  * With g the gradient of the losses and h that of lse (either may be NULL: none; a
  * stride of 1, or of 0: one number for all rows), p the probabilities:
  *   G = ((g + h) p - g [v = t]) / temperature     grad_x = G w     grad_w = G^T x
- * G is rounded to the inputs' type (of up to 32 rows what that leaves, rounded so
- * as well, is multiplied beside it, of up to 2048 and a sixteenth of V what it leaves
- * at the rows' own tokens); sums are float32, and rounded once.  A negative
+ * G is rounded to the inputs' type; of what that leaves is multiplied beside it, of
+ * up to 32 rows (up to 64 with V below 16 M) all, rounded so as well, and of more
+ * rows that at their own tokens; sums are float32, and rounded once.  A negative
  * token has no g, one of V or more has NaN for it.  The other arguments as in the
  * call whose stats are passed.
  */

@@ -7,20 +7,11 @@
 #pragma once
 
 #include "rs_linear.h"
+#include "rs_sort.h"
 
 namespace rs {
 
 constexpr int kTableInt8 = 3, kTableFp8 = 4;         // types of a table, next to RS_DTYPE_*
-
-struct TokenList {
-    const void *at;
-    int64_t     stride;
-    int32_t     is_64;
-    __device__ __forceinline__ int64_t operator[](int64_t i) const
-    {
-        return is_64 ? ((const int64_t *)at)[i * stride] : (int64_t)((const int32_t *)at)[i * stride];
-    }
-};
 
 struct EmbeddingParams {
     TokenList    tokens;

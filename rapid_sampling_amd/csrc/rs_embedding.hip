@@ -32,27 +32,67 @@ template <int WT> static void launch_embedding(const EmbeddingParams &p, int32_t
 // 53, 40; 16384 270, 80, 55 and 305, 63, 46; 32768 445, 157, 104 and 361, 68, 54.)
 static bool sorts_alone(uint32_t N, uint64_t clear) { return N <= kSortAlone / 2 || (N <= kSortAlone && clear >= 1ull << 28); }
 
-// Where a gradient's scratch lies.
-struct TableSpace {
-    uint64_t pairs[2], counts, parts, bytes = 0;
-    uint32_t digits, bits, chunk, chunks, groups;
-    uint64_t take(uint64_t n) { const uint64_t a = bytes; bytes += up(n, 256); return a; }
-};
-static TableSpace table_space(uint32_t N, uint32_t V, uint32_t K)
+static uint64_t take(uint64_t &bytes, uint64_t n)
 {
-    TableSpace s;
+    const uint64_t at = bytes;
+    bytes += up(n, 256);
+    return at;
+}
+SortSpace sort_space(uint32_t N, uint32_t V, uint64_t &bytes)
+{
+    SortSpace s;
     uint32_t bits = 1;
     while (bits < 32 && (V >> bits)) ++bits;             // of a token, or of V itself
     s.digits = (bits + kSortBits - 1) / kSortBits;
     s.bits = (bits + s.digits - 1) / s.digits;
     s.groups = (N + kSortTile - 1) / kSortTile;
+    for (int i = 0; i < 2; ++i) s.pairs[i] = take(bytes, 8ull * N);
+    s.counts = take(bytes, N <= kSortAlone / 2 ? 0 : 4ull * s.groups << s.bits);
+    return s;
+}
+
+const uint2 *launch_sort(const TokenList &tokens, uint32_t N, uint32_t V, const SortSpace &s, char *ws, void *clear_at, uint64_t clear_bytes, hipStream_t st)
+{
+    auto pairs = [&](uint32_t i) { return (uint2 *)(ws + s.pairs[i]); };
+    SortParams p = {};
+    p.tokens = tokens;
+    p.N = N; p.V = V; p.bits = s.bits; p.first = 1; p.digits = s.digits;
+    p.counts = (uint32_t *)(ws + s.counts);
+    const uint32_t lds = (kSortWaves << s.bits) * 4;
+    const ClearParams clear{(char *)clear_at, clear_bytes};
+    // (64 KB to a workgroup, one behind the other: 1 GiB in 168 us; in 1023 workgroups 189)
+    const uint32_t clears = clear.bytes ? (uint32_t)std::min<uint64_t>(32767, clear.bytes / 65536 + 1) : 0;
+    if (sorts_alone(N, clear.bytes)) {
+        p.out = pairs(0); p.out_b = pairs(1);
+        hipLaunchKernelGGL(sort_alone_kernel, dim3(1 + clears), dim3(kSortThreads), lds, st, p, clear);
+    } else {
+        if (clears) hipLaunchKernelGGL(clear_kernel, dim3(clears), dim3(kSortThreads), 0, st, clear);
+        for (uint32_t d = 0; d < s.digits; ++d) {
+            p.out = pairs(d & 1);
+            hipLaunchKernelGGL(sort_count_kernel, dim3(s.groups), dim3(kSortThreads), lds, st, p);
+            hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(kSortThreads), 0, st, p.counts, s.groups << s.bits);
+            hipLaunchKernelGGL(sort_place_kernel, dim3(s.groups), dim3(kSortThreads), lds, st, p);
+            p.first = 0; p.shift += s.bits; p.in = p.out;
+        }
+    }
+    return pairs((s.digits - 1) & 1);
+}
+
+// Where a gradient's scratch lies.
+struct TableSpace {
+    SortSpace sort;
+    uint64_t parts, bytes = 0;
+    uint32_t chunk, chunks;
+};
+static TableSpace table_space(uint32_t N, uint32_t V, uint32_t K)
+{
+    TableSpace s;
+    s.sort = sort_space(N, V, s.bytes);
     // Chunks of up to about the square root of the tokens: a token that makes up all of them has as many chunks to join as each has places.
     s.chunk = 4;
     while (s.chunk < 12 && (1ull << (2 * s.chunk + 4)) <= N) ++s.chunk;
     s.chunks = (N + (1u << s.chunk) - 1) >> s.chunk;
-    for (int i = 0; i < 2; ++i) s.pairs[i] = s.take(8ull * N);
-    s.counts = s.take(N <= kSortAlone / 2 ? 0 : 4ull * s.groups << s.bits);
-    s.parts = s.take((uint64_t)s.chunks * 2 * K * 4);
+    s.parts = take(s.bytes, (uint64_t)s.chunks * 2 * K * 4);
     return s;
 }
 
@@ -116,32 +156,10 @@ int rs_embedding_backward(const void *tokens, int32_t tokens_64, int64_t token_s
     if (workspace_bytes < s.bytes || ((uintptr_t)workspace & 255)) return RS_ERR_WORKSPACE;
     char *ws = (char *)workspace;
     const hipStream_t st = (hipStream_t)stream;
-    auto pairs = [&](uint32_t i) { return (uint2 *)(ws + s.pairs[i]); };
-    SortParams p = {};
-    p.tokens = TokenList{tokens, token_stride, tokens_64};
-    p.N = (uint32_t)M; p.V = (uint32_t)V; p.bits = s.bits; p.first = 1; p.digits = s.digits;
-    p.counts = (uint32_t *)(ws + s.counts);
-    const uint32_t lds = (kSortWaves << s.bits) * 4;
-    const ClearParams clear{(char *)dw, (uint64_t)V * K * size_of(dw_dtype)};
-    // (64 KB to a workgroup, one behind the other: 1 GiB in 168 us; in 1023 workgroups 189)
-    const uint32_t clears = (uint32_t)std::min<uint64_t>(32767, clear.bytes / 65536 + 1);
-    if (sorts_alone(p.N, clear.bytes)) {
-        p.out = pairs(0); p.out_b = pairs(1);
-        hipLaunchKernelGGL(sort_alone_kernel, dim3(1 + clears), dim3(kSortThreads), lds, st, p, clear);
-    } else {
-        hipLaunchKernelGGL(clear_kernel, dim3(clears), dim3(kSortThreads), 0, st, clear);
-        for (uint32_t d = 0; d < s.digits; ++d) {
-            p.out = pairs(d & 1);
-            hipLaunchKernelGGL(sort_count_kernel, dim3(s.groups), dim3(kSortThreads), lds, st, p);
-            hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(kSortThreads), 0, st, p.counts, s.groups << s.bits);
-            hipLaunchKernelGGL(sort_place_kernel, dim3(s.groups), dim3(kSortThreads), lds, st, p);
-            p.first = 0; p.shift += s.bits; p.in = p.out;
-        }
-    }
     TableGradParams t;
-    t.pairs = pairs((s.digits - 1) & 1);
+    t.pairs = launch_sort(TokenList{tokens, token_stride, tokens_64}, (uint32_t)M, (uint32_t)V, s.sort, ws, dw, (uint64_t)V * K * size_of(dw_dtype), st);
     t.g = g; t.g_stride = M > 1 ? g_stride : 0; t.parts = (float *)(ws + s.parts); t.dw = dw; t.scale = (float)scale;
-    t.N = p.N; t.V = p.V; t.K = (uint32_t)K; t.chunk = s.chunk;
+    t.N = (uint32_t)M; t.V = (uint32_t)V; t.K = (uint32_t)K; t.chunk = s.chunk;
     if (g_dtype == RS_DTYPE_F32) launch_sums<RS_DTYPE_F32>(t, s.chunks, dw_dtype, st);
     else if (g_dtype == RS_DTYPE_BF16) launch_sums<RS_DTYPE_BF16>(t, s.chunks, dw_dtype, st);
     else launch_sums<RS_DTYPE_F16>(t, s.chunks, dw_dtype, st);

@@ -11,10 +11,11 @@
 #pragma once
 
 #include "rs_product.h"
+#include "rs_sort.h"
 
 namespace rs {
 
-constexpr uint32_t kFewRows = 32, kHitRows = 2048;           // see G's rounding
+constexpr uint32_t kFewRows = 32, kCountRows = 2048;         // see G's rounding
 
 struct LossRow {                     // of one row, for G
     float   max, a, b;               // M, (g + h) / (S T), g / T
@@ -43,9 +44,8 @@ struct LossParams {
     uint32_t    rest;                // 0, or rows from one of G to what its rounding left, rounded too
     const float *sums;               // [share of the reduction][M][sum_stride] of the product, where it is shared out
     uint32_t    sum_stride, shares;
-    uint2      *order;               // null, or (token, row), by token and row
-    uint32_t   *rank;                // ... and each row's place there
-    float      *hit;                 // ... and what G's rounding left at the token, for each place
+    float      *hit;                 // null, or what G's rounding left at each row's token
+    const uint2 *order;              // null, or (token, row), by token and row
     uint32_t   *starts;              // ... and the first place of a token from kStretch s on, for every s
     uint32_t    n_starts;
 };
@@ -184,14 +184,14 @@ __global__ __launch_bounds__(256) void loss_shares_kernel(LossParams p)
 
 // ---------------------------------------------------------------- gradients --
 // G in 16 bits is rounded, to bfloat16 with 8 bits of its own size; in float16 it is made so large first (by a power of two, the same
-// for the whole call) that the largest possible is below 2^15, and a probability's share of it is lost from 2^-39 on.  That adds to the
-// gradients' own rounding another of its size (a row's or a column's many are off in all directions: 1.4 times as much in all).  What the
-// rounding left is made up for where few numbers of G make a gradient.  Of up to kFewRows rows (twice as many over small vocabularies) it is kept as
+// for the whole call) that the largest possible is below 2^15, and a probability's share of it is lost from 2^-39 on.  That would add to the
+// gradients' own rounding another of its size (a row's or a column's many are off in all directions: 1.41 times as much in all).  So what the
+// rounding left is made up for.  Of up to kFewRows rows (twice as many over less than sixteen times as many tokens) all of it is kept, as
 // rows of their own behind G's: the products are then of twice as many rows, and wait for memory all the same (forward and gradients of 1 row
-// of 4096 over 131072 in bfloat16 876 us without, 890 with; of 48 rows it would be 907 and 1012).  Of up to kHitRows that of each row at its own
-// token, the largest of the row as long as it is not learnt, is added to the two products' sums (385 x 50257 x 2000 in float16 498 us without, 521
-// with, and the errors 1.3 times the result's own rounding and 1.0), as long as a tile of dw has few of them (2000 x 7900 x 4096 in bfloat16 473 and
-// 547).  More rows are off by 1.35 to 1.41 times it whatever the data (8192 x 131072 x 4096 28.8 ms, and 29.9 with it).
+// of 4096 over 131072 in bfloat16 876 us without, 890 with; of 48 rows it would be 907 and 1012).  Of more rows that of each row at its own
+// token, the largest of the row as long as it is not learnt, is added to the two products' sums (loss_round_kernel, add_hits): errors are 1.00 to 1.01 times
+// the result's own rounding, and up to 1.07 over vocabularies of a few hundred tokens.  (us without and with it: 8192 x 131072 x 4096 in bfloat16 28620 and 28750, 4096 x
+// 50257 x 1024 in float16 1810 and 1860, 8192 x 8000 x 4096 1840 and 1920, 2000 x 7900 x 4096 476 and 528, 8192 x 512 x 4096 290 and 348.)
 __global__ __launch_bounds__(1024) void loss_scale_kernel(LossParams p)
 {
     __shared__ float tops[16];
@@ -215,15 +215,15 @@ __global__ __launch_bounds__(1024) void loss_scale_kernel(LossParams p)
     p.scale[1] = __builtin_ldexpf(1.0f, -e);
 }
 
-// The order of up to kHitRows rows, and then where stretches of the vocabulary begin in it: the number of (token, row) that come before, counted one by one
+// The order of up to kCountRows rows, and then where stretches of the vocabulary begin in it: the number of (token, row) that come before, counted one by one
 // by four threads (2000 rows over 32000 tokens 10 us; sorting them would be launches of its own).
-__device__ __forceinline__ void loss_order(const LossParams &p)
+__device__ __forceinline__ void loss_order(const LossParams &p, uint2 *order)
 {
-    __shared__ uint4 held[kHitRows / 4u];
+    __shared__ uint4 held[kCountRows / 4u];
     constexpr uint32_t kRowBits = 11;
-    static_assert(kHitRows == 1u << kRowBits, "token (20 bits, or none) and row in 32 bits");
+    static_assert(kCountRows == 1u << kRowBits, "token (20 bits, or none) and row in 32 bits");
 #pragma unroll
-    for (uint32_t e = 0; e < kHitRows / 256u; ++e) {
+    for (uint32_t e = 0; e < kCountRows / 256u; ++e) {
         const uint32_t j = e * 256u + threadIdx.x;
         if (e * 256u >= p.M) break;
         uint32_t pair = 0xFFFFFFFFu;
@@ -249,15 +249,26 @@ __device__ __forceinline__ void loss_order(const LossParams &p)
     if (quarter) return;
     if (!is_row) {
         if (m < p.n_starts) p.starts[m] = before;
-    } else if (m < p.M) {
-        p.order[before] = make_uint2(pair >> kRowBits, m);
-        p.rank[m] = before;
+    } else if (m < p.M) order[before] = make_uint2(pair >> kRowBits, m);
+}
+// More rows are sorted (rs_sort.h), and the stretches' beginnings looked for.
+__global__ __launch_bounds__(256) void loss_starts_kernel(LossParams p)
+{
+    const uint32_t s = blockIdx.x * 256u + threadIdx.x;
+    if (s >= p.n_starts) return;
+    uint32_t from = 0, to = p.M;                         // the first place whose token is not below is not before `from`, nor behind `to`
+    while (from < to) {
+        const uint32_t i = (from + to) / 2u, token = p.order[i].x;
+        if (token < p.V && token < s * kStretch) from = i + 1u;
+        else to = i;
     }
+    p.starts[s] = from;
 }
 
-__global__ __launch_bounds__(256) void loss_rows_kernel(LossParams p)
+// (order: null, or where to put it)
+__global__ __launch_bounds__(256) void loss_rows_kernel(LossParams p, uint2 *order)
 {
-    if (p.order) loss_order(p);
+    if (order) loss_order(p, order);
     const uint32_t m = blockIdx.x * 256u + threadIdx.x;
     if (m >= p.M) return;
     const float2 st = p.stats[m];
@@ -273,7 +284,6 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossParams p)
     p.rows[m] = r;
 }
 
-// (8192 rows, a piece of 8192 tokens, 4096 columns in bfloat16: 408 us, 1.35 PFLOP/s)
 // What is left of a number when it is rounded to 16 bits; nothing of one that is none.
 template <int DT> __device__ __forceinline__ float rounding_left(float v)
 {
@@ -283,6 +293,7 @@ template <int DT> __device__ __forceinline__ float rounding_left(float v)
     return d == d ? d : 0.0f;
 }
 
+// (8192 rows, a piece of 8192 tokens, 4096 columns in bfloat16: 408 us, 1.35 PFLOP/s)
 template <class T>
 __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
 {
@@ -306,7 +317,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
             for (int j = 0; j < 4; ++j)
                 if ((int32_t)(tile.n(u) + p.v0 + j) == r.token) {
                     v[u][j] -= r.b;
-                    if (T::DT != RS_DTYPE_F32 && p.hit && tile.m(t) < p.M) p.hit[p.rank[tile.m(t)]] = rounding_left<T::DT>(v[u][j]);
+                    if (T::DT != RS_DTYPE_F32 && p.hit && tile.m(t) < p.M) p.hit[tile.m(t)] = rounding_left<T::DT>(v[u][j]);
                 }
     };
     if constexpr (T::DT == RS_DTYPE_F32) {
@@ -358,7 +369,7 @@ __global__ __launch_bounds__(256) void loss_shares_grad_kernel(LossParams p)
         g[j] = r.a * __builtin_amdgcn_exp2f((g[j] - r.max) * p.c);
         if ((int32_t)(v + j) == r.token) {
             g[j] -= r.b;
-            if (p.hit) p.hit[p.rank[m]] = rounding_left<DT>(g[j]);
+            if (p.hit) p.hit[m] = rounding_left<DT>(g[j]);
         }
     }
     char *row = (char *)p.grad + (int64_t)m * p.grad_stride;
@@ -422,43 +433,88 @@ template <int DT> __device__ __forceinline__ float widen16(uint32_t v)
     else return __uint_as_float(v << 16);
 }
 
-// What G's rounding left at the tokens of a tile of dw: the rows' x, as much of them as the tile holds, by way of LDS.
+// What G's rounding left at the tokens of a tile of dw, added to its sums: for the rows whose token the tile holds, which lie side by side in the rows' order,
+// stages more of the same product, of those rows of x and a G that is 0 but at each row's token.  What is left is rounded as well, and what that leaves,
+// from a second such G: all of float32's 24 bits.  Half a stage for up to 32 rows; the next 64 are on their way while the last half is multiplied, and where they
+// are has been read before.  (Places behind the last row hold it once more, with a G of 0: an x that is no number has made its column of the tile none already.)
 template <class T> __device__ __forceinline__ void add_hits(const GradParams &p, const T &tile, char *lds, typename T::Acc &acc)
 {
-    constexpr uint32_t kBatch = 32, kPieces = T::kTileN / 8u;
-    static_assert(kBatch * (T::kTileN * 2u + 8u) <= T::kLds, "where the stages were");
-    uint2 *list = (uint2 *)(lds + kBatch * T::kTileN * 2u);                      // (token, what is left)
-    const uint32_t s = (p.v0 + tile.m0) / kStretch, K = p.a.p.rows;
+    constexpr uint32_t kX = T::P::kBytes, kG = T::Q::kBytes, kLoads = T::P::kLoads, kMany = T::kRed;
+    static_assert(2u * kX + 2u * kG <= T::kLds && kMany == 64u && T::kTileM % kStretch == 0u, "where the stages were");
+    const uint32_t s = (p.v0 + tile.m0) / kStretch;
     const uint32_t first = p.starts[s], last = p.starts[min(s + T::kTileM / kStretch, p.n_starts - 1u)];
-    for (uint32_t e0 = first; e0 < last; e0 += kBatch) {
-        const uint32_t many = min(last - e0, kBatch);
-        __syncthreads();
-        if (threadIdx.x < many) list[threadIdx.x] = make_uint2(p.order[e0 + threadIdx.x].x, __float_as_uint(p.hit[e0 + threadIdx.x]));
-        for (uint32_t i = threadIdx.x; i < many * kPieces; i += T::kThreads) {
-            const uint32_t k = tile.n0 + i % kPieces * 8u;
-            const uint16_t *row = (const uint16_t *)(p.x.at + (int64_t)p.order[e0 + i / kPieces].y * p.x.stride);
-            v4i v = {0, 0, 0, 0};
-            if (k + 8u <= K) v = *(const v4i *)(row + k);
-            else
+    if (first >= last) return;
+    char *const g_at = lds + 2u * kX;
+    const typename T::P::Reader rp(wave_id() % T::WN * (16u * T::NU));
+    const typename T::Q::Reader rq(wave_id() / T::WN * (16u * T::MT));
+    // the thread's pieces of 16 bytes of x's rows, as far as the rows go; what the last one holds behind a row's end belongs to columns that are not there
+    uint32_t rows[kLoads];
+    auto pair_of = [&](uint32_t e) { return p.order[min(e, last - 1u)]; };
+    auto ask = [&](uint32_t e0) {
 #pragma unroll
-                for (uint32_t j = 0; j < 7; ++j) if (k + j < K) v[j / 2] |= (int)((uint32_t)row[k + j] << (16 * (j % 2)));
-            *(v4i *)(lds + i * 16u) = v;
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            uint32_t e, byte;
+            T::P::source_of(T::P::place(i), e, byte);
+            rows[i] = pair_of(e0 + e).y;
         }
-        __syncthreads();
-        for (uint32_t e = 0; e < many; ++e) {
-            const uint2 at = list[e];
+    };
+    auto fetch = [&](char *to) {
 #pragma unroll
-            for (int t = 0; t < T::MT; ++t) {
-                if (tile.m(t) + p.v0 != at.x) continue;
-#pragma unroll
-                for (int u = 0; u < T::NU; ++u) {
-                    const uint2 four = *(const uint2 *)(lds + (e * T::kTileN + tile.n(u) - tile.n0) * 2u);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[u][t][j] += __uint_as_float(at.y) * widen16<T::DT>((j < 2 ? four.x : four.y) >> (16 * (j % 2)) & 0xFFFFu);
-                }
-            }
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            uint32_t e, byte;
+            T::P::source_of(T::P::place(i), e, byte);
+            const uint32_t k = tile.n0 * 2u + byte;
+            const char *from = p.x.at + (int64_t)rows[i] * p.x.stride + (k < p.a.p.rows * 2u ? k : 0u);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (LdsPtr)(to + (i * T::kWaves + wave_id()) * 1024u), 16, 0, 0);
         }
+    };
+    // a row of G to a thread: (token, row), what is left there, and its place
+    const uint32_t lane = threadIdx.x % kMany;
+    uint2 pair = pair_of(first + lane), next = pair_of(first + kMany + lane);
+    auto place_of = [&](uint32_t token) { return T::Q::place_of(lane, (token - p.v0 - tile.m0) * 2u); };
+    auto set = [&](uint32_t at, float v) {
+        put<T::DT>(g_at + at, 0, v);
+        put<T::DT>(g_at + kG + at, 0, rounding_left<T::DT>(v));
+    };
+    ask(first);
+    float left = p.hit[pair.y];
+    stage_barrier<0>();
+    for (uint32_t i = threadIdx.x * 16u; i < 2u * kG; i += T::kThreads * 16u) *(v4i *)(g_at + i) = v4i{0, 0, 0, 0};
+    fetch(lds);
+    ask(first + kMany);
+    stage_barrier<0>();
+    uint32_t now = 0;
+    for (uint32_t e0 = first; ; e0 += kMany) {
+        const uint32_t many = min(last - e0, kMany), at = place_of(pair.x);
+        if (threadIdx.x < many) set(at, left);
+        stage_barrier<0>();
+        v4i x[T::NU], g[T::MT], rest[T::MT];
+        auto read = [&](int half) {
+#pragma unroll
+            for (int u = 0; u < T::NU; ++u) x[u] = rp(lds + now, u, half);
+#pragma unroll
+            for (int t = 0; t < T::MT; ++t) { g[t] = rq(g_at, t, half); rest[t] = rq(g_at + kG, t, half); }
+        };
+        auto multiply_read = [&]() {
+            multiply_all<T::DT>(x, g, acc);
+            multiply_all<T::DT>(x, rest, acc);
+        };
+        read(0);
+        if (many > kMany / 2u) {
+            multiply_read();
+            read(1);
+        }
+        if (e0 + kMany < last) fetch(lds + (now ^ kX));
+        ask(e0 + 2u * kMany);
+        pair = next;
+        left = p.hit[pair.y];
+        next = pair_of(e0 + 2u * kMany + lane);
+        asm volatile("" ::: "memory");                           // (asked for before the products, not behind them)
+        multiply_read();
+        if (e0 + kMany >= last) return;
+        now ^= kX;
+        stage_barrier<63>();                                     // all have read G, and x may still be on its way
+        if (threadIdx.x < kMany) set(at, 0.0f);
     }
 }
 
@@ -499,8 +555,7 @@ struct RoundParams {
     const float   *sums;
     int64_t        part_stride, count;
     void          *y;
-    const float   *scale, *hit;      // hit: null, or as in LossParams, with rank
-    const uint32_t *rank;
+    const float   *scale, *hit;      // hit: null, or as in LossParams
     const LossRow *rows;
     Operand        w;
     uint32_t       parts, K;
@@ -524,14 +579,25 @@ __global__ __launch_bounds__(256) void loss_round_kernel(RoundParams p)
             for (int j = 0; j < 4; ++j)
                 for (uint32_t k = 0; i + j < p.count && k < p.parts; ++k) s[j] += p.sums[k * p.part_stride + i + j];
         if (DT != RS_DTYPE_F32 && p.hit) {
-            int64_t m = i / p.K;
+            int64_t m = p.count >> 32 ? i / p.K : (uint32_t)i / p.K;
             uint32_t k = (uint32_t)(i - m * p.K);
+            auto row_of = [&](int32_t token) { return (const uint16_t *)(p.w.at + (int64_t)token * p.w.stride); };
+            if (k + 4u <= p.K) {
+                const int32_t token = p.rows[m].token;
+                if (token >= 0) {
+                    uint2 w;
+                    __builtin_memcpy(&w, row_of(token) + k, 8);
+                    const float left = p.hit[m];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int32_t token = i + j < p.count ? p.rows[m].token : -1;
-                if (token >= 0) s[j] += p.hit[p.rank[m]] * widen16<DT>(((const uint16_t *)(p.w.at + (int64_t)token * p.w.stride))[k]);
-                if (++k == p.K) { k = 0; ++m; }
-            }
+                    for (int j = 0; j < 4; ++j) s[j] += left * widen16<DT>((j < 2 ? w.x : w.y) >> (16 * (j % 2)) & 0xFFFFu);
+                }
+            } else
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int32_t token = i + j < p.count ? p.rows[m].token : -1;
+                    if (token >= 0) s[j] += p.hit[m] * widen16<DT>(row_of(token)[k]);
+                    if (++k == p.K) { k = 0; ++m; }
+                }
         }
         s *= f;
         if (whole) put_four<DT>(p.y, i, s);

@@ -16,8 +16,9 @@ struct LossSpace {
     uint64_t grad_stride = 0;
     uint32_t shares = 1;                                // of the product's reduction
     uint64_t sums = 0, sum_stride = 0;
-    uint64_t hit = 0, order = 0, rank = 0, starts = 0;
-    uint32_t n_starts = 0;                              // 0: what G's rounding leaves at the tokens is not made up for
+    uint64_t hit = 0, order = 0, starts = 0;
+    SortSpace sort = {};                                // of more than kCountRows rows, in the place of order
+    uint32_t n_starts = 0;                              // 0: what G's rounding leaves at the tokens is not made up for by itself
     uint64_t take(uint64_t n) { const uint64_t at = bytes; bytes += up(n, 256); return at; }
 };
 
@@ -55,11 +56,11 @@ static LossSpace loss_space(int32_t M, int32_t V, int32_t K, int32_t dtype, bool
     }
     s.high = (M <= (int32_t)kFewRows || (M <= (int32_t)(2 * kFewRows) && 16 * M > V)) && dtype != RS_DTYPE_F32 ? 2 * M : M;
     if (s.high > (uint32_t)M) s.twice = s.take(s.high * up((uint64_t)K * size, 16));
-    else if (dtype != RS_DTYPE_F32 && M <= (int32_t)kHitRows && 16 * M <= V) {
+    else if (dtype != RS_DTYPE_F32) {
         s.n_starts = (uint32_t)(up(V, kStretch) / kStretch) + 1;
         s.hit = s.take((uint64_t)M * 4);
-        s.order = s.take((uint64_t)M * 8);
-        s.rank = s.take((uint64_t)M * 4);
+        if (M <= (int32_t)kCountRows) s.order = s.take((uint64_t)M * 8);
+        else s.sort = sort_space((uint32_t)M, (uint32_t)V, s.bytes);
         s.starts = s.take((uint64_t)s.n_starts * 4);
     }
     s.scale = s.take(8);
@@ -206,10 +207,19 @@ static void backward(LossParams p, const LossSpace &s, Operand x, Operand w, uin
     constexpr uint32_t size = kSize<DT>;
     if (DT == RS_DTYPE_F16) hipLaunchKernelGGL(loss_scale_kernel, dim3(1), dim3(1024), 0, st, p);
     else p.scale = nullptr;
+    uint2 *counted = nullptr;
     if (s.n_starts) {
-        p.hit = (float *)(ws + s.hit); p.order = (uint2 *)(ws + s.order); p.rank = (uint32_t *)(ws + s.rank); p.starts = (uint32_t *)(ws + s.starts); p.n_starts = s.n_starts;
+        p.hit = (float *)(ws + s.hit);
+        if (grad_w) {
+            p.starts = (uint32_t *)(ws + s.starts); p.n_starts = s.n_starts;
+            if (p.M <= kCountRows) p.order = counted = (uint2 *)(ws + s.order);
+            else {
+                p.order = launch_sort(TokenList{p.tokens, p.token_stride, p.tokens_64}, p.M, p.V, s.sort, ws, nullptr, 0, st);
+                hipLaunchKernelGGL(loss_starts_kernel, dim3((p.n_starts + 255) / 256), dim3(256), 0, st, p);
+            }
+        }
     }
-    hipLaunchKernelGGL(loss_rows_kernel, dim3(s.n_starts ? (p.M + 63) / 64 + (s.n_starts + 63) / 64 : (p.M + 255) / 256), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(loss_rows_kernel, dim3(counted ? (p.M + 63) / 64 + (p.n_starts + 63) / 64 : (p.M + 255) / 256), dim3(256), 0, st, p, counted);
     Operand xs = x;
     if (s.high > p.M) {
         p.rest = p.M;
@@ -251,7 +261,7 @@ static void backward(LossParams p, const LossSpace &s, Operand x, Operand w, uin
         RoundParams r = {};
         r.count = (int64_t)p.M * K;
         r.sums = (const float *)(ws + s.dx); r.part_stride = r.count; r.parts = s.split * (s.high / p.M);
-        r.y = grad_x; r.scale = p.scale; r.hit = p.hit; r.rank = p.rank; r.rows = p.rows; r.w = w; r.K = K;
+        r.y = grad_x; r.scale = p.scale; r.hit = p.hit; r.rows = p.rows; r.w = w; r.K = K;
         hipLaunchKernelGGL(loss_round_kernel<DT>, dim3((uint32_t)std::min<int64_t>((r.count + 1023) / 1024, 1 << 16)), dim3(256), 0, st, r);
     }
 }

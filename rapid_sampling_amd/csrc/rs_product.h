@@ -122,7 +122,9 @@ struct Side {
         if (kSize<DT> == 2) byte = ((byte / 32u) ^ turn(row)) * 32u + byte % 32u;
         else byte ^= (row / 8u & 3u) * 64u;
     }
-    __device__ __forceinline__ uint32_t place(uint32_t i) const { return (i * WAVES + wave_id()) * 1024u + threadIdx.x % 64u * 16u; }
+    // and where a byte of an r is held, of a transposed stage of 16 bits
+    static __device__ __forceinline__ uint32_t place_of(uint32_t row, uint32_t byte) { return row * kWide + ((byte / 32u) ^ turn(row)) * 32u + byte % 32u; }
+    static __device__ __forceinline__ uint32_t place(uint32_t i) { return (i * WAVES + wave_id()) * 1024u + threadIdx.x % 64u * 16u; }
 
     __device__ __forceinline__ Side(const Operand &o, uint32_t first)
     {
