@@ -74,7 +74,7 @@ not depend on what stands beside it.  No gradient, as linear_fp8.
 
 `linear_int8` shares linear_fp8's workspace of a stream, which its first call there or `reserve_workspace` makes; captured into a graph it has one of its own,
 as the others have their scratch memory: nothing needs to be reserved for any of these before a capture.
-A training step can be captured; while a graph of the same leaf that was made on another stream lives, that is refused.
+A training step can be captured; while a graph of the same leaf that was made on the default stream lives, that is refused.
 
 The functions live in the compiled extension `_sample` (host layer in
 csrc/sampling.cpp, kernels in csrc/rs_*.hip and csrc/rs_*.h behind the C ABI of

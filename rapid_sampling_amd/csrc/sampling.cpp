@@ -292,9 +292,10 @@ void refuse_tangent(const char *what, std::initializer_list<at::Tensor> inputs)
             throw std::invalid_argument(std::string(what) + " has no forward-mode derivative: call it on tensors without a tangent !\n");
 }
 
-// A leaf's gradient is summed on the stream on which the first graph alive that holds the leaf was made.  A backward pass that is captured on another would
-// pull that stream into the capture, or, of the default one, end it and the process: refused while the forward pass is captured.
-void refuse_other_graph(const char *what, std::initializer_list<at::Tensor> inputs)
+// A leaf's gradient is summed on the stream on which the first graph alive that holds the leaf was made.  A backward pass that is captured on another pulls
+// that stream into the capture, and joins it again (a warm-up on a side stream whose loss is still held); the default one cannot be
+// captured, and the attempt would end the capture and the process: refused while the forward pass is captured.
+void refuse_default_graph(const char *what, std::initializer_list<at::Tensor> inputs)
 {
     for (const at::Tensor &t : inputs) {
         if (!t.is_cuda() || !t.requires_grad() || !t.is_leaf()) continue;
@@ -302,10 +303,9 @@ void refuse_other_graph(const char *what, std::initializer_list<at::Tensor> inpu
         if (!sum) continue;
         const auto of = sum->stream();
         c10::hip::HIPGuardMasqueradingAsCUDA guard(t.device());
-        void *stream = current_stream(t);
-        if (is_capturing(stream) && of && (void *)c10::hip::HIPStreamMasqueradingAsCUDA(*of).stream() != stream)
-            throw std::runtime_error(std::string("rapid_sampling: ") + what + " is being captured while a graph of the same leaf from another stream lives; drop that "
-                                     "graph's outputs before the capture, or make it on the captured stream");
+        if (is_capturing(current_stream(t)) && of && !c10::hip::HIPStreamMasqueradingAsCUDA(*of).stream())
+            throw std::runtime_error(std::string("rapid_sampling: ") + what + " is being captured while a graph of the same leaf from another stream lives, the default "
+                                     "one, which cannot be captured; drop that graph's outputs before the capture, or make it on a stream of its own");
     }
 }
 
@@ -977,7 +977,7 @@ at::Tensor embedding(const at::Tensor &tokens, const at::Tensor &weight, double 
 {
     if (!weight.requires_grad() || !at::GradMode::is_enabled()) return embedding_forward(tokens, weight, scale, weight_scale, out_dtype);
     const TableCall c = read_table(tokens, weight, scale, weight_scale, out_dtype);
-    refuse_other_graph("embedding", {weight});
+    refuse_default_graph("embedding", {weight});
     return Embedding::apply(weight, tokens, scale, (int64_t)c.to);
 }
 
@@ -986,7 +986,7 @@ std::tuple<at::Tensor, at::Tensor> linear_cross_entropy(const at::Tensor &x, con
 {
     refuse_tangent("linear_cross_entropy", {x, weight});
     if ((x.requires_grad() || weight.requires_grad()) && at::GradMode::is_enabled()) {
-        refuse_other_graph("linear_cross_entropy", {x, weight});
+        refuse_default_graph("linear_cross_entropy", {x, weight});
         variable_list o = Loss::apply(x, weight, tokens, temperature);
         return {o[0], o[1]};
     }
