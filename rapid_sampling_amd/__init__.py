@@ -59,11 +59,13 @@ written whole: rows that no token names are 0.
 
 `linear_cross_entropy(x, weight, tokens, temperature=1.0)`: x (..., K) and weight (V, K) of one type, tokens (...).  `logsumexp` is
 ln sum e^(x . w / temperature), `loss` that minus the token's own x . w / temperature; 0 for a negative token, NaN for one
-outside the vocabulary.  Both have gradients by x and weight (once, in reverse mode; logsumexp's for an auxiliary loss).  The
-logits are never kept: the vocabulary is worked through in pieces of up to 128 MB of what takes their place (8192 columns at least), and made
-again in the backward pass.  What multiplies the operands there is rounded to their type, and what the rounding leaves is made up for: all of it for up to
-32 rows (64 over fewer than 16 times as many tokens), and at the rows' own tokens for more, so that gradients in 16 bits are off by little more than their own rounding; all sums are float32.  float32 operands are taken apart into three bfloat16
-numbers each, whose products are off by at most 2^-22 and by 2^-26 on average, in either direction.
+outside the vocabulary.  Both have gradients by x and weight (once, in reverse mode; logsumexp's for an auxiliary loss).  Logits
+are not kept for the gradients: the backward pass makes them again, in pieces of the vocabulary, and has of what takes their place at most 128 MB or rows x 8192 numbers, whichever
+is more (so all of it for a vocabulary of up to 8192, or for few rows), next to float32 sums of the size of x (up to 32 of them for few rows).  The forward pass has 8
+bytes for a row and 64 tokens.  (Small products of long rows leave partial logits in float32 in either pass, up to 17 MB.)  What multiplies the operands there is rounded to their type, and
+what the rounding leaves is made up for: all of it for up to 32 rows (64 over fewer than 16 times as many tokens), and at the rows' own tokens for more, so that gradients in 16 bits are off
+by little more than their own rounding; all sums are float32.  float32 operands are taken apart into three bfloat16 numbers each, whose products are off by at most 2^-22 and by 2^-26 on
+average, in either direction.
 Rows that do not begin at multiples of 16 bytes (K an odd number, say) are laid out anew by every call: for few rows of x that costs more than the product;
 under autograd the new table is kept for the gradients.
 

@@ -90,7 +90,7 @@ __device__ __forceinline__ void store8(void *y, int64_t at, uint32_t k, uint32_t
 }
 
 // 2^width threads to a row, eight values at a time.  Bound by the launch or by memory: 64 rows of 4096 in int8 2.6 us, 8192 in bfloat16 31 (4.3 TB/s,
-// read and written).
+// read and written), in int8 or e4m3 into bfloat16 16.5 (6.1).
 template <int WT, int DT>
 __global__ __launch_bounds__(256) void embedding_kernel(EmbeddingParams p)
 {

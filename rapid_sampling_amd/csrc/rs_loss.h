@@ -56,7 +56,7 @@ __device__ __forceinline__ int64_t loss_token(const LossParams &p, uint32_t m)
     return p.tokens_64 ? ((const int64_t *)p.tokens)[(int64_t)m * p.token_stride] : ((const int32_t *)p.tokens)[(int64_t)m * p.token_stride];
 }
 
-// Bound by the product, or for few rows by reading w: 8192 x 131072 x 4096 in bfloat16 6.4 ms (1.37 PFLOP/s), 1 x 65536 x 4096 91 us (5.9 TB/s).
+// Bound by the product, or for few rows by reading w: 8192 x 131072 x 4096 in bfloat16 6.3 ms (1.40 PFLOP/s), 1 x 65536 x 4096 90 us (6.0 TB/s).
 template <class T>
 __global__ __launch_bounds__(T::kThreads, 2) void loss_tile_kernel(LossParams p)
 {
@@ -128,7 +128,7 @@ __device__ __forceinline__ void finish_row(const LossParams &p, uint32_t m, floa
     if (p.stats) p.stats[m] = none ? make_float2(0.0f, __builtin_inff()) : sum;
 }
 
-// 2^WIDTH rows to a workgroup, 256 / 2^WIDTH threads to a row (8192 rows of 1024 stretches 62 us, one row 4).
+// 2^WIDTH rows to a workgroup, 256 / 2^WIDTH threads to a row (8192 rows of 1024 stretches 60 us, one row 4).
 __global__ __launch_bounds__(256) void loss_join_kernel(LossParams p, uint32_t width)
 {
     __shared__ float2 held[256];
@@ -293,7 +293,7 @@ template <int DT> __device__ __forceinline__ float rounding_left(float v)
     return d == d ? d : 0.0f;
 }
 
-// (8192 rows, a piece of 8192 tokens, 4096 columns in bfloat16: 408 us, 1.35 PFLOP/s)
+// (8192 rows, a piece of 8192 tokens, 4096 columns in bfloat16: 401 us, 1.37 PFLOP/s)
 template <class T>
 __global__ __launch_bounds__(T::kThreads, 2) void loss_grad_kernel(LossParams p)
 {
@@ -518,7 +518,7 @@ template <class T> __device__ __forceinline__ void add_hits(const GradParams &p,
     }
 }
 
-// dw of one piece, whole.  (The same piece: 473 us; both operands are turned.)
+// dw of one piece, whole.  (The same piece: 470 us; both operands are turned.)
 template <class T>
 __global__ __launch_bounds__(T::kThreads, 2) void loss_dw_kernel(GradParams p)
 {

@@ -30,7 +30,7 @@ static TileSize dx_size(uint64_t rows, uint64_t columns) { return rows <= 64 ? k
 // one and shared.  bfloat16: 64 x 1000 x 4096 31.8, 77.5 and 11.4, 39.0; 4 x 16000 x 4096 31.4, 120 and 29.6, 116; 64 x 1000 x 1024 14.7,
 // 40.2 and 10.4, 35.4; of 188 tiles, 64 x 24000 x 4096, 35.7, 172 and 43.2, 193.  float32, whose tiles take four times as long: 64 x 1000 x 4096 148, 321
 // and 18.8, 62.1; 64 x 8000 x 1024 44.5, 118 and 23.9, 77.8; of 188 tiles 156, 511 and 127, 483; of 243, 64 x 31000 x 1024, 45.7, 171 and
-// 44.1, 170.)
+// 44.1, 170, with products that took up to 3 % less than they do.)
 static uint32_t product_shares(uint64_t M, uint64_t V, uint64_t K, int32_t dtype)
 {
     const uint64_t tiles = tiles_of(M, V, 64, 128);
@@ -38,8 +38,9 @@ static uint32_t product_shares(uint64_t M, uint64_t V, uint64_t K, int32_t dtype
     return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({512 / tiles, K * size_of(dtype) / kRowBytes / 8, 32}));
 }
 
-// A piece of the vocabulary: G of the piece stays within the last cache (256 MB) with the piece's weights, in steps of 256 tokens and
-// at least 8192, so that the sums of dx that each piece reads and writes again (8 bytes) are little next to its products.
+// A piece of the vocabulary: 128 MB of G, half of the last cache, in steps of 256 tokens and at least 8192, so that the sums of dx that each piece reads and
+// writes again (8 bytes) are little next to its products.  For many rows the piece's weights stay there with it (8192 tokens of 4096 columns are 64 MB); for
+// up to a few hundred the piece is most of the vocabulary or all of it, and weights beyond the cache are read from memory by each of the products.
 static LossSpace loss_space(int32_t M, int32_t V, int32_t K, int32_t dtype, bool backward)
 {
     LossSpace s;
@@ -85,7 +86,7 @@ template <int DT, bool TP, bool TQ> using SmallTile = Tile<DT, TP, TQ, !TP && DT
 
 // float32 and up to 16 rows: 128 x 16 by two waves, which take a row of x apart once for four of w's and make no products for rows that are not there.
 // (Forward, and with gradients, us, 128 x 64 and so: 1 x 50000 x 1024 57.6, 219 and 44.1, 183; 16 x 24000 x 4096 112, 414 and 93, 378; 16 x 100000 x 4096
-// 417, 1544 and 342, 1325.  128 x 32 for up to 32 rows would save 2 to 10 of 100 more.)
+// 417, 1544 and 342, 1325, with products that took up to 3 % less.  128 x 32 for up to 32 rows would save 2 to 10 of 100 more.)
 constexpr uint32_t kNarrowRows = 16;
 template <int DT, bool TP, bool TQ> using NarrowTile = Tile<DT, TP, TQ, false, 2, 1, 4, 1, 4>;
 static bool narrow(int32_t dtype, uint32_t rows) { return dtype == RS_DTYPE_F32 && rows <= kNarrowRows; }
