@@ -189,8 +189,8 @@ __global__ __launch_bounds__(256) void loss_shares_kernel(LossParams p)
 // rounding left is made up for.  Of up to kFewRows rows (twice as many over less than sixteen times as many tokens) all of it is kept, as
 // rows of their own behind G's: the products are then of twice as many rows, and wait for memory all the same (forward and gradients of 1 row
 // of 4096 over 131072 in bfloat16 876 us without, 890 with; of 48 rows it would be 907 and 1012).  Of more rows that of each row at its own
-// token, the largest of the row as long as it is not learnt, is added to the two products' sums (loss_round_kernel, add_hits): errors are 1.00 to 1.01 times
-// the result's own rounding, and up to 1.07 over vocabularies of a few hundred tokens.  (us without and with it: 8192 x 131072 x 4096 in bfloat16 28620 and 28750, 4096 x
+// token, the largest of the row as long as it is not learnt, is added to the two products' sums (loss_round_kernel, add_hits): errors are 1.00 to 1.05 times
+// the result's own rounding (1.07 over 100 tokens; 1.03 to 1.14 at a temperature of 0.5, where other tokens have much of a row too).  (us without and with it: 8192 x 131072 x 4096 in bfloat16 28620 and 28750, 4096 x
 // 50257 x 1024 in float16 1810 and 1860, 8192 x 8000 x 4096 1840 and 1920, 2000 x 7900 x 4096 476 and 528, 8192 x 512 x 4096 290 and 348.)
 __global__ __launch_bounds__(1024) void loss_scale_kernel(LossParams p)
 {
